@@ -112,6 +112,16 @@ _SIGNATURES = {
     "fb_row_scales": [c_void_p, c_int, c_int, c_int, c_float, c_void_p, c_int, c_void_p],
     "fb_select_tokens": [c_void_p, c_ll, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                          c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p],
+    "fb_edit_logits": [c_void_p, c_ll, c_int, c_int, c_void_p, c_ll, c_void_p, c_void_p],
+    "fb_record_tokens": [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int,
+                         c_void_p],
+    "fb_sample_rules": [c_void_p, c_ll, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                        c_void_p],
+    "fb_adapter_shrink": [c_void_p, c_ll, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
+                          c_int, c_void_p, c_void_p],
+    "fb_adapter_expand": [c_void_p, c_int, c_ll, c_ll, c_void_p, c_void_p, c_int, c_void_p, c_int,
+                          c_int, c_int, c_int, c_void_p, c_int, c_ll, c_void_p],
     "fb_ln_add_ln": [c_void_p, c_int, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p,
                      c_void_p, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_int,
                      c_void_p],
@@ -1898,6 +1908,310 @@ def select_tokens(logits: torch.Tensor, out: torch.Tensor, temperature: Optional
           _arrival_counters(logits.device, n).data_ptr() if also is not None and chunks > 1 else 0,
           chunks, 0 if part_val is None else part_val.data_ptr(),
           0 if part_idx is None else part_idx.data_ptr(), _stream())
+    return out
+
+
+# --------------------------------------------------- what a request brings of its own: logits
+def _given(t, name: str, dtype: torch.dtype, shape, device) -> int:
+    """The address of a contiguous tensor that a caller hands over (None: 0): its type, its shape
+    (None: any), and the device of the call, which is the current one."""
+    if t is None:
+        return 0
+    if t.dtype != dtype:
+        raise KernelError(f"{name} has dtype {t.dtype}, expected {dtype}")
+    if shape is not None and tuple(t.shape) != shape:
+        raise KernelError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    if not t.is_contiguous():
+        raise KernelError(f"{name} is not contiguous")
+    if t.device != device:
+        raise KernelError(f"{name} is on {t.device}, the call's rows are on {device}")
+    return t.data_ptr()
+
+
+def _on_current_device(t: torch.Tensor, name: str) -> None:
+    if not t.is_cuda:
+        raise KernelError(f"{name} is on {t.device}; the kernels run on CUDA devices only")
+    if t.device.index != _current_device():
+        raise KernelError(f"{name} is on {t.device}, the current device is {_current_device()}")
+
+
+IN_PROMPT = 1 << 30  # FB_IN_PROMPT in csrc/logit_edits.cuh
+
+
+class TokenHistory:
+    """Which tokens each of several sequences holds: `counts` int32 [rows, vocab] (bits 0..29 how
+    often a token was generated, bit 30 whether the prompt holds it) and `seen` int32
+    [rows, ceil(vocab / 32)], a bit a token, set where its count is not zero. The penalties of
+    `LogitEdits` read a row of it; `record_tokens` writes it."""
+
+    def __init__(self, counts: torch.Tensor, seen: torch.Tensor):
+        if counts.dim() != 2 or seen.dim() != 2 or seen.shape[0] != counts.shape[0] or \
+                seen.shape[1] != (counts.shape[1] + 31) // 32:
+            raise KernelError(f"a history of {tuple(counts.shape)} counts has {tuple(seen.shape)} words "
+                              f"of bits")
+        self.counts, self.seen = counts, seen
+
+    @classmethod
+    def empty(cls, rows: int, vocab: int, device) -> "TokenHistory":
+        return cls(torch.zeros(rows, vocab, dtype=torch.int32, device=device),
+                   torch.zeros(rows, (vocab + 31) // 32, dtype=torch.int32, device=device))
+
+    @property
+    def rows(self) -> int:
+        return self.counts.shape[0]
+
+    @property
+    def vocab(self) -> int:
+        return self.counts.shape[1]
+
+    def clear(self, rows: Sequence[int]) -> None:
+        """These rows hold no token."""
+        zero_rows([t for r in rows for t in (self.counts[r], self.seen[r])])
+
+
+_RECORD = {"prompt": 0, "generated": 1, "taken back": 2}
+
+
+def record_tokens(history: TokenHistory, rows: torch.Tensor, tokens: torch.Tensor,
+                  what: str = "generated") -> None:
+    """Token i goes into the history's row `rows[i]` (int32 both; a row or a token outside of the
+    table is skipped): as one that the "prompt" holds, that was "generated" once more, or whose last
+    generation is "taken back". A token may come several times in one call."""
+    if what not in _RECORD:
+        raise KernelError(f"record_tokens: {what!r}; known: {sorted(_RECORD)}")
+    _on_current_device(history.counts, "counts")
+    device, n = history.counts.device, tokens.numel()
+    _call("fb_record_tokens",
+          _given(history.counts, "counts", torch.int32, None, device),
+          _given(history.seen, "seen", torch.int32, None, device), history.rows,
+          history.seen.shape[1], history.vocab, _given(rows, "rows", torch.int32, (n,), device),
+          _given(tokens, "tokens", torch.int32, (n,), device), n, _RECORD[what], _stream())
+
+
+class TokenBiases:
+    """What is added to some logits of each row: row r's are entries starts[r] to starts[r + 1] of
+    `ids` (int32, ascending within a row; equal ones add up; outside of the vocabulary: no effect)
+    and `values` (float32)."""
+
+    def __init__(self, starts: torch.Tensor, ids: torch.Tensor, values: torch.Tensor):
+        if ids.shape != values.shape or ids.dim() != 1 or starts.dim() != 1 or starts.numel() < 1:
+            raise KernelError(f"biases: starts {tuple(starts.shape)}, ids {tuple(ids.shape)}, values "
+                              f"{tuple(values.shape)}")
+        self.starts, self.ids, self.values = starts, ids, values
+
+    @classmethod
+    def from_rows(cls, rows: Sequence[Optional[dict]], device) -> "TokenBiases":
+        """One {token: bias} (or None) a row."""
+        starts, ids, values = [0], [], []
+        for row in rows:
+            for token in sorted(row or {}):
+                ids.append(int(token))
+                values.append(float(row[token]))
+            starts.append(len(ids))
+        at = lambda v, dtype: torch.tensor(v, dtype=dtype).to(device)  # noqa: E731
+        return cls(at(starts, torch.int32), at(ids, torch.int32), at(values, torch.float32))
+
+
+class LogitEdits:
+    """The edits of the rows of a step, all optional (csrc/logit_edits.cuh has the formulas):
+
+    `history` and `history_rows` (int32, a row's place in it; outside of it: no penalties) with
+    `repetition`, `frequency` and `presence` (float32, one a row; None: no effect);
+    `bias`, the rows' `TokenBiases`;
+    `allowed` (int32 [masks, ceil(vocab / 32)], a bit a token) and `allowed_rows` (int32, a row's
+    mask; outside of it: every token is allowed)."""
+
+    def __init__(self, history: Optional[TokenHistory] = None,
+                 history_rows: Optional[torch.Tensor] = None,
+                 repetition: Optional[torch.Tensor] = None,
+                 frequency: Optional[torch.Tensor] = None, presence: Optional[torch.Tensor] = None,
+                 bias: Optional[TokenBiases] = None, allowed: Optional[torch.Tensor] = None,
+                 allowed_rows: Optional[torch.Tensor] = None):
+        if (history is None) != (history_rows is None):
+            raise KernelError("a history comes with the rows' places in it")
+        if history is None and not (repetition is None and frequency is None and presence is None):
+            raise KernelError("penalties need a history")
+        if (allowed is None) != (allowed_rows is None):
+            raise KernelError("masks come with the rows' places among them")
+        self.history, self.history_rows = history, history_rows
+        self.repetition, self.frequency, self.presence = repetition, frequency, presence
+        self.bias, self.allowed, self.allowed_rows = bias, allowed, allowed_rows
+
+    def packed(self, n: int, vocab: int, device):
+        """The fields as the kernels take them, checked for `n` rows of `vocab` logits."""
+        words = (vocab + 31) // 32
+        out = [0] * 15
+        out[4] = words
+        h = self.history
+        if h is not None:
+            if h.vocab != vocab:
+                raise KernelError(f"a history of {h.vocab} tokens for logits of {vocab}")
+            out[:4] = (_given(h.counts, "counts", torch.int32, None, device),
+                       _given(h.seen, "seen", torch.int32, None, device),
+                       _given(self.history_rows, "history_rows", torch.int32, (n,), device), h.rows)
+            out[5:8] = (_given(self.repetition, "repetition", torch.float32, (n,), device),
+                        _given(self.frequency, "frequency", torch.float32, (n,), device),
+                        _given(self.presence, "presence", torch.float32, (n,), device))
+        b = self.bias
+        if b is not None:
+            out[8:12] = (_given(b.starts, "starts", torch.int32, (n + 1,), device),
+                         _given(b.ids, "ids", torch.int32, None, device),
+                         _given(b.values, "values", torch.float32, None, device), b.ids.numel())
+        if self.allowed is not None:
+            masks = self.allowed.shape[0]
+            out[12:] = (_given(self.allowed, "allowed", torch.int32, (masks, words), device),
+                        _given(self.allowed_rows, "allowed_rows", torch.int32, (n,), device), masks)
+            if masks == 0:
+                out[12] = 0
+        if h is not None and h.rows == 0:
+            out[0] = 0
+        return (c_ll * 15)(*out)
+
+
+def _logit_rows(logits: torch.Tensor, what: str):
+    if logits.dim() != 2 or logits.dtype != torch.float32:
+        raise KernelError(f"{what}: logits are float32 rows, got {logits.dtype} {tuple(logits.shape)}")
+    _on_current_device(logits, "logits")
+    stride = _rows(logits, "logits")
+    n, V = logits.shape
+    if V == 0:
+        raise KernelError(f"{what}: logits of no token")
+    return n, V, max(stride, V) if n <= 1 else stride
+
+
+def edit_logits(logits: torch.Tensor, edits: LogitEdits,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The edited logits of every row, float32 (a new tensor, or `out`, which may be `logits`)."""
+    n, V, stride = _logit_rows(logits, "edit_logits")
+    if out is None:
+        out = torch.empty((n, V), dtype=torch.float32, device=logits.device)
+    elif out.shape != logits.shape or out.dtype != torch.float32 or out.device != logits.device:
+        raise KernelError(f"edit_logits: out is {out.dtype} {tuple(out.shape)} on {out.device}")
+    packed = edits.packed(n, V, logits.device)
+    _call("fb_edit_logits", logits.data_ptr(), stride, n, V, out.data_ptr(),
+          max(_rows(out, "out"), V) if n <= 1 else _rows(out, "out"), ctypes.addressof(packed),
+          _stream(), tag=("n{} v{}", n, V))
+    return out
+
+
+class SampleRules:
+    """How the rows of a step draw their tokens, one entry a row (None: off): `temperature` float32
+    (0: the largest logit, the lowest index among equals), `top_k` int32 (0: off), `top_p` float32
+    (1: off), `min_p` float32 (0: off), and the random `streams` and `steps` of `select_tokens`,
+    int64."""
+
+    def __init__(self, temperature: Optional[torch.Tensor] = None,
+                 top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+                 min_p: Optional[torch.Tensor] = None, streams: Optional[torch.Tensor] = None,
+                 steps: Optional[torch.Tensor] = None):
+        self.temperature, self.top_k, self.top_p, self.min_p = temperature, top_k, top_p, min_p
+        self.streams, self.steps = streams, steps
+
+
+MAX_SAMPLE_VOCAB = 8 * 49152  # a cluster's shared memory (csrc/sample_rules.cu)
+
+
+def sample_tokens(logits: torch.Tensor, rules: SampleRules, edits: Optional[LogitEdits] = None,
+                  record: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                  logprobs: Optional[torch.Tensor] = None, also: Optional[torch.Tensor] = None):
+    """(tokens int32, logprobs float32), one a row, drawn under `rules` from the logits as `edits`
+    leaves them (csrc/sample_rules.cu): top-k, then top-p among those, then min-p; the log-probability
+    is the token's under softmax(edited / temperature) before anything is cut off. A row whose edits
+    leave no token gives -1 and -inf. `record` (int32, one a row): the tokens that the histories of
+    `edits` count as generated first (the step's inputs; no two rows may share a history then).
+    `also`: a second place for the tokens, the next step's input, where a row without a token gets 0."""
+    n, V, stride = _logit_rows(logits, "sample_tokens")
+    device = logits.device
+    if V > MAX_SAMPLE_VOCAB:
+        raise KernelError(f"sample_tokens: a vocabulary of {V} ({MAX_SAMPLE_VOCAB} at most)")
+    if out is None:
+        out = torch.empty(n, dtype=torch.int32, device=device)
+    if logprobs is None:
+        logprobs = torch.empty(n, dtype=torch.float32, device=device)
+    if record is not None and (edits is None or edits.history is None):
+        raise KernelError("sample_tokens: tokens to record, and no history")
+    packed = None if edits is None else edits.packed(n, V, device)
+    r, each = rules, (n,)
+    _call("fb_sample_rules", logits.data_ptr(), stride, n, V,
+          _given(r.temperature, "temperature", torch.float32, each, device),
+          _given(r.top_k, "top_k", torch.int32, each, device),
+          _given(r.top_p, "top_p", torch.float32, each, device),
+          _given(r.min_p, "min_p", torch.float32, each, device),
+          _given(r.streams, "streams", torch.int64, each, device),
+          _given(r.steps, "steps", torch.int64, each, device),
+          0 if packed is None else ctypes.addressof(packed),
+          _given(record, "record", torch.int32, each, device),
+          _given(out, "out", torch.int32, each, device),
+          _given(logprobs, "logprobs", torch.float32, each, device),
+          _given(also, "also", torch.int32, each, device), _stream(), tag=("n{} v{}", n, V))
+    return out, logprobs
+
+
+# ------------------------------------------- what a request brings of its own: an adapter
+MAX_ADAPTER_RANK = 512
+
+
+class AdapterBank:
+    """The low-rank adapters of one projection [N, K]: `a` [slots, rank, K] and `b` [slots, N, rank] in
+    the projection's type, `scales` float32 [slots]. An adapter of a smaller rank has zeros in the
+    rest."""
+
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor):
+        if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2] or \
+                tuple(scales.shape) != (a.shape[0],) or a.shape[0] == 0:
+            raise KernelError(f"adapters: a {tuple(a.shape)}, b {tuple(b.shape)}, scales "
+                              f"{tuple(scales.shape)}")
+        if a.shape[1] % 8 or not 8 <= a.shape[1] <= MAX_ADAPTER_RANK:
+            raise KernelError(f"adapters of rank {a.shape[1]}: a multiple of 8 up to {MAX_ADAPTER_RANK} "
+                              f"(fill up with zeros)")
+        self.a, self.b, self.scales = a, b, scales
+
+    @property
+    def slots(self) -> int:
+        return self.a.shape[0]
+
+    @property
+    def rank(self) -> int:
+        return self.a.shape[1]
+
+
+def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
+                    out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """y[t] = x[t] w^T + scale_a (x[t] a_a^T) b_a^T with a = index[t] (int32, one a token; outside of
+    the bank: no adapter). Sums are 32-bit, the ranks' numbers too, and y is rounded once, to
+    `out_dtype` (the input's type)."""
+    x = plain(x)
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise KernelError(f"adapted_product: x {tuple(x.shape)}, w {tuple(w.shape)}")
+    (T, K), N = x.shape, w.shape[0]
+    if w.dtype != x.dtype:
+        raise KernelError(f"adapted_product: x is {x.dtype}, w is {w.dtype}")
+    if tuple(bank.a.shape[1:]) != (bank.rank, K) or tuple(bank.b.shape[1:]) != (N, bank.rank):
+        raise KernelError(f"adapted_product: adapters {tuple(bank.a.shape)}, {tuple(bank.b.shape)} beside "
+                          f"a projection {tuple(w.shape)}")
+    _on_current_device(x, "x")
+    device = x.device
+    a = _given(bank.a, "a", x.dtype, None, device)
+    b = _given(bank.b, "b", x.dtype, None, device)
+    scales = _given(bank.scales, "scales", torch.float32, None, device)
+    which = _given(index, "index", torch.int32, (T,), device)
+    out = torch.empty((T, N), dtype=out_dtype or x.dtype, device=device)
+    if T == 0:
+        return out
+    if x.dtype == torch.float32:
+        base = gemm_simt(x, w, torch.empty((T, N), dtype=torch.float32, device=device))
+    else:
+        base = gemm_bf16(x, w, None, torch.float32, allow_planes=True)
+    planes = 1
+    if isinstance(base, Planes):
+        planes, base = base.count, base.tensor
+    low = torch.empty((T, bank.rank), dtype=torch.float32, device=device)
+    _call("fb_adapter_shrink", x.data_ptr(), _rows(x, "x"), code_of(x.dtype), a, scales, which,
+          bank.slots, bank.rank, T, K, low.data_ptr(), _stream(),
+          tag=("t{} k{} r{}", T, K, bank.rank))
+    _call("fb_adapter_expand", base.data_ptr(), planes, T * N, N, low.data_ptr(), b, code_of(x.dtype),
+          which, bank.slots, bank.rank, T, N, out.data_ptr(), code_of(out.dtype), N, _stream(),
+          tag=("t{} n{} r{}", T, N, bank.rank))
     return out
 
 

@@ -1,0 +1,135 @@
+"""A shared projection with low-rank adapters beside it, against the plain form in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import plain_requests as plain
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from foundry_b200.kernels import ops
+    return ops
+
+
+def case(ops, T, K, N, R, S, dtype, seed=0, pad=0, index=None):
+    g = torch.Generator().manual_seed(seed + 1000 * T + K + N + R)
+    normal = lambda *shape: torch.randn(*shape, generator=g)  # noqa: E731
+    x = normal(T, K + pad).to(dtype).to(DEV)[:, :K]
+    w = (normal(N, K) * 0.05).to(dtype).to(DEV)
+    a = (normal(S, R, K) / K ** 0.5).to(dtype).to(DEV)
+    b = (normal(S, N, R) * 0.2).to(dtype).to(DEV)
+    scales = (0.5 + torch.rand(S, generator=g)).to(DEV)
+    if index is None:
+        index = torch.randint(-1, S + 1, (T,), generator=g)  # S: outside of the bank
+    index = torch.as_tensor(index, dtype=torch.int32).to(DEV)
+    return x, w, ops.AdapterBank(a, b, scales), index
+
+
+def check(ops, x, w, bank, index, y, out_bf16):
+    host = lambda t: t.float().cpu().numpy()  # noqa: E731
+    want, size, much = plain.adapted(host(x), host(w), host(bank.a), host(bank.b), host(bank.scales),
+                                     index.cpu().numpy())
+    terms = x.shape[1] + bank.rank + 8
+    bound = plain.adapted_bound(want, size, much, terms, out_bf16)
+    if x.dtype == torch.bfloat16 and not out_bf16:
+        bound += 2.0 ** -8 * size
+    off = np.abs(host(y).astype(np.float64) - want)
+    assert (off <= bound).all(), (off / bound).max()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T", [1, 2, 7, 8, 9, 16, 17, 33, 64, 65, 130, 300])
+@pytest.mark.parametrize("K,N,R,S", [(256, 512, 16, 4), (520, 200, 24, 3), (1024, 328, 64, 9)])
+def test_against_the_plain_form(ops, T, K, N, R, S, dtype):
+    x, w, bank, index = case(ops, T, K, N, R, S, dtype)
+    check(ops, x, w, bank, index, ops.adapted_product(x, w, bank, index), dtype == torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("K,N,R", [(8, 8, 8), (64, 1, 8), (72, 77, 40), (100, 50, 16), (33, 17, 8), (4096, 1024, 512),
+                                   (2048, 2048, 96), (1000, 4104, 128)])
+@pytest.mark.parametrize("T", [1, 5, 40, 200])
+def test_odd_sizes(ops, T, K, N, R, dtype):
+    x, w, bank, index = case(ops, T, K, N, R, 2, dtype)
+    check(ops, x, w, bank, index, ops.adapted_product(x, w, bank, index), dtype == torch.bfloat16)
+
+
+@pytest.mark.parametrize("T", [3, 12, 50, 150, 700])
+def test_rows_of_a_wider_buffer_and_32_bit_results(ops, T):
+    x, w, bank, index = case(ops, T, 512, 264, 32, 3, torch.bfloat16, pad=24)
+    y = ops.adapted_product(x, w, bank, index, out_dtype=torch.float32)
+    assert y.dtype == torch.float32
+    check(ops, x, w, bank, index, y, False)
+
+
+@pytest.mark.parametrize("index", ["none", "one", "blocks", "every"])
+@pytest.mark.parametrize("T", [16, 48, 256, 777])
+def test_how_adapters_lie_among_the_tokens(ops, T, index):
+    S = 64
+    which = {"none": np.full(T, -1), "one": np.zeros(T), "blocks": np.arange(T) * 5 // T - 1,
+             "every": np.arange(T) % S}[index]
+    x, w, bank, index = case(ops, T, 512, 384, 16, S, torch.bfloat16, index=which.astype(np.int32))
+    check(ops, x, w, bank, index, ops.adapted_product(x, w, bank, index), True)
+
+
+def test_a_row_depends_on_its_own_adapter_alone(ops):
+    """Wild numbers in the adapters of other rows, and in slots that no row has, reach nobody."""
+    T = 40
+    x, w, bank, index = case(ops, T, 512, 264, 16, 4, torch.bfloat16, index=np.arange(T) % 3)
+    want = ops.adapted_product(x, w, bank, index)
+    bank.a[3], bank.b[3] = float("nan"), float("inf")
+    assert torch.equal(ops.adapted_product(x, w, bank, index), want)
+    bank.a[1], bank.b[1] = float("nan"), float("inf")
+    got = ops.adapted_product(x, w, bank, index)
+    others = (index != 1).nonzero()[:, 0]
+    assert torch.equal(got[others], want[others])
+
+
+def test_without_an_adapter_it_is_the_product(ops):
+    for T in (1, 16, 48, 300):
+        x, w, bank, index = case(ops, T, 1024, 512, 16, 2, torch.bfloat16, index=np.full(T, -1))
+        got = ops.adapted_product(x, w, bank, index).float()
+        want = (x.double() @ w.double().T).float()
+        assert torch.allclose(got, want, rtol=2.0 ** -8 * 1.01, atol=1024 * 2.0 ** -24 * 1024 * 0.05)
+
+
+def test_no_tokens(ops):
+    x, w, bank, index = case(ops, 0, 64, 32, 8, 1, torch.bfloat16, index=[])
+    assert ops.adapted_product(x, w, bank, index).shape == (0, 32)
+
+
+def test_a_row_scaled_input(ops):
+    """What a norm leaves for the products behind it: the scale is applied first."""
+    T, K = 9, 512
+    x, w, bank, index = case(ops, T, K, 256, 16, 3, torch.bfloat16)
+    shares = torch.rand(32, 16, device=DEV) * 40
+    scaled = ops.RowScaled(x.contiguous(), shares, 1e-5)
+    y = ops.adapted_product(scaled, w, bank, index)
+    check(ops, scaled.materialize(), w, bank, index, y, True)
+
+
+def test_on_another_stream_and_replayed(ops):
+    for T in (4, 40, 300):
+        x, w, bank, index = case(ops, T, 1024, 768, 32, 5, torch.bfloat16)
+        want = ops.adapted_product(x, w, bank, index)
+        torch.cuda.synchronize()
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side), ops.scratch_owner(("adapters", T)):
+            got = ops.adapted_product(x, w, bank, index)
+            side.synchronize()
+        assert torch.equal(got, want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = ops.adapted_product(x, w, bank, index)
+        x.copy_(x.flip(0))
+        index.copy_(index.flip(0))
+        for _ in range(2):
+            graph.replay()
+        torch.cuda.synchronize()
+        check(ops, x, w, bank, index, captured, True)
+        ops.release_scratch(("adapters", T))
