@@ -17,8 +17,10 @@
 namespace {
 
 constexpr int THREADS = 512;
-constexpr int MAX_CLUSTER = 8;
-constexpr int MAX_CHUNK = 46080;  // a block's logits in shared memory: 180 KB, beside 42 KB of bins
+constexpr int MAX_CLUSTER = 16;
+// A block's logits in shared memory, 129 KB. With more of them in one bin the fractions of their
+// weights could pass 32 bits (see Bins).
+constexpr int MAX_CHUNK = 33024;
 constexpr unsigned ID_BITS = 20, ID_MASK = (1u << ID_BITS) - 1;
 
 struct SampleArgs {
@@ -101,29 +103,56 @@ __device__ __forceinline__ void store_at(unsigned long long* mine, unsigned rank
 // What the blocks of a cluster tell each other: two sets by turns, so that a set is written again only
 // when every block has passed the barrier behind its last reading.
 struct Meeting {
-  unsigned long long said[2][MAX_CLUSTER];
-  unsigned long long warps[THREADS / 32];
+  unsigned long long said[2][2][MAX_CLUSTER];
+  unsigned long long warps[2][THREADS / 32];
 };
 
+// One value a thread -> one a row, joined in a fixed order, for every thread of the cluster; `meanwhile`
+// runs while the blocks wait for each other. The pair form takes two values with joins of their own.
+template <typename F, typename G, typename W>
+__device__ __forceinline__ void meet_pair(Meeting& m, int& turn, int blocks, unsigned rank,
+                                          unsigned long long& v, F&& join, unsigned long long* w, G&& join_w,
+                                          W&& meanwhile) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    v = join(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (w != nullptr) *w = join_w(*w, __shfl_xor_sync(0xffffffffu, *w, o));
+  }
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) {
+    m.warps[0][threadIdx.x >> 5] = v;
+    if (w != nullptr) m.warps[1][threadIdx.x >> 5] = *w;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    v = m.warps[0][lane & (THREADS / 32 - 1)];
+    if (w != nullptr) *w = m.warps[1][lane & (THREADS / 32 - 1)];
+#pragma unroll
+    for (int o = THREADS / 64; o > 0; o >>= 1) {
+      v = join(v, __shfl_xor_sync(0xffffffffu, v, o));
+      if (w != nullptr) *w = join_w(*w, __shfl_xor_sync(0xffffffffu, *w, o));
+    }
+    if (lane < blocks) {
+      store_at(&m.said[turn][0][rank], lane, v);
+      if (w != nullptr) store_at(&m.said[turn][1][rank], lane, *w);
+    }
+  }
+  cluster_arrive();
+  meanwhile();
+  cluster_wait();
+  // every warp joins what the blocks said
+  v = m.said[turn][0][lane & (blocks - 1)];
+  if (w != nullptr) *w = m.said[turn][1][lane & (blocks - 1)];
+  for (int o = blocks / 2; o > 0; o >>= 1) {
+    v = join(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (w != nullptr) *w = join_w(*w, __shfl_xor_sync(0xffffffffu, *w, o));
+  }
+  turn ^= 1;
+}
 template <typename F>
 __device__ __forceinline__ unsigned long long meet(Meeting& m, int& turn, int blocks, unsigned rank,
                                                    unsigned long long v, F&& join) {
-  // one value a thread -> one a row, joined in a fixed order, for every thread of the cluster
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = join(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) m.warps[threadIdx.x >> 5] = v;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    v = m.warps[threadIdx.x & (THREADS / 32 - 1)];
-#pragma unroll
-    for (int o = THREADS / 64; o > 0; o >>= 1) v = join(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if ((int)threadIdx.x < blocks) store_at(&m.said[turn][rank], threadIdx.x, v);
-  }
-  cluster_sync();
-  v = m.said[turn][0];
-  for (int b = 1; b < blocks; ++b) v = join(v, m.said[turn][b]);
-  turn ^= 1;
+  meet_pair(m, turn, blocks, rank, v, join, (unsigned long long*)nullptr, join, [] {});
   return v;
 }
 struct Larger {
@@ -152,17 +181,19 @@ __device__ __noinline__ unsigned long long cut_by_bits(F&& amount, unsigned long
   return cut;
 }
 
-// Tokens by their distance d = (M - v) / T from the best one: bins of 1 / 64, the last one for all
-// that is further. Inside a bin the weights exp(-d) are exp(-b / 64) (1 - part), with part below
-// 1 / 64; its 22-bit fraction adds up as whole numbers, so that the sums do not depend on the order
+// Tokens by their distance d = (M - v) / T from the best one: bins of 1 / 32, the last one for all
+// that is further than 32. Inside a bin the weights exp(-d) are exp(-b / 32) (1 - part), with part below
+// 0.031; its 22-bit fraction adds up as whole numbers, so that the sums do not depend on the order
 // in which threads come. What the last bin weighs (V exp(-32) at most) is left out of the sums.
-constexpr int BINS = 2048;
-constexpr float BINS_PER_UNIT = 64.f;
+// Bins half as wide (and a sorted list half as long) cost twice the exchange: see the launcher's note.
+constexpr int BINS = 1024;
+constexpr float BINS_PER_UNIT = 32.f;
 constexpr int PART_BITS = 22;
-constexpr int LISTED = 1024;  // tokens of a border's bin that are put in order in shared memory
+constexpr int LISTED = 512;  // tokens of a border's bin that are put in order in shared memory
+constexpr int SLICES = THREADS;
 
-// A distance in 64ths: its bin (an edge belongs to either side, always the same one), and 1 - exp(-x) of
-// what is left of it, x <= 1 / 64, by its series (the next term is below 2^-28), in units of 2^-22. Whole
+// A distance in 32nds: its bin (an edge belongs to either side, always the same one), and 1 - exp(-x) of
+// what is left of it, x <= 1 / 32, by its series (the next term is below 2^-31), in units of 2^-22. Whole
 // numbers are made and taken off by adding 1.5 * 2^23, which leaves them in the last bits.
 constexpr float TO_WHOLE = 12582912.f;
 __device__ __forceinline__ bool in_last_bin(float t) { return !(t < (float)(BINS - 1)); }
@@ -171,8 +202,13 @@ __device__ __forceinline__ int bin_of(float t) {
 }
 __device__ __forceinline__ unsigned part_of(float t) {  // of a token in front of the last bin
   const float x = t - (((t - 0.5f) + TO_WHOLE) - TO_WHOLE);  // exact
-  const float part = x * (65536.f - x * (512.f - x * (1024.f / 384.f)));
+  // 2^22 (y - y^2 / 2 + y^3 / 6 - y^4 / 24) at y = x / 32
+  const float part = x * (131072.f - x * (2048.f - x * (64.f / 3.f - x * (1.f / 6.f))));
   return (unsigned)__float_as_int(part + TO_WHOLE) & 0x3ffffu;
+}
+__device__ __forceinline__ int slice_of(float t) {  // of a token in front of the last bin
+  const float x = t - (((t - 0.5f) + TO_WHOLE) - TO_WHOLE);  // in [0, 1], exact
+  return min(SLICES - 1, (int)(x * (float)SLICES));
 }
 __device__ __forceinline__ unsigned weight_in_bin(float t) {
   return in_last_bin(t) ? 0u : (1u << PART_BITS) - part_of(t);
@@ -188,7 +224,14 @@ struct Bins {
   float all_weight[BINS];
   unsigned long long listed[LISTED];
   unsigned long long scan_warps[2][THREADS / 32];
-  unsigned counted;
+  // of each of the two borders: its bin + 1, this block's tokens in it so far, what stands in front
+  unsigned found[2], counted[2], count_front[2], tokens[2];
+  double weight_front[2];
+  // the same for a border's bin cut up once more, where it holds more tokens than the list: a slice a
+  // thread; weights in two halves of 11 bits, then whole
+  unsigned slice_count[SLICES], slice_low[SLICES], slice_high[SLICES], all_slice_count[SLICES];
+  unsigned long long all_slice_weight[SLICES], slice_weight_front[2];
+  unsigned slice_found[2], slice_count_front[2];
 };
 
 template <typename T>
@@ -208,7 +251,7 @@ __device__ __forceinline__ void store_word_at(void* mine, unsigned rank, unsigne
 }
 
 // A row by a cluster of `gridDim.z` blocks, each with `chunk` of its logits in shared memory.
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 2)
 sample_rules_kernel(const SampleArgs a) {
   cluster_arrive();  // waited for in front of the first word to another block: it has to be there
   fb_pdl_wait();
@@ -244,51 +287,80 @@ sample_rules_kernel(const SampleArgs a) {
     if (v > top) { top = v; top_at = i; }
     return v;
   };
-  auto come_in = [&](float v, int i, unsigned held, unsigned ok) {
-    if (held & 1u) v = fb_penalised(row, v, row.counts[lo + i]);
-    return biased ? v : settle(v, i, ok & 1u);
-  };
   const unsigned* seen = row.counts != nullptr ? row.seen + (lo >> 5) : nullptr;
   const unsigned* allowed = row.allowed != nullptr ? row.allowed + (lo >> 5) : nullptr;
   int done = 0;
   if ((reinterpret_cast<uintptr_t>(from) & 15) == 0) {
+    // four float4 a thread on their way together, then the words of their histories
     done = mine & ~3;
+    const bool whole_words = (reinterpret_cast<uintptr_t>(row.counts + lo) & 15) == 0;
     constexpr int AHEAD = 4;
     for (int i0 = tid * 4; i0 < done; i0 += THREADS * 4 * AHEAD) {
       float4 got[AHEAD];
+      unsigned held[AHEAD], ok[AHEAD];
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) {
         const int i = i0 + j * THREADS * 4;
-        if (i < done) got[j] = *reinterpret_cast<const float4*>(from + i);
+        held[j] = 0u;
+        ok[j] = ~0u;
+        if (i < done) {
+          got[j] = *reinterpret_cast<const float4*>(from + i);
+          if (seen != nullptr) held[j] = seen[i >> 5] >> (i & 31) & 15u;
+          if (allowed != nullptr) ok[j] = allowed[i >> 5] >> (i & 31);
+        }
+      }
+      if (seen != nullptr) {
+        int4 words[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) words[j] = fb_words_of(row, lo + i0 + j * THREADS * 4, held[j], whole_words);
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+          if (held[j] != 0u) fb_penalise(row, got[j], words[j], held[j]);
       }
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) {
         const int i = i0 + j * THREADS * 4;
         if (i >= done) break;
-        const unsigned held = seen != nullptr ? seen[i >> 5] >> (i & 31) : 0u;
-        const unsigned ok = allowed != nullptr ? allowed[i >> 5] >> (i & 31) : ~0u;
-        got[j].x = come_in(got[j].x, i, held, ok);
-        got[j].y = come_in(got[j].y, i + 1, held >> 1, ok >> 1);
-        got[j].z = come_in(got[j].z, i + 2, held >> 2, ok >> 2);
-        got[j].w = come_in(got[j].w, i + 3, held >> 3, ok >> 3);
+        if (!biased) {
+          got[j].x = settle(got[j].x, i, ok[j] & 1u);
+          got[j].y = settle(got[j].y, i + 1, ok[j] & 2u);
+          got[j].z = settle(got[j].z, i + 2, ok[j] & 4u);
+          got[j].w = settle(got[j].w, i + 3, ok[j] & 8u);
+        }
         *reinterpret_cast<float4*>(values + i) = got[j];
       }
     }
   }
   for (int i = done + tid; i < mine; i += THREADS) {
-    const unsigned held = seen != nullptr ? seen[i >> 5] >> (i & 31) : 0u;
-    const unsigned ok = allowed != nullptr ? allowed[i >> 5] >> (i & 31) : ~0u;
-    values[i] = come_in(from[i], i, held, ok);
+    float v = from[i];
+    if (seen != nullptr && (seen[i >> 5] >> (i & 31) & 1u)) v = fb_penalised(row, v, row.counts[lo + i]);
+    values[i] = biased ? v : settle(v, i, allowed != nullptr ? allowed[i >> 5] >> (i & 31) & 1u : 1u);
   }
-  if (cuts)
+  // what is looked at four by four ends with tokens that have no chance
+  const int padded = (mine + 3) & ~3;
+  if (mine + tid < padded) values[mine + tid] = -INFINITY;
+  if (cuts) {
     for (int b = tid; b < BINS; b += THREADS) bins.count[b] = bins.part[b] = 0;
-  __syncthreads();
+    if (tid < 2) bins.found[tid] = bins.counted[tid] = bins.slice_found[tid] = 0;
+  }
   if (biased) {
+    __syncthreads();
     fb_add_biases(a.edits, row, values, lo, hi);
     __syncthreads();
     for (int i = tid; i < mine; i += THREADS)
       values[i] = settle(values[i], i, allowed != nullptr ? allowed[i >> 5] >> (i & 31) & 1u : 1u);
   }
+  const float inv_t = greedy ? 1.f : 1.0f / T;
+  // exp(-(M - v) / T) as a power of two; the factor -log2(e) / T, log2(e) in two parts, rounded once
+  float log2_t = -1.44269502f * inv_t;
+  {
+    const float t = greedy ? 1.f : T;
+    const float q = 1.44269502f / t;
+    log2_t = -(q + (fmaf(-q, t, 1.44269502f) + 1.9259630e-8f) / t);
+  }
+  const unsigned long long stream = a.streams != nullptr ? (unsigned long long)a.streams[r] : 0ULL;
+  const unsigned long long step = a.steps != nullptr ? (unsigned long long)a.steps[r] : 0ULL;
+  const unsigned long long of_step = mix64(stream + GOLDEN * (step + 1));
   cluster_wait();
   // the first place of all: the greedy choice
   unsigned long long first = top_at >= 0 ? place_of(top, (unsigned)(lo + top_at)) : 0;
@@ -308,16 +380,11 @@ sample_rules_kernel(const SampleArgs a) {
     __syncthreads();
   }
   const float M = value_of(first);
-  const float inv_t = greedy ? 1.f : 1.0f / T;
-  // exp(-(M - v) / T) as a power of two, its factor rounded once from 64 bits
-  const float log2_t = (float)(-1.4426950408889634 / (greedy ? 1.0 : (double)T));
   auto weight_of = [&](float v) { return exp2_fast((M - v) * log2_t); };
   auto distance = [&](float v) { return (M - v) * inv_t; };
   const float bins_t = inv_t * BINS_PER_UNIT;
   auto binned = [&](float v) { return (M - v) * bins_t; };
-  const unsigned long long stream = a.streams != nullptr ? (unsigned long long)a.streams[r] : 0ULL;
-  const unsigned long long step = a.steps != nullptr ? (unsigned long long)a.steps[r] : 0ULL;
-  const unsigned long long of_step = mix64(stream + GOLDEN * (step + 1));
+  auto four_at = [&](int i) { return *reinterpret_cast<const float4*>(values + i); };
   // The winner of the draw so far, as a place of its score. A token of weight w beats score s where
   // -log u < w exp(-s), and -log u >= 1 - u: all but a few of the tokens need no logarithm (with a
   // thousandth more of the right side than rounding could ask for; 1 - u from 23 of its bits, a unit
@@ -325,9 +392,10 @@ sample_rules_kernel(const SampleArgs a) {
   const unsigned first_id = ID_MASK - (unsigned)(first & ID_MASK);
   unsigned long long best = greedy ? first : place_of(gumbel(random_of(of_step, first_id)), first_id);
   float beaten = greedy ? 0.f : 1.001f * expf(-value_of(best));
-  auto try_token = [&](float v, float w, unsigned id) {
-    const unsigned random = random_of(of_step, id);
-    if ((2.0f - 0x1p-22f) - __uint_as_float(random >> 9 | 0x3f800000u) > w * beaten) return;
+  auto may_win = [&](unsigned random, float w) {
+    return (2.0f - 0x1p-22f) - __uint_as_float(random >> 9 | 0x3f800000u) <= w * beaten && w >= least;
+  };
+  auto try_token = [&](float v, unsigned random, unsigned id) {
     const unsigned long long score = place_of(gumbel(random) - distance(v), id);
     if (score > best) {
       best = score;
@@ -337,44 +405,81 @@ sample_rules_kernel(const SampleArgs a) {
   double all = 0.0;
   if (!cuts) {  // one pass: the sum of the weights and the draw
     if (greedy) {
-#pragma unroll 4
-      for (int i = tid; i < mine; i += THREADS) all += (double)weight_of(values[i]);
+#pragma unroll 2
+      for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
+        const float4 v = four_at(i);
+        all += ((double)weight_of(v.x) + (double)weight_of(v.y)) + ((double)weight_of(v.z) + (double)weight_of(v.w));
+      }
     } else {
-#pragma unroll 4
-      for (int i = tid; i < mine; i += THREADS) {
-        const float v = values[i], w = weight_of(v);
-        all += (double)w;
-        if (w >= least && v != -INFINITY) try_token(v, w, (unsigned)(lo + i));
+#pragma unroll 2
+      for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
+        const float4 f = four_at(i);
+        const float v[4] = {f.x, f.y, f.z, f.w};
+        float w[4];
+        unsigned random[4];
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          w[j] = weight_of(v[j]);
+          random[j] = random_of(of_step, (unsigned)(lo + i + j));
+          any |= may_win(random[j], w[j]);
+        }
+        all += ((double)w[0] + (double)w[1]) + ((double)w[2] + (double)w[3]);
+        if (any) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (may_win(random[j], w[j])) try_token(v[j], random[j], (unsigned)(lo + i + j));
+        }
       }
     }
-    all = __longlong_as_double((long long)meet(m, turn, blocks, rank,
-                                               (unsigned long long)__double_as_longlong(all), SumDoubles{}));
   } else {
-#pragma unroll 4
-    for (int i = tid; i < mine; i += THREADS) {
-      const float v = values[i], t = binned(v);
-      if (!in_last_bin(t)) {
-        const int b = bin_of(t);
-        atomicAdd(&bins.count[b], 1u);
-        atomicAdd(&bins.part[b], part_of(t));
-      } else if (v != -INFINITY) {  // it may hold nearly all tokens: their number is made by warps
-        const unsigned together = __activemask();
-        if ((tid & 31) == __ffs(together) - 1) atomicAdd(&bins.count[BINS - 1], __popc(together));
+#pragma unroll 2
+    for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
+      const float4 f = four_at(i);
+      const float v[4] = {f.x, f.y, f.z, f.w};
+      unsigned far = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float t = binned(v[j]);
+        if (!in_last_bin(t)) {
+          const int b = bin_of(t);
+          atomicAdd(&bins.count[b], 1u);
+          atomicAdd(&bins.part[b], part_of(t));
+        } else {
+          far += v[j] != -INFINITY;
+        }
+      }
+      if (far != 0) {  // the last bin may hold nearly all tokens: their number is made by warps
+        const unsigned together = __activemask(), sum = __reduce_add_sync(together, far);
+        if ((tid & 31) == __ffs(together) - 1) atomicAdd(&bins.count[BINS - 1], sum);
       }
     }
-    cluster_sync();
     // each block adds up its share of the bins over the cluster and tells everybody
     const int share = BINS / blocks;
+    cluster_arrive();
+    double exact_unit = exp(-(double)((int)rank * share + tid) / BINS_PER_UNIT);
+    cluster_wait();
     for (int i = tid; i < share; i += THREADS) {
       const int b = (int)rank * share + i;
-      unsigned count = 0;
+      unsigned count = 0, counts[MAX_CLUSTER], parts[MAX_CLUSTER];
       unsigned long long part = 0;
-      for (int o = 0; o < blocks; ++o) {
-        count += load_at(&bins.count[b], o);
-        part += load_at(&bins.part[b], o);
+#pragma unroll
+      for (int o = 0; o < MAX_CLUSTER; ++o) {
+        if (o < blocks) {
+          counts[o] = load_at(&bins.count[b], o);
+          parts[o] = load_at(&bins.part[b], o);
+        }
       }
+#pragma unroll
+      for (int o = 0; o < MAX_CLUSTER; ++o) {
+        if (o < blocks) {
+          count += counts[o];
+          part += parts[o];
+        }
+      }
+      if (i != tid) exact_unit = exp(-(double)b / BINS_PER_UNIT);
       const double size = (double)(((unsigned long long)count << PART_BITS) - part) * (1.0 / (1 << PART_BITS));
-      const float weight = b == BINS - 1 ? 0.f : (float)(exp(-(double)b / BINS_PER_UNIT) * size);
+      const float weight = b == BINS - 1 ? 0.f : (float)(exact_unit * size);
       for (int o = 0; o < blocks; ++o) {
         store_word_at(&bins.all_count[b], o, count);
         store_word_at(&bins.all_weight[b], o, __float_as_uint(weight));
@@ -413,51 +518,40 @@ sample_rules_kernel(const SampleArgs a) {
       __syncthreads();
       unsigned front_c = 0;
       double front_w = 0.0;
+#pragma unroll
       for (int o = 0; o < THREADS / 32; ++o) {
+        const unsigned oc = (unsigned)bins.scan_warps[0][o];
         const double ow = __longlong_as_double((long long)bins.scan_warps[1][o]);
         if (o < (tid >> 5)) {
-          front_c += (unsigned)bins.scan_warps[0][o];
+          front_c += oc;
           front_w += ow;
         }
-        left += (unsigned)bins.scan_warps[0][o];
+        left += oc;
         all += ow;
       }
       count_before = front_c + upto_c - c;
       weight_before = front_w + (upto_w - w);
     }
     // The border of a rule: the last bin with tokens whose front is below `target`, put in order, and
-    // of its tokens the last one whose front is. `by_count`: fronts count tokens, else they weigh.
-    double front_sum = 0.0;  // what the last border keeps weighs
+    // of its tokens the last one whose front is. Rule 0: fronts count tokens, 1: they weigh.
+    double kept_sum = all;  // what the last border keeps weighs
     bool listed_before = false;
-    auto border = [&](bool by_count, double target) -> unsigned long long {
-      unsigned long long at = 0;  // (bin + 1, what stands in front of it: a thread of the block knows)
+    auto border = [&](int rule, double target) -> unsigned long long {
       {
-        unsigned c = count_before;
+        unsigned c = count_before, at = 0;
         double w = weight_before;
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
-          if (counts[j] != 0 && (by_count ? (double)c : w) < target) at = (unsigned long long)(tid * EACH + j + 1);
+          if (counts[j] != 0 && (rule == 0 ? (double)c : w) < target) at = tid * EACH + j + 1;
           c += counts[j];
           w += (double)weights[j];
         }
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const unsigned long long other = __shfl_xor_sync(0xffffffffu, at, o);
-        at = other > at ? other : at;
+        at = __reduce_max_sync(0xffffffffu, at);
+        if ((tid & 31) == 0 && at != 0) atomicMax(&bins.found[rule], at);
       }
       __syncthreads();
-      if ((tid & 31) == 0) bins.scan_warps[0][tid >> 5] = at;
-      if (tid == 0) bins.counted = 0;
-      __syncthreads();
-      for (int o = 0; o < THREADS / 32; ++o) at = bins.scan_warps[0][o] > at ? bins.scan_warps[0][o] : at;
-      if (at == 0) {  // a share of nothing
-        front_sum = 1.0;
-        return first;
-      }
-      const int b = (int)at - 1;
-      // the owner of that bin tells what stands in front of it
-      __syncthreads();
+      if (bins.found[rule] == 0) return first;  // a share of nothing
+      const int b = (int)bins.found[rule] - 1;
       if (tid == b / EACH) {
         unsigned c = count_before;
         double w = weight_before;
@@ -465,37 +559,158 @@ sample_rules_kernel(const SampleArgs a) {
         for (int j = 0; j < EACH; ++j) {
           if (j < b % EACH) { c += counts[j]; w += (double)weights[j]; }
         }
-        bins.scan_warps[0][0] = c;
-        bins.scan_warps[1][0] = (unsigned long long)__double_as_longlong(w);
+        bins.count_front[rule] = c;
+        bins.weight_front[rule] = w;
+        bins.tokens[rule] = bins.all_count[b];
       }
+      // (an error of 2^-23 of what this bin weighs, and none in the first bin)
+      const double unit = b == BINS - 1 ? 0.0 : (double)expf(-(float)b * (1.f / BINS_PER_UNIT)) * (1.0 / (1 << PART_BITS));
+      auto fixed = [&](float v) { return weight_in_bin(binned(v)); };
       __syncthreads();
-      const double c_front = (double)bins.scan_warps[0][0];
-      const double w_front = __longlong_as_double((long long)bins.scan_warps[1][0]);
-      const double unit = b == BINS - 1 ? 0.0 : exp(-(double)b / BINS_PER_UNIT) * (1.0 / (1 << PART_BITS));
-      const unsigned n = bins.all_count[b];
-      auto fixed = [&](float v) { return (unsigned long long)weight_in_bin(binned(v)); };
+      double c_front = (double)bins.count_front[rule];
+      const double w_front = bins.weight_front[rule];
+      unsigned long long front_in_bin = 0;  // in units of the bin
+      unsigned n = bins.tokens[rule];
+      int slice = -1;
+      if (n > LISTED && b != BINS - 1) {  // once more, inside the bin
+        bins.slice_count[tid] = bins.slice_low[tid] = bins.slice_high[tid] = 0;
+        __syncthreads();
+        for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
+          const float4 f = four_at(i);
+          const float v[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float t = binned(v[j]);
+            if (bin_of(t) != b) continue;
+            const int at = slice_of(t);
+            const unsigned w = weight_in_bin(t);
+            atomicAdd(&bins.slice_count[at], 1u);
+            atomicAdd(&bins.slice_low[at], w & 2047u);
+            atomicAdd(&bins.slice_high[at], w >> 11);
+          }
+        }
+        cluster_sync();
+        const int share = SLICES / blocks;
+        if (tid < share) {
+          const int at = (int)rank * share + tid;
+          unsigned counts[MAX_CLUSTER], low[MAX_CLUSTER], high[MAX_CLUSTER], count = 0;
+          unsigned long long weight = 0;
+#pragma unroll
+          for (int o = 0; o < MAX_CLUSTER; ++o) {
+            if (o < blocks) {
+              counts[o] = load_at(&bins.slice_count[at], o);
+              low[o] = load_at(&bins.slice_low[at], o);
+              high[o] = load_at(&bins.slice_high[at], o);
+            }
+          }
+#pragma unroll
+          for (int o = 0; o < MAX_CLUSTER; ++o) {
+            if (o < blocks) {
+              count += counts[o];
+              weight += low[o] + ((unsigned long long)high[o] << 11);
+            }
+          }
+          for (int o = 0; o < blocks; ++o) {
+            store_word_at(&bins.all_slice_count[at], o, count);
+            store_at(&bins.all_slice_weight[at], o, weight);
+          }
+        }
+        cluster_sync();
+        const unsigned mine_c = bins.all_slice_count[tid];
+        const unsigned long long mine_w = bins.all_slice_weight[tid];
+        unsigned upto_c = mine_c;
+        unsigned long long upto_w = mine_w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const unsigned oc = __shfl_up_sync(0xffffffffu, upto_c, o);
+          const unsigned long long ow = __shfl_up_sync(0xffffffffu, upto_w, o);
+          if ((tid & 31) >= o) { upto_c += oc; upto_w += ow; }
+        }
+        if ((tid & 31) == 31) {
+          bins.scan_warps[0][tid >> 5] = upto_c;
+          bins.scan_warps[1][tid >> 5] = upto_w;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int o = 0; o < THREADS / 32; ++o) {
+          if (o < (tid >> 5)) {
+            upto_c += (unsigned)bins.scan_warps[0][o];
+            upto_w += bins.scan_warps[1][o];
+          }
+        }
+        upto_c -= mine_c;  // in front of this thread's slice
+        upto_w -= mine_w;
+        const bool in_front = rule == 0 ? c_front + (double)upto_c < target : w_front + unit * (double)upto_w < target;
+        const unsigned at = __reduce_max_sync(0xffffffffu, mine_c != 0 && in_front ? tid + 1 : 0);
+        if ((tid & 31) == 0 && at != 0) atomicMax(&bins.slice_found[rule], at);
+        __syncthreads();
+        slice = max(0, (int)bins.slice_found[rule] - 1);
+        if (tid == slice) {
+          bins.slice_count_front[rule] = upto_c;
+          bins.slice_weight_front[rule] = upto_w;
+        }
+        __syncthreads();
+        c_front += (double)bins.slice_count_front[rule];
+        front_in_bin = bins.slice_weight_front[rule];
+        n = bins.all_slice_count[slice];
+      }
+      auto in_border = [&](float v) {
+        const float t = binned(v);
+        return bin_of(t) == b && v != -INFINITY && (slice < 0 || slice_of(t) == slice);
+      };
       if (n <= LISTED) {
         // everybody gets everybody's tokens of the bin; a block's stand behind those of lower ranks
         if (listed_before) cluster_sync();  // everybody is through with the list of the border before
         listed_before = true;
-        unsigned base = 0;
-        for (int o = 0; o < (int)rank; ++o) base += load_at(&bins.count[b], o);
-        for (int i = tid; i < mine; i += THREADS) {
-          const float v = values[i];
-          if (v == -INFINITY || bin_of(binned(v)) != b) continue;
-          const unsigned slot = base + atomicAdd(&bins.counted, 1u);
-          const unsigned long long place = place_of(v, (unsigned)(lo + i));
-          for (int o = 0; o < blocks; ++o) store_at(&bins.listed[slot], o, place);
+        const int lane = tid & 31;
+        const unsigned base = __reduce_add_sync(0xffffffffu, lane < (int)rank ?
+            load_at(slice < 0 ? &bins.count[b] : &bins.slice_count[slice], lane) : 0u);
+#pragma unroll 2
+        for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
+          const float4 f = four_at(i);
+          const float v[4] = {f.x, f.y, f.z, f.w};
+          bool in[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) in[j] = in_border(v[j]);
+          if (in[0] || in[1] || in[2] || in[3]) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (!in[j]) continue;
+              const unsigned slot = base + atomicAdd(&bins.counted[rule], 1u);
+              const unsigned long long place = place_of(v[j], (unsigned)(lo + i + j));
+              for (int o = 0; o < blocks; ++o) store_at(&bins.listed[slot], o, place);
+            }
+          }
         }
         cluster_sync();
+        if (n <= 32) {  // every warp for itself: how many are in front of each, and what do they weigh
+          const unsigned long long me = lane < (int)n ? bins.listed[lane] : 0ull;
+          const unsigned weighs = lane < (int)n ? fixed(value_of(me)) : 0u;
+          unsigned ahead = 0, in_front = 0;
+          for (unsigned j = 0; j < n; ++j) {
+            const unsigned long long other = __shfl_sync(0xffffffffu, me, j);
+            const unsigned w = __shfl_sync(0xffffffffu, weighs, j);
+            if (other > me) {
+              ++ahead;
+              in_front += w;
+            }
+          }
+          const bool kept = lane < (int)n &&
+              (rule == 0 ? c_front + (double)ahead : w_front + unit * (double)(front_in_bin + in_front)) < target;
+          const unsigned many = __reduce_max_sync(0xffffffffu, kept ? ahead + 1 : 0u);
+          const unsigned last = __ballot_sync(0xffffffffu, kept && ahead + 1 == many);
+          const int who = last != 0 ? __ffs(last) - 1 : 0;
+          kept_sum = w_front + unit * (double)(front_in_bin + __shfl_sync(0xffffffffu, in_front + weighs, who));
+          return __shfl_sync(0xffffffffu, me, who);
+        }
         // in order, the first place first (a bitonic network; zeros behind the tokens)
-        unsigned padded = 32;
-        while (padded < n) padded *= 2;
-        for (unsigned i = n + tid; i < padded; i += THREADS) bins.listed[i] = 0;
+        unsigned whole = 64;
+        while (whole < n) whole *= 2;
+        for (unsigned i = n + tid; i < whole; i += THREADS) bins.listed[i] = 0;
         __syncthreads();
-        for (unsigned size = 2; size <= padded; size *= 2) {
+        for (unsigned size = 2; size <= whole; size *= 2) {
           for (unsigned stride = size / 2; stride > 0; stride /= 2) {
-            if ((unsigned)tid < padded / 2) {
+            if ((unsigned)tid < whole / 2) {
               const unsigned i = 2 * tid - (tid & (stride - 1)), j = i + stride;
               const unsigned long long x = bins.listed[i], y = bins.listed[j];
               if ((x < y) == ((i & size) == 0)) { bins.listed[i] = y; bins.listed[j] = x; }
@@ -503,103 +718,122 @@ sample_rules_kernel(const SampleArgs a) {
             __syncthreads();
           }
         }
-        // a thread has two of them side by side: what stands in front of each, and is it kept
-        unsigned long long weighs[2], upto;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) weighs[j] = 2u * tid + j < n ? fixed(value_of(bins.listed[2 * tid + j])) : 0ull;
-        upto = weighs[0] + weighs[1];
+        // what stands in front of each (512 tokens weigh less than 2^31), and is it kept
+        const unsigned weighs = tid < (int)n ? fixed(value_of(bins.listed[tid])) : 0u;
+        unsigned upto = weighs;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-          const unsigned long long other = __shfl_up_sync(0xffffffffu, upto, o);
-          if ((tid & 31) >= o) upto += other;
+          const unsigned other = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += other;
         }
-        if ((tid & 31) == 31) bins.scan_warps[1][tid >> 5] = upto;
+        if (lane == 31) bins.scan_warps[1][tid >> 5] = upto;
         __syncthreads();
-        unsigned long long in_front = upto - weighs[0] - weighs[1];
-        for (int o = 0; o < (tid >> 5); ++o) in_front += bins.scan_warps[1][o];
-        unsigned long long kept = 0, many = 0;  // what the kept ones weigh, and how many they are
+        unsigned front = upto - weighs;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const unsigned i = 2 * tid + j;
-          if (i < n && (by_count ? c_front + (double)i : w_front + unit * (double)in_front) < target) {
-            kept = in_front + weighs[j];
-            many = i + 1;
-          }
-          in_front += weighs[j];
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {  // both grow along the list
-          const unsigned long long k2 = __shfl_xor_sync(0xffffffffu, kept, o);
-          const unsigned long long m2 = __shfl_xor_sync(0xffffffffu, many, o);
-          kept = k2 > kept ? k2 : kept;
-          many = m2 > many ? m2 : many;
-        }
+        for (int o = 0; o < THREADS / 32; ++o)
+          if (o < (tid >> 5)) front += (unsigned)bins.scan_warps[1][o];
+        const bool kept = tid < (int)n &&
+            (rule == 0 ? c_front + (double)tid : w_front + unit * (double)(front_in_bin + front)) < target;
+        // (kept ones stand at the list's front)
+        const unsigned many = (unsigned)__syncthreads_count(kept);
+        if (tid == (int)(many > 0 ? many - 1 : 0)) bins.weight_front[rule] = w_front + unit * (double)(front_in_bin + front + weighs);
         __syncthreads();
-        if ((tid & 31) == 0) {
-          bins.scan_warps[0][tid >> 5] = many;
-          bins.scan_warps[1][tid >> 5] = kept;
-        }
-        __syncthreads();
-        for (int o = 0; o < THREADS / 32; ++o) {
-          many = bins.scan_warps[0][o] > many ? bins.scan_warps[0][o] : many;
-          kept = bins.scan_warps[1][o] > kept ? bins.scan_warps[1][o] : kept;
-        }
-        const unsigned long long last = bins.listed[many > 0 ? many - 1 : 0];
-        __syncthreads();
-        front_sum = w_front + unit * (double)kept;
-        return last;
+        kept_sum = bins.weight_front[rule];
+        return bins.listed[many > 0 ? many - 1 : 0];
       }
       auto amount = [&](unsigned long long cut, bool count) {
         unsigned long long sum = 0;
         for (int i = tid; i < mine; i += THREADS) {
           const float v = values[i];
-          if (v == -INFINITY || place_of(v, (unsigned)(lo + i)) < cut || bin_of(binned(v)) != b) continue;
+          if (!in_border(v) || place_of(v, (unsigned)(lo + i)) < cut) continue;
           sum += count ? 1ull : fixed(v);
         }
         return meet(m, turn, blocks, rank, sum, Sum{});
       };
       unsigned long long need;
-      if (by_count) {
+      if (rule == 0) {
         need = (unsigned long long)(target - c_front);  // whole numbers
       } else {
-        const double missing = ceil((target - w_front) / unit);
+        const double missing = ceil((target - w_front) / unit) - (double)front_in_bin;
         need = missing < 1.0 ? 1ull : (unsigned long long)missing;
       }
-      const unsigned long long most = amount(0, by_count);
+      const unsigned long long most = amount(0, rule == 0);
       need = need < most ? need : most;
-      const unsigned long long cut = cut_by_bits([&](unsigned long long c) { return amount(c, by_count); }, need);
-      front_sum = w_front + unit * (double)amount(cut, false);
+      const unsigned long long cut = cut_by_bits([&](unsigned long long c) { return amount(c, rule == 0); }, need);
+      kept_sum = w_front + unit * (double)(front_in_bin + amount(cut, false));
       return cut;
     };
     unsigned long long cut = 0;
-    double kept_sum = all;
-    if (k > 0 && (unsigned)k < left) {
-      cut = border(true, (double)k);
-      kept_sum = front_sum;
-    }
+    if (k > 0 && (unsigned)k < left) cut = border(0, (double)k);
     if (p < 1.f) {
-      const unsigned long long by_share = border(false, (double)p * kept_sum);
+      const unsigned long long by_share = border(1, (double)p * kept_sum);
       cut = by_share > cut ? by_share : cut;
     }
     cut = cut < first ? cut : first;
     const float cut_value = cut == 0 ? -INFINITY : value_of(cut);
-#pragma unroll 4
-    for (int i = tid; i < mine; i += THREADS) {
-      const float v = values[i];
-      if (v < cut_value || v == -INFINITY) continue;
-      if (v == cut_value && place_of(v, (unsigned)(lo + i)) < cut) continue;
-      const float w = weight_of(v);
-      if (w >= least) try_token(v, w, (unsigned)(lo + i));
+#pragma unroll 2
+    for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
+      const float4 f = four_at(i);
+      if (!(fmaxf(fmaxf(f.x, f.y), fmaxf(f.z, f.w)) >= cut_value)) continue;
+      const float v[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (v[j] < cut_value || (v[j] == cut_value && place_of(v[j], (unsigned)(lo + i + j)) < cut)) continue;
+        const unsigned random = random_of(of_step, (unsigned)(lo + i + j));
+        if (may_win(random, weight_of(v[j]))) try_token(v[j], random, (unsigned)(lo + i + j));
+      }
     }
   }
-  if (!greedy) best = meet(m, turn, blocks, rank, best, Larger{});
+  double log_all = 0.0;
+  unsigned long long sum = (unsigned long long)__double_as_longlong(all);
+  if (cuts) {
+    meet_pair(m, turn, blocks, rank, best, Larger{}, (unsigned long long*)nullptr, SumDoubles{},
+              [&] { if (tid == 0) log_all = log(all); });
+  } else {
+    meet_pair(m, turn, blocks, rank, best, Larger{}, &sum, SumDoubles{}, [] {});
+    if (tid == 0) log_all = log(__longlong_as_double((long long)sum));
+  }
   const int token = (int)(ID_MASK - (unsigned)(best & ID_MASK));
   if (tid == 0 && token >= lo && token < hi) {
     a.out[r] = token;
     if (a.also != nullptr) a.also[r] = token;
-    a.logprobs[r] = (float)(-(double)distance(values[token - lo]) - log(all));
+    a.logprobs[r] = (float)(-(double)distance(values[token - lo]) - log_all);
   }
-  cluster_sync();  // nobody's words are still on their way to a block that has left
+  // (the last meeting's barrier is behind every word to another block)
+}
+
+// How many clusters of 16 blocks the device runs at once (0: none), with the kernel set up for it.
+int wide_clusters(int* count) {
+  static int of_device[64] = {};
+  int device = 0;
+  cudaGetDevice(&device);
+  if (device < 0 || device >= 64) device = 63;
+  if (of_device[device] == 0) {
+    const int most = MAX_CHUNK * 4 + (int)sizeof(Bins);
+    cudaError_t e = cudaFuncSetAttribute(sample_rules_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(sample_rules_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return fb_fail(2, "sample_rules: setting the kernel up: %s", cudaGetErrorString(e));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1, 1, 16);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = most;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 16;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, sample_rules_kernel, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      n = 0;
+    }
+    of_device[device] = n > 0 ? n : -1;
+  }
+  *count = of_device[device] > 0 ? of_device[device] : 0;
+  return 0;
 }
 }  // namespace
 
@@ -620,18 +854,16 @@ FB_API int fb_sample_rules(const float* logits, long long row_stride, int n, int
   FB_REQUIRE(record == nullptr || a.edits.counts != nullptr, "sample_rules: tokens to record, and no history");
   if (n == 0) return 0;
   int blocks = 1;
-  while (blocks < MAX_CLUSTER && V > 4096 * blocks) blocks *= 2;
+  while (blocks < 8 && V > 4096 * blocks) blocks *= 2;
+  int wide = 0;
+  if (int rc = wide_clusters(&wide)) return rc;
+  if (wide > 0 && (V > 8 * MAX_CHUNK || (V > 65536 && 16 * n <= sm_count()))) blocks = 16;
+  FB_REQUIRE(V <= blocks * MAX_CHUNK, "sample_rules: a vocabulary of %d (%d at most here)", V, blocks * MAX_CHUNK);
   a.logits = logits; a.row_stride = row_stride; a.V = V;
   a.chunk = ((V + blocks - 1) / blocks + 31) / 32 * 32;  // whole words of the bits
   a.temperature = temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p;
   a.streams = streams; a.steps = steps; a.record = record;
   a.out = out; a.logprobs = logprobs; a.also = also;
-  static bool seen[64] = {};
-  if (fb_first_use_on_device(seen)) {
-    cudaError_t e = cudaFuncSetAttribute(sample_rules_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         MAX_CHUNK * 4 + (int)sizeof(Bins));
-    if (e != cudaSuccess) return fb_fail(2, "sample_rules: shared memory opt-in: %s", cudaGetErrorString(e));
-  }
   fb_launch_cluster(sample_rules_kernel, dim3(n, 1, blocks), dim3(THREADS),
                     (size_t)a.chunk * 4 + sizeof(Bins), stream,
                     (unsigned)blocks, a);

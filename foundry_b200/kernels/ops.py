@@ -2108,7 +2108,7 @@ class SampleRules:
         self.streams, self.steps = streams, steps
 
 
-MAX_SAMPLE_VOCAB = 8 * 46080  # a cluster's shared memory (csrc/sample_rules.cu)
+MAX_SAMPLE_VOCAB = 16 * 33024  # a cluster's shared memory (csrc/sample_rules.cu)
 
 
 def sample_tokens(logits: torch.Tensor, rules: SampleRules, edits: Optional[LogitEdits] = None,

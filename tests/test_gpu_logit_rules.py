@@ -225,12 +225,25 @@ def test_draws_under_every_rule(ops, V, n, pad):
     check(ops, rows.device_logits, rows.edited(), rules_of(n, V), rows.edits)
 
 
+@pytest.mark.parametrize("spread", [0.0005, 0.02, 0.3, 1.0])
+@pytest.mark.parametrize("V", [3000, 32003, 100000])
+def test_borders_among_many_nearly_equal_logits(ops, V, spread):
+    """A flat row's border lies in a bin of more tokens than the sorted list holds; 32-bit logits close to
+    ten then have few values, and thousands of tokens share one."""
+    n = 12
+    rng = np.random.RandomState(V)
+    logits = (10 + spread * rng.randn(n, V)).astype(np.float32)
+    rules = dict(temperature=[0.5, 1.0, 2.0] * 4, top_k=[0, V // 2, 700, V - 1] * 3,
+                 top_p=[0.6, 0.1, 0.999] * 4, streams=list(range(n)), steps=[4] * n)
+    check(ops, dev(logits), logits, rules)
+
+
 def test_draws_of_a_large_vocabulary(ops):
     rows = Rows(ops, 12, 128256, seed=2)
     check(ops, rows.device_logits, rows.edited(), rules_of(12, 2, top_k=(0, 50, 1000, 100000)), rows.edits)
 
 
-@pytest.mark.parametrize("V", [131072, 131073, 368640])
+@pytest.mark.parametrize("V", [131072, 131073, 264192, 264193, 368640, 528384])
 def test_draws_of_the_largest_vocabularies(ops, V):
     rows = Rows(ops, 3, V, seed=4, history=False, biased=False, masked=False)
     check(ops, rows.device_logits, rows.logits, rules_of(3, 4, temperature=(0.9,)), None)
