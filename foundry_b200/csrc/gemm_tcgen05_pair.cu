@@ -64,6 +64,21 @@ __device__ __forceinline__ PairUnit pair_unit(const GemmParams& p, int u, int ti
   return w;
 }
 
+// More K behind a tile's own, for adapters beside the projection (adapter.cu): block `ta` of 256 rows has
+// counts[ta] adapters with tokens in it, the e-th of them slots[ta * most + e]; its rank numbers of the
+// block's rows, zero in rows of others, are rows (ta * most + e) * 256 .. of `u`, and its weights for
+// feature j row slot * rows_b + j of `b`. Each takes `kblocks` K blocks of 64, so a product with them is
+// one sum in tensor memory and one rounding. (A tile's last share of K carries them.)
+struct MoreK {
+  CUtensorMap u, b;
+  const int* counts;
+  const int* slots;
+  int most, kblocks;
+};
+struct NoMoreK {};
+template <bool MORE> struct MoreKArg { using type = NoMoreK; };
+template <> struct MoreKArg<true> { using type = MoreK; };
+
 // tiles_a counts 256-row blocks of A. gridDim.x is even: CTAs 2c and 2c + 1 are
 // cluster c, which walks the units c, c + clusters, ... A unit is a whole tile,
 // or, for the tiles of the last round when they would leave most pairs idle, one
@@ -71,11 +86,11 @@ __device__ __forceinline__ PairUnit pair_unit(const GemmParams& p, int u, int ti
 // float32 workspace; the epilogue warp that delivers a tile's last share (an
 // atomic counter per tile, CTA and warp, no waiting) sums the shares in share
 // order and runs the usual epilogue on the sum.
-template <int BN>
+template <int BN, bool MORE>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a,
                     const __grid_constant__ CUtensorMap map_b, const GemmParams p, int tiles_a,
-                    int tiles_b) {
+                    int tiles_b, const __grid_constant__ typename MoreKArg<MORE>::type more) {
   constexpr int STAGES = SmemPair<BN>::STAGES;
   constexpr int TMEM_COLS = 512;
   extern __shared__ uint8_t smem_raw[];
@@ -95,6 +110,11 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a,
   const int n_tiles = tiles_a * tiles_b;
   const int total_units =
       p.tail_splits > 1 ? p.full_tiles + (n_tiles - p.full_tiles) * p.tail_splits : n_tiles;
+  // K blocks of adapters behind a unit's own
+  auto more_blocks = [&](const PairUnit& w) {
+    if constexpr (MORE) return w.kb1 == nkb ? __ldcg(more.counts + w.ta) * more.kblocks : 0;
+    else return 0;
+  };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -153,7 +173,8 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a,
       bool ok = true;
       for (int u = cluster; u < total_units && ok; u += clusters) {
         const PairUnit w = pair_unit(p, u, tiles_a, nkb);
-        for (int kb = w.kb0 + (u == cluster ? early : 0); kb < w.kb1; ++kb) {
+        const int kb_end = w.kb1 + more_blocks(w);
+        for (int kb = w.kb0 + (u == cluster ? early : 0); kb < kb_end; ++kb) {
           const int use = it + (kb - w.kb0);
           const int s = use % STAGES;
           const uint32_t phase = (uint32_t)(use / STAGES) & 1u;
@@ -162,16 +183,26 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a,
           uint8_t* b_dst = a_dst + SmemPair<BN>::A_BYTES;
           if (leader) mbar_expect_tx(&full[s], 2 * SmemPair<BN>::STAGE_BYTES);
           const uint32_t bar = full_leader + (uint32_t)(s * 8);
+          if constexpr (MORE) {
+            if (kb >= nkb) {
+              const int e = (kb - nkb) / more.kblocks, k = (kb - nkb - e * more.kblocks) * BK;
+              const int slot = __ldcg(more.slots + w.ta * more.most + e);
+              tma_load_2d_pair(a_dst, &more.u, bar, k, (w.ta * more.most + e) * 2 * BM + (int)rank * BM);
+              tma_load_2d_pair(b_dst, &more.b, bar, k, slot * p.rows_b + w.tb * BN + (int)rank * (BN / 2));
+              continue;
+            }
+          }
           tma_load_2d_pair(a_dst, &map_a, bar, kb * BK, w.ta * 2 * BM + (int)rank * BM);
           tma_load_2d_pair(b_dst, &map_b, bar, kb * BK, w.tb * BN + (int)rank * (BN / 2));
         }
-        it += w.kb1 - w.kb0;
+        it += kb_end - w.kb0;
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------- MMA issuer (leader only)
     if (lane == 0 && leader) {
       constexpr uint32_t idesc = make_idesc(2 * BM, BN);
+      if constexpr (MORE) fb_pdl_wait();  // the adapters of a block are the work of an earlier kernel
       int it = 0, j = 0;
       bool ok = true;
       for (int u = cluster; u < total_units && ok; u += clusters, ++j) {
@@ -181,7 +212,8 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a,
         if (!ok) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + (uint32_t)(buf * BN);
-        for (int kb = w.kb0; kb < w.kb1; ++kb) {
+        const int kb_end = w.kb1 + more_blocks(w);
+        for (int kb = w.kb0; kb < kb_end; ++kb) {
           const int use = it + (kb - w.kb0);
           const int s = use % STAGES;
           const uint32_t phase = (uint32_t)(use / STAGES) & 1u;
@@ -199,7 +231,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a,
         }
         if (!ok) break;
         tc_commit_pair(&acc_full[buf]);
-        it += w.kb1 - w.kb0;
+        it += kb_end - w.kb0;
       }
     }
   } else {
@@ -323,10 +355,11 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a,
   }
 }
 
-template <int BN>
+template <int BN, bool MORE = false>
 int launch_pair(const CUtensorMap& ma, const CUtensorMap& mb, const GemmParams& p, int tiles_a,
                 int tiles_b, void* workspace, long long workspace_bytes, int* counters,
-                int counters_len, int share_min_kblocks, cudaStream_t stream) {
+                int counters_len, int share_min_kblocks, cudaStream_t stream,
+                const typename MoreKArg<MORE>::type& more = {}) {
   static int clusters_of_device[64] = {};  // CTA pairs that run at once, per device
   int device = 0;
   cudaGetDevice(&device);
@@ -345,14 +378,14 @@ int launch_pair(const CUtensorMap& ma, const CUtensorMap& mb, const GemmParams& 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   if (clusters_max == 0) {
-    cudaError_t e = cudaFuncSetAttribute(gemm_tc_pair_kernel<BN>,
+    cudaError_t e = cudaFuncSetAttribute(gemm_tc_pair_kernel<BN, MORE>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          SmemPair<BN>::BYTES);
     if (e != cudaSuccess) return fb_fail(2, "gemm_tc: shared memory opt-in: %s", cudaGetErrorString(e));
     cfg.gridDim = dim3(sm_count() / 2 * 2);
     cfg.numAttrs = 1;
     int n = 0;
-    e = cudaOccupancyMaxActiveClusters(&n, gemm_tc_pair_kernel<BN>, &cfg);
+    e = cudaOccupancyMaxActiveClusters(&n, gemm_tc_pair_kernel<BN, MORE>, &cfg);
     if (e != cudaSuccess || n <= 0)
       return fb_fail(2, "gemm_tc: no CTA pair of this kernel fits the device (%s)",
                      cudaGetErrorString(e));
@@ -397,7 +430,7 @@ int launch_pair(const CUtensorMap& ma, const CUtensorMap& mb, const GemmParams& 
   const int clusters = units < clusters_max ? units : clusters_max;
   cfg.gridDim = dim3(2 * clusters);
   cfg.numAttrs = g_fb_pdl ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, gemm_tc_pair_kernel<BN>, ma, mb, q, tiles_a, tiles_b);
+  cudaLaunchKernelEx(&cfg, gemm_tc_pair_kernel<BN, MORE>, ma, mb, q, tiles_a, tiles_b, more);
   return fb_check_launch("gemm_tc_pair");
 }
 
@@ -752,6 +785,55 @@ int fb_gemm_tc_pair(const void* a, long long lda, int rows_a, const void* b, lon
   }
 }
 
+// out[T, N] = x w^T + the adapters' share: u and b2 as MoreK has them, u [blocks * most * 256, rank], b2
+// [adapters * N, rank], counts [blocks], slots [blocks, most], written by fb_adapter_planes. bfloat16 or
+// float32 rows of `out`.
+FB_API int fb_gemm_tc_adapted(const void* x, long long ldx, int T, const void* w, long long ldw, int N, int K,
+                              const void* u, const void* b2, const int* counts, const int* slots, int most,
+                              int adapters, int rank, void* out, int out_f32, long long ldo, int bn,
+                              void* workspace, long long workspace_bytes, int* counters, int counters_len,
+                              const float* scale_ss, int scale_count, int scale_stride, int scale_dim,
+                              float scale_eps, cudaStream_t stream) {
+  FB_REQUIRE(T > 0 && N > 0 && K > 0 && most > 0 && adapters > 0 && ldo >= N, "gemm_tc_adapted: bad sizes");
+  FB_REQUIRE(K % 8 == 0 && ldx % 8 == 0 && ldw % 8 == 0 && rank > 0 && rank % 8 == 0 &&
+                 (((uintptr_t)x | (uintptr_t)w | (uintptr_t)u | (uintptr_t)b2) % 16) == 0,
+             "gemm_tc_adapted: K, the rank, the row strides and the operands must keep 16-byte alignment");
+  const int blocks = (T + 2 * BM - 1) / (2 * BM);
+  FB_REQUIRE((long long)blocks * most * 2 * BM < (1ll << 31) && (long long)adapters * N < (1ll << 31) - 256,
+             "gemm_tc_adapted: %d blocks of %d adapters pass 32-bit rows", blocks, most);
+  bind_status_mirror(stream);
+  GemmParams p{};
+  const int total_kb = (K + BK - 1) / BK;
+  p.rows_a = T; p.rows_b = N; p.K = K;
+  p.kblocks_per_split = total_kb;
+  p.stride_a = ldo; p.stride_b = 1;
+  p.out = out; p.out_f32 = out_f32;
+  p.constant_operand = 2;
+  p.tail_splits = 1; p.tail_kblocks = total_kb;
+  p.rows.scale_ss = scale_ss; p.rows.scale_count = scale_count; p.rows.scale_stride = scale_stride;
+  p.rows.scale_inv_dim = scale_dim > 0 ? 1.0f / (float)scale_dim : 0.f; p.rows.scale_eps = scale_eps;
+  CUtensorMap ma, mb;
+  MoreK more{};
+  int rc = make_map(&ma, x, T, K, ldx, BM);
+  if (!rc) rc = make_map(&mb, w, N, K, ldw, bn / 2);
+  if (!rc) rc = make_map(&more.u, u, (long long)blocks * most * 2 * BM, rank, rank, BM);
+  if (!rc) rc = make_map(&more.b, b2, (long long)adapters * N, rank, rank, bn / 2);
+  if (rc) return rc;
+  more.counts = counts; more.slots = slots; more.most = most; more.kblocks = (rank + BK - 1) / BK;
+  const int tiles_b = (N + bn - 1) / bn;
+  switch (bn) {
+#define FB_ADAPTED_CASE(W)                                                                                   \
+    case W:                                                                                                  \
+      return launch_pair<W, true>(ma, mb, p, blocks, tiles_b, workspace, workspace_bytes, counters,          \
+                                  counters_len, 32, stream, more);
+    FB_ADAPTED_CASE(128) FB_ADAPTED_CASE(144) FB_ADAPTED_CASE(160) FB_ADAPTED_CASE(176) FB_ADAPTED_CASE(192)
+    FB_ADAPTED_CASE(208) FB_ADAPTED_CASE(224) FB_ADAPTED_CASE(240) FB_ADAPTED_CASE(256)
+#undef FB_ADAPTED_CASE
+    default:
+      return fb_fail(1, "gemm_tc_adapted: tiles 128..256 (steps of 16) wide, not %d", bn);
+  }
+}
+
 // How many CTA pairs of the paired product (256-wide tiles) the device runs at
 // once: the number of tiles of one round. <= 0 on failure (see fb_last_error).
 FB_API int fb_gemm_tc_pair_slots() {
@@ -766,11 +848,11 @@ FB_API int fb_gemm_tc_pair_slots() {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaFuncSetAttribute(gemm_tc_pair_kernel<256>,
+  cudaError_t e = cudaFuncSetAttribute(gemm_tc_pair_kernel<256, false>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        SmemPair<256>::BYTES);
   int n = 0;
-  if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, gemm_tc_pair_kernel<256>, &cfg);
+  if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, gemm_tc_pair_kernel<256, false>, &cfg);
   if (e != cudaSuccess) return -fb_fail(2, "gemm_tc_pair_slots: %s", cudaGetErrorString(e));
   return n;
 }

@@ -120,6 +120,12 @@ _SIGNATURES = {
                         c_void_p],
     "fb_adapter_shrink": [c_void_p, c_ll, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                           c_int, c_void_p, c_void_p],
+    "fb_adapter_planes": [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+                          c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
+    "fb_gemm_tc_adapted": [c_void_p, c_ll, c_int, c_void_p, c_ll, c_int, c_int, c_void_p, c_void_p,
+                           c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_ll, c_int,
+                           c_void_p, c_ll, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_float,
+                           c_void_p],
     "fb_adapter_expand": [c_void_p, c_int, c_ll, c_ll, c_void_p, c_void_p, c_int, c_void_p, c_int,
                           c_int, c_int, c_int, c_void_p, c_int, c_ll, c_void_p],
     "fb_ln_add_ln": [c_void_p, c_int, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p,
@@ -2154,7 +2160,7 @@ MAX_ADAPTER_RANK = 512
 class AdapterBank:
     """The low-rank adapters of one projection [N, K]: `a` [slots, rank, K] and `b` [slots, N, rank] in
     the projection's type, `scales` float32 [slots]. An adapter of a smaller rank has zeros in the
-    rest."""
+    rest. `b` has to be finite: with many tokens, zeros of other rows meet it."""
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor):
         if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2] or \
@@ -2175,11 +2181,50 @@ class AdapterBank:
         return self.a.shape[1]
 
 
+ADAPTER_BLOCK = 256      # tokens whose adapters share the planes of a tile (csrc/adapter.cu)
+ADAPTER_PIECE = 8192     # tokens of one launch: the planes' workspace is made for this many
+MAX_ADAPTER_SLOTS = 1024
+
+
+def _planes_fit(x: torch.Tensor, w: torch.Tensor, bank: AdapterBank) -> bool:
+    """Whether adapters may ride behind the projection's own K in the paired product."""
+    return (x.dtype == torch.bfloat16 and x.shape[0] > SKINNY_ROWS and w.shape[0] >= 128 and PAIRED
+            and PERSISTENT and bank.slots <= MAX_ADAPTER_SLOTS and _tc_usable(x, w, w))
+
+
+def _adapted_planes(x: torch.Tensor, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
+                    out: torch.Tensor) -> None:
+    (T, K), N = x.shape, w.shape[0]
+    blocks = (T + ADAPTER_BLOCK - 1) // ADAPTER_BLOCK
+    most = min(bank.slots, ADAPTER_BLOCK, T)
+    u = torch.empty((blocks * most * ADAPTER_BLOCK, bank.rank), dtype=torch.bfloat16, device=x.device)
+    lists = torch.empty(blocks * (1 + most), dtype=torch.int32, device=x.device)
+    counts, slots = lists.data_ptr(), lists.data_ptr() + 4 * blocks
+    # K is split over as many blocks as keep the SMs busy, two adapters a block of tokens taken for usual
+    work = (T + 31) // 32 * min(most, 2)
+    shares = 1
+    while shares < 8 and work * shares * 2 <= sm_count() and K >= 1024 * shares:
+        shares *= 2
+    _call("fb_adapter_planes", x.data_ptr(), _rows(x, "x"), bank.a.data_ptr(), bank.scales.data_ptr(),
+          index.data_ptr(), bank.slots, bank.rank, T, K, most, shares, u.data_ptr(), counts, slots,
+          _stream(), tag=("t{} k{} r{}", T, K, bank.rank))
+    bn = prompt_plan(T, N)[0]
+    scratch = (0, 0, 0, 0)
+    if PAIR_TAIL_SHARES:
+        work, counters = _pair_scratch(x.device)
+        scratch = (work.data_ptr(), work.numel() * 4, counters.data_ptr(), counters.numel())
+    _call("fb_gemm_tc_adapted", x.data_ptr(), _rows(x, "x"), T, w.data_ptr(), _rows(w, "w"), N, K,
+          u.data_ptr(), bank.b.data_ptr(), counts, slots, most, bank.slots, bank.rank, out.data_ptr(),
+          1 if out.dtype == torch.float32 else 0, out.stride(0), bn, *scratch, *_NO_SCALE, _stream(),
+          tag=("t{} n{} k{} r{} tile{}", T, N, K, bank.rank, bn))
+
+
 def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
                     out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """y[t] = x[t] w^T + scale_a (x[t] a_a^T) b_a^T with a = index[t] (int32, one a token; outside of
-    the bank: no adapter). Sums are 32-bit, the ranks' numbers too, and y is rounded once, to
-    `out_dtype` (the input's type)."""
+    the bank: no adapter). Sums are 32-bit and y is rounded once, to `out_dtype` (the input's type);
+    in bfloat16 with more than 16 tokens the rank numbers are rounded to bfloat16 for the tensor
+    cores (csrc/adapter.cu says which kernels run)."""
     x = plain(x)
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
         raise KernelError(f"adapted_product: x {tuple(x.shape)}, w {tuple(w.shape)}")
@@ -2191,13 +2236,30 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
                           f"a projection {tuple(w.shape)}")
     _on_current_device(x, "x")
     device = x.device
+    if w.device != device:
+        raise KernelError(f"w is on {w.device}, the call's rows are on {device}")
     a = _given(bank.a, "a", x.dtype, None, device)
     b = _given(bank.b, "b", x.dtype, None, device)
     scales = _given(bank.scales, "scales", torch.float32, None, device)
     which = _given(index, "index", torch.int32, (T,), device)
+    if (a | b) % 16:
+        raise KernelError("adapted_product: the adapters must start on 16-byte boundaries")
     out = torch.empty((T, N), dtype=out_dtype or x.dtype, device=device)
+    code_of(out.dtype)
     if T == 0:
         return out
+    if T > ADAPTER_PIECE:
+        for t in range(0, T, ADAPTER_PIECE):
+            out[t:t + ADAPTER_PIECE] = adapted_product(x[t:t + ADAPTER_PIECE], w, bank,
+                                                       index[t:t + ADAPTER_PIECE], out.dtype)
+        return out
+    if _planes_fit(x, w, bank):
+        _adapted_planes(x, w, bank, index, out)
+        return out
+    low = torch.empty((T, bank.rank), dtype=torch.float32, device=device)
+    _call("fb_adapter_shrink", x.data_ptr(), _rows(x, "x"), code_of(x.dtype), a, scales, which,
+          bank.slots, bank.rank, T, K, low.data_ptr(), _stream(),
+          tag=("t{} k{} r{}", T, K, bank.rank))
     if x.dtype == torch.float32:
         base = gemm_simt(x, w, torch.empty((T, N), dtype=torch.float32, device=device))
     else:
@@ -2205,10 +2267,6 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
     planes = 1
     if isinstance(base, Planes):
         planes, base = base.count, base.tensor
-    low = torch.empty((T, bank.rank), dtype=torch.float32, device=device)
-    _call("fb_adapter_shrink", x.data_ptr(), _rows(x, "x"), code_of(x.dtype), a, scales, which,
-          bank.slots, bank.rank, T, K, low.data_ptr(), _stream(),
-          tag=("t{} k{} r{}", T, K, bank.rank))
     _call("fb_adapter_expand", base.data_ptr(), planes, T * N, N, low.data_ptr(), b, code_of(x.dtype),
           which, bank.slots, bank.rank, T, N, out.data_ptr(), code_of(out.dtype), N, _stream(),
           tag=("t{} n{} r{}", T, N, bank.rank))
