@@ -4,13 +4,15 @@
 //
 // What it has to read beside the projection is small (a rank of 16 beside 4,096 -> 4,096: 1/128 of W for
 // every adapter in the step), so what counts is that the projection's kernels run as they do without it.
-//   More than 16 tokens, bfloat16: `adapter_planes` makes the rank numbers of each block of 256 tokens, a
-//   plane for every adapter that has tokens in the block (zero in the rows of others), and the paired
-//   tcgen05 product takes them as more K behind its own, [x | planes] [W | B]^T: one sum in tensor
-//   memory, one rounding (gemm_tcgen05_pair.cu, MoreK). The rank numbers are rounded to bfloat16 for
-//   that, 2^-9 of the adapter's part on average.
-//   Else: `adapter_shrink` makes a token's rank numbers in 32 bits, the projection leaves 32-bit sums
-//   (planes), and `adapter_expand` adds up planes and adapter and rounds once.
+//   Where the projection itself runs as the paired tcgen05 product (hundreds of tokens, bfloat16):
+//   `adapter_low` (adapter_tcgen05.cu) makes the rank numbers of each block of 256 tokens as planes, one for every adapter that
+//   has tokens in the block (zero in the rows of others), and the product takes them as more K behind its
+//   own, [x | planes] [W | B]^T: one sum in tensor memory, one rounding (gemm_tcgen05_pair.cu, MoreK). The
+//   rank numbers are rounded to bfloat16 for that, 2^-9 of the adapter's part on average.
+//   More than 16 tokens, else: `adapter_low` leaves them as 32-bit rows, the projection leaves 32-bit sums
+//   (split-K planes), and `adapter_expand_mma` adds up sums and adapters on the tensor cores (again of
+//   bfloat16 rank numbers) and rounds once.
+//   A few tokens, and float32: the same in three with plain multiply-adds, nothing rounded in between.
 #include "common.cuh"
 
 namespace {
@@ -133,166 +135,120 @@ adapter_expand_kernel(const float* base, int planes, long long plane_stride, lon
   out[(size_t)t * ldo + n] = fb_from_float<Out>(v);
 }
 
-// ------------------------------------------------------------ the planes of a block
-constexpr int BLOCK_ROWS = 256;  // tokens of a block: a tile of the paired product
-constexpr int TOKENS = 32;       // tokens of a CTA
-constexpr int RANKS = 64;        // ranks of a turn
-constexpr int WARPS = THREADS / 32;
-constexpr int MAX_SLOTS = 1024;
-constexpr int CHUNK = 64;
+// ------------------------------------------------------- the other side on tensor cores
+constexpr int FEATURES = 64;        // of a CTA, 16 a warp
+constexpr int TOKENS = 32;
+constexpr int EXPAND_THREADS = 128;
+constexpr int STEPS = 8;            // k steps of 16 whose loads are on their way together
 
-__device__ __forceinline__ void cluster_sync() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float ld_peer(const float* mine, unsigned rank) {
-  unsigned there;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
-               : "=r"(there) : "r"((unsigned)__cvta_generic_to_shared(mine)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
-  return v;
-}
-
-struct PlaneShared {
-  unsigned present[MAX_SLOTS / 32];
-  int slot, count, any;
-  int index[TOKENS];
-  float part[RANKS][TOKENS + 1];          // this CTA's share of K
-  float warps[WARPS][RANKS][TOKENS + 1];  // each warp's
-};
-
-// CTA (i, e, z): of 32 tokens, the rank numbers of the e-th adapter of their block, zero in the rows of
-// others; K is split over the warps and over the z CTAs of a cluster, which read each other's sums in
-// order. Rows of A are the instruction's 16 rows, tokens its 8 columns, and both come straight from
-// global memory in the order that the instruction wants (a thread has 16 neighbouring elements of K, as
-// in gemm_skinny.cu): every warp has other bytes, so shared memory would not save any.
-__global__ void __launch_bounds__(THREADS)
-adapter_planes_kernel(const __nv_bfloat16* x, long long ldx, const __nv_bfloat16* a, const float* scales,
-                      const int* index, int slots, int rank, int T, int K, int most, __nv_bfloat16* u,
-                      int* counts, int* slots_of) {
+// out[t, n] = sum over the planes of base[., t, n] + sum_j low[t, j] B[a][n, j] for 32 tokens and 64
+// features. The adapters of the 32 tokens come one after another, 16 ranks a step; tokens of others have
+// zeros there. B comes straight from global memory: a thread takes four neighbouring ranks of a row,
+// which the instruction gets as its k slots (2q, 2q + 1, 2q + 8, 2q + 9) on both sides.
+template <typename Out>
+__global__ void __launch_bounds__(EXPAND_THREADS)
+adapter_expand_mma_kernel(const float* base, int planes, long long plane_stride, long long ldb, const float* low,
+                          const __nv_bfloat16* b, const int* index, int slots, int rank, int T, int N, Out* out,
+                          long long ldo) {
   extern __shared__ __align__(16) unsigned char raw[];
-  PlaneShared& s = *reinterpret_cast<PlaneShared*>(raw);
+  float (*sums)[FEATURES + 4] = reinterpret_cast<float (*)[FEATURES + 4]>(raw);                // [TOKENS]
+  __nv_bfloat16* u = reinterpret_cast<__nv_bfloat16*>(raw + TOKENS * (FEATURES + 4) * 4);      // [TOKENS][ld]
+  __shared__ int s_index[TOKENS], s_slots[TOKENS], s_count;
+  const int ld = rank + 8;
   fb_pdl_wait();
   fb_pdl_launch();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
-  const int t0 = blockIdx.x * TOKENS, block = t0 / BLOCK_ROWS, e = blockIdx.y;
-  const int shares = gridDim.z, share = blockIdx.z;
-  for (int i = tid; i < MAX_SLOTS / 32; i += THREADS) s.present[i] = 0u;
-  if (tid == 0) s.any = 0;
-  __syncthreads();
-  {
-    const int t = block * BLOCK_ROWS + tid;  // (THREADS tokens of the block)
-    int slot = t < T ? index[t] : -1;
+  const int t0 = blockIdx.y * TOKENS, n0 = blockIdx.x * FEATURES;
+  if (warp == 0) {  // the adapters of these tokens, each once
+    int slot = t0 + lane < T ? index[t0 + lane] : -1;
     if (slot >= slots) slot = -1;
-    if (slot >= 0) atomicOr(&s.present[slot >> 5], 1u << (slot & 31));
-    const int here = t - t0;
-    if (here >= 0 && here < TOKENS) s.index[here] = slot;
+    s_index[lane] = slot;
+    const unsigned same = __match_any_sync(0xffffffffu, slot);
+    const bool first = slot >= 0 && __ffs(same) - 1 == lane;
+    const unsigned firsts = __ballot_sync(0xffffffffu, first);
+    if (first) s_slots[__popc(firsts & ((1u << lane) - 1))] = slot;
+    if (lane == 0) s_count = __popc(firsts);
   }
   __syncthreads();
-  if (warp == 0) {  // the e-th adapter of the block, by its slot
-    const unsigned word = s.present[lane];
-    unsigned upto = __popc(word);
+  for (int i = tid; i < TOKENS * (rank / 4); i += EXPAND_THREADS) {
+    const int t = i / (rank / 4), j = i % (rank / 4) * 4;
+    if (s_index[t] < 0) continue;  // (no adapter takes its row)
+    const float4 f = __ldcg(reinterpret_cast<const float4*>(low + (size_t)(t0 + t) * rank + j));
+    __nv_bfloat162* to = reinterpret_cast<__nv_bfloat162*>(u + t * ld + j);
+    to[0] = __floats2bfloat162_rn(f.x, f.y);
+    to[1] = __floats2bfloat162_rn(f.z, f.w);
+  }
+  __syncthreads();
+  float acc[TOKENS / 8][4];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned other = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += other;
+  for (int n = 0; n < TOKENS / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+  const int row0 = min(n0 + warp * 16 + g, N - 1), row1 = min(n0 + warp * 16 + g + 8, N - 1);
+  const int per = (rank + 15) / 16, steps = s_count * per;
+  for (int s0 = 0; s0 < steps; s0 += STEPS) {
+    uint2 w[STEPS][2];
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const int e = (s0 + i) / per, k = (s0 + i - e * per) * 16 + 4 * q;
+      w[i][0] = w[i][1] = make_uint2(0u, 0u);
+      if (s0 + i < steps && k < rank) {
+        const __nv_bfloat16* from = b + (size_t)s_slots[e] * N * rank + k;
+        w[i][0] = __ldcg(reinterpret_cast<const uint2*>(from + (size_t)row0 * rank));
+        w[i][1] = __ldcg(reinterpret_cast<const uint2*>(from + (size_t)row1 * rank));
+      }
     }
-    if (lane == 31) s.count = (int)upto;
-    const int before = (int)upto - __popc(word);
-    if (e >= before && e < (int)upto) s.slot = lane * 32 + (int)__fns(word, 0, e - before + 1);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      if (s0 + i >= steps) break;
+      const int e = (s0 + i) / per, k = (s0 + i - e * per) * 16 + 4 * q, slot = s_slots[e];
+#pragma unroll
+      for (int n = 0; n < TOKENS / 8; ++n) {
+        const int t = n * 8 + g;
+        uint2 v = make_uint2(0u, 0u);
+        if (s_index[t] == slot && k < rank) v = *reinterpret_cast<const uint2*>(u + t * ld + k);
+        mma_bf16(acc[n], w[i][0].x, w[i][1].x, w[i][0].y, w[i][1].y, v.x, v.y);
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < TOKENS / 8; ++n) {
+    sums[n * 8 + 2 * q][warp * 16 + g] = acc[n][0];
+    sums[n * 8 + 2 * q + 1][warp * 16 + g] = acc[n][1];
+    sums[n * 8 + 2 * q][warp * 16 + g + 8] = acc[n][2];
+    sums[n * 8 + 2 * q + 1][warp * 16 + g + 8] = acc[n][3];
   }
   __syncthreads();
-  const bool tells = t0 % BLOCK_ROWS == 0 && share == 0 && tid == 0;
-  if (tells && e == 0) counts[block] = s.count;
-  if (e >= s.count) return;  // (every CTA of the cluster)
-  const int slot = s.slot;
-  if (tells) slots_of[block * most + e] = slot;
-  __nv_bfloat16* rows = u + ((size_t)(block * most + e) * BLOCK_ROWS + t0 % BLOCK_ROWS) * rank;
-  if (tid < TOKENS && s.index[tid] == slot) s.any = 1;
-  __syncthreads();
-  if (s.any == 0) {  // none of these tokens: zeros
-    if (share == 0)
-      for (int i = tid; i < TOKENS * rank / 8; i += THREADS)
-        reinterpret_cast<uint4*>(rows)[i] = make_uint4(0u, 0u, 0u, 0u);
+  const bool four = (((uintptr_t)base | (uintptr_t)out) % 16) == 0 && ldb % 4 == 0 && plane_stride % 4 == 0 &&
+                    ldo % 4 == 0 && n0 + FEATURES <= N;
+  if (four) {
+    constexpr int GROUPS = FEATURES / 4;
+#pragma unroll
+    for (int i0 = 0; i0 < TOKENS * GROUPS; i0 += EXPAND_THREADS) {
+      const int t = (i0 + tid) / GROUPS, f = (i0 + tid) % GROUPS * 4;
+      if (t0 + t >= T) continue;
+      float4 v = *reinterpret_cast<const float4*>(&sums[t][f]);
+      for (int p = 0; p < planes; ++p) {
+        const float4 o = __ldcg(reinterpret_cast<const float4*>(base + (size_t)p * plane_stride + (size_t)(t0 + t) * ldb + n0 + f));
+        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+      }
+      Out* to = out + (size_t)(t0 + t) * ldo + n0 + f;
+      if constexpr (sizeof(Out) == 4) {
+        *reinterpret_cast<float4*>(to) = v;
+      } else {
+        uint2 pk;
+        const __nv_bfloat162 h0 = __floats2bfloat162_rn(v.x, v.y), h1 = __floats2bfloat162_rn(v.z, v.w);
+        pk.x = *reinterpret_cast<const uint32_t*>(&h0);
+        pk.y = *reinterpret_cast<const uint32_t*>(&h1);
+        *reinterpret_cast<uint2*>(to) = pk;
+      }
+    }
     return;
   }
-  const float scale = scales[slot];
-  const int chunks = (K + CHUNK - 1) / CHUNK;
-  const int each = (chunks + shares * WARPS - 1) / (shares * WARPS);
-  const int c0 = (share * WARPS + warp) * each, c1 = min(chunks, c0 + each);
-  const __nv_bfloat16* xr[TOKENS / 8];
-#pragma unroll
-  for (int n = 0; n < TOKENS / 8; ++n) xr[n] = x + (size_t)min(t0 + n * 8 + g, T - 1) * ldx + q * 8;
-  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  for (int r0 = 0; r0 < rank; r0 += RANKS) {
-    const int tiles = (min(RANKS, rank - r0) + 15) / 16;
-    float acc[RANKS / 16][TOKENS / 8][4];
-#pragma unroll
-    for (int m = 0; m < RANKS / 16; ++m)
-#pragma unroll
-      for (int n = 0; n < TOKENS / 8; ++n) acc[m][n][0] = acc[m][n][1] = acc[m][n][2] = acc[m][n][3] = 0.f;
-    for (int c = c0; c < c1; ++c) {
-      const int k = c * CHUNK + q * 8;
-      const bool lo = k + 8 <= K, hi = k + 40 <= K;
-      uint4 b[TOKENS / 8][2];
-#pragma unroll
-      for (int n = 0; n < TOKENS / 8; ++n) {
-        b[n][0] = lo ? ld16(xr[n] + (size_t)c * CHUNK) : zero;
-        b[n][1] = hi ? ld16(xr[n] + (size_t)c * CHUNK + 32) : zero;
-      }
-#pragma unroll
-      for (int m = 0; m < RANKS / 16; ++m) {
-        if (m >= tiles) break;
-        const __nv_bfloat16* w0 = a + ((size_t)slot * rank + min(r0 + m * 16 + g, rank - 1)) * K + k;
-        const __nv_bfloat16* w1 = a + ((size_t)slot * rank + min(r0 + m * 16 + g + 8, rank - 1)) * K + k;
-        const uint4 w[4] = {lo ? ld16(w0) : zero, hi ? ld16(w0 + 32) : zero, lo ? ld16(w1) : zero,
-                            hi ? ld16(w1 + 32) : zero};
-        const uint32_t* a0 = reinterpret_cast<const uint32_t*>(&w[0]);
-        const uint32_t* a1 = reinterpret_cast<const uint32_t*>(&w[2]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int n = 0; n < TOKENS / 8; ++n) {
-            const uint32_t* bx = reinterpret_cast<const uint32_t*>(&b[n][0]);
-            mma_bf16(acc[m][n], a0[2 * i], a1[2 * i], a0[2 * i + 1], a1[2 * i + 1], bx[2 * i], bx[2 * i + 1]);
-          }
-      }
-    }
-#pragma unroll
-    for (int m = 0; m < RANKS / 16; ++m) {
-      if (m >= tiles) break;
-#pragma unroll
-      for (int n = 0; n < TOKENS / 8; ++n) {
-        s.warps[warp][m * 16 + g][n * 8 + 2 * q] = acc[m][n][0];
-        s.warps[warp][m * 16 + g][n * 8 + 2 * q + 1] = acc[m][n][1];
-        s.warps[warp][m * 16 + g + 8][n * 8 + 2 * q] = acc[m][n][2];
-        s.warps[warp][m * 16 + g + 8][n * 8 + 2 * q + 1] = acc[m][n][3];
-      }
-    }
-    __syncthreads();
-    for (int i = tid; i < tiles * 16 * TOKENS; i += THREADS) {
-      const int j = i / TOKENS, t = i % TOKENS;
-      float v = 0.f;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) v += s.warps[w][j][t];
-      s.part[j][t] = v;
-    }
-    if (shares > 1) cluster_sync(); else __syncthreads();
-    // the tokens' rows are shared by the cluster's CTAs; ranks side by side
-    const int wide = min(RANKS, rank - r0), mine = TOKENS / shares;
-    for (int i = tid; i < mine * wide; i += THREADS) {
-      const int t = share * mine + i / wide, j = i % wide;
-      float v = 0.f;
-      if (shares > 1) {
-        for (int z = 0; z < shares; ++z) v += ld_peer(&s.part[j][t], z);
-      } else {
-        v = s.part[j][t];
-      }
-      rows[(size_t)t * rank + r0 + j] = __float2bfloat16_rn(s.index[t] == slot ? scale * v : 0.f);
-    }
-    // nobody's sums are overwritten, or gone, while a peer still reads them
-    if (shares > 1) cluster_sync(); else __syncthreads();
+  for (int i = tid; i < TOKENS * FEATURES; i += EXPAND_THREADS) {
+    const int t = i / FEATURES, f = i % FEATURES;
+    if (t0 + t >= T || n0 + f >= N) continue;
+    float v = sums[t][f];
+    for (int p = 0; p < planes; ++p) v += __ldcg(base + (size_t)p * plane_stride + (size_t)(t0 + t) * ldb + n0 + f);
+    out[(size_t)(t0 + t) * ldo + n0 + f] = fb_from_float<Out>(v);
   }
 }
 }  // namespace
@@ -326,29 +282,18 @@ FB_API int fb_adapter_expand(const float* base, int planes, long long plane_stri
   return fb_check_launch("adapter_expand");
 }
 
-// u [ceil(T / 256) * most * 256, rank] bfloat16, counts [blocks], slots_of [blocks, most]: what
-// fb_gemm_tc_adapted takes beside x and W. most: at least the adapters that one block of 256 tokens can
-// have. shares: CTAs that split K (1, 2, 4 or 8).
-FB_API int fb_adapter_planes(const void* x, long long ldx, const void* a, const float* scales, const int* index,
-                             int slots, int rank, int T, int K, int most, int shares, void* u, int* counts,
-                             int* slots_of, cudaStream_t stream) {
-  FB_REQUIRE(T > 0 && K > 0 && rank > 0 && rank % 8 == 0 && slots > 0 && slots <= MAX_SLOTS && ldx >= K,
-             "adapter_planes: bad sizes T=%d K=%d rank=%d slots=%d", T, K, rank, slots);
-  FB_REQUIRE(most >= (slots < BLOCK_ROWS ? slots : BLOCK_ROWS) || most >= T, "adapter_planes: room for %d adapters a block", most);
-  FB_REQUIRE(K % 8 == 0 && ldx % 8 == 0 && (((uintptr_t)x | (uintptr_t)a | (uintptr_t)u) % 16) == 0,
-             "adapter_planes: K, the row stride and the operands must keep 16-byte alignment");
-  FB_REQUIRE(shares == 1 || shares == 2 || shares == 4 || shares == 8, "adapter_planes: %d shares of K", shares);
-  static bool seen[64] = {};
-  if (fb_first_use_on_device(seen)) {
-    cudaError_t e = cudaFuncSetAttribute(adapter_planes_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)sizeof(PlaneShared));
-    if (e != cudaSuccess) return fb_fail(2, "adapter_planes: shared memory opt-in: %s", cudaGetErrorString(e));
-  }
-  // every row of every block is written, those behind the last token too: the product reads them
-  const int blocks = (T + BLOCK_ROWS - 1) / BLOCK_ROWS;
-  const dim3 grid(blocks * (BLOCK_ROWS / TOKENS), most < slots ? most : slots, shares);
-  fb_launch_cluster(adapter_planes_kernel, grid, dim3(THREADS), sizeof(PlaneShared), stream, (unsigned)shares,
-                    (const __nv_bfloat16*)x, ldx, (const __nv_bfloat16*)a, scales, index, slots, rank, T, K,
-                    most, (__nv_bfloat16*)u, counts, slots_of);
-  return fb_check_launch("adapter_planes");
+// As fb_adapter_expand for bfloat16 adapters, on the tensor cores.
+FB_API int fb_adapter_expand_mma(const float* base, int planes, long long plane_stride, long long ldb,
+                                 const float* low, const void* b, const int* index, int slots, int rank, int T,
+                                 int N, void* out, int out_dtype, long long ldo, cudaStream_t stream) {
+  FB_REQUIRE(T > 0 && N > 0 && rank > 0 && rank <= 512 && rank % 8 == 0 && slots > 0 && planes > 0 && ldb >= N &&
+                 ldo >= N && (((uintptr_t)b | (uintptr_t)low) % 16) == 0,
+             "adapter_expand_mma: bad sizes T=%d N=%d rank=%d, or operands not on 16-byte boundaries", T, N, rank);
+  FB_REQUIRE((T + TOKENS - 1) / TOKENS <= 65535, "adapter_expand_mma: %d tokens", T);
+  const size_t shared = TOKENS * (FEATURES + 4) * 4 + (size_t)TOKENS * (rank + 8) * 2;  // (42 KB at rank 512)
+  const dim3 grid((N + FEATURES - 1) / FEATURES, (T + TOKENS - 1) / TOKENS);
+  FB_DISPATCH_DTYPE(out_dtype, O,
+      fb_launch(adapter_expand_mma_kernel<O>, grid, dim3(EXPAND_THREADS), shared, stream, base, planes,
+                plane_stride, ldb, low, (const __nv_bfloat16*)b, index, slots, rank, T, N, (O*)out, ldo));
+  return fb_check_launch("adapter_expand_mma");
 }

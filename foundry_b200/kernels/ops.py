@@ -109,6 +109,7 @@ _SIGNATURES = {
     "fb_wait_for_stream": [c_void_p],
     "fb_zero_rows": [c_void_p, c_void_p, c_int, c_void_p],
     "fb_gemm_f32_status": [c_void_p],
+    "fb_adapter_status": [c_void_p],
     "fb_row_scales": [c_void_p, c_int, c_int, c_int, c_float, c_void_p, c_int, c_void_p],
     "fb_select_tokens": [c_void_p, c_ll, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                          c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p],
@@ -120,8 +121,10 @@ _SIGNATURES = {
                         c_void_p],
     "fb_adapter_shrink": [c_void_p, c_ll, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                           c_int, c_void_p, c_void_p],
-    "fb_adapter_planes": [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
-                          c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
+    "fb_adapter_low": [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+                       c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    "fb_adapter_expand_mma": [c_void_p, c_int, c_ll, c_ll, c_void_p, c_void_p, c_void_p, c_int,
+                              c_int, c_int, c_int, c_void_p, c_int, c_ll, c_void_p],
     "fb_gemm_tc_adapted": [c_void_p, c_ll, c_int, c_void_p, c_ll, c_int, c_int, c_void_p, c_void_p,
                            c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_ll, c_int,
                            c_void_p, c_ll, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_float,
@@ -1368,10 +1371,11 @@ if _os.environ.get("FOUNDRY_B200_PDL", "1") == "0":
 
 
 _STATUS_READERS = ("fb_gemm_tc_status", "fb_gemm_tc_pair_status", "fb_attention_tc_status",
-                   "fb_gemm_rows_status", "fb_gemm_f32_status")
+                   "fb_gemm_rows_status", "fb_gemm_f32_status", "fb_adapter_status")
 # kernel codes of the host-visible failure record (FB_STATUS_KERNEL in csrc)
 _STATUS_KERNELS = {1: "tcgen05 product", 2: "paired tcgen05 product", 3: "tcgen05 prompt attention",
-                   4: "tcgen05 product for few token rows", 5: "32-bit tcgen05 product"}
+                   4: "tcgen05 product for few token rows", 5: "32-bit tcgen05 product",
+                   6: "tcgen05 product of adapters"}
 _STATUS_ROLES = {1: "tile loads", 2: "matrix instructions", 3: "epilogue",
                  4: "accumulators", 5: "tiles to split", 6: "room for pieces", 20: "shared-memory alignment"}
 _MIRROR = []
@@ -2186,10 +2190,32 @@ ADAPTER_PIECE = 8192     # tokens of one launch: the planes' workspace is made f
 MAX_ADAPTER_SLOTS = 1024
 
 
-def _planes_fit(x: torch.Tensor, w: torch.Tensor, bank: AdapterBank) -> bool:
-    """Whether adapters may ride behind the projection's own K in the paired product."""
-    return (x.dtype == torch.bfloat16 and x.shape[0] > SKINNY_ROWS and w.shape[0] >= 128 and PAIRED
-            and PERSISTENT and bank.slots <= MAX_ADAPTER_SLOTS and _tc_usable(x, w, w))
+def _low_fits(x: torch.Tensor, w: torch.Tensor, bank: AdapterBank) -> bool:
+    """Whether the rank numbers are the tensor cores' (csrc/adapter.cu)."""
+    return (x.dtype == torch.bfloat16 and x.shape[0] > SKINNY_ROWS
+            and bank.slots <= MAX_ADAPTER_SLOTS and _tc_usable(x, w, w))
+
+
+def _planes_pay(T: int, N: int, K: int) -> bool:
+    """Whether adapters ride behind the projection's own K: where that runs as the paired product
+    anyway. (Where it would not, the paired form costs more than the two launches it saves: 4,096 ->
+    4,096 with rank 16 in graph replays, 128 tokens.)"""
+    if not (PAIRED and PERSISTENT) or N < 128 or T <= 128:
+        return False
+    return not (T <= ONE_TILE_ROWS and _one_tile_plan(T, N, K)[1])
+
+
+def _adapter_low(x: torch.Tensor, bank: AdapterBank, index: torch.Tensor, most: int, u: int, counts: int,
+                 slots: int, low: int) -> None:
+    T, K = x.shape
+    tiles = (T + 127) // 128
+    side = max(1, min(most, sm_count() // tiles))
+    shares = 1
+    while shares < 8 and 2 * shares * tiles * side <= sm_count() and K >= 256 * shares:
+        shares *= 2
+    _call("fb_adapter_low", x.data_ptr(), _rows(x, "x"), bank.a.data_ptr(), bank.scales.data_ptr(),
+          index.data_ptr(), bank.slots, bank.rank, T, K, most, side, shares, u, counts, slots, low,
+          _stream(), tag=("t{} k{} r{}", T, K, bank.rank))
 
 
 def _adapted_planes(x: torch.Tensor, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
@@ -2200,14 +2226,7 @@ def _adapted_planes(x: torch.Tensor, w: torch.Tensor, bank: AdapterBank, index: 
     u = torch.empty((blocks * most * ADAPTER_BLOCK, bank.rank), dtype=torch.bfloat16, device=x.device)
     lists = torch.empty(blocks * (1 + most), dtype=torch.int32, device=x.device)
     counts, slots = lists.data_ptr(), lists.data_ptr() + 4 * blocks
-    # K is split over as many blocks as keep the SMs busy, two adapters a block of tokens taken for usual
-    work = (T + 31) // 32 * min(most, 2)
-    shares = 1
-    while shares < 8 and work * shares * 2 <= sm_count() and K >= 1024 * shares:
-        shares *= 2
-    _call("fb_adapter_planes", x.data_ptr(), _rows(x, "x"), bank.a.data_ptr(), bank.scales.data_ptr(),
-          index.data_ptr(), bank.slots, bank.rank, T, K, most, shares, u.data_ptr(), counts, slots,
-          _stream(), tag=("t{} k{} r{}", T, K, bank.rank))
+    _adapter_low(x, bank, index, most, u.data_ptr(), counts, slots, 0)
     bn = prompt_plan(T, N)[0]
     scratch = (0, 0, 0, 0)
     if PAIR_TAIL_SHARES:
@@ -2253,13 +2272,17 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
             out[t:t + ADAPTER_PIECE] = adapted_product(x[t:t + ADAPTER_PIECE], w, bank,
                                                        index[t:t + ADAPTER_PIECE], out.dtype)
         return out
-    if _planes_fit(x, w, bank):
+    on_tensor_cores = _low_fits(x, w, bank)
+    if on_tensor_cores and _planes_pay(T, N, K):
         _adapted_planes(x, w, bank, index, out)
         return out
     low = torch.empty((T, bank.rank), dtype=torch.float32, device=device)
-    _call("fb_adapter_shrink", x.data_ptr(), _rows(x, "x"), code_of(x.dtype), a, scales, which,
-          bank.slots, bank.rank, T, K, low.data_ptr(), _stream(),
-          tag=("t{} k{} r{}", T, K, bank.rank))
+    if on_tensor_cores:
+        _adapter_low(x, bank, index, min(bank.slots, 128, T), 0, 0, 0, low.data_ptr())
+    else:
+        _call("fb_adapter_shrink", x.data_ptr(), _rows(x, "x"), code_of(x.dtype), a, scales, which,
+              bank.slots, bank.rank, T, K, low.data_ptr(), _stream(),
+              tag=("t{} k{} r{}", T, K, bank.rank))
     if x.dtype == torch.float32:
         base = gemm_simt(x, w, torch.empty((T, N), dtype=torch.float32, device=device))
     else:
@@ -2267,6 +2290,11 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
     planes = 1
     if isinstance(base, Planes):
         planes, base = base.count, base.tensor
+    if on_tensor_cores:
+        _call("fb_adapter_expand_mma", base.data_ptr(), planes, T * N, N, low.data_ptr(), b, which,
+              bank.slots, bank.rank, T, N, out.data_ptr(), code_of(out.dtype), N, _stream(),
+              tag=("t{} n{} r{}", T, N, bank.rank))
+        return out
     _call("fb_adapter_expand", base.data_ptr(), planes, T * N, N, low.data_ptr(), b, code_of(x.dtype),
           which, bank.slots, bank.rank, T, N, out.data_ptr(), code_of(out.dtype), N, _stream(),
           tag=("t{} n{} r{}", T, N, bank.rank))
