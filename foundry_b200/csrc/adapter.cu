@@ -9,24 +9,14 @@
 //   has tokens in the block (zero in the rows of others), and the product takes them as more K behind its
 //   own, [x | planes] [W | B]^T: one sum in tensor memory, one rounding (gemm_tcgen05_pair.cu, MoreK). The
 //   rank numbers are rounded to bfloat16 for that, 2^-9 of the adapter's part on average.
-//   More than 16 tokens, else: `adapter_low` leaves them as 32-bit rows, the projection leaves 32-bit sums
-//   (split-K planes), and `adapter_expand_mma` adds up sums and adapters on the tensor cores (again of
-//   bfloat16 rank numbers) and rounds once.
-//   A few tokens, and float32: the same in three with plain multiply-adds, nothing rounded in between.
+//   Else: `adapter_shrink` (or, for many numbers, `adapter_low`) leaves them as 32-bit rows, the projection
+//   leaves 32-bit sums (split-K planes), and `adapter_expand` adds up sums and adapters and rounds once.
 #include "common.cuh"
 
 namespace {
 
 constexpr int THREADS = 256;
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ uint4 ld16(const void* p) {  // never by the non-coherent path
   uint4 v;
   asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
@@ -44,31 +34,35 @@ __device__ __forceinline__ float dot8(const uint4& a, const uint4& b, float sum)
   return sum;
 }
 
-// Block (j, t): low[t, 8 j + warp] = scale * sum_k x[t, k] A[a][.., k], a warp a rank. `wide`: rows are
-// on 16-byte boundaries.
-template <typename T>
+// low[t, j] = scale * sum_k x[t, k] A[a][j, k], PARTS warps of a block a rank, each with a share of K, so that
+// a warp has few rounds of loads one after another (K = 14,336, 48 tokens, rank 16: one warp a rank 24 us).
+// Block (i, t) has the ranks from i * 8 / PARTS on. `wide`: rows are on 16-byte boundaries.
+template <typename T, int PARTS>
 __global__ void __launch_bounds__(THREADS)
 adapter_shrink_kernel(const T* x, long long ldx, const T* a, const float* scales, const int* index, int slots,
                       int rank, int K, int wide, float* low) {
+  __shared__ float sums[THREADS / 32];
   fb_pdl_wait();
   fb_pdl_launch();
   const int t = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int j = blockIdx.x * (THREADS / 32) + warp;
+  const int j = blockIdx.x * (THREADS / 32 / PARTS) + warp / PARTS;
   const int slot = index[t];
-  if (slot < 0 || slot >= slots || j >= rank) return;
+  if (slot < 0 || slot >= slots) return;  // (the whole block)
+  constexpr int EACH = 16 / sizeof(T), ROUND = 32 * EACH;
+  const int rounds = (K + ROUND - 1) / ROUND, each = (rounds + PARTS - 1) / PARTS;
+  const int from = (warp % PARTS) * each * ROUND, to = min(K, from + each * ROUND);
   const T* row = x + (size_t)t * ldx;
-  const T* w = a + ((size_t)slot * rank + j) * K;
-  constexpr int EACH = 16 / sizeof(T);
+  const T* w = a + ((size_t)slot * rank + min(j, rank - 1)) * K;
   float sum = 0.f;
-  int k = lane * EACH;
+  int k = from + lane * EACH;
   if (wide) {
     constexpr int AHEAD = 4;
-    for (; k + (AHEAD - 1) * 32 * EACH < K; k += AHEAD * 32 * EACH) {  // (K is a multiple of EACH)
+    for (; k + (AHEAD - 1) * ROUND < to; k += AHEAD * ROUND) {  // (K is a multiple of EACH)
       uint4 u[AHEAD], v[AHEAD];
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
-        v[i] = ld16(w + k + i * 32 * EACH);
-        u[i] = ld16(row + k + i * 32 * EACH);
+        v[i] = ld16(w + k + i * ROUND);
+        u[i] = ld16(row + k + i * ROUND);
       }
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
@@ -83,173 +77,218 @@ adapter_shrink_kernel(const T* x, long long ldx, const T* a, const float* scales
       }
     }
   }
-  for (; k < K; k += 32 * EACH) {
+  for (; k < to; k += ROUND) {
 #pragma unroll
     for (int e = 0; e < EACH; ++e)
-      if (k + e < K) sum = fmaf(fb_load_coherent(row + k + e), fb_load_coherent(w + k + e), sum);
+      if (k + e < to) sum = fmaf(fb_load_coherent(row + k + e), fb_load_coherent(w + k + e), sum);
   }
   sum = fb_warp_sum(sum);
-  if (lane == 0) low[(size_t)t * rank + j] = scales[slot] * sum;
-}
-
-// out[t, n] = sum over the planes of base[., t, n] + sum_j low[t, j] B[a][n, j], a thread a feature.
-template <typename T, typename Out>
-__global__ void __launch_bounds__(THREADS)
-adapter_expand_kernel(const float* base, int planes, long long plane_stride, long long ldb, const float* low,
-                      const T* b, const int* index, int slots, int rank, int N, Out* out, long long ldo) {
-  fb_pdl_wait();
-  extern __shared__ __align__(16) float mine[];
-  const int t = blockIdx.y, n = blockIdx.x * THREADS + threadIdx.x;
-  int slot = index[t];
-  if (slot >= slots) slot = -1;
-  if (slot >= 0) {
-    for (int j = threadIdx.x; j < rank; j += THREADS) mine[j] = __ldcg(low + (size_t)t * rank + j);
+  if constexpr (PARTS > 1) {
+    if (lane == 0) sums[warp] = sum;
     __syncthreads();
-  }
-  if (n >= N) return;
-  float v = 0.f;
-  for (int p = 0; p < planes; ++p) v += __ldcg(base + (size_t)p * plane_stride + (size_t)t * ldb + n);
-  if (slot >= 0) {
-    const T* w = b + ((size_t)slot * N + n) * rank;
-    float sum = 0.f;
-#pragma unroll 4
-    for (int j = 0; j < rank; j += 8) {  // (a multiple of 8)
-      if constexpr (sizeof(T) == 2) {
-        const uint4 q = ld16(w + j);
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
+    if (warp % PARTS != 0) return;
+    sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = __bfloat1622float2(h[e]);
-          sum = fmaf(mine[j + 2 * e], f.x, sum);
-          sum = fmaf(mine[j + 2 * e + 1], f.y, sum);
-        }
-      } else {
-        const uint4 q[2] = {ld16(w + j), ld16(w + j + 4)};
-        const float* f = reinterpret_cast<const float*>(q);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf(mine[j + e], f[e], sum);
-      }
-    }
-    v += sum;
+    for (int i = 0; i < PARTS; ++i) sum += sums[warp + i];
   }
-  out[(size_t)t * ldo + n] = fb_from_float<Out>(v);
+  if (lane == 0 && j < rank) low[(size_t)t * rank + j] = scales[slot] * sum;
 }
 
-// ------------------------------------------------------- the other side on tensor cores
-constexpr int FEATURES = 64;        // of a CTA, 16 a warp
-constexpr int TOKENS = 32;
-constexpr int EXPAND_THREADS = 128;
-constexpr int STEPS = 8;            // k steps of 16 whose loads are on their way together
+template <typename T, int PARTS>
+void launch_shrink(const T* x, long long ldx, const T* a, const float* scales, const int* index, int slots,
+                   int rank, int tokens, int K, int wide, float* low, cudaStream_t stream) {
+  constexpr int RANKS = THREADS / 32 / PARTS;
+  fb_launch(adapter_shrink_kernel<T, PARTS>, dim3((rank + RANKS - 1) / RANKS, tokens), dim3(THREADS), 0, stream,
+            x, ldx, a, scales, index, slots, rank, K, wide, low);
+}
+template <typename T>
+void shrink_by_size(const T* x, long long ldx, const T* a, const float* scales, const int* index, int slots,
+                    int rank, int tokens, int K, int wide, float* low, cudaStream_t stream) {
+  const int rounds = K / (32 * (16 / (int)sizeof(T)));  // of a warp's loads: four go out together
+  if (rounds <= 8) launch_shrink<T, 1>(x, ldx, a, scales, index, slots, rank, tokens, K, wide, low, stream);
+  else if (rounds <= 16) launch_shrink<T, 2>(x, ldx, a, scales, index, slots, rank, tokens, K, wide, low, stream);
+  else launch_shrink<T, 4>(x, ldx, a, scales, index, slots, rank, tokens, K, wide, low, stream);
+}
 
-// out[t, n] = sum over the planes of base[., t, n] + sum_j low[t, j] B[a][n, j] for 32 tokens and 64
-// features. The adapters of the 32 tokens come one after another, 16 ranks a step; tokens of others have
-// zeros there. B comes straight from global memory: a thread takes four neighbouring ranks of a row,
-// which the instruction gets as its k slots (2q, 2q + 1, 2q + 8, 2q + 9) on both sides.
-template <typename Out>
-__global__ void __launch_bounds__(EXPAND_THREADS)
-adapter_expand_mma_kernel(const float* base, int planes, long long plane_stride, long long ldb, const float* low,
-                          const __nv_bfloat16* b, const int* index, int slots, int rank, int T, int N, Out* out,
-                          long long ldo) {
-  extern __shared__ __align__(16) unsigned char raw[];
-  float (*sums)[FEATURES + 4] = reinterpret_cast<float (*)[FEATURES + 4]>(raw);                // [TOKENS]
-  __nv_bfloat16* u = reinterpret_cast<__nv_bfloat16*>(raw + TOKENS * (FEATURES + 4) * 4);      // [TOKENS][ld]
-  __shared__ int s_index[TOKENS], s_slots[TOKENS], s_count;
-  const int ld = rank + 8;
+// out[t, n] = sum over the planes of base[., t, n] + sum_j low[t, j] B[a][n, j].
+//
+// A row of B is read by L neighbouring lanes, 16 bytes each, so that a load of the warp takes 512 bytes that
+// lie side by side (a thread a feature, which reads its row alone, made 32 lines of every load: 48 tokens,
+// 4,096 features, rank 64, 11 us for the kernel). A lane keeps its few ranks' numbers of a token, multiplies
+// L features, and the lanes exchange sums so that each ends with the whole sum of one feature. Four tokens
+// a block: neighbours with the same adapter use the row that is there.
+constexpr int EXPAND_THREADS = 128;
+constexpr int EXPAND_TOKENS = 4;
+template <int L> constexpr int ROUNDS_OF = L >= 4 ? 1 : 4 / L;  // of 32 features a warp
+
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& q, float (&f)[16 / sizeof(T)]) {
+  if constexpr (sizeof(T) == 2) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 v = __bfloat1622float2(h[e]);
+      f[2 * e] = v.x;
+      f[2 * e + 1] = v.y;
+    }
+  } else {
+    const float4 v = *reinterpret_cast<const float4*>(&q);
+    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+  }
+}
+
+// L sums a lane, one a feature -> the sum over the L lanes of the lane's own feature.
+template <int L>
+__device__ __forceinline__ float share_out(float (&v)[L], int li) {
+#pragma unroll
+  for (int s = L / 2; s > 0; s >>= 1) {
+    const bool upper = (li & s) != 0;
+#pragma unroll
+    for (int i = 0; i < s; ++i) {
+      const float send = upper ? v[i] : v[i + s], keep = upper ? v[i + s] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, s);
+    }
+  }
+  return v[0];
+}
+
+template <typename T, typename Out, int L>
+__global__ void __launch_bounds__(EXPAND_THREADS, L <= 8 ? 6 : 3)
+adapter_expand_kernel(const float* base, int planes, long long plane_stride, long long ldb, const float* low,
+                      const T* b, const int* index, int slots, int rank, int tokens, int N, Out* out,
+                      long long ldo) {
+  constexpr int EACH = 16 / sizeof(T), ROUNDS = ROUNDS_OF<L>, GROUPS = 32 / L;
+  extern __shared__ __align__(16) float mine[];  // [EXPAND_TOKENS][rank]
+  __shared__ int s_slot[EXPAND_TOKENS];
   fb_pdl_wait();
-  fb_pdl_launch();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
-  const int t0 = blockIdx.y * TOKENS, n0 = blockIdx.x * FEATURES;
-  if (warp == 0) {  // the adapters of these tokens, each once
-    int slot = t0 + lane < T ? index[t0 + lane] : -1;
-    if (slot >= slots) slot = -1;
-    s_index[lane] = slot;
-    const unsigned same = __match_any_sync(0xffffffffu, slot);
-    const bool first = slot >= 0 && __ffs(same) - 1 == lane;
-    const unsigned firsts = __ballot_sync(0xffffffffu, first);
-    if (first) s_slots[__popc(firsts & ((1u << lane) - 1))] = slot;
-    if (lane == 0) s_count = __popc(firsts);
+  const int tid = threadIdx.x, lane = tid & 31, li = lane % L, group = lane / L;
+  const int t0 = blockIdx.y * EXPAND_TOKENS, live = min(EXPAND_TOKENS, tokens - t0);
+  const int n0 = (blockIdx.x * (EXPAND_THREADS / 32) + (tid >> 5)) * 32 * ROUNDS;
+  if (tid < EXPAND_TOKENS) {
+    const int slot = tid < live ? index[t0 + tid] : -1;
+    s_slot[tid] = slot < slots ? slot : -1;
   }
-  __syncthreads();
-  for (int i = tid; i < TOKENS * (rank / 4); i += EXPAND_THREADS) {
-    const int t = i / (rank / 4), j = i % (rank / 4) * 4;
-    if (s_index[t] < 0) continue;  // (no adapter takes its row)
-    const float4 f = __ldcg(reinterpret_cast<const float4*>(low + (size_t)(t0 + t) * rank + j));
-    __nv_bfloat162* to = reinterpret_cast<__nv_bfloat162*>(u + t * ld + j);
-    to[0] = __floats2bfloat162_rn(f.x, f.y);
-    to[1] = __floats2bfloat162_rn(f.z, f.w);
-  }
-  __syncthreads();
-  float acc[TOKENS / 8][4];
+  // what the projection left for this lane's features
+  float sum[EXPAND_TOKENS][ROUNDS];
 #pragma unroll
-  for (int n = 0; n < TOKENS / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-  const int row0 = min(n0 + warp * 16 + g, N - 1), row1 = min(n0 + warp * 16 + g + 8, N - 1);
-  const int per = (rank + 15) / 16, steps = s_count * per;
-  for (int s0 = 0; s0 < steps; s0 += STEPS) {
-    uint2 w[STEPS][2];
+  for (int t = 0; t < EXPAND_TOKENS; ++t)
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-      const int e = (s0 + i) / per, k = (s0 + i - e * per) * 16 + 4 * q;
-      w[i][0] = w[i][1] = make_uint2(0u, 0u);
-      if (s0 + i < steps && k < rank) {
-        const __nv_bfloat16* from = b + (size_t)s_slots[e] * N * rank + k;
-        w[i][0] = __ldcg(reinterpret_cast<const uint2*>(from + (size_t)row0 * rank));
-        w[i][1] = __ldcg(reinterpret_cast<const uint2*>(from + (size_t)row1 * rank));
+    for (int r = 0; r < ROUNDS; ++r) {
+      const int n = n0 + r * 32 + li * GROUPS + group;
+      sum[t][r] = t < live && n < N ? __ldcg(base + (size_t)(t0 + t) * ldb + n) : 0.f;
+    }
+  for (int i = tid; i < live * rank / 4; i += EXPAND_THREADS)  // (rows of tokens without an adapter go unused)
+    reinterpret_cast<float4*>(mine)[i] = __ldcg(reinterpret_cast<const float4*>(low + (size_t)t0 * rank) + i);
+#pragma unroll 2
+  for (int p = 1; p < planes; ++p)
+#pragma unroll
+    for (int t = 0; t < EXPAND_TOKENS; ++t)
+#pragma unroll
+      for (int r = 0; r < ROUNDS; ++r) {
+        const int n = n0 + r * 32 + li * GROUPS + group;
+        if (t < live && n < N) sum[t][r] += __ldcg(base + (size_t)p * plane_stride + (size_t)(t0 + t) * ldb + n);
+      }
+  __syncthreads();
+  auto row_at = [&](int slot, int r, int i) {  // (features past the last one read the last one's row)
+    return b + ((size_t)slot * N + min(n0 + r * 32 + i * GROUPS + group, N - 1)) * rank;
+  };
+  if constexpr (L <= 8) {  // four or eight rows a lane, kept from token to token as they are stored
+    uint4 raw[ROUNDS * L];
+    int there = -1;
+#pragma unroll
+    for (int t = 0; t < EXPAND_TOKENS; ++t) {
+      const int slot = s_slot[t];
+      if (slot < 0) continue;
+      const bool in = li * EACH < rank;
+      if (slot != there) {
+#pragma unroll
+        for (int i = 0; i < ROUNDS * L; ++i)
+          raw[i] = in ? ld16(row_at(slot, i / L, i % L) + li * EACH) : make_uint4(0u, 0u, 0u, 0u);
+        there = slot;
+      }
+      float f[EACH];
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) f[e] = in ? mine[t * rank + li * EACH + e] : 0.f;
+#pragma unroll
+      for (int r = 0; r < ROUNDS; ++r) {
+        float v[L];
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+          float w[EACH];
+          unpack<T>(raw[r * L + i], w);
+          v[i] = w[0] * f[0];
+#pragma unroll
+          for (int e = 1; e < EACH; ++e) v[i] = fmaf(w[e], f[e], v[i]);
+        }
+        sum[t][r] += share_out<L>(v, li);
       }
     }
+  } else {
+    for (int t = 0; t < live; ++t) {
+      const int slot = s_slot[t];
+      if (slot < 0) continue;
+      float v[L];
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-      if (s0 + i >= steps) break;
-      const int e = (s0 + i) / per, k = (s0 + i - e * per) * 16 + 4 * q, slot = s_slots[e];
+      for (int i = 0; i < L; ++i) v[i] = 0.f;
+      for (int j = li * EACH; j - li * EACH < rank; j += L * EACH) {
+        const bool in = j < rank;
+        float f[EACH];
 #pragma unroll
-      for (int n = 0; n < TOKENS / 8; ++n) {
-        const int t = n * 8 + g;
-        uint2 v = make_uint2(0u, 0u);
-        if (s_index[t] == slot && k < rank) v = *reinterpret_cast<const uint2*>(u + t * ld + k);
-        mma_bf16(acc[n], w[i][0].x, w[i][1].x, w[i][0].y, w[i][1].y, v.x, v.y);
+        for (int e = 0; e < EACH; ++e) f[e] = in ? mine[t * rank + j + e] : 0.f;
+#pragma unroll
+        for (int i0 = 0; i0 < L; i0 += 8) {
+          uint4 raw[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) raw[i] = in ? ld16(row_at(slot, 0, i0 + i) + j) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float w[EACH];
+            unpack<T>(raw[i], w);
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) v[i0 + i] = fmaf(w[e], f[e], v[i0 + i]);
+          }
+        }
       }
+      const float whole = share_out<L>(v, li);
+#pragma unroll
+      for (int q = 0; q < EXPAND_TOKENS; ++q)  // (registers have no runtime index)
+        if (q == t) sum[q][0] += whole;
     }
   }
 #pragma unroll
-  for (int n = 0; n < TOKENS / 8; ++n) {
-    sums[n * 8 + 2 * q][warp * 16 + g] = acc[n][0];
-    sums[n * 8 + 2 * q + 1][warp * 16 + g] = acc[n][1];
-    sums[n * 8 + 2 * q][warp * 16 + g + 8] = acc[n][2];
-    sums[n * 8 + 2 * q + 1][warp * 16 + g + 8] = acc[n][3];
-  }
-  __syncthreads();
-  const bool four = (((uintptr_t)base | (uintptr_t)out) % 16) == 0 && ldb % 4 == 0 && plane_stride % 4 == 0 &&
-                    ldo % 4 == 0 && n0 + FEATURES <= N;
-  if (four) {
-    constexpr int GROUPS = FEATURES / 4;
+  for (int t = 0; t < EXPAND_TOKENS; ++t)
 #pragma unroll
-    for (int i0 = 0; i0 < TOKENS * GROUPS; i0 += EXPAND_THREADS) {
-      const int t = (i0 + tid) / GROUPS, f = (i0 + tid) % GROUPS * 4;
-      if (t0 + t >= T) continue;
-      float4 v = *reinterpret_cast<const float4*>(&sums[t][f]);
-      for (int p = 0; p < planes; ++p) {
-        const float4 o = __ldcg(reinterpret_cast<const float4*>(base + (size_t)p * plane_stride + (size_t)(t0 + t) * ldb + n0 + f));
-        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-      }
-      Out* to = out + (size_t)(t0 + t) * ldo + n0 + f;
-      if constexpr (sizeof(Out) == 4) {
-        *reinterpret_cast<float4*>(to) = v;
-      } else {
-        uint2 pk;
-        const __nv_bfloat162 h0 = __floats2bfloat162_rn(v.x, v.y), h1 = __floats2bfloat162_rn(v.z, v.w);
-        pk.x = *reinterpret_cast<const uint32_t*>(&h0);
-        pk.y = *reinterpret_cast<const uint32_t*>(&h1);
-        *reinterpret_cast<uint2*>(to) = pk;
-      }
+    for (int r = 0; r < ROUNDS; ++r) {
+      const int n = n0 + r * 32 + li * GROUPS + group;
+      if (t < live && n < N) out[(size_t)(t0 + t) * ldo + n] = fb_from_float<Out>(sum[t][r]);
     }
-    return;
-  }
-  for (int i = tid; i < TOKENS * FEATURES; i += EXPAND_THREADS) {
-    const int t = i / FEATURES, f = i % FEATURES;
-    if (t0 + t >= T || n0 + f >= N) continue;
-    float v = sums[t][f];
-    for (int p = 0; p < planes; ++p) v += __ldcg(base + (size_t)p * plane_stride + (size_t)(t0 + t) * ldb + n0 + f);
-    out[(size_t)(t0 + t) * ldo + n0 + f] = fb_from_float<Out>(v);
-  }
+}
+
+template <typename T, typename Out, int L>
+void launch_expand(const float* base, int planes, long long plane_stride, long long ldb, const float* low,
+                   const T* b, const int* index, int slots, int rank, int tokens, int N, Out* out, long long ldo,
+                   cudaStream_t stream) {
+  constexpr int FEATURES = EXPAND_THREADS * ROUNDS_OF<L>;
+  const dim3 grid((N + FEATURES - 1) / FEATURES, (tokens + EXPAND_TOKENS - 1) / EXPAND_TOKENS);
+  fb_launch(adapter_expand_kernel<T, Out, L>, grid, dim3(EXPAND_THREADS), (size_t)EXPAND_TOKENS * rank * 4, stream,
+            base, planes, plane_stride, ldb, low, b, index, slots, rank, tokens, N, out, ldo);
+}
+
+// As many lanes a row of B as it has pieces of 16 bytes (a power of two, 32 at most).
+template <typename T, typename Out>
+void expand_by_rank(const float* base, int planes, long long plane_stride, long long ldb, const float* low,
+                    const T* b, const int* index, int slots, int rank, int tokens, int N, Out* out,
+                    long long ldo, cudaStream_t stream) {
+  const int pieces = rank / (16 / (int)sizeof(T));
+#define FB_EXPAND(L) \
+  launch_expand<T, Out, L>(base, planes, plane_stride, ldb, low, b, index, slots, rank, tokens, N, out, ldo, stream)
+  if (pieces <= 1) FB_EXPAND(1);
+  else if (pieces <= 2) FB_EXPAND(2);
+  else if (pieces <= 4) FB_EXPAND(4);
+  else if (pieces <= 8) FB_EXPAND(8);
+  else if (pieces <= 16) FB_EXPAND(16);
+  else FB_EXPAND(32);
+#undef FB_EXPAND
 }
 }  // namespace
 
@@ -261,39 +300,21 @@ FB_API int fb_adapter_shrink(const void* x, long long ldx, int dtype, const void
   if (T == 0) return 0;
   const int each = dtype == FB_BF16 ? 8 : 4;
   const int wide = K % each == 0 && ldx % each == 0 && (((uintptr_t)x | (uintptr_t)a) % 16) == 0;
-  const dim3 grid((rank + THREADS / 32 - 1) / (THREADS / 32), T);
-  FB_DISPATCH_DTYPE(dtype, E, fb_launch(adapter_shrink_kernel<E>, grid, dim3(THREADS), 0, stream, (const E*)x,
-                                        ldx, (const E*)a, scales, index, slots, rank, K, wide, low));
+  FB_DISPATCH_DTYPE(dtype, E, shrink_by_size((const E*)x, ldx, (const E*)a, scales, index, slots, rank, T, K, wide,
+                                             low, stream));
   return fb_check_launch("adapter_shrink");
 }
 
 FB_API int fb_adapter_expand(const float* base, int planes, long long plane_stride, long long ldb,
                              const float* low, const void* b, int dtype, const int* index, int slots, int rank,
                              int T, int N, void* out, int out_dtype, long long ldo, cudaStream_t stream) {
-  FB_REQUIRE(T >= 0 && N > 0 && rank > 0 && rank <= 1024 && rank % 8 == 0 && slots > 0 && planes > 0 &&
-                 ldb >= N && ldo >= N && ((uintptr_t)b % 16) == 0,
-             "adapter_expand: bad sizes T=%d N=%d rank=%d, or B not on a 16-byte boundary", T, N, rank);
-  FB_REQUIRE(T <= 65535, "adapter_expand: %d tokens (65535 at most)", T);
-  if (T == 0) return 0;
-  const dim3 grid((N + THREADS - 1) / THREADS, T);
-  FB_DISPATCH_DTYPE(dtype, E, FB_DISPATCH_DTYPE(out_dtype, O,
-      fb_launch(adapter_expand_kernel<E, O>, grid, dim3(THREADS), (size_t)rank * 4, stream, base, planes,
-                plane_stride, ldb, low, (const E*)b, index, slots, rank, N, (O*)out, ldo)));
-  return fb_check_launch("adapter_expand");
-}
-
-// As fb_adapter_expand for bfloat16 adapters, on the tensor cores.
-FB_API int fb_adapter_expand_mma(const float* base, int planes, long long plane_stride, long long ldb,
-                                 const float* low, const void* b, const int* index, int slots, int rank, int T,
-                                 int N, void* out, int out_dtype, long long ldo, cudaStream_t stream) {
-  FB_REQUIRE(T > 0 && N > 0 && rank > 0 && rank <= 512 && rank % 8 == 0 && slots > 0 && planes > 0 && ldb >= N &&
+  FB_REQUIRE(T >= 0 && N > 0 && rank > 0 && rank <= 512 && rank % 8 == 0 && slots > 0 && planes > 0 && ldb >= N &&
                  ldo >= N && (((uintptr_t)b | (uintptr_t)low) % 16) == 0,
-             "adapter_expand_mma: bad sizes T=%d N=%d rank=%d, or operands not on 16-byte boundaries", T, N, rank);
-  FB_REQUIRE((T + TOKENS - 1) / TOKENS <= 65535, "adapter_expand_mma: %d tokens", T);
-  const size_t shared = TOKENS * (FEATURES + 4) * 4 + (size_t)TOKENS * (rank + 8) * 2;  // (42 KB at rank 512)
-  const dim3 grid((N + FEATURES - 1) / FEATURES, (T + TOKENS - 1) / TOKENS);
-  FB_DISPATCH_DTYPE(out_dtype, O,
-      fb_launch(adapter_expand_mma_kernel<O>, grid, dim3(EXPAND_THREADS), shared, stream, base, planes,
-                plane_stride, ldb, low, (const __nv_bfloat16*)b, index, slots, rank, T, N, (O*)out, ldo));
-  return fb_check_launch("adapter_expand_mma");
+             "adapter_expand: bad sizes T=%d N=%d rank=%d, or operands not on 16-byte boundaries", T, N, rank);
+  FB_REQUIRE(T <= 4 * 65535, "adapter_expand: %d tokens (262140 at most)", T);
+  if (T == 0) return 0;
+  FB_DISPATCH_DTYPE(dtype, E, FB_DISPATCH_DTYPE(out_dtype, O,
+      expand_by_rank(base, planes, plane_stride, ldb, low, (const E*)b, index, slots, rank, T, N, (O*)out, ldo,
+                     stream)));
+  return fb_check_launch("adapter_expand");
 }

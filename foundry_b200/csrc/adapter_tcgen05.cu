@@ -23,7 +23,8 @@ struct LowSmem {
   static constexpr int X_BYTES = BM * BK * 2;
   static constexpr int STAGE_BYTES = X_BYTES + RB * BK * 2;
   static constexpr int PART_BYTES = BM * (RB + 1) * 4;  // this CTA's share of K
-  static constexpr int STAGES = 7;
+  // two CTAs an SM: the start and the end of one beside the stream of the other
+  static constexpr int STAGES = RB <= 32 ? 4 : 3;
   static constexpr int BYTES = STAGES * STAGE_BYTES + 1024 /*align*/ + PART_BYTES + 256;
 };
 
@@ -44,7 +45,7 @@ __device__ __forceinline__ float ld_peer(const float* mine, unsigned rank) {
 // is 256 tokens, and every adapter of it gets a plane of bfloat16 rows, zero in those of others; else a
 // block is the tile, and a token's own rank numbers go to its row of `low`.
 template <int RB, bool PLANES>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(THREADS, 2)
 adapter_low_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a,
                    const float* scales, const int* index, int slots, int rank, int T, int K, int most,
                    __nv_bfloat16* u, int* counts, int* slots_of, float* low) {

@@ -123,8 +123,6 @@ _SIGNATURES = {
                           c_int, c_void_p, c_void_p],
     "fb_adapter_low": [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                        c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
-    "fb_adapter_expand_mma": [c_void_p, c_int, c_ll, c_ll, c_void_p, c_void_p, c_void_p, c_int,
-                              c_int, c_int, c_int, c_void_p, c_int, c_ll, c_void_p],
     "fb_gemm_tc_adapted": [c_void_p, c_ll, c_int, c_void_p, c_ll, c_int, c_int, c_void_p, c_void_p,
                            c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_ll, c_int,
                            c_void_p, c_ll, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_float,
@@ -2196,23 +2194,24 @@ def _low_fits(x: torch.Tensor, w: torch.Tensor, bank: AdapterBank) -> bool:
             and bank.slots <= MAX_ADAPTER_SLOTS and _tc_usable(x, w, w))
 
 
-def _planes_pay(T: int, N: int, K: int) -> bool:
-    """Whether adapters ride behind the projection's own K: where that runs as the paired product
-    anyway. (Where it would not, the paired form costs more than the two launches it saves: 4,096 ->
-    4,096 with rank 16 in graph replays, 128 tokens.)"""
-    if not (PAIRED and PERSISTENT) or N < 128 or T <= 128:
-        return False
-    return not (T <= ONE_TILE_ROWS and _one_tile_plan(T, N, K)[1])
+def _planes_pay(T: int, N: int) -> bool:
+    """Whether adapters ride behind the projection's own K in the paired product. Otherwise the
+    projection's best form leaves its 32-bit sums to be read again, T * N of them; the paired one, which is
+    not the best for few tokens, saves that (4,096 -> 4,096, rank 16: 256 tokens 25 us against 31, 512
+    41 against 34; 4,096 -> 28,672, rank 32: 48 tokens 61 against 64, 128 86 against 66)."""
+    return PAIRED and PERSISTENT and N >= 128 and T > 64 and T * N >= 3 << 19
 
 
 def _adapter_low(x: torch.Tensor, bank: AdapterBank, index: torch.Tensor, most: int, u: int, counts: int,
                  slots: int, low: int) -> None:
     T, K = x.shape
     tiles = (T + 127) // 128
-    side = max(1, min(most, sm_count() // tiles))
-    shares = 1
-    while shares < 8 and 2 * shares * tiles * side <= sm_count() and K >= 256 * shares:
-        shares *= 2
+    # two CTAs fit an SM; K in eight shares of two blocks of 64 at least, then the adapters side by side
+    # (2,048 tokens of 4,096, rank 48, one or two adapters a block: 8 x 2 9.9 us, 8 x 1 14.8, 4 x 2 11.8)
+    shares = 8
+    while shares > 1 and (tiles * shares > 2 * sm_count() or K < 128 * shares):
+        shares //= 2
+    side = max(1, min(most, 2 * sm_count() // (tiles * shares)))
     _call("fb_adapter_low", x.data_ptr(), _rows(x, "x"), bank.a.data_ptr(), bank.scales.data_ptr(),
           index.data_ptr(), bank.slots, bank.rank, T, K, most, side, shares, u, counts, slots, low,
           _stream(), tag=("t{} k{} r{}", T, K, bank.rank))
@@ -2242,8 +2241,8 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
                     out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """y[t] = x[t] w^T + scale_a (x[t] a_a^T) b_a^T with a = index[t] (int32, one a token; outside of
     the bank: no adapter). Sums are 32-bit and y is rounded once, to `out_dtype` (the input's type);
-    in bfloat16 with more than 16 tokens the rank numbers are rounded to bfloat16 for the tensor
-    cores (csrc/adapter.cu says which kernels run)."""
+    where the projection runs as the paired tcgen05 product (hundreds of tokens) the rank numbers are
+    rounded to bfloat16 for it (csrc/adapter.cu says which kernels run)."""
     x = plain(x)
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
         raise KernelError(f"adapted_product: x {tuple(x.shape)}, w {tuple(w.shape)}")
@@ -2273,11 +2272,13 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
                                                        index[t:t + ADAPTER_PIECE], out.dtype)
         return out
     on_tensor_cores = _low_fits(x, w, bank)
-    if on_tensor_cores and _planes_pay(T, N, K):
+    if on_tensor_cores and _planes_pay(T, N):
         _adapted_planes(x, w, bank, index, out)
         return out
     low = torch.empty((T, bank.rank), dtype=torch.float32, device=device)
-    if on_tensor_cores:
+    # up to this many rank numbers one warp a number is ahead (64 tokens x 64 ranks of 4,096: 6.9 us
+    # against 12; 256 x 64: 14.3 against 12.3; 512 x 16: 9.1 against 7.3)
+    if on_tensor_cores and T * bank.rank > 8192:
         _adapter_low(x, bank, index, min(bank.slots, 128, T), 0, 0, 0, low.data_ptr())
     else:
         _call("fb_adapter_shrink", x.data_ptr(), _rows(x, "x"), code_of(x.dtype), a, scales, which,
@@ -2290,11 +2291,6 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
     planes = 1
     if isinstance(base, Planes):
         planes, base = base.count, base.tensor
-    if on_tensor_cores:
-        _call("fb_adapter_expand_mma", base.data_ptr(), planes, T * N, N, low.data_ptr(), b, which,
-              bank.slots, bank.rank, T, N, out.data_ptr(), code_of(out.dtype), N, _stream(),
-              tag=("t{} n{} r{}", T, N, bank.rank))
-        return out
     _call("fb_adapter_expand", base.data_ptr(), planes, T * N, N, low.data_ptr(), b, code_of(x.dtype),
           which, bank.slots, bank.rank, T, N, out.data_ptr(), code_of(out.dtype), N, _stream(),
           tag=("t{} n{} r{}", T, N, bank.rank))
