@@ -9,6 +9,8 @@
 //   has tokens in the block (zero in the rows of others), and the product takes them as more K behind its
 //   own, [x | planes] [W | B]^T: one sum in tensor memory, one rounding (gemm_tcgen05_pair.cu, MoreK). The
 //   rank numbers are rounded to bfloat16 for that, 2^-9 of the adapter's part on average.
+//   Up to 16 tokens, bfloat16: `adapter_shrink` leaves them as 32-bit rows, and the weight-streaming product
+//   adds their product with B in its epilogue (gemm_skinny.cu, MODE_ADAPT). Nothing is rounded in between.
 //   Else: `adapter_shrink` (or, for many numbers, `adapter_low`) leaves them as 32-bit rows, the projection
 //   leaves 32-bit sums (split-K planes), and `adapter_expand` adds up sums and adapters and rounds once.
 #include "common.cuh"
@@ -107,7 +109,8 @@ void shrink_by_size(const T* x, long long ldx, const T* a, const float* scales, 
   const int rounds = K / (32 * (16 / (int)sizeof(T)));  // of a warp's loads: four go out together
   if (rounds <= 8) launch_shrink<T, 1>(x, ldx, a, scales, index, slots, rank, tokens, K, wide, low, stream);
   else if (rounds <= 16) launch_shrink<T, 2>(x, ldx, a, scales, index, slots, rank, tokens, K, wide, low, stream);
-  else launch_shrink<T, 4>(x, ldx, a, scales, index, slots, rank, tokens, K, wide, low, stream);
+  else if (rounds <= 32) launch_shrink<T, 4>(x, ldx, a, scales, index, slots, rank, tokens, K, wide, low, stream);
+  else launch_shrink<T, 8>(x, ldx, a, scales, index, slots, rank, tokens, K, wide, low, stream);
 }
 
 // out[t, n] = sum over the planes of base[., t, n] + sum_j low[t, j] B[a][n, j].

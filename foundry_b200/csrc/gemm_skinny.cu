@@ -141,9 +141,19 @@ constexpr int MODE_ROPE = 1;   // rotate and write queries, keys, values
 constexpr int MODE_SINK = 2;   // add into the residual rows in front of a norm
 constexpr int MODE_MANY = 3;   // store; the grid holds several products
 constexpr int MODE_CLAMP = 4;  // (gate, up) pairs with clamped halves and biases
+constexpr int MODE_ADAPT = 5;  // store, each token's low-rank adapter added (adapter.cu)
+// What MODE_ADAPT adds to feature n of token t: sum_j low[t, j] b[index[t]][n, j] (an index outside of
+// the bank: nothing), in front of the row scale.
+struct AdapterAdd {
+  const float* low;         // [T, rank]
+  const __nv_bfloat16* b;   // [slots, N, rank]
+  const int* index;         // [T]
+  int slots, rank;          // rank: a multiple of 8
+};
 template <int MODE> struct EndArg { using type = NoSink; };
 template <> struct EndArg<MODE_SINK> { using type = ResidualSink; };
 template <> struct EndArg<MODE_CLAMP> { using type = FbGluClamp; };
+template <> struct EndArg<MODE_ADAPT> { using type = AdapterAdd; };
 
 // NT: token tiles of 8 (1 or 2). WARPS: warps per CTA, each with a K range.
 // UNROLL: chunks whose loads are in flight together.
@@ -484,6 +494,48 @@ gemm_skinny_kernel(const __nv_bfloat16* x, long long ldx,
       out_h[(size_t)tok * ldo + (row >> 1)] =
           __float2bfloat16_rn(fb_glu_clamped(sink, gate * rs + b0, up * rs + b1));
     }
+  } else if constexpr (MODE == MODE_ADAPT) {
+    // Neighbouring lanes share a row of b, 16 bytes each and round; as many as there are threads for the
+    // 16 * T sums, and pieces in a row.
+    const int pieces = sink.rank >> 3;
+    int lanes = 1;
+    while (lanes < 32 && lanes < pieces && 2 * lanes * 16 * T <= WARPS * 32) lanes *= 2;
+    const int part = lane & (lanes - 1);
+    for (int at = threadIdx.x / lanes; at < (16 * T + 31) / 32 * 32; at += WARPS * 32 / lanes) {  // (whole warps)
+      const int row = at & 15, tok = at >> 4;
+      const bool live = tok < T && n0 + row < N;
+      const int slot = live ? *reinterpret_cast<const volatile int*>(sink.index + tok) : -1;
+      float v = 0.f;
+      if (slot >= 0 && slot < sink.slots) {
+        const __nv_bfloat16* brow = sink.b + ((size_t)slot * N + n0 + row) * sink.rank;
+        const float* low = sink.low + (size_t)tok * sink.rank;
+        for (int i = part; i < pieces; i += lanes) {
+          const uint4 q = ld_cached(brow + i * 8);
+          const uint4 lo = ld_cached(low + i * 8), hi = ld_cached(low + i * 8 + 4);
+          const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
+          const float* f0 = reinterpret_cast<const float*>(&lo);
+          const float* f1 = reinterpret_cast<const float*>(&hi);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 b0 = __bfloat1622float2(h[e]), b1 = __bfloat1622float2(h[e + 2]);
+            v = fmaf(f0[2 * e], b0.x, v);
+            v = fmaf(f0[2 * e + 1], b0.y, v);
+            v = fmaf(f1[2 * e], b1.x, v);
+            v = fmaf(f1[2 * e + 1], b1.y, v);
+          }
+        }
+      }
+      for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (live && part == 0) {
+        float whole = 0.f;
+#pragma unroll
+        for (int wi = 0; wi < WARPS; ++wi) whole += red[wi][row][tok];
+        v = (whole + v) * row_scale(tok);
+        const size_t o = (size_t)tok * ldo + n0 + row;
+        if (out_f32) out_f[o] = v;
+        else out_h[o] = __float2bfloat16_rn(v);
+      }
+    }
   } else {
     if (epilogue == 0 || epilogue == 5) {
       for (int idx = threadIdx.x; idx < 16 * T; idx += WARPS * 32) {
@@ -527,7 +579,8 @@ int launch_skinny(const void* x, long long ldx, const void* w, long long ldw, vo
                   long long next_bytes, int ksplit, long long plane_stride, int warps,
                   int late_trigger, const RopeWrite& rw, const RowScale& scale,
                   const ResidualSink& sink, cudaStream_t stream,
-                  MoreProducts more = MoreProducts{}, const FbGluClamp& clamp = FbGluClamp{}) {
+                  MoreProducts more = MoreProducts{}, const FbGluClamp& clamp = FbGluClamp{},
+                  const AdapterAdd& adapter = AdapterAdd{}) {
   FB_REQUIRE(next_bytes >= 0 && next_bytes % 16 == 0 && ((uintptr_t)next % 16) == 0,
              "gemm_skinny: the prefetch range must be 16-byte aligned and a multiple of 16 bytes");
   FB_REQUIRE(T > 0 && T <= 16 && N > 0 && K > 0, "gemm_skinny: bad sizes T=%d N=%d K=%d", T, N, K);
@@ -582,6 +635,7 @@ int launch_skinny(const void* x, long long ldx, const void* w, long long ldw, vo
     if (epilogue == 2) FB_SKINNY_R(NT, W, U, MODE_ROPE, rw, NoSink{}, NoMore{});            \
     else if (epilogue == 3) FB_SKINNY_R(NT, W, U, MODE_SINK, NoRope{}, sink, NoMore{});     \
     else if (epilogue == 6) FB_SKINNY_R(NT, W, U, MODE_CLAMP, NoRope{}, clamp, NoMore{});   \
+    else if (adapter.low != nullptr) FB_SKINNY_R(NT, W, U, MODE_ADAPT, NoRope{}, adapter, NoMore{}); \
     else if (more.count > 0) FB_SKINNY_R(NT, W, U, MODE_MANY, NoRope{}, NoSink{}, more);      \
     else FB_SKINNY_R(NT, W, U, MODE_PLAIN, NoRope{}, NoSink{}, NoMore{});                   \
   } while (0)
@@ -736,4 +790,31 @@ FB_API int fb_gemm_skinny_rope(const void* x, long long ldx, const void* w, long
                        scale_dim > 0 ? 1.0f / (float)scale_dim : 0.f, scale_eps};
   return launch_skinny(x, ldx, w, ldw, q_out, q_stride, 0, T, (A + 2 * Kh) * D, K, 2, next,
                        next_bytes, 1, 0, warps, late_trigger, rw, scale, ResidualSink{}, stream);
+}
+
+// adapter.cu
+extern "C" int fb_adapter_shrink(const void* x, long long ldx, int dtype, const void* a, const float* scales,
+                                 const int* index, int slots, int rank, int T, int K, float* low,
+                                 cudaStream_t stream);
+
+// out[t] = scale of t's row * (x[t] w^T + scales[i] (x[t] a[i]^T) b[i]^T), i = index[t] (outside of the bank:
+// without the second part), for up to 16 tokens: two kernels, the rank numbers (low [T, rank] float32,
+// written here) and the product with them in its epilogue. a [slots, rank, K], b [slots, N, rank] bfloat16.
+// scale_*: as in fb_gemm_skinny.
+FB_API int fb_gemm_skinny_adapted(const void* x, long long ldx, const void* w, long long ldw, void* out,
+                                  long long ldo, int out_f32, int T, int N, int K, const void* a, const void* b,
+                                  const float* scales, const int* index, int slots, int rank, float* low,
+                                  const void* next, long long next_bytes, int warps, const float* scale_ss,
+                                  int scale_count, int scale_stride, int scale_dim, float scale_eps,
+                                  cudaStream_t stream) {
+  FB_REQUIRE(slots > 0 && rank > 0 && rank % 8 == 0 && a && b && scales && index && low &&
+                 (((uintptr_t)b | (uintptr_t)low) % 16) == 0,
+             "gemm_skinny_adapted: a bank of %d adapters of rank %d, or operands not on 16-byte boundaries", slots,
+             rank);
+  if (int rc = fb_adapter_shrink(x, ldx, FB_BF16, a, scales, index, slots, rank, T, K, low, stream)) return rc;
+  const RowScale scale{scale_ss, scale_count, scale_stride,
+                       scale_dim > 0 ? 1.0f / (float)scale_dim : 0.f, scale_eps};
+  return launch_skinny(x, ldx, w, ldw, out, ldo, out_f32, T, N, K, 0, next, next_bytes, 1, 0, warps, 1,
+                       RopeWrite{}, scale, ResidualSink{}, stream, MoreProducts{}, FbGluClamp{},
+                       AdapterAdd{low, (const __nv_bfloat16*)b, index, slots, rank});
 }

@@ -121,6 +121,10 @@ _SIGNATURES = {
                         c_void_p],
     "fb_adapter_shrink": [c_void_p, c_ll, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                           c_int, c_void_p, c_void_p],
+    "fb_gemm_skinny_adapted": [c_void_p, c_ll, c_void_p, c_ll, c_void_p, c_ll, c_int, c_int, c_int,
+                               c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p,
+                               c_void_p, c_ll, c_int, c_void_p, c_int, c_int, c_int, c_float,
+                               c_void_p],
     "fb_adapter_low": [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                        c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     "fb_gemm_tc_adapted": [c_void_p, c_ll, c_int, c_void_p, c_ll, c_int, c_int, c_void_p, c_void_p,
@@ -1920,26 +1924,26 @@ def select_tokens(logits: torch.Tensor, out: torch.Tensor, temperature: Optional
 
 
 # --------------------------------------------------- what a request brings of its own: logits
-def _given(t, name: str, dtype: torch.dtype, shape, device) -> int:
+def _given(t, name: str, dtype: torch.dtype, shape, device: int) -> int:
     """The address of a contiguous tensor that a caller hands over (None: 0): its type, its shape
-    (None: any), and the device of the call, which is the current one."""
+    (None: any), and the number of the call's device."""
     if t is None:
         return 0
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise KernelError(f"{name} has dtype {t.dtype}, expected {dtype}")
-    if shape is not None and tuple(t.shape) != shape:
+    if shape is not None and t.shape != shape:
         raise KernelError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
     if not t.is_contiguous():
         raise KernelError(f"{name} is not contiguous")
-    if t.device != device:
-        raise KernelError(f"{name} is on {t.device}, the call's rows are on {device}")
+    if t.get_device() != device:
+        raise KernelError(f"{name} is on {t.device}, the call's rows are on cuda:{device}")
     return t.data_ptr()
 
 
 def _on_current_device(t: torch.Tensor, name: str) -> None:
     if not t.is_cuda:
         raise KernelError(f"{name} is on {t.device}; the kernels run on CUDA devices only")
-    if t.device.index != _current_device():
+    if t.get_device() != _current_device():
         raise KernelError(f"{name} is on {t.device}, the current device is {_current_device()}")
 
 
@@ -1988,7 +1992,7 @@ def record_tokens(history: TokenHistory, rows: torch.Tensor, tokens: torch.Tenso
     if what not in _RECORD:
         raise KernelError(f"record_tokens: {what!r}; known: {sorted(_RECORD)}")
     _on_current_device(history.counts, "counts")
-    device, n = history.counts.device, tokens.numel()
+    device, n = history.counts.get_device(), tokens.numel()
     _call("fb_record_tokens",
           _given(history.counts, "counts", torch.int32, None, device),
           _given(history.seen, "seen", torch.int32, None, device), history.rows,
@@ -2095,7 +2099,7 @@ def edit_logits(logits: torch.Tensor, edits: LogitEdits,
         out = torch.empty((n, V), dtype=torch.float32, device=logits.device)
     elif out.shape != logits.shape or out.dtype != torch.float32 or out.device != logits.device:
         raise KernelError(f"edit_logits: out is {out.dtype} {tuple(out.shape)} on {out.device}")
-    packed = edits.packed(n, V, logits.device)
+    packed = edits.packed(n, V, logits.get_device())
     _call("fb_edit_logits", logits.data_ptr(), stride, n, V, out.data_ptr(),
           max(_rows(out, "out"), V) if n <= 1 else _rows(out, "out"), ctypes.addressof(packed),
           _stream(), tag=("n{} v{}", n, V))
@@ -2138,20 +2142,21 @@ def sample_tokens(logits: torch.Tensor, rules: SampleRules, edits: Optional[Logi
         logprobs = torch.empty(n, dtype=torch.float32, device=device)
     if record is not None and (edits is None or edits.history is None):
         raise KernelError("sample_tokens: tokens to record, and no history")
-    packed = None if edits is None else edits.packed(n, V, device)
+    at = logits.get_device()
+    packed = None if edits is None else edits.packed(n, V, at)
     r, each = rules, (n,)
     _call("fb_sample_rules", logits.data_ptr(), stride, n, V,
-          _given(r.temperature, "temperature", torch.float32, each, device),
-          _given(r.top_k, "top_k", torch.int32, each, device),
-          _given(r.top_p, "top_p", torch.float32, each, device),
-          _given(r.min_p, "min_p", torch.float32, each, device),
-          _given(r.streams, "streams", torch.int64, each, device),
-          _given(r.steps, "steps", torch.int64, each, device),
+          _given(r.temperature, "temperature", torch.float32, each, at),
+          _given(r.top_k, "top_k", torch.int32, each, at),
+          _given(r.top_p, "top_p", torch.float32, each, at),
+          _given(r.min_p, "min_p", torch.float32, each, at),
+          _given(r.streams, "streams", torch.int64, each, at),
+          _given(r.steps, "steps", torch.int64, each, at),
           0 if packed is None else ctypes.addressof(packed),
-          _given(record, "record", torch.int32, each, device),
-          _given(out, "out", torch.int32, each, device),
-          _given(logprobs, "logprobs", torch.float32, each, device),
-          _given(also, "also", torch.int32, each, device), _stream(), tag=("n{} v{}", n, V))
+          _given(record, "record", torch.int32, each, at),
+          _given(out, "out", torch.int32, each, at),
+          _given(logprobs, "logprobs", torch.float32, each, at),
+          _given(also, "also", torch.int32, each, at), _stream(), tag=("n{} v{}", n, V))
     return out, logprobs
 
 
@@ -2238,62 +2243,76 @@ def _adapted_planes(x: torch.Tensor, w: torch.Tensor, bank: AdapterBank, index: 
 
 
 def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
-                    out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+                    out_dtype: Optional[torch.dtype] = None,
+                    then_reads: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y[t] = x[t] w^T + scale_a (x[t] a_a^T) b_a^T with a = index[t] (int32, one a token; outside of
     the bank: no adapter). Sums are 32-bit and y is rounded once, to `out_dtype` (the input's type);
     where the projection runs as the paired tcgen05 product (hundreds of tokens) the rank numbers are
-    rounded to bfloat16 for it (csrc/adapter.cu says which kernels run)."""
-    x = plain(x)
-    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
-        raise KernelError(f"adapted_product: x {tuple(x.shape)}, w {tuple(w.shape)}")
-    (T, K), N = x.shape, w.shape[0]
-    if w.dtype != x.dtype:
-        raise KernelError(f"adapted_product: x is {x.dtype}, w is {w.dtype}")
-    if tuple(bank.a.shape[1:]) != (bank.rank, K) or tuple(bank.b.shape[1:]) != (N, bank.rank):
+    rounded to bfloat16 for it (csrc/adapter.cu says which kernels run). `x` may be a `RowScaled`;
+    `then_reads` names the weights that the step streams next, a hint."""
+    values = x.values if isinstance(x, RowScaled) else x
+    if values.dim() != 2 or w.dim() != 2 or values.shape[1] != w.shape[1]:
+        raise KernelError(f"adapted_product: x {tuple(values.shape)}, w {tuple(w.shape)}")
+    (T, K), N, dtype = values.shape, w.shape[0], values.dtype
+    slots, rank = bank.slots, bank.rank
+    if w.dtype != dtype:
+        raise KernelError(f"adapted_product: x is {dtype}, w is {w.dtype}")
+    if bank.a.shape[2] != K or bank.b.shape[1] != N:
         raise KernelError(f"adapted_product: adapters {tuple(bank.a.shape)}, {tuple(bank.b.shape)} beside "
                           f"a projection {tuple(w.shape)}")
-    _on_current_device(x, "x")
-    device = x.device
-    if w.device != device:
-        raise KernelError(f"w is on {w.device}, the call's rows are on {device}")
-    a = _given(bank.a, "a", x.dtype, None, device)
-    b = _given(bank.b, "b", x.dtype, None, device)
-    scales = _given(bank.scales, "scales", torch.float32, None, device)
-    which = _given(index, "index", torch.int32, (T,), device)
+    _on_current_device(values, "x")
+    at = values.get_device()
+    if w.get_device() != at:
+        raise KernelError(f"w is on {w.device}, the call's rows are on {values.device}")
+    a = _given(bank.a, "a", dtype, None, at)
+    b = _given(bank.b, "b", dtype, None, at)
+    scales = _given(bank.scales, "scales", torch.float32, None, at)
+    which = _given(index, "index", torch.int32, (T,), at)
     if (a | b) % 16:
         raise KernelError("adapted_product: the adapters must start on 16-byte boundaries")
-    out = torch.empty((T, N), dtype=out_dtype or x.dtype, device=device)
-    code_of(out.dtype)
+    out_dtype = out_dtype or dtype
+    code = code_of(out_dtype)
+    out = torch.empty((T, N), dtype=out_dtype, device=values.device)
     if T == 0:
         return out
+    bf16 = dtype == torch.bfloat16
+    if bf16 and T <= SKINNY_ROWS and _tc_usable(values, w, w):
+        low = torch.empty((T, rank), dtype=torch.float32, device=values.device)
+        scale, values = _scale_of(x)
+        _COUNT[0] += 1  # the rank numbers' kernel
+        _call("fb_gemm_skinny_adapted", values.data_ptr(), values.stride(0), w.data_ptr(), w.stride(0),
+              out.data_ptr(), N, 1 - code, T, N, K, a, b, scales, which, slots, rank, low.data_ptr(),
+              *_prefetch_range(then_reads), skinny_plan(N, K, False)[1], *scale, _stream(),
+              tag=("t{} n{} k{} r{}", T, N, K, rank))
+        return out
+    x = plain(x)
     if T > ADAPTER_PIECE:
         for t in range(0, T, ADAPTER_PIECE):
             out[t:t + ADAPTER_PIECE] = adapted_product(x[t:t + ADAPTER_PIECE], w, bank,
-                                                       index[t:t + ADAPTER_PIECE], out.dtype)
+                                                       index[t:t + ADAPTER_PIECE], out_dtype)
         return out
     on_tensor_cores = _low_fits(x, w, bank)
     if on_tensor_cores and _planes_pay(T, N):
         _adapted_planes(x, w, bank, index, out)
         return out
-    low = torch.empty((T, bank.rank), dtype=torch.float32, device=device)
+    low = torch.empty((T, rank), dtype=torch.float32, device=x.device)
     # up to this many rank numbers one warp a number is ahead (64 tokens x 64 ranks of 4,096: 6.9 us
     # against 12; 256 x 64: 14.3 against 12.3; 512 x 16: 9.1 against 7.3)
-    if on_tensor_cores and T * bank.rank > 8192:
-        _adapter_low(x, bank, index, min(bank.slots, 128, T), 0, 0, 0, low.data_ptr())
+    if on_tensor_cores and T * rank > 8192:
+        _adapter_low(x, bank, index, min(slots, 128, T), 0, 0, 0, low.data_ptr())
     else:
-        _call("fb_adapter_shrink", x.data_ptr(), _rows(x, "x"), code_of(x.dtype), a, scales, which,
-              bank.slots, bank.rank, T, K, low.data_ptr(), _stream(),
-              tag=("t{} k{} r{}", T, K, bank.rank))
-    if x.dtype == torch.float32:
-        base = gemm_simt(x, w, torch.empty((T, N), dtype=torch.float32, device=device))
-    else:
+        _call("fb_adapter_shrink", x.data_ptr(), _rows(x, "x"), code_of(dtype), a, scales, which,
+              slots, rank, T, K, low.data_ptr(), _stream(), tag=("t{} k{} r{}", T, K, rank))
+    if bf16:
         base = gemm_bf16(x, w, None, torch.float32, allow_planes=True)
+    else:
+        base = gemm_simt(x, w, torch.empty((T, N), dtype=torch.float32, device=x.device))
     planes = 1
     if isinstance(base, Planes):
         planes, base = base.count, base.tensor
-    _call("fb_adapter_expand", base.data_ptr(), planes, T * N, N, low.data_ptr(), b, code_of(x.dtype),
-          which, bank.slots, bank.rank, T, N, out.data_ptr(), code_of(out.dtype), N, _stream(),
-          tag=("t{} n{} r{}", T, N, bank.rank))
+    _call("fb_adapter_expand", base.data_ptr(), planes, T * N, N, low.data_ptr(), b, code_of(dtype),
+          which, slots, rank, T, N, out.data_ptr(), code, N, _stream(),
+          tag=("t{} n{} r{}", T, N, rank))
     return out
 
 

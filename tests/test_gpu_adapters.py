@@ -107,14 +107,23 @@ def test_no_tokens(ops):
     assert ops.adapted_product(x, w, bank, index).shape == (0, 32)
 
 
-def test_a_row_scaled_input(ops):
-    """What a norm leaves for the products behind it: the scale is applied first."""
-    T, K = 9, 512
+@pytest.mark.parametrize("T", [9, 16, 40])
+def test_a_row_scaled_input(ops, T):
+    """What a norm leaves for the products behind it: scale_t * values. A few tokens' product is linear in
+    the scale and takes it behind its sums; otherwise the rows are scaled first, and rounded again (2^-8 of
+    every factor, so of the products' absolute sum)."""
+    K = 512
     x, w, bank, index = case(ops, T, K, 256, 16, 3, torch.bfloat16)
-    shares = torch.rand(32, 16, device=DEV) * 40
+    shares = torch.rand(32, (T + 15) // 16 * 16, device=DEV) * 40
     scaled = ops.RowScaled(x.contiguous(), shares, 1e-5)
-    y = ops.adapted_product(scaled, w, bank, index)
-    check(ops, scaled.materialize(), w, bank, index, y, True)
+    y = ops.adapted_product(scaled, w, bank, index).float().cpu().numpy().astype(np.float64)
+    host = lambda t: t.float().cpu().numpy()  # noqa: E731
+    scale = 1 / np.sqrt(host(shares).astype(np.float64).sum(0)[:T] / K + 1e-5)
+    want, size, much = plain.adapted(host(x), host(w), host(bank.a), host(bank.b), host(bank.scales),
+                                     index.cpu().numpy())
+    want, size, much = (v * scale[:, None] for v in (want, size, much))
+    bound = plain.adapted_bound(want, size, much, K + bank.rank + 40, True) + (2.0 ** -8 * much if T > 16 else 0)
+    assert (np.abs(y - want) <= bound).all(), (np.abs(y - want) / bound).max()
 
 
 def test_on_another_stream_and_replayed(ops):

@@ -34,7 +34,7 @@ def test_edits_come_in_pairs():
 
 
 def test_edits_fit_the_rows():
-    cpu = torch.device("cpu")
+    cpu = -1  # the number of the CPU's tensors
     history = ops.TokenHistory(i32(2, 40), i32(2, 2))
     fits = ops.LogitEdits(history, i32(3), torch.ones(3), allowed=i32(1, 2), allowed_rows=i32(3))
     fits.packed(3, 40, cpu)
