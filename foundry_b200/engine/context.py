@@ -62,6 +62,9 @@ class StepContext:
     fresh: bool = False
     # The wanted rows are all rows, in their order (fixed when a step is captured)
     wants_every_row: bool = False
+    # int32 [n_tokens]: the place of each token's low-rank adapter in the parts' banks (-1: none),
+    # or None in a step of which no sequence has one
+    adapters: Optional[torch.Tensor] = None
     _tables: Dict[int, torch.Tensor] = field(default_factory=dict)
     # The weight that the step streams after the part being run (a prefetch
     # hint, set by the model and the blocks as they go; None = unknown).
@@ -193,9 +196,11 @@ def lengths_are_unequal(lengths: Sequence[int]) -> bool:
 
 def build_context(cache: SequenceCache, steps: Sequence[SequenceStep], vocab_size: int,
                   device: torch.device, max_positions: Optional[int] = None,
-                  plan: Optional[StepPlan] = None) -> StepContext:
+                  plan: Optional[StepPlan] = None,
+                  adapters: Optional[Sequence[int]] = None) -> StepContext:
     """Validate a step, reserve its cache pages, and upload its description
-    (or upload a step already planned)."""
+    (or upload a step already planned). `adapters`: the place of each sequence's
+    adapter, or None where no sequence has one."""
     if plan is None:
         plan = plan_step(cache, steps, vocab_size, max_positions)
     n_seqs, T = len(plan.slots), int(plan.token_ids.size)
@@ -206,6 +211,8 @@ def build_context(cache: SequenceCache, steps: Sequence[SequenceStep], vocab_siz
               np.asarray(plan.kv_lens, np.int32)]
     for _, _, rows in plan.tables:
         fields.append(np.asarray(rows, np.int32).reshape(-1))
+    if adapters is not None:
+        fields.append(np.repeat(np.asarray(adapters, np.int32), lens))
     offsets = np.cumsum([0] + [f.size for f in fields])
     packed = torch.from_numpy(np.concatenate(fields)).to(device)
     part = [packed[offsets[i]:offsets[i + 1]] for i in range(len(fields))]
@@ -219,4 +226,6 @@ def build_context(cache: SequenceCache, steps: Sequence[SequenceStep], vocab_siz
         fresh=all(plan.kv_lens[i] == lens[i] for i in range(n_seqs)))
     for i, (group, width, _) in enumerate(plan.tables):
         ctx._tables[id(group)] = part[7 + i].view(n_seqs, width)
+    if adapters is not None:
+        ctx.adapters = part[-1]
     return ctx

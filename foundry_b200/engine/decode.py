@@ -33,8 +33,10 @@ import torch
 
 from ..cache.pages import PAGE
 from ..kernels import ops
-from ..sampling.params import SamplingParams
+from ..sampling.params import SamplingParams, is_ruled, params_of_rows
+from ..sampling.rules import RowRules, bias_room, check_vocabulary
 from .context import StepContext, lengths_are_unequal
+from .generate import NoTokenLeft
 from .staging import StagingRing
 
 
@@ -47,16 +49,19 @@ def bucket_of(n: int) -> int:
 
 class DecodeRunner:
     """Fixed buffers and the captured graph for `bucket` rows and page tables
-    `width` pages wide."""
+    `width` pages wide. `rules`: None, or (room for biases, whether rows have masks, whether rows
+    have histories) of a step whose rows draw under rules of their own; `adapted`: rows may have an
+    adapter."""
 
-    def __init__(self, engine, bucket: int, width: int, unequal: bool = False):
+    def __init__(self, engine, bucket: int, width: int, unequal: bool = False, rules=None,
+                 adapted: bool = False):
         self.engine, self.bucket, self.width, self.unequal = engine, bucket, width, unequal
         dev = engine.device
         groups = engine.cache.groups
         b = bucket
         # packed int32 fields: token ids | positions | seq_of_token | want_rows | slots |
-        # cu_tokens | kv_lens | one page table per group
-        sizes = [b, b, b, b, b, b + 1, b] + [b * width for _ in groups]
+        # cu_tokens | kv_lens | one page table per group (| adapters)
+        sizes = [b, b, b, b, b, b + 1, b] + [b * width for _ in groups] + [b] * adapted
         offsets = [int(o) for o in np.cumsum([0] + sizes)]
         # the host may prepare steps ahead of the device: uploads go through a ring
         self.fields = StagingRing(offsets[-1], torch.int32, dev)
@@ -79,6 +84,15 @@ class DecodeRunner:
         for i, group in enumerate(groups):
             self.ctx._tables[id(group)] = part[7 + i].view(b, width)
         self.h_tables = [self.h[7 + i].reshape(b, width) for i in range(len(groups))]
+        if adapted:
+            self.ctx.adapters = part[-1]
+        self.adapted = adapted
+        self.rules = None
+        if rules is not None:
+            room, masks, histories = rules
+            self.rules = RowRules(b, engine.spec.vocab_size, dev,
+                                  engine.token_history() if histories else None, room, masks, ahead=True)
+        self.rules_of = None  # what the rules were last filled with
         self.row_sig: List[Optional[Tuple[int, int, int]]] = [None] * b
         self.filled_for: Optional[List[int]] = None  # the slots that the rows stand for
         self.h[3][:] = np.arange(b)  # every row's logits are wanted
@@ -90,6 +104,7 @@ class DecodeRunner:
         self.meta64 = self.sampling_fields.dev
         self.next_tokens = torch.zeros(b, dtype=torch.int32, device=dev)
         self.tokens_host = torch.zeros(b, dtype=torch.int32).pin_memory()
+        self.logprobs_host = torch.zeros(b, dtype=torch.float32).pin_memory()
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.kernels_per_step = 0
         self.kernel_histogram: Dict[str, int] = {}
@@ -100,6 +115,10 @@ class DecodeRunner:
         b = self.bucket
         with ops.scratch_owner(engine.scratch):
             self.logits = engine.model.forward(self.ctx, engine.cache)
+            if self.rules is not None:  # the step's inputs join the histories first
+                self.rules.draw(self.logits, self.next_tokens, record=self.ctx.token_ids,
+                                also=self.ctx.token_ids)
+                return
             ops.select_tokens(self.logits, self.next_tokens, self.temperature, self.meta64[:b],
                               self.meta64[b:], also=self.ctx.token_ids)
 
@@ -145,21 +164,33 @@ class DecodeRunner:
 class DecodeSession:
     """Decode steps of a set of open sequences, row i being `slots[i]`.
     `keys[i]` names row i's random stream and `counts[i]` is how many tokens
-    its sequence has generated (both only matter when sampling)."""
+    its sequence has generated (both only matter when sampling). `sampling`:
+    one `SamplingParams` for all rows, or one each."""
 
     def __init__(self, engine, slots: Sequence[int], sampling: SamplingParams = SamplingParams(),
                  keys: Optional[Sequence[int]] = None, counts: Optional[Sequence[int]] = None):
         from ..sampling.sampler import stream_key
         self.engine = engine
         self.slots = list(slots)
-        self.sampling = sampling
+        self.sampling = sampling if isinstance(sampling, SamplingParams) else list(sampling)
+        self.params = params_of_rows(sampling, len(self.slots))
         keys = list(keys) if keys is not None else list(range(len(slots)))
         self.keys = keys
-        self.streams = [stream_key(sampling.seed, k) for k in keys]
+        self.streams = [stream_key(p.seed, k) for p, k in zip(self.params, keys)]
+        self.rules = None  # what a runner of these rows needs (see DecodeRunner)
+        self.history_rows = [-1] * len(self.slots)
+        if is_ruled(self.sampling):
+            check_vocabulary(self.params, engine.spec.vocab_size)
+            self.rules = (bias_room(self.params), any(p.allowed_tokens is not None for p in self.params),
+                          any(p.needs_history for p in self.params))
+            self.history_rows = [engine.history_row(s) if p.needs_history else -1
+                                 for s, p in zip(self.slots, self.params)]
+        self.adapters = engine.adapters_of(self.slots)
         self.counts = list(counts) if counts is not None else [0] * len(slots)
         self.runner: Optional[DecodeRunner] = None
         self.h2d_bytes_per_step = 0
         self.d2h_bytes_per_step = 0
+        self.last_logprobs: List[float] = []
         self._ahead: Optional[dict] = None  # the step that was started on a guess
         self._read = torch.cuda.Event()     # behind the copy of a step's tokens to the host
 
@@ -186,7 +217,8 @@ class DecodeSession:
             while width < need:
                 width *= 2
             previous = runner
-            runner = self.runner = engine.decode_runner(bucket, width, unequal)
+            runner = self.runner = engine.decode_runner(bucket, width, unequal, self.rules,
+                                                        self.adapters is not None)
             if previous is not None and previous is not runner and previous.bucket == bucket:
                 # tokens that stay on the device (`step`) move on with the session
                 runner.ctx.token_ids.copy_(previous.next_tokens)
@@ -200,6 +232,9 @@ class DecodeSession:
             h[6][n:] = 0
             runner.row_sig[n:] = [None] * (bucket - n)
             runner.filled_for = list(slots)
+        if runner.adapted:  # (a slot may have been opened again with another)
+            h[-1][:n] = self.adapters
+            h[-1][n:] = -1
         h[1][:n] = lengths
         h[6][:n] = h[1][:n] + 1
         epoch = table.epoch
@@ -224,7 +259,18 @@ class DecodeSession:
             runner.host_np[n:runner.bucket] = 0
             start = 0
         self.h2d_bytes_per_step = runner.fields.upload(start)
-        temperature = float(self.sampling.temperature)
+        if runner.rules is not None:
+            filled = (self.params, self.history_rows)
+            if runner.rules_of != filled:
+                self.h2d_bytes_per_step += runner.rules.fill(*filled)
+                runner.rules_of = filled
+            if self.rules[1]:
+                self.h2d_bytes_per_step += runner.rules.set_masks(
+                    [None if p.allowed_tokens is None else p.allowed_tokens(self.engine.tokens_said(s))
+                     for s, p in zip(self.slots, self.params)])
+            self.h2d_bytes_per_step += runner.rules.set_steps(self.streams, self.counts)
+            return
+        temperature = float(self.params[0].temperature)
         if runner.temperature_value != temperature:
             runner.temperature.fill_(temperature)
             runner.temperature_value = temperature
@@ -243,6 +289,8 @@ class DecodeSession:
     def step(self) -> None:
         """One step whose input tokens are the previous step's choices, which
         stay on the device."""
+        if self.rules is not None and self.rules[1]:
+            raise ValueError("a grammar's masks depend on the tokens: use step_host")
         self.cancel_ahead()
         self._launch(getattr(self, "_pending_tokens", None))
         self._pending_tokens = None
@@ -265,6 +313,8 @@ class DecodeSession:
         engine, cache = self.engine, self.engine.cache
         if cache.state or not engine.model.replay_safe() or not engine.use_graphs:
             return False
+        if self.rules is not None and self.rules[1]:  # the next masks depend on this step's tokens
+            return False
         lengths = [cache.length(s) for s in self.slots]
         if any(n + 1 > engine.spec.max_positions for n in lengths):
             return False
@@ -279,10 +329,16 @@ class DecodeSession:
         if ahead is None:
             return
         table = self.engine.cache.table
-        for slot, epoch, length in ahead["slots"]:
+        unsaid = []  # (history row, the input token that the step recorded)
+        for (slot, epoch, length), token, row in zip(ahead["slots"], ahead["tokens"], self.history_rows):
             if table.slots.is_held(slot) and table.epoch[slot] == epoch \
                     and table.length[slot] == length + 1:
                 self.engine.cache.forget_from(slot, length)
+                if row >= 0:
+                    unsaid.append((row, token))
+        if unsaid:
+            pairs = torch.tensor(unsaid, dtype=torch.int32).t().contiguous().to(self.engine.device)
+            ops.record_tokens(self.engine.token_history(), pairs[0], pairs[1], "taken back")
         self.counts = list(ahead["counts"])
 
     def _started(self, tokens: List[int], counts: Optional[Sequence[int]] = None) -> DecodeRunner:
@@ -317,9 +373,15 @@ class DecodeSession:
         (sampling only). `more`: the caller expects to come back with the same
         rows and the tokens returned here, so the step after this one is
         started before this one's tokens are handed out."""
+        if self.rules is not None and self.rules[1]:
+            for slot, p, token in zip(self.slots, self.params, tokens):
+                if p.allowed_tokens is not None:
+                    self.engine.tokens_said(slot).append(int(token))
         runner = self._started([int(t) for t in tokens], counts)
         n = len(self.slots)
         runner.tokens_host[:n].copy_(runner.next_tokens[:n], non_blocking=True)
+        if runner.rules is not None:
+            runner.logprobs_host[:n].copy_(runner.rules.logprobs[:n], non_blocking=True)
         self._read.record()
         guess = None
         if more and self._may_run_ahead():
@@ -331,9 +393,14 @@ class DecodeSession:
         ops.raise_on_device_failure()
         self.d2h_bytes_per_step = n * 4
         out = runner.tokens_host[:n].tolist()
+        if runner.rules is not None:
+            self.last_logprobs = runner.logprobs_host[:n].tolist()
+            self.d2h_bytes_per_step = n * 8
         if guess is not None:
-            guess["tokens"] = out
+            guess["tokens"] = [max(t, 0) for t in out]  # (no token: the step was fed token 0)
             self._ahead = guess
+        if runner.rules is not None and min(out) < 0:
+            raise NoTokenLeft(f"row {out.index(min(out))}: what its sampling allows leaves no token")
         return out
 
     def logits(self) -> torch.Tensor:

@@ -11,17 +11,18 @@ from __future__ import annotations
 
 import itertools
 import weakref
-from typing import List, Optional, Sequence
+from typing import Dict, List, Optional, Sequence
 
 import torch
 
 from ..cache.store import SequenceCache
 from ..config import load_model_config
 from ..config.spec import ModelSpec
-from ..sampling import Sampler, SamplingParams
+from ..sampling import Sampler, SamplingParams, is_ruled, params_of_rows
 from ..weights.safetensors_io import WeightFiles
 from . import generate as loop
 from ..cache.pages import CacheFull
+from .adapters import AdapterStore
 from .context import SequenceStep, build_context, check_steps
 from .prompt import PromptRunners
 from .decode import DecodeRunner, DecodeSession
@@ -66,6 +67,12 @@ class Engine:
         self._graph_pool = None
         self._session = None
         self._prompts = None  # graphs of short prompt steps, made at the first one
+        self._history: Optional[ops.TokenHistory] = None  # made for the first row with a penalty
+        self._unread = set()  # slots whose row of the history is another sequence's
+        self._said: Dict[int, List[int]] = {}  # tokens generated, for rows with a grammar
+        self._last_logprobs: List[float] = []
+        self.adapters: Optional[AdapterStore] = None
+        self._adapter_of: Dict[int, int] = {}  # slot -> place of its adapter
         # scratch memory that kernels share between their CTAs is this engine's own
         self.scratch = ("engine", next(_ENGINE_NUMBERS))
         weakref.finalize(self, ops.release_scratch, self.scratch)
@@ -119,11 +126,75 @@ class Engine:
                                    self.device)
 
     # ------------------------------------------------------- StepBackend
-    def open_sequence(self) -> int:
-        return self.cache.open_sequence()
+    def open_sequence(self, adapter: Optional[str] = None) -> int:
+        """A new sequence, with the adapter of that name (`load_adapter`) or none."""
+        place = None if adapter is None else self._adapters().place_of(adapter)
+        slot = self.cache.open_sequence()
+        self._unread.add(slot)
+        self._said.pop(slot, None)
+        self._adapter_of.pop(slot, None)
+        if place is not None:
+            self._adapter_of[slot] = place
+            self.adapters.hold(place)
+        return slot
 
     def close_sequence(self, slot: int) -> None:
         self.cache.close_sequence(slot)
+        place = self._adapter_of.pop(slot, None)
+        if place is not None:
+            self.adapters.release(place)
+
+    # ------------------------------------------------------------ adapters
+    def enable_adapters(self, max_adapters: int = 8, max_rank: int = 16) -> None:
+        """Make room for low-rank adapters beside the projections that take them (q, k, v, o, gate, up
+        and down of the Llama decoder): `max_adapters` at a time, of rank `max_rank` at most."""
+        if self.adapters is not None:
+            raise ValueError("adapters are enabled already")
+        self.adapters = AdapterStore(self.model, max_adapters, max_rank, self.dtype, self.device)
+
+    def _adapters(self) -> AdapterStore:
+        if self.adapters is None:
+            raise ValueError("no adapters: call enable_adapters first")
+        return self.adapters
+
+    def load_adapter(self, name: str, source, scale: Optional[float] = None) -> None:
+        """An adapter from a folder (adapter_config.json, adapter_model.safetensors) or from
+        {"<projection>.lora_A.weight": tensor, "<projection>.lora_B.weight": tensor}; `scale` (of a
+        folder: lora_alpha / r unless given) multiplies its part."""
+        self._settle()
+        self._adapters().load(name, source, scale)
+
+    def unload_adapter(self, name: str) -> None:
+        self._adapters().unload(name)
+
+    def adapters_of(self, slots: Sequence[int]) -> Optional[List[int]]:
+        """The places of these sequences' adapters (-1: none), or None if no one has one."""
+        places = [self._adapter_of.get(s, -1) for s in slots]
+        return places if any(p >= 0 for p in places) else None
+
+    # ----------------------------------------------------------- histories
+    def token_history(self) -> ops.TokenHistory:
+        """Which tokens each slot's sequence holds; a slot's row is its number."""
+        if self._history is None:
+            self._history = ops.TokenHistory.empty(self.cache.scratch_slot + 1, self.spec.vocab_size,
+                                                   self.device)
+        return self._history
+
+    def history_row(self, slot: int) -> int:
+        """The slot's row of the history, cleared if another sequence's tokens are in it."""
+        history = self.token_history()
+        if slot in self._unread:
+            history.clear([slot])
+            self._unread.discard(slot)
+        return slot
+
+    def tokens_said(self, slot: int) -> List[int]:
+        """The tokens that the slot's sequence has generated, as far as a grammar was asked."""
+        return self._said.setdefault(slot, [])
+
+    def last_logprobs(self) -> List[float]:
+        """The log-probabilities of the tokens that the last `step_select` returned."""
+        return self._last_logprobs
 
     def _settle(self) -> None:
         """Take back a decode step that the engine's session started on a guess
@@ -160,7 +231,8 @@ class Engine:
             logits = self._prompts.step(steps)
         else:
             ctx = build_context(self.cache, steps, self.spec.vocab_size, self.device,
-                                self.spec.max_positions)
+                                self.spec.max_positions,
+                                adapters=self.adapters_of([s.slot for s in steps]))
             with ops.scratch_owner(self.scratch):
                 logits = self.model.forward(ctx, self.cache)
         if logits.shape[0]:
@@ -206,13 +278,50 @@ class Engine:
         only the token ids cross to the host. `more`: the caller expects to
         come back with the same sequences, each with the token returned here
         (a generation loop whose rows all go on unless a stop token ends one);
-        single-token steps then start the next step before they return."""
-        if self._is_decode(steps):
+        single-token steps then start the next step before they return.
+        `params`: one `SamplingParams` for all wanted rows, or one each (in a
+        step of several tokens every sequence then wants one row). The penalties'
+        histories count what a row brings as the prompt's while its count is 0,
+        and as generated afterwards."""
+        ruled = is_ruled(params)
+        # (a row that has generated nothing yet brings a prompt, of a single token maybe)
+        if self._is_decode(steps) and not (ruled and any(c == 0 for c in counts)):
             session = self._session_of(steps, params, keys, counts)
-            return session.step_host([int(s.tokens[0]) for s in steps], more, counts)
+            tokens = session.step_host([int(s.tokens[0]) for s in steps], more, counts)
+            self._last_logprobs = session.last_logprobs
+            return tokens
+        if ruled:
+            return self._draw_behind(steps, params_of_rows(params, len(steps)), keys, counts)
         logits = self.step(steps)
         tokens = self.sampler.select(logits, params, keys, counts)
         return tokens.tolist()
+
+    def _draw_behind(self, steps, params, keys, counts) -> List[int]:
+        """A step of several tokens whose rows draw under rules of their own."""
+        if any(len(s.want) != 1 for s in steps):
+            raise ValueError("rows that draw under rules of their own want one place each")
+        logits = self.step(steps)
+        said = [p.needs_history for p in params]
+        rows = [self.history_row(s.slot) if h else -1 for s, h in zip(steps, said)]
+        for what, wanted in (("prompt", lambda c: c == 0), ("generated", lambda c: c > 0)):
+            pairs = [(row, int(t)) for s, row, c in zip(steps, rows, counts) if row >= 0 and wanted(c)
+                     for t in s.tokens]
+            if pairs:
+                where = torch.tensor(pairs, dtype=torch.int32).t().contiguous().to(self.device)
+                ops.record_tokens(self.token_history(), where[0], where[1], what)
+        for s, p, c in zip(steps, params, counts):
+            if p.allowed_tokens is not None and c > 0:
+                self.tokens_said(s.slot).extend(int(t) for t in s.tokens)
+        masks = [None if p.allowed_tokens is None else p.allowed_tokens(self.tokens_said(s.slot))
+                 for s, p in zip(steps, params)]
+        tokens, logprobs = self.sampler.draw(logits, params, keys, counts,
+                                             self.token_history() if any(said) else None, rows, masks)
+        self._last_logprobs = logprobs.tolist()
+        tokens = tokens.tolist()
+        if min(tokens) < 0:
+            raise loop.NoTokenLeft(f"row {tokens.index(min(tokens))}: what its sampling allows leaves "
+                                   f"no token")
+        return tokens
 
     @staticmethod
     def _is_decode(steps: Sequence[SequenceStep]) -> bool:
@@ -233,7 +342,8 @@ class Engine:
         keys = list(range(len(slots))) if keys is None else list(keys)
         session = self._session
         if session is None or session.slots != slots or session.sampling != params \
-                or session.keys != keys:
+                or session.keys != keys or session.adapters != self.adapters_of(slots) \
+                or (session.rules is not None and any(s in self._unread for s in slots)):
             self._settle()
             session = self._session = DecodeSession(self, slots, params, keys, counts)
         return session
@@ -245,13 +355,18 @@ class Engine:
         self._settle()
         return DecodeSession(self, slots, sampling, keys, counts)
 
-    def decode_runner(self, bucket: int, width: int, unequal: bool = False) -> "DecodeRunner":
+    def decode_runner(self, bucket: int, width: int, unequal: bool = False, rules=None,
+                      adapted: bool = False) -> "DecodeRunner":
         """The captured step for `bucket` rows, page tables `width` pages wide, and
         sequences of about equal or of unequal lengths (the attention shares its
-        work differently)."""
+        work differently); `rules` and `adapted` as `DecodeRunner` has them."""
         key = (bucket, width) if not unequal else (bucket, width, "unequal")
+        if rules is not None:
+            key += (rules,)
+        if adapted:
+            key += ("adapted",)
         if key not in self._runners:
-            self._runners[key] = DecodeRunner(self, bucket, width, unequal)
+            self._runners[key] = DecodeRunner(self, bucket, width, unequal, rules, adapted)
         return self._runners[key]
 
     def graph_pool(self):
@@ -263,6 +378,10 @@ class Engine:
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int,
                  eos_token_id: Optional[Sequence[int]] = None,
                  sampling: SamplingParams = SamplingParams(), max_batch: Optional[int] = None,
-                 ignore_eos: bool = False) -> loop.Generation:
+                 ignore_eos: bool = False,
+                 adapters: Optional[Sequence[Optional[str]]] = None) -> loop.Generation:
+        """`sampling`: one `SamplingParams` for all prompts, or one each; `adapters`: the name of each
+        prompt's adapter, or None."""
         stops = self.spec.eos_token_ids if eos_token_id is None else tuple(eos_token_id)
-        return loop.generate(self, prompts, max_new_tokens, stops, sampling, max_batch, ignore_eos)
+        return loop.generate(self, prompts, max_new_tokens, stops, sampling, max_batch, ignore_eos,
+                             adapters)

@@ -23,7 +23,7 @@ from dataclasses import dataclass, field
 from typing import List, Optional, Protocol, Sequence
 
 from ..cache.pages import PAGE, pages_for
-from ..sampling.params import SamplingParams
+from ..sampling.params import SamplingParams, params_of_rows
 from .context import SequenceStep
 
 
@@ -34,6 +34,7 @@ class GenerateError(ValueError):
 class EmptyBatch(GenerateError): pass
 class EmptyPrompt(GenerateError): pass
 class PromptTooLong(GenerateError): pass
+class NoTokenLeft(GenerateError): pass
 
 
 @dataclass
@@ -45,6 +46,8 @@ class Generation:
     prefill: float = 0.0  # seconds, summed over batches
     decode_steps: List[float] = field(default_factory=list)
     batches: List[List[int]] = field(default_factory=list)  # request indices of each batch
+    # log-probabilities of the new tokens, for requests whose sampling asks for them (else empty rows)
+    logprobs: List[List[float]] = field(default_factory=list)
 
 
 class StepBackend(Protocol):
@@ -56,6 +59,9 @@ class StepBackend(Protocol):
     def max_positions(self) -> int: ...
     def step_select(self, steps: Sequence[SequenceStep], params: SamplingParams,
                     keys: Sequence[int], counts: Sequence[int], more: bool = False) -> List[int]: ...
+    # where requests bring their own: `params` is then a list, a row each, `open_sequence` gets the
+    # request's adapter, and the tokens' log-probabilities are those of the last `step_select`
+    def last_logprobs(self) -> List[float]: ...
 
 
 def is_stopped(row: Sequence[int], eos_token_ids: Sequence[int]) -> bool:
@@ -87,14 +93,22 @@ def plan_batch(pending: Sequence[int], prompt_lens: Sequence[int], max_new_token
 
 
 def generate(backend: StepBackend, prompts: Sequence[Sequence[int]], max_new_tokens: int,
-             eos_token_ids: Sequence[int] = (), sampling: SamplingParams = SamplingParams(),
-             max_batch: Optional[int] = None, ignore_eos: bool = False) -> Generation:
+             eos_token_ids: Sequence[int] = (), sampling=SamplingParams(),
+             max_batch: Optional[int] = None, ignore_eos: bool = False,
+             adapters: Optional[Sequence[Optional[str]]] = None) -> Generation:
+    """`sampling`: one `SamplingParams` for all requests, or one each. `adapters`: the name of each
+    request's adapter, or None."""
     if len(prompts) == 0:
         raise EmptyBatch("the batch holds no prompt")
     if any(len(p) == 0 for p in prompts):
         raise EmptyPrompt("a prompt holds no token")
     n = len(prompts)
-    result = Generation(token_ids=[[] for _ in range(n)], finish_reason=["length"] * n)
+    if not isinstance(sampling, SamplingParams):
+        sampling = params_of_rows(sampling, n)
+    if adapters is not None and len(adapters) != n:
+        raise GenerateError(f"{len(adapters)} adapters for {n} requests")
+    result = Generation(token_ids=[[] for _ in range(n)], finish_reason=["length"] * n,
+                        logprobs=[[] for _ in range(n)])
     if max_new_tokens <= 0:
         return result
     lens = [len(p) for p in prompts]
@@ -115,18 +129,28 @@ def generate(backend: StepBackend, prompts: Sequence[Sequence[int]], max_new_tok
             raise PromptTooLong(f"request {pending[0]} does not fit the free cache")
         pending = pending[len(batch):]
         result.batches.append(list(batch))
-        _run_batch(backend, batch, prompts, max_new_tokens, stops, sampling, result)
+        _run_batch(backend, batch, prompts, max_new_tokens, stops, sampling, result, adapters)
     return result
 
 
-def _run_batch(backend, batch, prompts, max_new_tokens, stops, sampling, result) -> None:
-    slot_of = {r: backend.open_sequence() for r in batch}
-    live = list(batch)
+def _sampling_of(sampling, live):
+    return sampling if isinstance(sampling, SamplingParams) else [sampling[r] for r in live]
+
+
+def _run_batch(backend, batch, prompts, max_new_tokens, stops, sampling, result,
+               adapters=None) -> None:
+    slot_of = {}
+    live = []
     try:
+        for r in batch:
+            name = None if adapters is None else adapters[r]
+            slot_of[r] = backend.open_sequence() if name is None else backend.open_sequence(name)
+            live.append(r)
         started = time.perf_counter()
         steps = [SequenceStep(slot_of[r], list(prompts[r]), [len(prompts[r]) - 1]) for r in live]
-        tokens = backend.step_select(steps, sampling, live, [0] * len(live))
+        tokens = backend.step_select(steps, _sampling_of(sampling, live), live, [0] * len(live))
         result.prefill += time.perf_counter() - started
+        _note_logprobs(backend, live, sampling, result)
         live = _append(backend, live, tokens, slot_of, stops, max_new_tokens, result)
         while live:
             started = time.perf_counter()
@@ -135,12 +159,21 @@ def _run_batch(backend, batch, prompts, max_new_tokens, stops, sampling, result)
             # unless a stop token ends a row, the same rows come back with the tokens
             # of this step: the backend may start that step before it returns
             more = all(c + 1 < max_new_tokens for c in counts)
-            tokens = backend.step_select(steps, sampling, live, counts, more)
+            tokens = backend.step_select(steps, _sampling_of(sampling, live), live, counts, more)
             result.decode_steps.append(time.perf_counter() - started)
+            _note_logprobs(backend, live, sampling, result)
             live = _append(backend, live, tokens, slot_of, stops, max_new_tokens, result)
     finally:
         for r in live:  # only after an error: give back what is still held
             backend.close_sequence(slot_of[r])
+
+
+def _note_logprobs(backend, live, sampling, result) -> None:
+    params = params_of_rows(_sampling_of(sampling, live), len(live))
+    if any(p.logprobs for p in params):
+        for r, p, value in zip(live, params, backend.last_logprobs()):
+            if p.logprobs:
+                result.logprobs[r].append(float(value))
 
 
 def _append(backend, live, tokens, slot_of, stops, max_new_tokens, result) -> List[int]:

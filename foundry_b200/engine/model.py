@@ -118,15 +118,23 @@ class Model:
             total += count * size
         return total
 
+    @staticmethod
+    def _parts_of(block):
+        listed = getattr(block, "parts", None)  # a block may list its parts itself
+        return list(listed()) if callable(listed) else [
+            getattr(block, name, None) for name in ("mixer", "feed_forward", "mixer_norm",
+                                                    "feed_forward_norm")]
+
+    def parts(self):
+        """Every block's parts, in order."""
+        return [part for block in self.blocks for part in self._parts_of(block) if part is not None]
+
     def replay_safe(self) -> bool:
         """Whether every part says that its forward reads nothing of the step
         on the host (`replay_safe = True`, see parts/base.py): only then may a
         step of this model be captured once and replayed."""
         for block in self.blocks:
-            listed = getattr(block, "parts", None)  # a block may list its parts itself
-            parts = [block] + (list(listed()) if callable(listed) else
-                               [getattr(block, name, None) for name in
-                                ("mixer", "feed_forward", "mixer_norm", "feed_forward_norm")])
+            parts = [block] + self._parts_of(block)
             if not all(p is not None and getattr(p, "replay_safe", False) for p in parts):
                 return False
         others = [self.final_norm] + self.junctions + ([self.embedder] if self.embedder else [])

@@ -52,14 +52,13 @@ class PromptRunner:
     """Fixed buffers and the captured graph of one bucket."""
 
     def __init__(self, engine, tokens: int, seqs: int, width: int, want: int, long_queries: bool,
-                 fresh: bool = False):
+                 fresh: bool = False, adapted: bool = False):
         self.engine = engine
-        self.key = (tokens, seqs, width, want, long_queries, fresh)
         dev = engine.device
         groups = engine.cache.groups
         t, s = tokens, seqs
         # packed int32 fields, as in build_context
-        sizes = [t, t, t, want, s, s + 1, s] + [s * width for _ in groups]
+        sizes = [t, t, t, want, s, s + 1, s] + [s * width for _ in groups] + [t] * adapted
         offsets = [int(o) for o in np.cumsum([0] + sizes)]
         # steps may be queued ahead of the device (portions of a prompt whose logits
         # nobody waits for): the upload goes through a ring of pinned buffers
@@ -78,12 +77,14 @@ class PromptRunner:
             query_blocks_bound=(t + 63) // 64 + s, long_queries=long_queries, fresh=fresh)
         for i, group in enumerate(groups):
             self.ctx._tables[id(group)] = part[7 + i].view(s, width)
+        if adapted:
+            self.ctx.adapters = part[-1]
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.kernels_per_step = 0
         self.kernel_histogram: Dict[str, int] = {}
         self.logits: Optional[torch.Tensor] = None
 
-    def fill(self, plan: StepPlan, scratch_slot: int) -> None:
+    def fill(self, plan: StepPlan, scratch_slot: int, adapters: Optional[Sequence[int]] = None) -> None:
         h = self.h
         T, S, W = int(plan.token_ids.size), len(plan.slots), len(plan.want_rows)
         h[0][:T] = plan.token_ids
@@ -102,6 +103,9 @@ class PromptRunner:
         h[6][S:] = 0
         for table, (_, w, rows) in zip(self.h_tables, plan.tables):
             table[:S, :w] = np.asarray(rows, np.int32).reshape(S, w)
+        if adapters is not None:
+            h[-1][:T] = np.repeat(np.asarray(adapters, np.int32), np.diff(plan.cu))
+            h[-1][T:] = -1
         self.fields.upload()
 
     def _body(self) -> None:
@@ -152,7 +156,7 @@ class PromptRunners:
     def __init__(self, engine):
         self.engine = engine
         self.enabled = replay_safe(engine.model)
-        self._runners: Dict[Tuple[int, int, int, int, bool, bool], PromptRunner] = {}
+        self._runners: Dict[Tuple, PromptRunner] = {}
 
     def wants(self, steps: Sequence[SequenceStep]) -> bool:
         if not self.enabled or not self.engine.use_graphs or PROMPT_GRAPH_TOKENS <= 0:
@@ -172,13 +176,16 @@ class PromptRunners:
         key = (token_bucket(int(plan.token_ids.size)), bucket_of(len(plan.slots)), width,
                bucket_of(len(plan.want_rows)) if plan.want_rows else 0, longest >= 64,
                all(plan.kv_lens[i] == plan.cu[i + 1] - plan.cu[i] for i in range(len(plan.slots))))
+        adapters = engine.adapters_of([s.slot for s in steps])
+        if adapters is not None:
+            key += (True,)
         runner = self._runners.pop(key, None)
         if runner is None:
             if len(self._runners) >= MAX_RUNNERS:
                 self._runners.pop(next(iter(self._runners)))
             runner = PromptRunner(engine, *key)
         self._runners[key] = runner  # most recently used last
-        runner.fill(plan, engine.cache.scratch_slot)
+        runner.fill(plan, engine.cache.scratch_slot, adapters)
         logits = runner.run()
         return logits[:len(plan.want_rows)].clone()
 

@@ -23,6 +23,7 @@ from ..cache.store import KVRequest, KVView
 from ..config.spec import PartSpec
 from ..kernels import ops
 from ..weights.loader import ExpectedTensor
+from .adapters import AdapterSite
 from .base import POSITION_ENCODINGS, Fetch, Part, register_mixer
 from .linear import Linear, matmul_nt
 
@@ -102,6 +103,7 @@ class GQAAttention(Part):
             host = getattr(enc, "inv_freq_host", None)
             self.angles_key = ("rotary angles", host.tobytes() if host is not None else id(enc))
         self.scale = factor / math.sqrt(head_dim)
+        self.qkv_site = self.o_site = None  # room for adapters, named when the weights are loaded
 
     # ----------------------------------------------------------------- setup
     def expected_tensors(self, prefix: str) -> Dict[str, ExpectedTensor]:
@@ -110,6 +112,9 @@ class GQAAttention(Part):
     def load(self, prefix: str, fetch: Fetch) -> None:
         self.qkv.load(prefix, fetch)
         self.o.load(prefix, fetch)
+        self.qkv_site = AdapterSite([(f"{prefix}.{name}", rows) for name, rows in self.qkv.outs],
+                                    self.hidden_size)
+        self.o_site = AdapterSite([(f"{prefix}.o_proj", self.hidden_size)], self.q_size)
         if self.rotary_dim and self.pairing == "half":
             # Store the rows of every query and key head so that the two features a
             # frequency turns are neighbours (2i, 2i + 1) instead of half a rotary width
@@ -117,7 +122,8 @@ class GQAAttention(Part):
             # values between neighbouring lanes. Scores are dot products over a head's
             # features, so any order serves as long as queries and keys share it; values
             # and the output projection are untouched.
-            self.qkv.weight = self.qkv.weight.index_select(0, self._neighbour_order()).contiguous()
+            self.qkv_site.order = self._neighbour_order()
+            self.qkv.weight = self.qkv.weight.index_select(0, self.qkv_site.order).contiguous()
             self.pairing = "interleaved"
 
     def _neighbour_order(self) -> torch.Tensor:
@@ -132,6 +138,9 @@ class GQAAttention(Part):
             order += [head * self.head_dim + e for e in within]
         order += list(range(len(order), len(order) + self.kv_size))  # the value heads as they are
         return torch.tensor(order, dtype=torch.long, device=self.qkv.weight.device)
+
+    def adapter_sites(self):
+        return [self.qkv_site, self.o_site]
 
     def cache_request(self) -> KVRequest:
         return KVRequest(self.num_kv_heads, self.head_dim, self.window)
@@ -151,13 +160,27 @@ class GQAAttention(Part):
     # ------------------------------------------------------------------- run
     def forward(self, ctx, x, cache: KVView):
         table = ctx.page_table(cache.group)
-        q = rotated_projection(ctx, x, self.qkv.weight, self.inv_freq, self.rotary_dim,
-                               self.pairing, self.angles_key, cache, self.num_heads,
-                               self.num_kv_heads, self.head_dim)
+        adapters = getattr(ctx, "adapters", None)
+        if adapters is None:
+            q = rotated_projection(ctx, x, self.qkv.weight, self.inv_freq, self.rotary_dim,
+                                   self.pairing, self.angles_key, cache, self.num_heads,
+                                   self.num_kv_heads, self.head_dim)
+        else:  # 32-bit sums of projection and adapters, then rotation and cache write
+            qkv = ops.adapted_product(x, self.qkv.weight, self.qkv_site.bank, adapters,
+                                      out_dtype=torch.float32, then_reads=self.o.weight)
+            q = ops.rope_kv_write(ops.Planes(qkv[None]), ctx.positions, ctx.seq_of_token, table,
+                                  self.inv_freq, self.rotary_dim, cache.k, cache.v, self.num_heads,
+                                  self.num_kv_heads, self.head_dim,
+                                  ring_pages=cache.group.ring_pages, write_cache=cache.writes,
+                                  dtype=x.dtype, pairing=self.pairing)
         attn = torch.empty((x.shape[0], self.q_size), dtype=x.dtype, device=x.device)
         ops.attention(ctx, q, attn, table, cache.k, cache.v, self.num_heads, self.num_kv_heads,
                       self.head_dim, self.scale, window=cache.group.window,
                       ring_pages=cache.group.ring_pages, then_reads=self.o.weight)
+        if adapters is not None:  # 32-bit sums for whoever adds them to the stream
+            return ops.Planes(ops.adapted_product(
+                attn, self.o.weight, self.o_site.bank, adapters, out_dtype=torch.float32,
+                then_reads=getattr(ctx, "reads_after_part", None))[None])
         return self.o.forward(attn, allow_planes=True,
                               then_reads=getattr(ctx, "reads_after_part", None),
                               residual=getattr(ctx, "residual_sink", None))

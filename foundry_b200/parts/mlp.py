@@ -13,6 +13,7 @@ import torch
 
 from ..kernels import ops
 from ..weights.loader import ExpectedTensor
+from .adapters import AdapterSite
 from .base import Fetch, Part, register_feed_forward
 from .linear import Linear, matmul_nt
 from .products import product_f32, product_planes
@@ -35,6 +36,7 @@ class SwiGLU(Part):
         self.dtype, self.device = dtype, device
         self.names, self.suffix = tuple(names), suffix  # the three projections in the files
         self.gate_up: torch.Tensor = None  # [2I, H]: row 2i is gate i, row 2i+1 is up i
+        self.gate_up_site = self.down_site = None  # room for adapters, named when the weights are loaded
         self.down = Linear(intermediate_size, [(self.names[2], hidden_size)], dtype=dtype,
                            device=device, suffix=suffix)
 
@@ -53,9 +55,27 @@ class SwiGLU(Part):
         self.gate_up = torch.stack([gate, up], 1).reshape(2 * self.intermediate_size,
                                                           self.hidden_size).contiguous()
         self.down.load(prefix, fetch)
+        wide = self.intermediate_size
+        self.gate_up_site = AdapterSite(
+            [(f"{prefix}.{self.names[0]}", wide), (f"{prefix}.{self.names[1]}", wide)],
+            self.hidden_size, torch.arange(2 * wide).view(2, wide).t().reshape(-1))
+        self.down_site = AdapterSite([(f"{prefix}.{self.names[2]}", self.hidden_size)], wide)
+
+    def adapter_sites(self):
+        return [self.gate_up_site, self.down_site]
 
     def first_weight(self):
         return self.gate_up
+
+    def _adapted(self, ctx, x, adapters: torch.Tensor):
+        """`forward` of a step of which some tokens have an adapter."""
+        both = ops.adapted_product(x, self.gate_up, self.gate_up_site.bank, adapters,
+                                   out_dtype=torch.float32, then_reads=self.down.weight)
+        hidden = torch.empty((x.shape[0], self.intermediate_size), dtype=x.dtype, device=x.device)
+        ops.silu_mul(both, hidden, interleaved=True, act=self.activation)
+        return ops.Planes(ops.adapted_product(
+            hidden, self.down.weight, self.down_site.bank, adapters, out_dtype=torch.float32,
+            then_reads=getattr(ctx, "reads_after_part", None))[None])
 
     def hidden(self, x) -> torch.Tensor:
         """act(gate(x)) * up(x) in the activation type: what the down projection reads."""
@@ -69,6 +89,9 @@ class SwiGLU(Part):
         return hidden
 
     def forward(self, ctx, x):
+        adapters = getattr(ctx, "adapters", None)
+        if adapters is not None:
+            return self._adapted(ctx, x, adapters)
         hidden = self.hidden(x)
         return self.down.forward(hidden, out_dtype=self.out_dtype, allow_planes=True,
                                  then_reads=getattr(ctx, "reads_after_part", None),

@@ -11,7 +11,8 @@ import numpy as np
 import torch
 
 from ..kernels import ops
-from .params import SamplingParams
+from .params import SamplingParams, params_of_rows
+from .rules import RowRules, bias_room, check_vocabulary
 
 _M1, _M2, _GOLDEN = 0xbf58476d1ce4e5b9, 0x94d049bb133111eb, 0x9e3779b97f4a7c15
 _MASK = (1 << 64) - 1
@@ -55,6 +56,22 @@ def gumbel_scores(logits: np.ndarray, temperature: float, seed: int, key: int,
 class Sampler:
     def __init__(self, device: torch.device):
         self.device = device
+
+    def draw(self, logits: torch.Tensor, params, keys: Sequence[int], steps: Sequence[int],
+             history: Optional[ops.TokenHistory], history_rows: Sequence[int], masks):
+        """(tokens, log-probabilities) of rows that draw under rules of their own: `history_rows` are
+        the rows' places in `history`, `masks` the tokens that each row allows (None: all)."""
+        n, vocab = logits.shape
+        rows = params_of_rows(params, n)
+        check_vocabulary(rows, vocab)
+        rules = RowRules(n, vocab, logits.device, history, bias_room(rows),
+                         any(m is not None for m in masks))
+        rules.fill(rows, history_rows)
+        rules.set_steps([stream_key(p.seed, int(k)) for p, k in zip(rows, keys)], list(steps))
+        if rules.bits is not None:
+            rules.set_masks(masks)
+        out = torch.empty(n, dtype=torch.int32, device=logits.device)
+        return rules.draw(logits, out)
 
     def select(self, logits: torch.Tensor, params: SamplingParams,
                keys: Optional[Sequence[int]] = None,
