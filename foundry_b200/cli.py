@@ -68,6 +68,20 @@ def build_parser() -> argparse.ArgumentParser:
     run.add_argument("--temperature", type=float, default=0.0,
                      help="Sampling temperature; 0 always takes the most likely token.")
     run.add_argument("--seed", type=int, default=0, help="Seed of the sampling streams.")
+    run.add_argument("--top-k", type=int, default=0, help="Draw among this many most likely tokens (0: all).")
+    run.add_argument("--top-p", type=float, default=1.0,
+                     help="Draw among the fewest tokens whose probability reaches this.")
+    run.add_argument("--min-p", type=float, default=0.0,
+                     help="Draw among tokens at least this many times as likely as the likeliest.")
+    run.add_argument("--repetition-penalty", type=float, default=1.0,
+                     help="Divides positive logits of tokens that were there already, multiplies others.")
+    run.add_argument("--frequency-penalty", type=float, default=0.0,
+                     help="Taken off a token's logit for every time it was generated.")
+    run.add_argument("--presence-penalty", type=float, default=0.0,
+                     help="Taken off the logit of every token that was generated.")
+    run.add_argument("--adapter", metavar="DIR",
+                     help="Folder with adapter_config.json and adapter_model.safetensors: a low-rank "
+                          "adapter for all prompts.")
     run.add_argument("--ignore-eos", action="store_true", help="Do not stop at stop tokens.")
 
     bench = sub.add_parser("bench", help="Time prompt processing and greedy decoding on seeded "
@@ -179,9 +193,25 @@ def _git_commit() -> Optional[str]:
         return None
 
 
+def sampling_of(args):
+    """The sampling parameters that the options of `run` name."""
+    from .sampling import SamplingParams
+    return SamplingParams(args.temperature, args.seed, args.top_k, args.top_p, args.min_p,
+                          args.repetition_penalty, args.frequency_penalty, args.presence_penalty)
+
+
+def load_adapter(engine, folder: str) -> str:
+    """Make room for the folder's adapter and load it; returns its name."""
+    from .engine.adapters import pairs_of, read_folder
+    tensors, scale = read_folder(folder)
+    engine.enable_adapters(1, max(a.shape[0] for a, _ in pairs_of(tensors).values()))
+    engine.load_adapter(folder, tensors, scale)
+    return folder
+
+
 def cmd_run(args) -> int:
     from .cache.pages import PAGE, pages_for
-    from .sampling import SamplingParams
+    sampling = sampling_of(args)
     check_token_ids(args.prompt_ids, _vocab_size(args))
     # the cache holds prompt + new tokens of every prompt (src/cli/command.rs:91-101)
     per_seq = [len(p) + args.max_new_tokens for p in args.prompt_ids]
@@ -192,9 +222,9 @@ def cmd_run(args) -> int:
         per_seq = [args.max_seq_len] * len(per_seq)
     need = sum(pages_for(n) * PAGE for n in per_seq)
     engine, _ = open_engine(args, need, len(args.prompt_ids))
-    out = engine.generate(args.prompt_ids, args.max_new_tokens,
-                          sampling=SamplingParams(args.temperature, args.seed),
-                          ignore_eos=args.ignore_eos)
+    adapters = [load_adapter(engine, args.adapter)] * len(args.prompt_ids) if args.adapter else None
+    out = engine.generate(args.prompt_ids, args.max_new_tokens, sampling=sampling,
+                          ignore_eos=args.ignore_eos, adapters=adapters)
     log.info("Generated tokens. prompt_tokens=%s generated_tokens=%s prefill_ms=%.1f "
              "decode_steps=%d decode_ms_total=%.1f", [len(p) for p in args.prompt_ids],
              [len(r) for r in out.token_ids], out.prefill * 1e3, len(out.decode_steps),

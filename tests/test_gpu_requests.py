@@ -346,3 +346,18 @@ def test_a_slot_forgets_the_sequence_before(setting):
         prompt = tiny.random_tokens(90 + seed, 6 + seed, V)
         assert engine.generate([prompt], 6, eos_token_id=[], sampling=p).token_ids == [
             simulate(setting, prompt, p, 0, 6)[0]]
+
+
+def test_the_command_line_with_an_adapter_and_rules(setting, tmp_path, capsys):
+    import json
+    from foundry_b200 import SamplingParams
+    from foundry_b200.cli import main
+    from foundry_b200.weights.safetensors_io import save_file
+    save_file(setting["tensors"]["one"], str(tmp_path / "adapter_model.safetensors"))
+    (tmp_path / "adapter_config.json").write_text(json.dumps({"r": 4, "lora_alpha": 6}))
+    prompt = tiny.random_tokens(8, 10, setting["cfg"]["vocab_size"])
+    assert main(["run", "--model", setting["folder"], "--dtype", "float32", "--prompt-ids", ",".join(map(str, prompt)),
+                 "--max-new-tokens", "7", "--ignore-eos", "--temperature", "0.7", "--seed", "3", "--top-k", "6",
+                 "--frequency-penalty", "0.5", "--adapter", str(tmp_path)]) == 0
+    p = SamplingParams(0.7, 3, top_k=6, frequency_penalty=0.5)
+    assert json.loads(capsys.readouterr().out) == simulate(setting, prompt, p, 0, 7, "one")[0]

@@ -213,3 +213,13 @@ def test_an_adapters_folder(tmp_path):
         config(**more)
         with pytest.raises(adapters.AdapterError):
             adapters.read_folder(str(tmp_path))
+
+
+def test_the_command_lines_options():
+    from foundry_b200.cli import build_parser, sampling_of
+    base = ["run", "--model", "m", "--prompt-ids", "1,2", "--max-new-tokens", "3"]
+    assert sampling_of(build_parser().parse_args(base)) == SamplingParams()
+    args = build_parser().parse_args(base + [
+        "--temperature", "0.8", "--seed", "4", "--top-k", "40", "--top-p", "0.9", "--min-p", "0.05",
+        "--repetition-penalty", "1.1", "--frequency-penalty", "0.2", "--presence-penalty", "0.3", "--adapter", "d"])
+    assert sampling_of(args) == SamplingParams(0.8, 4, 40, 0.9, 0.05, 1.1, 0.2, 0.3) and args.adapter == "d"
