@@ -14,6 +14,8 @@
 // (ordered bits of v) << 20 | (2^20 - 1 - i), larger = earlier, and a cut keeps the places >= cut.
 #include "logit_edits.cuh"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int THREADS = 512;
@@ -100,61 +102,6 @@ __device__ __forceinline__ void store_at(unsigned long long* mine, unsigned rank
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(there), "l"(v) : "memory");
 }
 
-// What the blocks of a cluster tell each other: two sets by turns, so that a set is written again only
-// when every block has passed the barrier behind its last reading.
-struct Meeting {
-  unsigned long long said[2][2][MAX_CLUSTER];
-  unsigned long long warps[2][THREADS / 32];
-};
-
-// One value a thread -> one a row, joined in a fixed order, for every thread of the cluster; `meanwhile`
-// runs while the blocks wait for each other. The pair form takes two values with joins of their own.
-template <typename F, typename G, typename W>
-__device__ __forceinline__ void meet_pair(Meeting& m, int& turn, int blocks, unsigned rank,
-                                          unsigned long long& v, F&& join, unsigned long long* w, G&& join_w,
-                                          W&& meanwhile) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    v = join(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if (w != nullptr) *w = join_w(*w, __shfl_xor_sync(0xffffffffu, *w, o));
-  }
-  const int lane = threadIdx.x & 31;
-  if (lane == 0) {
-    m.warps[0][threadIdx.x >> 5] = v;
-    if (w != nullptr) m.warps[1][threadIdx.x >> 5] = *w;
-  }
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    v = m.warps[0][lane & (THREADS / 32 - 1)];
-    if (w != nullptr) *w = m.warps[1][lane & (THREADS / 32 - 1)];
-#pragma unroll
-    for (int o = THREADS / 64; o > 0; o >>= 1) {
-      v = join(v, __shfl_xor_sync(0xffffffffu, v, o));
-      if (w != nullptr) *w = join_w(*w, __shfl_xor_sync(0xffffffffu, *w, o));
-    }
-    if (lane < blocks) {
-      store_at(&m.said[turn][0][rank], lane, v);
-      if (w != nullptr) store_at(&m.said[turn][1][rank], lane, *w);
-    }
-  }
-  cluster_arrive();
-  meanwhile();
-  cluster_wait();
-  // every warp joins what the blocks said
-  v = m.said[turn][0][lane & (blocks - 1)];
-  if (w != nullptr) *w = m.said[turn][1][lane & (blocks - 1)];
-  for (int o = blocks / 2; o > 0; o >>= 1) {
-    v = join(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if (w != nullptr) *w = join_w(*w, __shfl_xor_sync(0xffffffffu, *w, o));
-  }
-  turn ^= 1;
-}
-template <typename F>
-__device__ __forceinline__ unsigned long long meet(Meeting& m, int& turn, int blocks, unsigned rank,
-                                                   unsigned long long v, F&& join) {
-  meet_pair(m, turn, blocks, rank, v, join, (unsigned long long*)nullptr, join, [] {});
-  return v;
-}
 struct Larger {
   __device__ unsigned long long operator()(unsigned long long a, unsigned long long b) const { return a > b ? a : b; }
 };
@@ -168,6 +115,74 @@ struct SumDoubles {
   }
 };
 
+// What the blocks of a cluster tell each other: two sets by turns, so that a set is written again only
+// when every block has passed the barrier behind its last reading.
+struct Meeting {
+  unsigned long long said[2][2][MAX_CLUSTER];
+  unsigned long long warps[2][THREADS / 32];
+};
+
+// One value a thread -> one a row, joined in a fixed order, for every thread of the cluster; `meanwhile`
+// runs while the blocks wait for each other. The pair form takes two values with joins of their own.
+// The join of a warp's values, for every lane. The larger of two places: their upper 32 bits, then the
+// lower ones of those that have them, by the warp's own reductions.
+template <int LANES, typename F>
+__device__ __forceinline__ unsigned long long over_warp(unsigned long long v, F&& join) {
+  if constexpr (std::is_same_v<std::remove_cv_t<std::remove_reference_t<F>>, Larger>) {
+    const unsigned upper = (unsigned)(v >> ID_BITS);
+    const unsigned most = __reduce_max_sync(0xffffffffu, upper);
+    const unsigned lower = __reduce_max_sync(0xffffffffu, upper == most ? (unsigned)v & ID_MASK : 0u);
+    return ((unsigned long long)most << ID_BITS) | lower;
+  } else {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v = join(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  }
+}
+
+template <typename F, typename G, typename W>
+__device__ __forceinline__ void meet_pair(Meeting& m, int& turn, int blocks, unsigned rank,
+                                          unsigned long long& v, F&& join, unsigned long long* w, G&& join_w,
+                                          W&& meanwhile) {
+  v = over_warp<32>(v, join);
+  if (w != nullptr) *w = over_warp<32>(*w, join_w);
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) {
+    m.warps[0][threadIdx.x >> 5] = v;
+    if (w != nullptr) m.warps[1][threadIdx.x >> 5] = *w;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    v = m.warps[0][lane & (THREADS / 32 - 1)];
+    if (w != nullptr) *w = m.warps[1][lane & (THREADS / 32 - 1)];
+    v = over_warp<THREADS / 32>(v, join);
+    if (w != nullptr) *w = over_warp<THREADS / 32>(*w, join_w);
+    if (lane < blocks) {
+      store_at(&m.said[turn][0][rank], lane, v);
+      if (w != nullptr) store_at(&m.said[turn][1][rank], lane, *w);
+    }
+  }
+  cluster_arrive();
+  meanwhile();
+  cluster_wait();
+  // every warp joins what the blocks said
+  v = m.said[turn][0][lane & (blocks - 1)];
+  if (w != nullptr) *w = m.said[turn][1][lane & (blocks - 1)];
+  if constexpr (std::is_same_v<std::remove_cv_t<std::remove_reference_t<F>>, Larger>) {
+    v = over_warp<32>(v, join);
+  } else {
+    for (int o = blocks / 2; o > 0; o >>= 1) v = join(v, __shfl_xor_sync(0xffffffffu, v, o));
+  }
+  if (w != nullptr)
+    for (int o = blocks / 2; o > 0; o >>= 1) *w = join_w(*w, __shfl_xor_sync(0xffffffffu, *w, o));
+  turn ^= 1;
+}
+template <typename F>
+__device__ __forceinline__ unsigned long long meet(Meeting& m, int& turn, int blocks, unsigned rank,
+                                                   unsigned long long v, F&& join) {
+  meet_pair(m, turn, blocks, rank, v, join, (unsigned long long*)nullptr, join, [] {});
+  return v;
+}
 // The border of a rule between the tokens of one bin of weights, found where it lies between too many
 // equal or nearly equal ones for the list in shared memory: a bit of the place a meeting, 52 meetings.
 // The largest cut for which `amount(cut)`, the cluster's sum over the bin's places >= cut, reaches `need`.
@@ -665,10 +680,18 @@ sample_rules_kernel(const SampleArgs a) {
         const int lane = tid & 31;
         const unsigned base = __reduce_add_sync(0xffffffffu, lane < (int)rank ?
             load_at(slice < 0 ? &bins.count[b] : &bins.slice_count[slice], lane) : 0u);
+        // (values a bin further on either side than the border's bin, and what rounding could make of
+        // that; most tokens lie outside)
+        const float far = (float)(b + 2) / bins_t, room = 0x1p-21f * (fabsf(M) + far);
+        const float v_from = b == BINS - 1 ? -INFINITY : (M - far) - room;
+        const float v_to = (M - (float)(b - 1) / bins_t) + room;
 #pragma unroll 2
         for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
           const float4 f = four_at(i);
           const float v[4] = {f.x, f.y, f.z, f.w};
+          if (!((v[0] >= v_from && v[0] <= v_to) || (v[1] >= v_from && v[1] <= v_to) ||
+                (v[2] >= v_from && v[2] <= v_to) || (v[3] >= v_from && v[3] <= v_to)))
+            continue;
           bool in[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) in[j] = in_border(v[j]);

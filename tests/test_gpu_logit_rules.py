@@ -238,6 +238,19 @@ def test_borders_among_many_nearly_equal_logits(ops, V, spread):
     check(ops, dev(logits), logits, rules)
 
 
+@pytest.mark.parametrize("size,heat", [(1e6, 0.01), (3e7, 2.0), (1e-30, 1e-31), (200.0, 0.003), (1.0, 1e5)])
+def test_logits_and_temperatures_of_any_size(ops, size, heat):
+    """Steps between neighbouring 32-bit logits wider than a bin of the histogram, logits near the
+    smallest numbers, temperatures that make all tokens or one of them likely."""
+    n, V = 12, 6000
+    rng = np.random.RandomState(3)
+    logits = (size * (1 + 1e-6 * rng.randn(n, V))).astype(np.float32)
+    logits[::2] = (size * rng.randn(6, V)).astype(np.float32)
+    rules = dict(temperature=[heat] * n, top_k=[0, 0, 700, 50] * 3, top_p=[0.9, 0.5, 0.7] * 4,
+                 streams=list(range(n)), steps=[4] * n)
+    check(ops, dev(logits), logits, rules)
+
+
 def test_draws_of_a_large_vocabulary(ops):
     rows = Rows(ops, 12, 128256, seed=2)
     check(ops, rows.device_logits, rows.edited(), rules_of(12, 2, top_k=(0, 50, 1000, 100000)), rows.edits)
