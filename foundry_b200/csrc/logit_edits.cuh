@@ -72,28 +72,6 @@ __device__ __forceinline__ float fb_penalised(const FbRowEdits& e, float v, int 
   return v;
 }
 
-// Four neighbouring logits i..i+3 of a row, i a multiple of 4, whose bits of the history are
-// `held & 15`: the words of those whose bit is set, in one load where `aligned` says that it may be one
-// (the words of the others are not looked at).
-__device__ __forceinline__ int4 fb_words_of(const FbRowEdits& e, int i, unsigned held, bool aligned) {
-  int4 w = make_int4(0, 0, 0, 0);
-  if (aligned) {
-    if (held & 15u) w = *reinterpret_cast<const int4*>(e.counts + i);
-  } else {
-    if (held & 1u) w.x = e.counts[i];
-    if (held & 2u) w.y = e.counts[i + 1];
-    if (held & 4u) w.z = e.counts[i + 2];
-    if (held & 8u) w.w = e.counts[i + 3];
-  }
-  return w;
-}
-__device__ __forceinline__ void fb_penalise(const FbRowEdits& e, float4& v, const int4& w, unsigned held) {
-  if (held & 1u) v.x = fb_penalised(e, v.x, w.x);
-  if (held & 2u) v.y = fb_penalised(e, v.y, w.y);
-  if (held & 4u) v.z = fb_penalised(e, v.z, w.z);
-  if (held & 8u) v.w = fb_penalised(e, v.w, w.w);
-}
-
 // The biases of a row that fall into [lo, hi), added to values that lie in shared memory from lo
 // on. Threads look at the row's whole list side by side (a request has some hundreds at most). Equal
 // ids stand side by side, and the first one's thread adds them all, in order.

@@ -294,6 +294,15 @@ sample_rules_kernel(const SampleArgs a) {
     __syncthreads();
   }
   const bool biased = row.bias_from < row.bias_to;
+  // Rows with a history or biases: the logits go to shared memory as they are, with the places of the
+  // history's tokens on a list (in the bins' room, which nobody needs yet), and the block's threads work
+  // the list off, one load of a count each, all at once (logit_edits.cu says what that saves).
+  const bool deferred = biased || row.counts != nullptr;
+  __shared__ int hit_count;
+  unsigned short* hits = reinterpret_cast<unsigned short*>(&bins);
+  constexpr int MOST_HITS = sizeof(Bins) / 2;
+  if (deferred && tid == 0) hit_count = 0;
+  if (deferred) __syncthreads();
   float top = -INFINITY;  // the thread's best value, and where it comes first
   int top_at = -1;
   // a value on its way out of the edits: NaN has no chance, like a token that is not allowed
@@ -304,11 +313,19 @@ sample_rules_kernel(const SampleArgs a) {
   };
   const unsigned* seen = row.counts != nullptr ? row.seen + (lo >> 5) : nullptr;
   const unsigned* allowed = row.allowed != nullptr ? row.allowed + (lo >> 5) : nullptr;
+  // tokens i + (the set bits of `held`) of this block; those that find no room are seen to at once
+  auto list_hits = [&](int i, unsigned held) {
+    int at = atomicAdd(&hit_count, __popc(held));
+    for (; held != 0u; held &= held - 1, ++at) {
+      const int where = i + __ffs(held) - 1;
+      if (at < MOST_HITS) hits[at] = (unsigned short)where;
+      else values[where] = fb_penalised(row, values[where], row.counts[lo + where]);
+    }
+  };
   int done = 0;
   if ((reinterpret_cast<uintptr_t>(from) & 15) == 0) {
-    // four float4 a thread on their way together, then the words of their histories
+    // four float4 a thread on their way together
     done = mine & ~3;
-    const bool whole_words = (reinterpret_cast<uintptr_t>(row.counts + lo) & 15) == 0;
     constexpr int AHEAD = 4;
     for (int i0 = tid * 4; i0 < done; i0 += THREADS * 4 * AHEAD) {
       float4 got[AHEAD];
@@ -321,49 +338,57 @@ sample_rules_kernel(const SampleArgs a) {
         if (i < done) {
           got[j] = *reinterpret_cast<const float4*>(from + i);
           if (seen != nullptr) held[j] = seen[i >> 5] >> (i & 31) & 15u;
-          if (allowed != nullptr) ok[j] = allowed[i >> 5] >> (i & 31);
+          if (allowed != nullptr && !deferred) ok[j] = allowed[i >> 5] >> (i & 31);
         }
-      }
-      if (seen != nullptr) {
-        int4 words[AHEAD];
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j) words[j] = fb_words_of(row, lo + i0 + j * THREADS * 4, held[j], whole_words);
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j)
-          if (held[j] != 0u) fb_penalise(row, got[j], words[j], held[j]);
       }
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) {
         const int i = i0 + j * THREADS * 4;
         if (i >= done) break;
-        if (!biased) {
+        if (!deferred) {
           got[j].x = settle(got[j].x, i, ok[j] & 1u);
           got[j].y = settle(got[j].y, i + 1, ok[j] & 2u);
           got[j].z = settle(got[j].z, i + 2, ok[j] & 4u);
           got[j].w = settle(got[j].w, i + 3, ok[j] & 8u);
         }
         *reinterpret_cast<float4*>(values + i) = got[j];
+        if (held[j] != 0u) list_hits(i, held[j]);
       }
     }
   }
   for (int i = done + tid; i < mine; i += THREADS) {
-    float v = from[i];
-    if (seen != nullptr && (seen[i >> 5] >> (i & 31) & 1u)) v = fb_penalised(row, v, row.counts[lo + i]);
-    values[i] = biased ? v : settle(v, i, allowed != nullptr ? allowed[i >> 5] >> (i & 31) & 1u : 1u);
+    values[i] = deferred ? from[i] : settle(from[i], i, allowed != nullptr ? allowed[i >> 5] >> (i & 31) & 1u : 1u);
+    if (seen != nullptr && (seen[i >> 5] >> (i & 31) & 1u)) list_hits(i, 1u);
   }
   // what is looked at four by four ends with tokens that have no chance
   const int padded = (mine + 3) & ~3;
   if (mine + tid < padded) values[mine + tid] = -INFINITY;
+  if (deferred) {
+    __syncthreads();
+    const int listed = min(hit_count, MOST_HITS);
+    for (int i = tid; i < listed; i += THREADS) {
+      const int where = hits[i];
+      values[where] = fb_penalised(row, values[where], row.counts[lo + where]);
+    }
+    __syncthreads();
+    if (biased) {
+      fb_add_biases(a.edits, row, values, lo, hi);
+      __syncthreads();
+    }
+#pragma unroll 2
+    for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
+      float4 f = *reinterpret_cast<float4*>(values + i);
+      const unsigned ok = allowed != nullptr ? allowed[i >> 5] >> (i & 31) : ~0u;
+      f.x = settle(f.x, i, ok & 1u);
+      f.y = settle(f.y, i + 1, ok & 2u);
+      f.z = settle(f.z, i + 2, ok & 4u);
+      f.w = settle(f.w, i + 3, ok & 8u);
+      *reinterpret_cast<float4*>(values + i) = f;
+    }
+  }
   if (cuts) {
     for (int b = tid; b < BINS; b += THREADS) bins.count[b] = bins.part[b] = 0;
     if (tid < 2) bins.found[tid] = bins.counted[tid] = bins.slice_found[tid] = 0;
-  }
-  if (biased) {
-    __syncthreads();
-    fb_add_biases(a.edits, row, values, lo, hi);
-    __syncthreads();
-    for (int i = tid; i < mine; i += THREADS)
-      values[i] = settle(values[i], i, allowed != nullptr ? allowed[i >> 5] >> (i & 31) & 1u : 1u);
   }
   const float inv_t = greedy ? 1.f : 1.0f / T;
   // exp(-(M - v) / T) as a power of two; the factor -log2(e) / T, log2(e) in two parts, rounded once
@@ -448,27 +473,27 @@ sample_rules_kernel(const SampleArgs a) {
       }
     }
   } else {
+    unsigned far = 0;
 #pragma unroll 2
     for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
       const float4 f = four_at(i);
       const float v[4] = {f.x, f.y, f.z, f.w};
-      unsigned far = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float t = binned(v[j]);
-        if (!in_last_bin(t)) {
-          const int b = bin_of(t);
+        const bool near = !in_last_bin(t);
+        const unsigned part = part_of(t);
+        const int b = bin_of(t);
+        if (near) {
           atomicAdd(&bins.count[b], 1u);
-          atomicAdd(&bins.part[b], part_of(t));
-        } else {
-          far += v[j] != -INFINITY;
+          atomicAdd(&bins.part[b], part);
         }
-      }
-      if (far != 0) {  // the last bin may hold nearly all tokens: their number is made by warps
-        const unsigned together = __activemask(), sum = __reduce_add_sync(together, far);
-        if ((tid & 31) == __ffs(together) - 1) atomicAdd(&bins.count[BINS - 1], sum);
+        far += !near && v[j] != -INFINITY;
       }
     }
+    // the last bin may hold nearly all tokens: their number is made by warps
+    far = __reduce_add_sync(0xffffffffu, far);
+    if ((tid & 31) == 0 && far != 0) atomicAdd(&bins.count[BINS - 1], far);
     // each block adds up its share of the bins over the cluster and tells everybody
     const int share = BINS / blocks;
     cluster_arrive();

@@ -251,6 +251,22 @@ def test_logits_and_temperatures_of_any_size(ops, size, heat):
     check(ops, dev(logits), logits, rules)
 
 
+def test_a_history_of_nearly_all_tokens(ops):
+    """More of the history's tokens in a block's share of a row than its list has room for."""
+    n, V = 10, 150016
+    rng = np.random.RandomState(8)
+    logits = (rng.randn(n, V) * 3).astype(np.float32)
+    table = rng.randint(0, 4, (n, V)).astype(np.int32)
+    table[rng.rand(n, V) < 0.3] |= plain.IN_PROMPT
+    table[0] = 1
+    rep, freq, pres = (np.full(n, v, np.float32) for v in (1.3, 0.2, 0.1))
+    edits = ops.LogitEdits(ops.TokenHistory(dev(table), dev(plain.pack_bits(table != 0))), torch.arange(n, dtype=torch.int32, device=DEV),
+                           dev(rep), dev(freq), dev(pres))
+    edited = np.stack([plain.edited(logits[r], table[r], rep[r], freq[r], pres[r]) for r in range(n)])
+    same(ops.edit_logits(dev(logits), edits), edited)
+    check(ops, dev(logits), edited, rules_of(n, 8), edits)
+
+
 def test_draws_of_a_large_vocabulary(ops):
     rows = Rows(ops, 12, 128256, seed=2)
     check(ops, rows.device_logits, rows.edited(), rules_of(12, 2, top_k=(0, 50, 1000, 100000)), rows.edits)
