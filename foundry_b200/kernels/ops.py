@@ -1940,6 +1940,20 @@ def _given(t, name: str, dtype: torch.dtype, shape, device: int) -> int:
     return t.data_ptr()
 
 
+def _a_row_each(n: int, device: int, given):
+    """The addresses of (name, tensor or None, type) with one entry for each of `n` rows."""
+    out = []
+    for name, t, dtype in given:
+        if t is None:
+            out.append(0)
+        elif t.dtype is dtype and t.numel() == n and t.dim() == 1 and t.is_contiguous() \
+                and t.get_device() == device:
+            out.append(t.data_ptr())
+        else:
+            out.append(_given(t, name, dtype, (n,), device))  # says what is wrong
+    return out
+
+
 def _on_current_device(t: torch.Tensor, name: str) -> None:
     if not t.is_cuda:
         raise KernelError(f"{name} is on {t.device}; the kernels run on CUDA devices only")
@@ -2058,12 +2072,13 @@ class LogitEdits:
         if h is not None:
             if h.vocab != vocab:
                 raise KernelError(f"a history of {h.vocab} tokens for logits of {vocab}")
-            out[:4] = (_given(h.counts, "counts", torch.int32, None, device),
-                       _given(h.seen, "seen", torch.int32, None, device),
-                       _given(self.history_rows, "history_rows", torch.int32, (n,), device), h.rows)
-            out[5:8] = (_given(self.repetition, "repetition", torch.float32, (n,), device),
-                        _given(self.frequency, "frequency", torch.float32, (n,), device),
-                        _given(self.presence, "presence", torch.float32, (n,), device))
+            i32, f32 = torch.int32, torch.float32
+            out[0] = _given(h.counts, "counts", i32, None, device)
+            out[1] = _given(h.seen, "seen", i32, None, device)
+            out[3] = h.rows
+            out[2], out[5], out[6], out[7] = _a_row_each(n, device, (
+                ("history_rows", self.history_rows, i32), ("repetition", self.repetition, f32),
+                ("frequency", self.frequency, f32), ("presence", self.presence, f32)))
         b = self.bias
         if b is not None:
             out[8:12] = (_given(b.starts, "starts", torch.int32, (n + 1,), device),
@@ -2144,19 +2159,14 @@ def sample_tokens(logits: torch.Tensor, rules: SampleRules, edits: Optional[Logi
         raise KernelError("sample_tokens: tokens to record, and no history")
     at = logits.get_device()
     packed = None if edits is None else edits.packed(n, V, at)
-    r, each = rules, (n,)
-    _call("fb_sample_rules", logits.data_ptr(), stride, n, V,
-          _given(r.temperature, "temperature", torch.float32, each, at),
-          _given(r.top_k, "top_k", torch.int32, each, at),
-          _given(r.top_p, "top_p", torch.float32, each, at),
-          _given(r.min_p, "min_p", torch.float32, each, at),
-          _given(r.streams, "streams", torch.int64, each, at),
-          _given(r.steps, "steps", torch.int64, each, at),
-          0 if packed is None else ctypes.addressof(packed),
-          _given(record, "record", torch.int32, each, at),
-          _given(out, "out", torch.int32, each, at),
-          _given(logprobs, "logprobs", torch.float32, each, at),
-          _given(also, "also", torch.int32, each, at), _stream(), tag=("n{} v{}", n, V))
+    r, f32, i32, i64 = rules, torch.float32, torch.int32, torch.int64
+    rows = _a_row_each(n, at, (
+        ("temperature", r.temperature, f32), ("top_k", r.top_k, i32), ("top_p", r.top_p, f32),
+        ("min_p", r.min_p, f32), ("streams", r.streams, i64), ("steps", r.steps, i64),
+        ("record", record, i32), ("out", out, i32), ("logprobs", logprobs, f32), ("also", also, i32)))
+    _call("fb_sample_rules", logits.data_ptr(), stride, n, V, *rows[:6],
+          0 if packed is None else ctypes.addressof(packed), *rows[6:], _stream(),
+          tag=("n{} v{}", n, V))
     return out, logprobs
 
 
