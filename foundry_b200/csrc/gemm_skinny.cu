@@ -142,6 +142,7 @@ constexpr int MODE_SINK = 2;   // add into the residual rows in front of a norm
 constexpr int MODE_MANY = 3;   // store; the grid holds several products
 constexpr int MODE_CLAMP = 4;  // (gate, up) pairs with clamped halves and biases
 constexpr int MODE_ADAPT = 5;  // store, each token's low-rank adapter added (adapter.cu)
+constexpr int STAGED_LOW = 1024;  // rank numbers that its blocks fetch ahead
 // What MODE_ADAPT adds to feature n of token t: sum_j low[t, j] b[index[t]][n, j] (an index outside of
 // the bank: nothing), in front of the row scale.
 struct AdapterAdd {
@@ -179,6 +180,11 @@ gemm_skinny_kernel(const __nv_bfloat16* x, long long ldx,
   __shared__ float red[WARPS][16][8 * NT + 1];
   __shared__ float scale_part[4][16];
   extern __shared__ __align__(16) float shares[];  // [scale.count][16] when there is a row scale
+  constexpr bool ADAPT = MODE == MODE_ADAPT;
+  constexpr bool AHEAD = ADAPT && NT == 1;  // (the registers of 16 tokens are full)
+  constexpr int STAGED = AHEAD ? (WARPS == 4 ? 4 : 2) : 0;  // pieces of b a thread
+  __shared__ __align__(16) uint4 b_staged[STAGED + 1][AHEAD ? WARPS * 32 : 1];
+  __shared__ __align__(16) float low_staged[AHEAD ? STAGED_LOW : 4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   int group = blockIdx.x;
@@ -277,8 +283,25 @@ gemm_skinny_kernel(const __nv_bfloat16* x, long long ldx,
   // thread's old residual values and norm weights into registers.
   constexpr int SINK_ITEMS = SINK ? (16 * 8 * NT + WARPS * 32 - 1) / (WARPS * 32) : 1;
   float old_resid[SINK_ITEMS], gamma[SINK_ITEMS];
+  // MODE_ADAPT: neighbouring lanes share a (token, feature)'s row of b, 16 bytes each and round; as many as
+  // there are threads for the 16 * T sums, and pieces in a row. A thread has two sums at most.
+  constexpr int SUMS = ADAPT ? (16 * 8 * NT + WARPS * 32 - 1) / (WARPS * 32) : 1;
+  int sum_lanes = 1, slot_of[SUMS];
+  if constexpr (ADAPT)
+    while (sum_lanes < 32 && 8 * sum_lanes < sink.rank && 2 * sum_lanes * 16 * T <= WARPS * 32) sum_lanes *= 2;
+  auto read_slots = [&]() {
+    if constexpr (ADAPT) {
+#pragma unroll
+      for (int it = 0; it < SUMS; ++it) {
+        const int at = threadIdx.x / sum_lanes + it * (WARPS * 32 / sum_lanes);
+        slot_of[it] = (at >> 4) < T && n0 + (at & 15) < N
+                          ? *reinterpret_cast<const volatile int*>(sink.index + (at >> 4)) : -1;
+      }
+    }
+  };
   auto after_wait = [&]() {
     fb_pdl_wait();
+    if constexpr (AHEAD) read_slots();
     if (scale.ss != nullptr) {
       // Every CTA of the grid wants the same few lines: through L1 (.ca), so that
       // the CTAs of an SM ask L2 once, and only the T floats of a row that count.
@@ -326,6 +349,32 @@ gemm_skinny_kernel(const __nv_bfloat16* x, long long ldx,
       if (lane < TOKS) scale_part[warp][lane] = sum;
     }
   };
+  // The first pieces of b and the rank numbers are asked for beside the weight stream, as the row scale is:
+  // fetched by the epilogue, one after the other, they cost 8 tokens of 4,096 -> 28,672 4 us.
+  bool low_ahead = false;
+  if constexpr (AHEAD) low_ahead = T * sink.rank <= STAGED_LOW;
+  auto ask_for_adapter = [&]() {
+    if constexpr (AHEAD) {
+      int n = 0;
+#pragma unroll
+      for (int it = 0; it < SUMS; ++it) {
+        const int at = threadIdx.x / sum_lanes + it * (WARPS * 32 / sum_lanes);
+        const __nv_bfloat16* brow = sink.b + ((size_t)max(slot_of[it], 0) * N + n0 + (at & 15)) * sink.rank;
+        for (int i = lane & (sum_lanes - 1); i < (sink.rank >> 3) && n < STAGED; i += sum_lanes, ++n) {
+          if (slot_of[it] < 0 || slot_of[it] >= sink.slots) continue;
+          const uint32_t dst = (uint32_t)__cvta_generic_to_shared(&b_staged[n][threadIdx.x]);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(brow + i * 8) : "memory");
+        }
+      }
+      if (low_ahead) {
+        for (int i = threadIdx.x * 4; i < T * sink.rank; i += WARPS * 128) {
+          const uint32_t dst = (uint32_t)__cvta_generic_to_shared(low_staged + i);
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(sink.low + i) : "memory");
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  };
   for (; c + UNROLL <= full_end; c += UNROLL) {
     uint4 a[UNROLL][4];
 #pragma unroll
@@ -353,7 +402,7 @@ gemm_skinny_kernel(const __nv_bfloat16* x, long long ldx,
       uint4 b[UNROLL][NT][2];
 #pragma unroll
       for (int u = 0; u < UNROLL; ++u) load_x(b[u], u);
-      if (first) finish_scale();
+      if (first) { finish_scale(); ask_for_adapter(); }
 #pragma unroll
       for (int u = 0; u < UNROLL; ++u) multiply(a[u], b[u]);
     } else {
@@ -363,7 +412,7 @@ gemm_skinny_kernel(const __nv_bfloat16* x, long long ldx,
       // and ran three CTAs to an SM, or spilled under the cap).
       uint4 b[2][NT][2];
       load_x(b[0], 0);
-      if (first) finish_scale();
+      if (first) { finish_scale(); ask_for_adapter(); }
 #pragma unroll
       for (int u = 0; u < UNROLL; ++u) {
         if (u + 1 < UNROLL) load_x(b[(u + 1) & 1], u + 1);
@@ -374,6 +423,7 @@ gemm_skinny_kernel(const __nv_bfloat16* x, long long ldx,
   if (!waited) {
     after_wait();
     finish_scale();
+    ask_for_adapter();
   }
   // the rest: single chunks, the last of which may reach beyond K
   for (; c < c1; ++c) {
@@ -408,6 +458,7 @@ gemm_skinny_kernel(const __nv_bfloat16* x, long long ldx,
     red[warp][g + 8][j * 8 + 2 * t] = acc[j][2];
     red[warp][g + 8][j * 8 + 2 * t + 1] = acc[j][3];
   }
+  if constexpr (AHEAD) asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
   // token `tok`'s scale, by whoever needs it (no barrier more for a shared copy)
   auto row_scale = [&](int tok) {
@@ -495,34 +546,32 @@ gemm_skinny_kernel(const __nv_bfloat16* x, long long ldx,
           __float2bfloat16_rn(fb_glu_clamped(sink, gate * rs + b0, up * rs + b1));
     }
   } else if constexpr (MODE == MODE_ADAPT) {
-    // Neighbouring lanes share a row of b, 16 bytes each and round; as many as there are threads for the
-    // 16 * T sums, and pieces in a row.
-    const int pieces = sink.rank >> 3;
-    int lanes = 1;
-    while (lanes < 32 && lanes < pieces && 2 * lanes * 16 * T <= WARPS * 32) lanes *= 2;
-    const int part = lane & (lanes - 1);
-    for (int at = threadIdx.x / lanes; at < (16 * T + 31) / 32 * 32; at += WARPS * 32 / lanes) {  // (whole warps)
-      const int row = at & 15, tok = at >> 4;
-      const bool live = tok < T && n0 + row < N;
-      const int slot = live ? *reinterpret_cast<const volatile int*>(sink.index + tok) : -1;
-      float v = 0.f;
-      if (slot >= 0 && slot < sink.slots) {
-        const __nv_bfloat16* brow = sink.b + ((size_t)slot * N + n0 + row) * sink.rank;
-        const float* low = sink.low + (size_t)tok * sink.rank;
-        for (int i = part; i < pieces; i += lanes) {
-          const uint4 q = ld_cached(brow + i * 8);
-          const uint4 lo = ld_cached(low + i * 8), hi = ld_cached(low + i * 8 + 4);
-          const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
-          const float* f0 = reinterpret_cast<const float*>(&lo);
-          const float* f1 = reinterpret_cast<const float*>(&hi);
+    const int lanes = sum_lanes, pieces = sink.rank >> 3, part = lane & (lanes - 1);
+    if constexpr (!AHEAD) read_slots();
+    int n = 0;  // of the staged pieces
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float2 b0 = __bfloat1622float2(h[e]), b1 = __bfloat1622float2(h[e + 2]);
-            v = fmaf(f0[2 * e], b0.x, v);
-            v = fmaf(f0[2 * e + 1], b0.y, v);
-            v = fmaf(f1[2 * e], b1.x, v);
-            v = fmaf(f1[2 * e + 1], b1.y, v);
-          }
+    for (int it = 0; it < SUMS; ++it) {
+      const int at = threadIdx.x / lanes + it * (WARPS * 32 / lanes);
+      const int row = at & 15, tok = at >> 4, slot = slot_of[it];
+      const bool live = tok < T && n0 + row < N;
+      float v = 0.f;
+      const __nv_bfloat16* brow = sink.b + ((size_t)max(slot, 0) * N + n0 + row) * sink.rank;
+      for (int i = part; i < pieces; i += lanes, ++n) {
+        if (slot < 0 || slot >= sink.slots) continue;
+        const float* low = (low_ahead ? low_staged : sink.low) + tok * sink.rank + i * 8;
+        const uint4 q = n < STAGED ? b_staged[n][threadIdx.x] : ld_cached(brow + i * 8);
+        const uint4 lo = low_ahead ? *reinterpret_cast<const uint4*>(low) : ld_cached(low);
+        const uint4 hi = low_ahead ? *reinterpret_cast<const uint4*>(low + 4) : ld_cached(low + 4);
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
+        const float* f0 = reinterpret_cast<const float*>(&lo);
+        const float* f1 = reinterpret_cast<const float*>(&hi);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 b0 = __bfloat1622float2(h[e]), b1 = __bfloat1622float2(h[e + 2]);
+          v = fmaf(f0[2 * e], b0.x, v);
+          v = fmaf(f0[2 * e + 1], b0.y, v);
+          v = fmaf(f1[2 * e], b1.x, v);
+          v = fmaf(f1[2 * e + 1], b1.y, v);
         }
       }
       for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

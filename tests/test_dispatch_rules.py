@@ -124,3 +124,22 @@ def test_low_rank_kernel_by_rank_tokens_and_type():
     (200, 2048, False, 2), (500, 8192, False, 1), (600, 8192, False, 2)])
 def test_form_of_the_experts_products_by_rows_an_expert(rows, K, gated, form):
     assert ops.grouped_form(16 * rows, 16, K, gated) == form
+
+
+@pytest.mark.parametrize("T,N,pays", [(16, 1 << 20, False), (64, 1 << 20, False), (65, 28672, True), (48, 28672, False),
+                                      (256, 4096, False), (384, 4096, True), (512, 4096, True), (512, 2048, False),
+                                      (8192, 128, False), (12288, 128, True), (1 << 20, 127, False)])
+def test_adapters_behind_k_by_the_sums_that_it_saves(T, N, pays):
+    assert ops._planes_pay(T, N) == pays
+
+
+def test_rank_numbers_on_tensor_maps_by_alignment_and_places():
+    """Rows that a tensor map cannot take, and more places than the kernel keeps marks for, go elsewhere."""
+    def fits(K=64, slots=4, dtype=torch.bfloat16, pad=0):
+        x = torch.zeros(300, K + pad, dtype=dtype)[:, :K]
+        w = torch.zeros(64, K, dtype=dtype)
+        bank = types.SimpleNamespace(a=torch.zeros(slots, 8, K, dtype=dtype), b=torch.zeros(slots, 64, 8, dtype=dtype),
+                                     slots=slots, rank=8)
+        return ops._low_fits(x, w, bank)
+    assert fits() and fits(pad=8) and fits(slots=1024)
+    assert not fits(slots=1025) and not fits(K=60) and not fits(pad=4) and not fits(dtype=torch.float32)

@@ -102,6 +102,40 @@ def test_without_an_adapter_it_is_the_product(ops):
         assert torch.allclose(got, want, rtol=2.0 ** -8 * 1.01, atol=1024 * 2.0 ** -24 * 1024 * 0.05)
 
 
+@pytest.mark.parametrize("N", [64, 256])  # the rank numbers as rows, and as planes behind K
+@pytest.mark.parametrize("T", [8192, 8193, 8200, 16500])
+def test_more_tokens_than_one_launch_takes(ops, T, N):
+    x, w, bank, index = case(ops, T, 64, N, 8, 3, torch.bfloat16, pad=8)
+    check(ops, x, w, bank, index, ops.adapted_product(x, w, bank, index), True)
+
+
+@pytest.mark.parametrize("T", [5, 300, 7000])
+@pytest.mark.parametrize("S", [1024, 1025, 3000])
+def test_banks_of_thousands_of_places(ops, T, S):
+    """More than the tensor cores' kernel keeps its marks for; blocks with as many adapters as tokens."""
+    x, w, bank, index = case(ops, T, 64, 256, 8, S, torch.bfloat16)
+    check(ops, x, w, bank, index, ops.adapted_product(x, w, bank, index), True)
+
+
+def test_prompts_and_single_tokens_on_two_streams(ops):
+    """One bank and index for projections of prompts and of single tokens, in turn and on two streams."""
+    x, w, bank, index = case(ops, 600, 512, 4096, 16, 4, torch.bfloat16)
+    few = [x[i:i + 3].contiguous() for i in range(0, 30, 3)]
+    of_few = [index[i:i + 3].contiguous() for i in range(0, 30, 3)]
+    want, want_few = ops.adapted_product(x, w, bank, index), [
+        ops.adapted_product(t, w, bank, i) for t, i in zip(few, of_few)]
+    torch.cuda.synchronize()
+    side, got_few = torch.cuda.Stream(), []
+    for _ in range(3):
+        got = ops.adapted_product(x, w, bank, index)
+        with torch.cuda.stream(side), ops.scratch_owner("adapters beside"):
+            got_few = [ops.adapted_product(t, w, bank, i) for t, i in zip(few, of_few)]
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    assert all(torch.equal(g, v) for g, v in zip(got_few, want_few))
+    ops.release_scratch("adapters beside")
+
+
 def test_no_tokens(ops):
     x, w, bank, index = case(ops, 0, 64, 32, 8, 1, torch.bfloat16, index=[])
     assert ops.adapted_product(x, w, bank, index).shape == (0, 32)

@@ -210,6 +210,45 @@ def test_adapters_beside_the_feed_forwards_of_another_architecture(tmp_path):
     assert np.abs(results[2] - results[1]).max() > 1e-2 * scale
 
 
+@pytest.mark.parametrize("family,name,names", [
+    ("tokovik", "mixed", ("l0.mlp.gate", "l2.mlp.up", "l2.mlp.down")),
+    ("tokovik", "other", ("l0.mlp.down", "l1.mlp.gate", "l1.mlp.up")),
+    ("vonulorn", "mixed", ("l0.mlp.up", "l2.mlp.gate", "l3.mlp.down")),
+    ("vonulorn", "other", ("l1.mlp.gate", "l2.mlp.down"))])
+def test_adapters_under_every_arrangement_of_parts(tmp_path, family, name, names):
+    """The same where a constant scales the parts' outputs, norms stand behind them, or the layers' streams
+    are summed: what a part with adapters returns is taken like what it returns without."""
+    import importlib
+    from foundry_b200 import Engine, SequenceStep
+    from foundry_b200.weights.safetensors_io import SINGLE_FILE, save_file
+    made = importlib.import_module(f"{family}_tiny")
+    folder, weights = made.write_folder(str(tmp_path / "plain"), name)
+    merged_folder, _ = made.write_folder(str(tmp_path / "merged"), name)
+    g = torch.Generator().manual_seed(0)
+    tensors, merged = {}, dict(weights)
+    for where in names:
+        rows, cols = weights[where].shape
+        a, b = torch.randn(8, cols, generator=g) / cols ** 0.5, torch.randn(rows, 8, generator=g) * 0.3
+        tensors[f"{where}.lora_A.weight"], tensors[f"{where}.lora_B.weight"] = a, b
+        merged[where] = (weights[where].double() + 0.5 * b.double() @ a.double()).float()
+    save_file(merged, str(tmp_path / "merged" / SINGLE_FILE), metadata={"format": "pt"})
+    tokens = tiny.random_tokens(3, 30, made.CONFIGS[name].get("vocab_size", made.CONFIGS[name].get("vocab", 64)))
+    results = []
+    for where, adapter in ((folder, "x"), (merged_folder, None), (folder, None)):
+        engine = Engine.from_folder(where, dtype="float32", max_tokens=1024, max_slots=4)
+        if adapter:
+            engine.enable_adapters(2, 8)
+            engine.load_adapter("x", tensors, 0.5)
+        slot = engine.open_sequence(adapter) if adapter else engine.open_sequence()
+        rows = [engine.step([SequenceStep(slot, tokens[:26], [25])])[0].cpu()]
+        rows += [engine.step([SequenceStep(slot, [t], [0])])[0].cpu() for t in tokens[26:]]
+        results.append(torch.stack(rows).double().numpy())
+    # (both are within 2e-5 of the logit scale of the exact sums)
+    scale = max(1.0, np.abs(results[1]).max())
+    assert np.abs(results[0] - results[1]).max() <= 4e-5 * scale
+    assert np.abs(results[2] - results[1]).max() > 1e-2 * scale
+
+
 # ------------------------------------------------------------- rules and edits
 def simulate(setting, prompt, params, key, steps, name=None, stops=()):
     """The plain model's tokens under a request's rules, their log-probabilities, and how far 32-bit ones
