@@ -118,10 +118,8 @@ void shrink_by_size(const T* x, long long ldx, const T* a, const float* scales, 
 // A row of B is read by L neighbouring lanes, 16 bytes each, so that a load of the warp takes 512 bytes that
 // lie side by side (a thread a feature, which reads its row alone, made 32 lines of every load: 48 tokens,
 // 4,096 features, rank 64, 11 us for the kernel). A lane keeps its few ranks' numbers of a token, multiplies
-// L features, and the lanes exchange sums so that each ends with the whole sum of one feature. Four tokens
-// a block: neighbours with the same adapter use the row that is there.
+// L features, and the lanes exchange sums so that each ends with the whole sum of one feature.
 constexpr int EXPAND_THREADS = 128;
-constexpr int EXPAND_TOKENS = 4;
 template <int L> constexpr int ROUNDS_OF = L >= 4 ? 1 : 4 / L;  // of 32 features a warp
 
 template <typename T>
@@ -155,26 +153,26 @@ __device__ __forceinline__ float share_out(float (&v)[L], int li) {
   return v[0];
 }
 
-template <typename T, typename Out, int L>
+template <typename T, typename Out, int L, int TOKENS>
 __global__ void __launch_bounds__(EXPAND_THREADS, L <= 8 ? 6 : 3)
 adapter_expand_kernel(const float* base, int planes, long long plane_stride, long long ldb, const float* low,
                       const T* b, const int* index, int slots, int rank, int tokens, int N, Out* out,
                       long long ldo) {
   constexpr int EACH = 16 / sizeof(T), ROUNDS = ROUNDS_OF<L>, GROUPS = 32 / L;
-  extern __shared__ __align__(16) float mine[];  // [EXPAND_TOKENS][rank]
-  __shared__ int s_slot[EXPAND_TOKENS];
+  extern __shared__ __align__(16) float mine[];  // [TOKENS][rank]
+  __shared__ int s_slot[TOKENS];
   fb_pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, li = lane % L, group = lane / L;
-  const int t0 = blockIdx.y * EXPAND_TOKENS, live = min(EXPAND_TOKENS, tokens - t0);
+  const int t0 = blockIdx.y * TOKENS, live = min(TOKENS, tokens - t0);
   const int n0 = (blockIdx.x * (EXPAND_THREADS / 32) + (tid >> 5)) * 32 * ROUNDS;
-  if (tid < EXPAND_TOKENS) {
+  if (tid < TOKENS) {
     const int slot = tid < live ? index[t0 + tid] : -1;
     s_slot[tid] = slot < slots ? slot : -1;
   }
   // what the projection left for this lane's features
-  float sum[EXPAND_TOKENS][ROUNDS];
+  float sum[TOKENS][ROUNDS];
 #pragma unroll
-  for (int t = 0; t < EXPAND_TOKENS; ++t)
+  for (int t = 0; t < TOKENS; ++t)
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
       const int n = n0 + r * 32 + li * GROUPS + group;
@@ -185,7 +183,7 @@ adapter_expand_kernel(const float* base, int planes, long long plane_stride, lon
 #pragma unroll 2
   for (int p = 1; p < planes; ++p)
 #pragma unroll
-    for (int t = 0; t < EXPAND_TOKENS; ++t)
+    for (int t = 0; t < TOKENS; ++t)
 #pragma unroll
       for (int r = 0; r < ROUNDS; ++r) {
         const int n = n0 + r * 32 + li * GROUPS + group;
@@ -199,7 +197,7 @@ adapter_expand_kernel(const float* base, int planes, long long plane_stride, lon
     uint4 raw[ROUNDS * L];
     int there = -1;
 #pragma unroll
-    for (int t = 0; t < EXPAND_TOKENS; ++t) {
+    for (int t = 0; t < TOKENS; ++t) {
       const int slot = s_slot[t];
       if (slot < 0) continue;
       const bool in = li * EACH < rank;
@@ -254,12 +252,12 @@ adapter_expand_kernel(const float* base, int planes, long long plane_stride, lon
       }
       const float whole = share_out<L>(v, li);
 #pragma unroll
-      for (int q = 0; q < EXPAND_TOKENS; ++q)  // (registers have no runtime index)
+      for (int q = 0; q < TOKENS; ++q)  // (registers have no runtime index)
         if (q == t) sum[q][0] += whole;
     }
   }
 #pragma unroll
-  for (int t = 0; t < EXPAND_TOKENS; ++t)
+  for (int t = 0; t < TOKENS; ++t)
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
       const int n = n0 + r * 32 + li * GROUPS + group;
@@ -267,14 +265,24 @@ adapter_expand_kernel(const float* base, int planes, long long plane_stride, lon
     }
 }
 
+// Tokens a block: one until that makes more blocks than the SMs hold at a time, then two or four, which
+// reuse a row of B where neighbours share it (2,048 -> 4,096, rank 16, 4 adapters, the whole operator with one,
+// two and four: 17 tokens 11.0, 11.4, 11.6 us; 128 tokens 15.8, 14.5, 15.1; 256 21.2, 19.1, 18.0; 2,048 ->
+// 28,672, rank 32, 64 tokens 48, 42, 40. With eight: 15.3 at 64 tokens against 13.3, and never ahead by 2%).
 template <typename T, typename Out, int L>
 void launch_expand(const float* base, int planes, long long plane_stride, long long ldb, const float* low,
                    const T* b, const int* index, int slots, int rank, int tokens, int N, Out* out, long long ldo,
                    cudaStream_t stream) {
   constexpr int FEATURES = EXPAND_THREADS * ROUNDS_OF<L>;
-  const dim3 grid((N + FEATURES - 1) / FEATURES, (tokens + EXPAND_TOKENS - 1) / EXPAND_TOKENS);
-  fb_launch(adapter_expand_kernel<T, Out, L>, grid, dim3(EXPAND_THREADS), (size_t)EXPAND_TOKENS * rank * 4, stream,
-            base, planes, plane_stride, ldb, low, b, index, slots, rank, tokens, N, out, ldo);
+  const int columns = (N + FEATURES - 1) / FEATURES;
+  const long long once = 12LL * sm_count();
+  auto launch = [&](auto kernel, int each) {
+    fb_launch(kernel, dim3(columns, (tokens + each - 1) / each), dim3(EXPAND_THREADS), (size_t)each * rank * 4,
+              stream, base, planes, plane_stride, ldb, low, b, index, slots, rank, tokens, N, out, ldo);
+  };
+  if ((long long)columns * tokens <= once) launch(adapter_expand_kernel<T, Out, L, 1>, 1);
+  else if ((long long)columns * tokens <= 2 * once) launch(adapter_expand_kernel<T, Out, L, 2>, 2);
+  else launch(adapter_expand_kernel<T, Out, L, 4>, 4);
 }
 
 // As many lanes a row of B as it has pieces of 16 bytes (a power of two, 32 at most).
@@ -314,7 +322,7 @@ FB_API int fb_adapter_expand(const float* base, int planes, long long plane_stri
   FB_REQUIRE(T >= 0 && N > 0 && rank > 0 && rank <= 512 && rank % 8 == 0 && slots > 0 && planes > 0 && ldb >= N &&
                  ldo >= N && (((uintptr_t)b | (uintptr_t)low) % 16) == 0,
              "adapter_expand: bad sizes T=%d N=%d rank=%d, or operands not on 16-byte boundaries", T, N, rank);
-  FB_REQUIRE(T <= 4 * 65535, "adapter_expand: %d tokens (262140 at most)", T);
+  FB_REQUIRE(T <= 65535, "adapter_expand: %d tokens (65535 at most)", T);
   if (T == 0) return 0;
   FB_DISPATCH_DTYPE(dtype, E, FB_DISPATCH_DTYPE(out_dtype, O,
       expand_by_rank(base, planes, plane_stride, ldb, low, (const E*)b, index, slots, rank, T, N, (O*)out, ldo,
