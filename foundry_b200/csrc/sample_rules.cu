@@ -12,6 +12,13 @@
 //
 // Both borders are cuts in one order: token i of value v has the 52-bit place
 // (ordered bits of v) << 20 | (2^20 - 1 - i), larger = earlier, and a cut keeps the places >= cut.
+//
+// A row is read once, into the shared memory of a cluster. What bounds it is not those bytes (64 rows of
+// 128,256: 34.7 MB, 5.3 us at the copy rate) but the passes over shared memory (116 instructions a logit
+// under mixed rules, a third of the SMs' issue slots), and for few rows the meetings of the cluster one
+// after another, 1.2 to 1.7 us each: the maximum, the bins, a border, the winner. Device times in graph
+// replays at 128,256 tokens, by rule (greedy, plain, top-k, top-p): one row 6.0, 7.7, 14.6, 15 us; 8 rows
+// 8.1, 10.8, 19.8, 28; 64 rows 24, 34, 53, 85 (two rounds of clusters).
 #include "logit_edits.cuh"
 
 #include <type_traits>
@@ -200,7 +207,8 @@ __device__ __noinline__ unsigned long long cut_by_bits(F&& amount, unsigned long
 // that is further than 32. Inside a bin the weights exp(-d) are exp(-b / 32) (1 - part), with part below
 // 0.031; its 22-bit fraction adds up as whole numbers, so that the sums do not depend on the order
 // in which threads come. What the last bin weighs (V exp(-32) at most) is left out of the sums.
-// Bins half as wide (and a sorted list half as long) cost twice the exchange: see the launcher's note.
+// Wider or finer was not better: with the near bins and the rest in two zones, or a list of 1,024, 64 rows of
+// 128,256 under every kind of rule took 86 us and more where this takes 73.
 constexpr int BINS = 1024;
 constexpr float BINS_PER_UNIT = 32.f;
 constexpr int PART_BITS = 22;
@@ -356,9 +364,29 @@ sample_rules_kernel(const SampleArgs a) {
       }
     }
   }
-  for (int i = done + tid; i < mine; i += THREADS) {
-    values[i] = deferred ? from[i] : settle(from[i], i, allowed != nullptr ? allowed[i >> 5] >> (i & 31) & 1u : 1u);
-    if (seen != nullptr && (seen[i >> 5] >> (i & 31) & 1u)) list_hits(i, 1u);
+  // rows that start elsewhere, and the last tokens: eight loads a thread on their way together
+  constexpr int ONES = 8;
+  for (int i0 = done + tid; i0 < mine; i0 += THREADS * ONES) {
+    float got[ONES];
+    unsigned held[ONES], ok[ONES];
+#pragma unroll
+    for (int j = 0; j < ONES; ++j) {
+      const int i = i0 + j * THREADS;
+      held[j] = 0u;
+      ok[j] = 1u;
+      if (i < mine) {
+        got[j] = from[i];
+        if (seen != nullptr) held[j] = seen[i >> 5] >> (i & 31) & 1u;
+        if (allowed != nullptr && !deferred) ok[j] = allowed[i >> 5] >> (i & 31) & 1u;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < ONES; ++j) {
+      const int i = i0 + j * THREADS;
+      if (i >= mine) break;
+      values[i] = deferred ? got[j] : settle(got[j], i, ok[j]);
+      if (held[j] != 0u) list_hits(i, 1u);
+    }
   }
   // what is looked at four by four ends with tokens that have no chance
   const int padded = (mine + 3) & ~3;
@@ -850,37 +878,70 @@ sample_rules_kernel(const SampleArgs a) {
   // (the last meeting's barrier is behind every word to another block)
 }
 
-// How many clusters of 16 blocks the device runs at once (0: none), with the kernel set up for it.
-int wide_clusters(int* count) {
-  static int of_device[64] = {};
+// How many clusters of 1, 2, 4, 8 and 16 blocks the device runs at once where an SM has one block (0: none),
+// with the kernel set up for it.
+int clusters_at_once(const int** counts) {
+  static int of_device[64][6] = {};  // the last number: made
   int device = 0;
   cudaGetDevice(&device);
   if (device < 0 || device >= 64) device = 63;
-  if (of_device[device] == 0) {
+  int* const of = of_device[device];
+  if (of[5] == 0) {
     const int most = MAX_CHUNK * 4 + (int)sizeof(Bins);
     cudaError_t e = cudaFuncSetAttribute(sample_rules_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(sample_rules_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return fb_fail(2, "sample_rules: setting the kernel up: %s", cudaGetErrorString(e));
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(1, 1, 16);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = most;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 16;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, sample_rules_kernel, &cfg) != cudaSuccess) {
-      cudaGetLastError();
-      n = 0;
+    for (int i = 0; i < 5; ++i) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(1, 1, 1 << i);
+      cfg.blockDim = dim3(THREADS);
+      cfg.dynamicSmemBytes = most;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 1;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1 << i;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, sample_rules_kernel, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n = 0;
+      }
+      of[i] = n;
     }
-    of_device[device] = n > 0 ? n : -1;
+    of[5] = 1;
   }
-  *count = of_device[device] > 0 ? of_device[device] : 0;
+  *counts = of;
+  return 0;
+}
+
+// Blocks a row. The most that leave every block an SM of its own (eight; sixteen for long rows), down to 1,000
+// logits a block; where even the fewest that hold a row do not, the fewest of which two fit an SM. Measured with
+// 1, 2, 4, 8, 16 blocks, plain draws and top-p:
+//   1 row of 128,256: -, -, 15.9 and 22.7, 11.0 and 18.6, 8.2 and 15.5 us;
+//   33 rows of 32,000: 16.0 and 43, 11.2 and 31, 8.7 and 22, 9.4 and 27, 19.5 and 52;
+//   64 rows of 32,000: 16.2 and 43, 11.5 and 32, 11.8 and 30, 18.3 and 45, 35 and 84;
+//   256 rows of 8,000: 12 and 30, 17 and 40, 28 and 63, 51 and 123, 115 and 286.
+int blocks_a_row(int n, int V, int* blocks) {
+  const int* at_once;
+  if (int rc = clusters_at_once(&at_once)) return rc;
+  const bool wide = at_once[4] > 0;
+  if (wide && (V > 8 * MAX_CHUNK || (V >= 65536 && 16 * n <= sm_count()))) {
+    *blocks = 16;
+    return 0;
+  }
+  for (int i = 3; i >= 0; --i) {
+    if ((i > 0 && V < 1000 << i) || V > MAX_CHUNK << i) continue;
+    if (n <= at_once[i]) {
+      *blocks = 1 << i;
+      return 0;
+    }
+  }
+  constexpr int TWO_AN_SM = 20000;
+  *blocks = 1;
+  while (*blocks < 8 && V > TWO_AN_SM * *blocks) *blocks *= 2;
   return 0;
 }
 }  // namespace
@@ -901,11 +962,8 @@ FB_API int fb_sample_rules(const float* logits, long long row_stride, int n, int
   if (int rc = fb_check_edits("sample_rules", a.edits, V)) return rc;
   FB_REQUIRE(record == nullptr || a.edits.counts != nullptr, "sample_rules: tokens to record, and no history");
   if (n == 0) return 0;
-  int blocks = 1;
-  while (blocks < 8 && V > 4096 * blocks) blocks *= 2;
-  int wide = 0;
-  if (int rc = wide_clusters(&wide)) return rc;
-  if (wide > 0 && (V > 8 * MAX_CHUNK || (V > 65536 && 16 * n <= sm_count()))) blocks = 16;
+  int blocks = 0;
+  if (int rc = blocks_a_row(n, V, &blocks)) return rc;
   FB_REQUIRE(V <= blocks * MAX_CHUNK, "sample_rules: a vocabulary of %d (%d at most here)", V, blocks * MAX_CHUNK);
   a.logits = logits; a.row_stride = row_stride; a.V = V;
   a.chunk = ((V + blocks - 1) / blocks + 31) / 32 * 32;  // whole words of the bits
