@@ -273,8 +273,16 @@ __device__ __forceinline__ void store_word_at(void* mine, unsigned rank, unsigne
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there), "r"(v) : "memory");
 }
 
+template <int BYTES>
+__device__ __forceinline__ void copy_async(float* to, const float* from) {
+  const unsigned there = (unsigned)__cvta_generic_to_shared(to);
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(there), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(there), "l"(from) : "memory");
+}
+
 // A row by a cluster of `gridDim.z` blocks, each with `chunk` of its logits in shared memory.
-__global__ void __launch_bounds__(THREADS, 2)
+template <int AN_SM>
+__global__ void __launch_bounds__(THREADS, AN_SM)
 sample_rules_kernel(const SampleArgs a) {
   cluster_arrive();  // waited for in front of the first word to another block: it has to be there
   fb_pdl_wait();
@@ -302,117 +310,67 @@ sample_rules_kernel(const SampleArgs a) {
     __syncthreads();
   }
   const bool biased = row.bias_from < row.bias_to;
-  // Rows with a history or biases: the logits go to shared memory as they are, with the places of the
-  // history's tokens on a list (in the bins' room, which nobody needs yet), and the block's threads work
-  // the list off, one load of a count each, all at once (logit_edits.cu says what that saves).
-  const bool deferred = biased || row.counts != nullptr;
+  // The logits go to shared memory as they are, all asked for at once (loads into registers took a trip to
+  // memory for every 8,192 of a block). Meanwhile the places of the history's tokens are put on a list (in the
+  // bins' room, which nobody needs yet), which the block's threads then work off, one load of a count each, all
+  // at once (logit_edits.cu says what that saves).
   __shared__ int hit_count;
   unsigned short* hits = reinterpret_cast<unsigned short*>(&bins);
   constexpr int MOST_HITS = sizeof(Bins) / 2;
-  if (deferred && tid == 0) hit_count = 0;
-  if (deferred) __syncthreads();
+  int done = 0;
+  if ((reinterpret_cast<uintptr_t>(from) & 15) == 0) {
+    done = mine & ~3;
+    for (int i = 4 * tid; i < done; i += 4 * THREADS) copy_async<16>(values + i, from + i);
+  }
+  for (int i = done + tid; i < mine; i += THREADS) copy_async<4>(values + i, from + i);
+  // what is looked at four by four ends with tokens that have no chance
+  const int padded = (mine + 3) & ~3;
+  if (mine + tid < padded) values[mine + tid] = -INFINITY;
+  const unsigned* allowed = row.allowed != nullptr ? row.allowed + (lo >> 5) : nullptr;
+  if (row.counts != nullptr) {
+    if (tid == 0) hit_count = 0;
+    __syncthreads();
+    for (int w = tid; 32 * w < mine; w += THREADS) {
+      unsigned held = row.seen[(lo >> 5) + w];
+      if (mine - 32 * w < 32) held &= (1u << (mine - 32 * w)) - 1;
+      if (held == 0u) continue;
+      int at = atomicAdd(&hit_count, __popc(held));
+      for (; held != 0u && at < MOST_HITS; held &= held - 1, ++at) hits[at] = (unsigned short)(32 * w + __ffs(held) - 1);
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  if (row.counts != nullptr) {
+    auto penalise = [&](int i) { values[i] = fb_penalised(row, values[i], row.counts[lo + i]); };
+    if (hit_count <= MOST_HITS) {
+      for (int i = tid; i < hit_count; i += THREADS) penalise(hits[i]);
+    } else {  // (the list has no room for so many)
+      for (int i = tid; i < mine; i += THREADS)
+        if (row.seen[(lo + i) >> 5] >> (i & 31) & 1u) penalise(i);
+    }
+    __syncthreads();
+  }
+  if (biased) {
+    fb_add_biases(a.edits, row, values, lo, hi);
+    __syncthreads();
+  }
+  // NaN has no chance, like a token that is not allowed
   float top = -INFINITY;  // the thread's best value, and where it comes first
   int top_at = -1;
-  // a value on its way out of the edits: NaN has no chance, like a token that is not allowed
   auto settle = [&](float v, int i, unsigned ok) {
     v = ok ? fmaxf(v, -INFINITY) : -INFINITY;
     if (v > top) { top = v; top_at = i; }
     return v;
   };
-  const unsigned* seen = row.counts != nullptr ? row.seen + (lo >> 5) : nullptr;
-  const unsigned* allowed = row.allowed != nullptr ? row.allowed + (lo >> 5) : nullptr;
-  // tokens i + (the set bits of `held`) of this block; those that find no room are seen to at once
-  auto list_hits = [&](int i, unsigned held) {
-    int at = atomicAdd(&hit_count, __popc(held));
-    for (; held != 0u; held &= held - 1, ++at) {
-      const int where = i + __ffs(held) - 1;
-      if (at < MOST_HITS) hits[at] = (unsigned short)where;
-      else values[where] = fb_penalised(row, values[where], row.counts[lo + where]);
-    }
-  };
-  int done = 0;
-  if ((reinterpret_cast<uintptr_t>(from) & 15) == 0) {
-    // four float4 a thread on their way together
-    done = mine & ~3;
-    constexpr int AHEAD = 4;
-    for (int i0 = tid * 4; i0 < done; i0 += THREADS * 4 * AHEAD) {
-      float4 got[AHEAD];
-      unsigned held[AHEAD], ok[AHEAD];
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        const int i = i0 + j * THREADS * 4;
-        held[j] = 0u;
-        ok[j] = ~0u;
-        if (i < done) {
-          got[j] = *reinterpret_cast<const float4*>(from + i);
-          if (seen != nullptr) held[j] = seen[i >> 5] >> (i & 31) & 15u;
-          if (allowed != nullptr && !deferred) ok[j] = allowed[i >> 5] >> (i & 31);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        const int i = i0 + j * THREADS * 4;
-        if (i >= done) break;
-        if (!deferred) {
-          got[j].x = settle(got[j].x, i, ok[j] & 1u);
-          got[j].y = settle(got[j].y, i + 1, ok[j] & 2u);
-          got[j].z = settle(got[j].z, i + 2, ok[j] & 4u);
-          got[j].w = settle(got[j].w, i + 3, ok[j] & 8u);
-        }
-        *reinterpret_cast<float4*>(values + i) = got[j];
-        if (held[j] != 0u) list_hits(i, held[j]);
-      }
-    }
-  }
-  // rows that start elsewhere, and the last tokens: eight loads a thread on their way together
-  constexpr int ONES = 8;
-  for (int i0 = done + tid; i0 < mine; i0 += THREADS * ONES) {
-    float got[ONES];
-    unsigned held[ONES], ok[ONES];
-#pragma unroll
-    for (int j = 0; j < ONES; ++j) {
-      const int i = i0 + j * THREADS;
-      held[j] = 0u;
-      ok[j] = 1u;
-      if (i < mine) {
-        got[j] = from[i];
-        if (seen != nullptr) held[j] = seen[i >> 5] >> (i & 31) & 1u;
-        if (allowed != nullptr && !deferred) ok[j] = allowed[i >> 5] >> (i & 31) & 1u;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < ONES; ++j) {
-      const int i = i0 + j * THREADS;
-      if (i >= mine) break;
-      values[i] = deferred ? got[j] : settle(got[j], i, ok[j]);
-      if (held[j] != 0u) list_hits(i, 1u);
-    }
-  }
-  // what is looked at four by four ends with tokens that have no chance
-  const int padded = (mine + 3) & ~3;
-  if (mine + tid < padded) values[mine + tid] = -INFINITY;
-  if (deferred) {
-    __syncthreads();
-    const int listed = min(hit_count, MOST_HITS);
-    for (int i = tid; i < listed; i += THREADS) {
-      const int where = hits[i];
-      values[where] = fb_penalised(row, values[where], row.counts[lo + where]);
-    }
-    __syncthreads();
-    if (biased) {
-      fb_add_biases(a.edits, row, values, lo, hi);
-      __syncthreads();
-    }
 #pragma unroll 2
-    for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
-      float4 f = *reinterpret_cast<float4*>(values + i);
-      const unsigned ok = allowed != nullptr ? allowed[i >> 5] >> (i & 31) : ~0u;
-      f.x = settle(f.x, i, ok & 1u);
-      f.y = settle(f.y, i + 1, ok & 2u);
-      f.z = settle(f.z, i + 2, ok & 4u);
-      f.w = settle(f.w, i + 3, ok & 8u);
-      *reinterpret_cast<float4*>(values + i) = f;
-    }
+  for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
+    float4 f = *reinterpret_cast<float4*>(values + i);
+    const unsigned ok = allowed != nullptr ? allowed[i >> 5] >> (i & 31) : ~0u;
+    f.x = settle(f.x, i, ok & 1u);
+    f.y = settle(f.y, i + 1, ok & 2u);
+    f.z = settle(f.z, i + 2, ok & 4u);
+    f.w = settle(f.w, i + 3, ok & 8u);
+    *reinterpret_cast<float4*>(values + i) = f;
   }
   if (cuts) {
     for (int b = tid; b < BINS; b += THREADS) bins.count[b] = bins.part[b] = 0;
@@ -888,9 +846,11 @@ int clusters_at_once(const int** counts) {
   int* const of = of_device[device];
   if (of[5] == 0) {
     const int most = MAX_CHUNK * 4 + (int)sizeof(Bins);
-    cudaError_t e = cudaFuncSetAttribute(sample_rules_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(sample_rules_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    cudaError_t e = cudaSuccess;
+    for (auto kernel : {sample_rules_kernel<1>, sample_rules_kernel<2>}) {
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    }
     if (e != cudaSuccess) return fb_fail(2, "sample_rules: setting the kernel up: %s", cudaGetErrorString(e));
     for (int i = 0; i < 5; ++i) {
       cudaLaunchConfig_t cfg = {};
@@ -905,7 +865,7 @@ int clusters_at_once(const int** counts) {
       cfg.attrs = attr;
       cfg.numAttrs = 1;
       int n = 0;
-      if (cudaOccupancyMaxActiveClusters(&n, sample_rules_kernel, &cfg) != cudaSuccess) {
+      if (cudaOccupancyMaxActiveClusters(&n, sample_rules_kernel<1>, &cfg) != cudaSuccess) {
         cudaGetLastError();
         n = 0;
       }
@@ -917,6 +877,8 @@ int clusters_at_once(const int** counts) {
   return 0;
 }
 
+constexpr int TWO_AN_SM = 20000;  // logits a block at most for two of them on an SM
+
 // Blocks a row. The most that leave every block an SM of its own (eight; sixteen for long rows), down to 1,000
 // logits a block; where even the fewest that hold a row do not, the fewest of which two fit an SM. Measured with
 // 1, 2, 4, 8, 16 blocks, plain draws and top-p:
@@ -924,12 +886,14 @@ int clusters_at_once(const int** counts) {
 //   33 rows of 32,000: 16.0 and 43, 11.2 and 31, 8.7 and 22, 9.4 and 27, 19.5 and 52;
 //   64 rows of 32,000: 16.2 and 43, 11.5 and 32, 11.8 and 30, 18.3 and 45, 35 and 84;
 //   256 rows of 8,000: 12 and 30, 17 and 40, 28 and 63, 51 and 123, 115 and 286.
-int blocks_a_row(int n, int V, int* blocks) {
+int blocks_a_row(int n, int V, int* blocks, int* an_sm) {
   const int* at_once;
   if (int rc = clusters_at_once(&at_once)) return rc;
   const bool wide = at_once[4] > 0;
+  *an_sm = 1;
   if (wide && (V > 8 * MAX_CHUNK || (V >= 65536 && 16 * n <= sm_count()))) {
     *blocks = 16;
+    if (n > at_once[4] && V <= 16 * TWO_AN_SM) *an_sm = 2;
     return 0;
   }
   for (int i = 3; i >= 0; --i) {
@@ -939,9 +903,9 @@ int blocks_a_row(int n, int V, int* blocks) {
       return 0;
     }
   }
-  constexpr int TWO_AN_SM = 20000;
   *blocks = 1;
   while (*blocks < 8 && V > TWO_AN_SM * *blocks) *blocks *= 2;
+  if (V <= TWO_AN_SM * *blocks) *an_sm = 2;
   return 0;
 }
 }  // namespace
@@ -962,15 +926,15 @@ FB_API int fb_sample_rules(const float* logits, long long row_stride, int n, int
   if (int rc = fb_check_edits("sample_rules", a.edits, V)) return rc;
   FB_REQUIRE(record == nullptr || a.edits.counts != nullptr, "sample_rules: tokens to record, and no history");
   if (n == 0) return 0;
-  int blocks = 0;
-  if (int rc = blocks_a_row(n, V, &blocks)) return rc;
+  int blocks = 0, an_sm = 1;
+  if (int rc = blocks_a_row(n, V, &blocks, &an_sm)) return rc;
   FB_REQUIRE(V <= blocks * MAX_CHUNK, "sample_rules: a vocabulary of %d (%d at most here)", V, blocks * MAX_CHUNK);
   a.logits = logits; a.row_stride = row_stride; a.V = V;
   a.chunk = ((V + blocks - 1) / blocks + 31) / 32 * 32;  // whole words of the bits
   a.temperature = temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p;
   a.streams = streams; a.steps = steps; a.record = record;
   a.out = out; a.logprobs = logprobs; a.also = also;
-  fb_launch_cluster(sample_rules_kernel, dim3(n, 1, blocks), dim3(THREADS),
+  fb_launch_cluster(an_sm == 2 ? sample_rules_kernel<2> : sample_rules_kernel<1>, dim3(n, 1, blocks), dim3(THREADS),
                     (size_t)a.chunk * 4 + sizeof(Bins), stream,
                     (unsigned)blocks, a);
   return fb_check_launch("sample_rules");
