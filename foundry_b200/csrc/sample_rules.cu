@@ -57,12 +57,14 @@ __device__ __forceinline__ unsigned long long mix64(unsigned long long z) {
 }
 constexpr unsigned long long GOLDEN = 0x9e3779b97f4a7c15ULL;
 
+__device__ __forceinline__ unsigned random_at(unsigned long long z) {
+  z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ULL;
+  return (unsigned)(((z ^ (z >> 27)) * 0x94d049bb133111ebULL) >> 32);
+}
 // The upper half of token i's random number; its top 24 bits are those of the number that sampling.cu
 // makes (whose last exclusive-or does not reach them).
 __device__ __forceinline__ unsigned random_of(unsigned long long of_step, unsigned i) {
-  unsigned long long z = of_step + GOLDEN * ((unsigned long long)i + 1);
-  z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ULL;
-  return (unsigned)(((z ^ (z >> 27)) * 0x94d049bb133111ebULL) >> 32);
+  return random_at(of_step + GOLDEN * ((unsigned long long)i + 1));
 }
 // -log(-log u). 24 bits and a half are 25, and the largest rounds u to one, whose noise would be
 // infinite: any token would win with it. u stays below one.
@@ -75,6 +77,13 @@ __device__ __forceinline__ float exp2_fast(float a) {
   float v;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v) : "f"(a));
   return v;
+}
+
+// A weight in 64 bits: it is positive or zero and no denormal number, so its bits need only be moved (zero
+// becomes 2^-127, nothing beside the largest weight, which is one). The conversion runs at an eighth of the rate.
+__device__ __forceinline__ double widened(float w) {
+  const unsigned b = __float_as_uint(w);
+  return __hiloint2double((int)((b >> 3) + (896u << 20)), (int)(b << 29));
 }
 
 __device__ __forceinline__ unsigned ordered(float v) {
@@ -212,8 +221,9 @@ __device__ __noinline__ unsigned long long cut_by_bits(F&& amount, unsigned long
 constexpr int BINS = 1024;
 constexpr float BINS_PER_UNIT = 32.f;
 constexpr int PART_BITS = 22;
-constexpr int LISTED = 512;  // tokens of a border's bin that are put in order in shared memory
+constexpr int LISTED = 128;  // tokens of a border's bin that are compared with each other in shared memory
 constexpr int SLICES = THREADS;
+static_assert(LISTED * 4 == THREADS, "four threads a token of the list, or more");
 
 // A distance in 32nds: its bin (an edge belongs to either side, always the same one), and 1 - exp(-x) of
 // what is left of it, x <= 1 / 32, by its series (the next term is below 2^-31), in units of 2^-22. Whole
@@ -245,11 +255,12 @@ struct Bins {
   unsigned count[BINS], part[BINS];      // this block's tokens
   unsigned all_count[BINS];              // the row's
   float all_weight[BINS];
-  unsigned long long listed[LISTED];
+  unsigned long long listed[LISTED], own[LISTED];  // the row's, and this block's part of them
   unsigned long long scan_warps[2][THREADS / 32];
   // of each of the two borders: its bin + 1, this block's tokens in it so far, what stands in front
-  unsigned found[2], counted[2], count_front[2], tokens[2];
+  unsigned found[2], counted[2], last[2], count_front[2], tokens[2], weighs[LISTED];
   double weight_front[2];
+  unsigned long long cut[2];
   // the same for a border's bin cut up once more, where it holds more tokens than the list: a slice a
   // thread; weights in two halves of 11 bits, then whole
   unsigned slice_count[SLICES], slice_low[SLICES], slice_high[SLICES], all_slice_count[SLICES];
@@ -355,26 +366,47 @@ sample_rules_kernel(const SampleArgs a) {
     __syncthreads();
   }
   // NaN has no chance, like a token that is not allowed
-  float top = -INFINITY;  // the thread's best value, and where it comes first
-  int top_at = -1;
-  auto settle = [&](float v, int i, unsigned ok) {
-    v = ok ? fmaxf(v, -INFINITY) : -INFINITY;
-    if (v > top) { top = v; top_at = i; }
-    return v;
-  };
+  float top = -INFINITY;  // the thread's best value
+  if (allowed != nullptr) {
 #pragma unroll 2
-  for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
-    float4 f = *reinterpret_cast<float4*>(values + i);
-    const unsigned ok = allowed != nullptr ? allowed[i >> 5] >> (i & 31) : ~0u;
-    f.x = settle(f.x, i, ok & 1u);
-    f.y = settle(f.y, i + 1, ok & 2u);
-    f.z = settle(f.z, i + 2, ok & 4u);
-    f.w = settle(f.w, i + 3, ok & 8u);
-    *reinterpret_cast<float4*>(values + i) = f;
+    for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
+      float4 f = *reinterpret_cast<float4*>(values + i);
+      const unsigned ok = allowed[i >> 5] >> (i & 31);
+      f.x = ok & 1u ? fmaxf(f.x, -INFINITY) : -INFINITY;
+      f.y = ok & 2u ? fmaxf(f.y, -INFINITY) : -INFINITY;
+      f.z = ok & 4u ? fmaxf(f.z, -INFINITY) : -INFINITY;
+      f.w = ok & 8u ? fmaxf(f.w, -INFINITY) : -INFINITY;
+      top = fmaxf(fmaxf(top, fmaxf(f.x, f.y)), fmaxf(f.z, f.w));
+      *reinterpret_cast<float4*>(values + i) = f;
+    }
+  } else {
+#pragma unroll 2
+    for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
+      float4 f = *reinterpret_cast<float4*>(values + i);
+      if (isnan((f.x + f.y) + (f.z + f.w))) {  // (or infinities of both signs)
+        f.x = fmaxf(f.x, -INFINITY);
+        f.y = fmaxf(f.y, -INFINITY);
+        f.z = fmaxf(f.z, -INFINITY);
+        f.w = fmaxf(f.w, -INFINITY);
+        *reinterpret_cast<float4*>(values + i) = f;
+      }
+      top = fmaxf(fmaxf(top, fmaxf(f.x, f.y)), fmaxf(f.z, f.w));
+    }
+  }
+  // where it comes first: looked for by the threads that have their warp's best value alone
+  int top_at = -1;
+  if (top > -INFINITY && ordered(top) == __reduce_max_sync(__activemask(), ordered(top))) {
+    for (int i = 4 * tid; top_at < 0; i += 4 * THREADS) {
+      const float4 f = *reinterpret_cast<float4*>(values + i);
+      if (f.x == top) top_at = i;
+      else if (f.y == top) top_at = i + 1;
+      else if (f.z == top) top_at = i + 2;
+      else if (f.w == top) top_at = i + 3;
+    }
   }
   if (cuts) {
     for (int b = tid; b < BINS; b += THREADS) bins.count[b] = bins.part[b] = 0;
-    if (tid < 2) bins.found[tid] = bins.counted[tid] = bins.slice_found[tid] = 0;
+    if (tid < 2) bins.found[tid] = bins.counted[tid] = bins.last[tid] = bins.slice_found[tid] = 0;
   }
   const float inv_t = greedy ? 1.f : 1.0f / T;
   // exp(-(M - v) / T) as a power of two; the factor -log2(e) / T, log2(e) in two parts, rounded once
@@ -428,18 +460,23 @@ sample_rules_kernel(const SampleArgs a) {
       beaten = 1.001f * expf(-value_of(best));
     }
   };
+  // The best of a warp is what its other threads' tokens have to beat as well: of a flat row's tokens nearly
+  // every one that a thread looks at first beats its own best so far.
+  auto share_the_best = [&] { beaten = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(beaten))); };
   double all = 0.0;
   if (!cuts) {  // one pass: the sum of the weights and the draw
     if (greedy) {
 #pragma unroll 2
       for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
         const float4 v = four_at(i);
-        all += ((double)weight_of(v.x) + (double)weight_of(v.y)) + ((double)weight_of(v.z) + (double)weight_of(v.w));
+        all += (widened(weight_of(v.x)) + widened(weight_of(v.y))) + (widened(weight_of(v.z)) + widened(weight_of(v.w)));
       }
     } else {
+      unsigned long long z = of_step + GOLDEN * ((unsigned long long)(lo + 4 * tid) + 1);
 #pragma unroll 2
-      for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
-        const float4 f = four_at(i);
+      for (int i0 = 0; i0 < padded; i0 += 4 * THREADS, z += 4 * THREADS * GOLDEN) {  // (whole warps)
+        const int i = i0 + 4 * tid;
+        const float4 f = i < padded ? four_at(i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
         const float v[4] = {f.x, f.y, f.z, f.w};
         float w[4];
         unsigned random[4];
@@ -447,14 +484,15 @@ sample_rules_kernel(const SampleArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           w[j] = weight_of(v[j]);
-          random[j] = random_of(of_step, (unsigned)(lo + i + j));
+          random[j] = random_at(z + j * GOLDEN);
           any |= may_win(random[j], w[j]);
         }
-        all += ((double)w[0] + (double)w[1]) + ((double)w[2] + (double)w[3]);
-        if (any) {
+        all += (widened(w[0]) + widened(w[1])) + (widened(w[2]) + widened(w[3]));
+        if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             if (may_win(random[j], w[j])) try_token(v[j], random[j], (unsigned)(lo + i + j));
+          share_the_best();
         }
       }
     }
@@ -480,33 +518,28 @@ sample_rules_kernel(const SampleArgs a) {
     // the last bin may hold nearly all tokens: their number is made by warps
     far = __reduce_add_sync(0xffffffffu, far);
     if ((tid & 31) == 0 && far != 0) atomicAdd(&bins.count[BINS - 1], far);
-    // each block adds up its share of the bins over the cluster and tells everybody
-    const int share = BINS / blocks;
+    // Each block adds up its share of the bins over the cluster and tells everybody: blocks / 2 neighbouring
+    // lanes a bin, each with two of the blocks (one thread a bin, asking them all in a row, took 2 us).
+    const int share = BINS / blocks, lanes = max(1, blocks / 2), part_of_bin = tid & (lanes - 1);
     cluster_arrive();
-    double exact_unit = exp(-(double)((int)rank * share + tid) / BINS_PER_UNIT);
+    const double exact_unit = exp(-(double)((int)rank * share + tid / lanes) / BINS_PER_UNIT);
     cluster_wait();
-    for (int i = tid; i < share; i += THREADS) {
+    for (int i = tid / lanes; i < share; i += THREADS / lanes) {  // (a second round only for one block's bins)
       const int b = (int)rank * share + i;
-      unsigned count = 0, counts[MAX_CLUSTER], parts[MAX_CLUSTER];
+      unsigned count = 0;
       unsigned long long part = 0;
-#pragma unroll
-      for (int o = 0; o < MAX_CLUSTER; ++o) {
-        if (o < blocks) {
-          counts[o] = load_at(&bins.count[b], o);
-          parts[o] = load_at(&bins.part[b], o);
-        }
+      for (int o = part_of_bin; o < blocks; o += lanes) {
+        count += load_at(&bins.count[b], o);
+        part += load_at(&bins.part[b], o);
       }
-#pragma unroll
-      for (int o = 0; o < MAX_CLUSTER; ++o) {
-        if (o < blocks) {
-          count += counts[o];
-          part += parts[o];
-        }
+      for (int o = lanes / 2; o > 0; o /= 2) {
+        count += __shfl_xor_sync(0xffffffffu, count, o);
+        part += __shfl_xor_sync(0xffffffffu, part, o);
       }
-      if (i != tid) exact_unit = exp(-(double)b / BINS_PER_UNIT);
+      const double unit = i < THREADS / lanes ? exact_unit : exp(-(double)b / BINS_PER_UNIT);
       const double size = (double)(((unsigned long long)count << PART_BITS) - part) * (1.0 / (1 << PART_BITS));
-      const float weight = b == BINS - 1 ? 0.f : (float)(exact_unit * size);
-      for (int o = 0; o < blocks; ++o) {
+      const float weight = b == BINS - 1 ? 0.f : (float)(unit * size);
+      for (int o = part_of_bin; o < blocks; o += lanes) {
         store_word_at(&bins.all_count[b], o, count);
         store_word_at(&bins.all_weight[b], o, __float_as_uint(weight));
       }
@@ -598,12 +631,23 @@ sample_rules_kernel(const SampleArgs a) {
       unsigned long long front_in_bin = 0;  // in units of the bin
       unsigned n = bins.tokens[rule];
       int slice = -1;
+      // (values a bin further on either side than the border's bin, and what rounding could make of
+      // that; most tokens lie outside)
+      const float far = (float)(b + 2) / bins_t, room = 0x1p-21f * (fabsf(M) + far);
+      const float v_from = b == BINS - 1 ? -INFINITY : (M - far) - room;
+      const float v_to = (M - (float)(b - 1) / bins_t) + room;
+      auto none_near = [&](const float (&v)[4]) {
+        return !((v[0] >= v_from && v[0] <= v_to) || (v[1] >= v_from && v[1] <= v_to) ||
+                 (v[2] >= v_from && v[2] <= v_to) || (v[3] >= v_from && v[3] <= v_to));
+      };
       if (n > LISTED && b != BINS - 1) {  // once more, inside the bin
         bins.slice_count[tid] = bins.slice_low[tid] = bins.slice_high[tid] = 0;
         __syncthreads();
+#pragma unroll 2
         for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
           const float4 f = four_at(i);
           const float v[4] = {f.x, f.y, f.z, f.w};
+          if (none_near(v)) continue;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float t = binned(v[j]);
@@ -616,30 +660,16 @@ sample_rules_kernel(const SampleArgs a) {
           }
         }
         cluster_sync();
-        const int share = SLICES / blocks;
-        if (tid < share) {
-          const int at = (int)rank * share + tid;
-          unsigned counts[MAX_CLUSTER], low[MAX_CLUSTER], high[MAX_CLUSTER], count = 0;
-          unsigned long long weight = 0;
-#pragma unroll
-          for (int o = 0; o < MAX_CLUSTER; ++o) {
-            if (o < blocks) {
-              counts[o] = load_at(&bins.slice_count[at], o);
-              low[o] = load_at(&bins.slice_low[at], o);
-              high[o] = load_at(&bins.slice_high[at], o);
-            }
+        {  // as the bins: a thread a block and a slice
+          const int at = (int)rank * (SLICES / blocks) + tid / blocks, o = tid & (blocks - 1);
+          unsigned count = load_at(&bins.slice_count[at], o);
+          unsigned long long weight = load_at(&bins.slice_low[at], o) + ((unsigned long long)load_at(&bins.slice_high[at], o) << 11);
+          for (int l = blocks / 2; l > 0; l /= 2) {
+            count += __shfl_xor_sync(0xffffffffu, count, l);
+            weight += __shfl_xor_sync(0xffffffffu, weight, l);
           }
-#pragma unroll
-          for (int o = 0; o < MAX_CLUSTER; ++o) {
-            if (o < blocks) {
-              count += counts[o];
-              weight += low[o] + ((unsigned long long)high[o] << 11);
-            }
-          }
-          for (int o = 0; o < blocks; ++o) {
-            store_word_at(&bins.all_slice_count[at], o, count);
-            store_at(&bins.all_slice_weight[at], o, weight);
-          }
+          store_word_at(&bins.all_slice_count[at], o, count);
+          store_at(&bins.all_slice_weight[at], o, weight);
         }
         cluster_sync();
         const unsigned mine_c = bins.all_slice_count[tid];
@@ -691,30 +721,24 @@ sample_rules_kernel(const SampleArgs a) {
         const int lane = tid & 31;
         const unsigned base = __reduce_add_sync(0xffffffffu, lane < (int)rank ?
             load_at(slice < 0 ? &bins.count[b] : &bins.slice_count[slice], lane) : 0u);
-        // (values a bin further on either side than the border's bin, and what rounding could make of
-        // that; most tokens lie outside)
-        const float far = (float)(b + 2) / bins_t, room = 0x1p-21f * (fabsf(M) + far);
-        const float v_from = b == BINS - 1 ? -INFINITY : (M - far) - room;
-        const float v_to = (M - (float)(b - 1) / bins_t) + room;
 #pragma unroll 2
         for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
           const float4 f = four_at(i);
           const float v[4] = {f.x, f.y, f.z, f.w};
-          if (!((v[0] >= v_from && v[0] <= v_to) || (v[1] >= v_from && v[1] <= v_to) ||
-                (v[2] >= v_from && v[2] <= v_to) || (v[3] >= v_from && v[3] <= v_to)))
-            continue;
+          if (none_near(v)) continue;
           bool in[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) in[j] = in_border(v[j]);
           if (in[0] || in[1] || in[2] || in[3]) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              if (!in[j]) continue;
-              const unsigned slot = base + atomicAdd(&bins.counted[rule], 1u);
-              const unsigned long long place = place_of(v[j], (unsigned)(lo + i + j));
-              for (int o = 0; o < blocks; ++o) store_at(&bins.listed[slot], o, place);
-            }
+            for (int j = 0; j < 4; ++j)
+              if (in[j]) bins.own[atomicAdd(&bins.counted[rule], 1u)] = place_of(v[j], (unsigned)(lo + i + j));
           }
+        }
+        __syncthreads();
+        for (unsigned i = tid; i < bins.counted[rule] * blocks; i += THREADS) {
+          const unsigned k = i / blocks;
+          store_at(&bins.listed[base + k], i - k * blocks, bins.own[k]);
         }
         cluster_sync();
         if (n <= 32) {  // every warp for itself: how many are in front of each, and what do they weigh
@@ -737,43 +761,38 @@ sample_rules_kernel(const SampleArgs a) {
           kept_sum = w_front + unit * (double)(front_in_bin + __shfl_sync(0xffffffffu, in_front + weighs, who));
           return __shfl_sync(0xffffffffu, me, who);
         }
-        // in order, the first place first (a bitonic network; zeros behind the tokens)
-        unsigned whole = 64;
-        while (whole < n) whole *= 2;
-        for (unsigned i = n + tid; i < whole; i += THREADS) bins.listed[i] = 0;
+        // a group of neighbouring threads a token: how many are in front of it, and what do they weigh (128
+        // tokens less than 2^29)
+        unsigned each = THREADS / 64;  // threads a token
+        while (each * n > THREADS) each /= 2;
+        const unsigned who = tid / each;
+        const unsigned long long me = who < n ? bins.listed[who] : 0ull;
+        if (tid < (int)n) bins.weighs[tid] = fixed(value_of(bins.listed[tid]));
         __syncthreads();
-        for (unsigned size = 2; size <= whole; size *= 2) {
-          for (unsigned stride = size / 2; stride > 0; stride /= 2) {
-            if ((unsigned)tid < whole / 2) {
-              const unsigned i = 2 * tid - (tid & (stride - 1)), j = i + stride;
-              const unsigned long long x = bins.listed[i], y = bins.listed[j];
-              if ((x < y) == ((i & size) == 0)) { bins.listed[i] = y; bins.listed[j] = x; }
-            }
-            __syncthreads();
+        unsigned ahead = 0, in_front = 0;
+#pragma unroll 4
+        for (unsigned j = tid & (each - 1); j < n; j += each) {
+          if (bins.listed[j] > me) {
+            ++ahead;
+            in_front += bins.weighs[j];
           }
         }
-        // what stands in front of each (512 tokens weigh less than 2^31), and is it kept
-        const unsigned weighs = tid < (int)n ? fixed(value_of(bins.listed[tid])) : 0u;
-        unsigned upto = weighs;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const unsigned other = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += other;
+        for (unsigned o = each / 2; o > 0; o /= 2) {
+          ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+          in_front += __shfl_xor_sync(0xffffffffu, in_front, o);
         }
-        if (lane == 31) bins.scan_warps[1][tid >> 5] = upto;
+        const bool kept = who < n &&
+            (rule == 0 ? c_front + (double)ahead : w_front + unit * (double)(front_in_bin + in_front)) < target;
+        const unsigned many = __reduce_max_sync(0xffffffffu, kept ? ahead + 1 : 0u);
+        if (lane == 0 && many != 0) atomicMax(&bins.last[rule], many);
         __syncthreads();
-        unsigned front = upto - weighs;
-#pragma unroll
-        for (int o = 0; o < THREADS / 32; ++o)
-          if (o < (tid >> 5)) front += (unsigned)bins.scan_warps[1][o];
-        const bool kept = tid < (int)n &&
-            (rule == 0 ? c_front + (double)tid : w_front + unit * (double)(front_in_bin + front)) < target;
-        // (kept ones stand at the list's front)
-        const unsigned many = (unsigned)__syncthreads_count(kept);
-        if (tid == (int)(many > 0 ? many - 1 : 0)) bins.weight_front[rule] = w_front + unit * (double)(front_in_bin + front + weighs);
+        if (who < n && ahead + 1 == max(1u, bins.last[rule]) && (tid & (each - 1)) == 0) {
+          bins.cut[rule] = me;
+          bins.weight_front[rule] = w_front + unit * (double)(front_in_bin + in_front + bins.weighs[who]);
+        }
         __syncthreads();
         kept_sum = bins.weight_front[rule];
-        return bins.listed[many > 0 ? many - 1 : 0];
+        return bins.cut[rule];
       }
       auto amount = [&](unsigned long long cut, bool count) {
         unsigned long long sum = 0;
@@ -806,15 +825,26 @@ sample_rules_kernel(const SampleArgs a) {
     cut = cut < first ? cut : first;
     const float cut_value = cut == 0 ? -INFINITY : value_of(cut);
 #pragma unroll 2
-    for (int i = 4 * tid; i < padded; i += 4 * THREADS) {
-      const float4 f = four_at(i);
-      if (!(fmaxf(fmaxf(f.x, f.y), fmaxf(f.z, f.w)) >= cut_value)) continue;
+    for (int i0 = 0; i0 < padded; i0 += 4 * THREADS) {  // (whole warps)
+      const int i = i0 + 4 * tid;
+      const float4 f = i < padded ? four_at(i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      if (!__any_sync(0xffffffffu, fmaxf(fmaxf(f.x, f.y), fmaxf(f.z, f.w)) >= cut_value)) continue;
       const float v[4] = {f.x, f.y, f.z, f.w};
+      unsigned random[4];
+      bool tried[4], any = false;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (v[j] < cut_value || (v[j] == cut_value && place_of(v[j], (unsigned)(lo + i + j)) < cut)) continue;
-        const unsigned random = random_of(of_step, (unsigned)(lo + i + j));
-        if (may_win(random, weight_of(v[j]))) try_token(v[j], random, (unsigned)(lo + i + j));
+        tried[j] = false;
+        if (v[j] >= cut_value && (v[j] > cut_value || place_of(v[j], (unsigned)(lo + i + j)) >= cut)) {
+          random[j] = random_of(of_step, (unsigned)(lo + i + j));
+          any |= tried[j] = may_win(random[j], weight_of(v[j]));
+        }
+      }
+      if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (tried[j]) try_token(v[j], random[j], (unsigned)(lo + i + j));
+        share_the_best();
       }
     }
   }
