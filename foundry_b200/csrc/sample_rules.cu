@@ -14,11 +14,11 @@
 // (ordered bits of v) << 20 | (2^20 - 1 - i), larger = earlier, and a cut keeps the places >= cut.
 //
 // A row is read once, into the shared memory of a cluster. What bounds it is not those bytes (64 rows of
-// 128,256: 34.7 MB, 5.3 us at the copy rate) but the passes over shared memory (116 instructions a logit
-// under mixed rules, a third of the SMs' issue slots), and for few rows the meetings of the cluster one
-// after another, 1.2 to 1.7 us each: the maximum, the bins, a border, the winner. Device times in graph
-// replays at 128,256 tokens, by rule (greedy, plain, top-k, top-p): one row 6.0, 7.7, 14.6, 15 us; 8 rows
-// 8.1, 10.8, 19.8, 28; 64 rows 24, 34, 53, 85 (two rounds of clusters).
+// 128,256: 34.7 MB, 5.3 us at the copy rate) but the passes over shared memory (some 100 instructions a logit
+// under mixed rules) and the meetings of the cluster one after another, 1 to 1.5 us each: the maximum, the bins,
+// a border, the winner. Device times in graph replays at 128,256 tokens, by rule (greedy, plain, top-k, top-p):
+// one row 6.1, 7.4, 14.1, 14.4 us; 8 rows 7.7, 10.8, 19, 27; 33 rows 10.1, 15.4, 23.5, 41; 64 rows, two rounds
+// of clusters, 19, 32, 51, 77.
 #include "logit_edits.cuh"
 
 #include <type_traits>
@@ -216,8 +216,8 @@ __device__ __noinline__ unsigned long long cut_by_bits(F&& amount, unsigned long
 // that is further than 32. Inside a bin the weights exp(-d) are exp(-b / 32) (1 - part), with part below
 // 0.031; its 22-bit fraction adds up as whole numbers, so that the sums do not depend on the order
 // in which threads come. What the last bin weighs (V exp(-32) at most) is left out of the sums.
-// Wider or finer was not better: with the near bins and the rest in two zones, or a list of 1,024, 64 rows of
-// 128,256 under every kind of rule took 86 us and more where this takes 73.
+// Two zones, near bins and the rest, were slower (64 rows of 128,256 under every kind of rule 86 us where one zone
+// took 82).
 constexpr int BINS = 1024;
 constexpr float BINS_PER_UNIT = 32.f;
 constexpr int PART_BITS = 22;
@@ -292,6 +292,8 @@ __device__ __forceinline__ void copy_async(float* to, const float* from) {
 }
 
 // A row by a cluster of `gridDim.z` blocks, each with `chunk` of its logits in shared memory.
+// AN_SM blocks of it run on an SM: alone there it may use more registers (32,000 tokens a row, top-p 12.3 us
+// against 13.0 for one row, 26.2 against 27.2 for 64).
 template <int AN_SM>
 __global__ void __launch_bounds__(THREADS, AN_SM)
 sample_rules_kernel(const SampleArgs a) {

@@ -238,6 +238,26 @@ def test_borders_among_many_nearly_equal_logits(ops, V, spread):
     check(ops, dev(logits), logits, rules)
 
 
+@pytest.mark.parametrize("m", [1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 257, 600, 3000])
+@pytest.mark.parametrize("V,n", [(7000, 6), (70000, 6), (7000, 200)])
+def test_borders_in_a_bin_of_so_many_tokens(ops, V, n, m):
+    """`m` tokens within a thirtieth of each other, a few in front of them, nothing to speak of behind:
+    both rules' borders among them, in the bin's first, a middle and its last token."""
+    rng = np.random.RandomState(m)
+    logits = np.full((n, V), -40.0, np.float32)
+    for r in range(n):
+        at = rng.permutation(V)[:m + 3]
+        logits[r, at[:3]] = (3.0, 2.5, 2.0)
+        logits[r, at[3:]] = (1.0 + 0.029 * rng.rand(m)).astype(np.float32)
+    first = np.exp(np.array([0.0, -0.5, -1.0])).sum()
+    inside = m * np.exp(-2.0 + 0.0145)
+    share = lambda x: float(np.float32((first + x * inside) / (first + inside)))  # noqa: E731
+    k = [0, 3 + (m + 1) // 2, 4, 0, 3 + m, 3 + (m + 1) // 2]
+    p = [share(0.5), 1.0, 1.0, share(0.02), share(0.99), 0.8]
+    rules = dict(temperature=[1.0] * n, top_k=(k * n)[:n], top_p=(p * n)[:n], streams=list(range(n)), steps=[m] * n)
+    check(ops, dev(logits), logits, rules)
+
+
 @pytest.mark.parametrize("size,heat", [(1e6, 0.01), (3e7, 2.0), (1e-30, 1e-31), (200.0, 0.003), (1.0, 1e5)])
 def test_logits_and_temperatures_of_any_size(ops, size, heat):
     """Steps between neighbouring 32-bit logits wider than a bin of the histogram, logits near the
