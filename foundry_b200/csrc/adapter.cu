@@ -9,6 +9,9 @@
 //   has tokens in the block (zero in the rows of others), and the product takes them as more K behind its
 //   own, [x | planes] [W | B]^T: one sum in tensor memory, one rounding (gemm_tcgen05_pair.cu, MoreK). The
 //   rank numbers are rounded to bfloat16 for that, 2^-9 of the adapter's part on average.
+//   17 to 64 tokens, bfloat16, few adapters: the same with planes by `adapter_shrink` behind the K of the product
+//   that shares K in a cluster (gemm_rows_tcgen05.cu, RowsMore): 48 tokens of 4,096 -> 4,096 with 12 adapters of
+//   rank 64 17.3 us, 19.4 with a pass of its own for the sums; 10.1 without adapters.
 //   Up to 16 tokens, bfloat16: `adapter_shrink` leaves them as 32-bit rows, and the weight-streaming product
 //   adds their product with B in its epilogue (gemm_skinny.cu, MODE_ADAPT). Nothing is rounded in between.
 //   Else: `adapter_shrink` (or, for many numbers, `adapter_low`) leaves them as 32-bit rows, the projection
@@ -36,20 +39,74 @@ __device__ __forceinline__ float dot8(const uint4& a, const uint4& b, float sum)
   return sum;
 }
 
+// The rank numbers as planes for a product that takes them as more K (fb_gemm_rows_adapted): adapter by
+// adapter [256 rows, rank] bfloat16, zero in the rows of other adapters' tokens.
+struct ShrinkPlanes {
+  __nv_bfloat16* u;
+  int* counts;    // [1]: adapters with tokens
+  int* slots_of;  // which they are, in ascending order
+};
+constexpr int PLANE_ROWS = 256, PLANE_SLOTS = 1024;
+
 // low[t, j] = scale * sum_k x[t, k] A[a][j, k], PARTS warps of a block a rank, each with a share of K, so that
 // a warp has few rounds of loads one after another (K = 14,336, 48 tokens, rank 16: one warp a rank 24 us).
-// Block (i, t) has the ranks from i * 8 / PARTS on. `wide`: rows are on 16-byte boundaries.
-template <typename T, int PARTS>
+// Block (i, t) has the ranks from i * 8 / PARTS on. `wide`: rows are on 16-byte boundaries. PLANES: the numbers
+// go to the token's row of its adapter's plane, and zeros to its row of the others.
+template <typename T, int PARTS, bool PLANES>
 __global__ void __launch_bounds__(THREADS)
 adapter_shrink_kernel(const T* x, long long ldx, const T* a, const float* scales, const int* index, int slots,
-                      int rank, int K, int wide, float* low) {
+                      int rank, int K, int wide, float* low, const ShrinkPlanes planes) {
   __shared__ float sums[THREADS / 32];
   fb_pdl_wait();
   fb_pdl_launch();
   const int t = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int j = blockIdx.x * (THREADS / 32 / PARTS) + warp / PARTS;
   const int slot = index[t];
-  if (slot < 0 || slot >= slots) return;  // (the whole block)
+  const bool own = slot >= 0 && slot < slots;
+  __shared__ int s_order;
+  if constexpr (PLANES) {
+    __shared__ unsigned s_present[PLANE_SLOTS / 32];
+    __shared__ int s_count;
+    const int tid = threadIdx.x;
+    if (tid < PLANE_SLOTS / 32) s_present[tid] = 0u;
+    __syncthreads();
+    if (tid < (int)gridDim.y) {  // (256 tokens at most)
+      const int other = index[tid];
+      if (other >= 0 && other < slots) atomicOr(&s_present[other >> 5], 1u << (other & 31));
+    }
+    __syncthreads();
+    if (warp == 0) {
+      const unsigned marks = s_present[lane];
+      const int here = __popc(marks), word = own ? slot >> 5 : 0;
+      const unsigned below = own ? (1u << (slot & 31)) - 1 : 0u;
+      const int count = __reduce_add_sync(0xffffffffu, here);
+      const int order = __reduce_add_sync(0xffffffffu, lane < word ? here : lane == word ? __popc(marks & below) : 0);
+      if (lane == 0) {
+        s_count = count;
+        s_order = order;
+      }
+      if (blockIdx.x == 0 && t == 0) {
+        int at = here;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int front = __shfl_up_sync(0xffffffffu, at, o);
+          if (lane >= o) at += front;
+        }
+        at -= here;
+        for (unsigned left = marks; left != 0u; left &= left - 1) planes.slots_of[at++] = lane * 32 + __ffs(left) - 1;
+        if (lane == 0) planes.counts[0] = count;
+      }
+    }
+    __syncthreads();
+    constexpr int RANKS = THREADS / 32 / PARTS;
+    const int j0 = blockIdx.x * RANKS, live = min(RANKS, rank - j0);
+    for (int i = tid; i < s_count * live; i += THREADS) {
+      const int e = i / live;
+      if (!own || e != s_order)
+        planes.u[((size_t)e * PLANE_ROWS + t) * rank + j0 + i % live] = __float2bfloat16_rn(0.f);
+    }
+  }
+  if (!own) return;  // (the whole block)
   constexpr int EACH = 16 / sizeof(T), ROUND = 32 * EACH;
   const int rounds = (K + ROUND - 1) / ROUND, each = (rounds + PARTS - 1) / PARTS;
   const int from = (warp % PARTS) * each * ROUND, to = min(K, from + each * ROUND);
@@ -93,24 +150,32 @@ adapter_shrink_kernel(const T* x, long long ldx, const T* a, const float* scales
 #pragma unroll
     for (int i = 0; i < PARTS; ++i) sum += sums[warp + i];
   }
-  if (lane == 0 && j < rank) low[(size_t)t * rank + j] = scales[slot] * sum;
+  if (lane == 0 && j < rank) {
+    if constexpr (PLANES)
+      planes.u[((size_t)s_order * PLANE_ROWS + t) * rank + j] = __float2bfloat16_rn(scales[slot] * sum);
+    else
+      low[(size_t)t * rank + j] = scales[slot] * sum;
+  }
 }
 
-template <typename T, int PARTS>
+template <typename T, int PARTS, bool PLANES>
 void launch_shrink(const T* x, long long ldx, const T* a, const float* scales, const int* index, int slots,
-                   int rank, int tokens, int K, int wide, float* low, cudaStream_t stream) {
+                   int rank, int tokens, int K, int wide, float* low, const ShrinkPlanes& planes, cudaStream_t stream) {
   constexpr int RANKS = THREADS / 32 / PARTS;
-  fb_launch(adapter_shrink_kernel<T, PARTS>, dim3((rank + RANKS - 1) / RANKS, tokens), dim3(THREADS), 0, stream,
-            x, ldx, a, scales, index, slots, rank, K, wide, low);
+  fb_launch(adapter_shrink_kernel<T, PARTS, PLANES>, dim3((rank + RANKS - 1) / RANKS, tokens), dim3(THREADS), 0,
+            stream, x, ldx, a, scales, index, slots, rank, K, wide, low, planes);
 }
-template <typename T>
+template <typename T, bool PLANES>
 void shrink_by_size(const T* x, long long ldx, const T* a, const float* scales, const int* index, int slots,
-                    int rank, int tokens, int K, int wide, float* low, cudaStream_t stream) {
+                    int rank, int tokens, int K, int wide, float* low, const ShrinkPlanes& planes, cudaStream_t stream) {
   const int rounds = K / (32 * (16 / (int)sizeof(T)));  // of a warp's loads: four go out together
-  if (rounds <= 8) launch_shrink<T, 1>(x, ldx, a, scales, index, slots, rank, tokens, K, wide, low, stream);
-  else if (rounds <= 16) launch_shrink<T, 2>(x, ldx, a, scales, index, slots, rank, tokens, K, wide, low, stream);
-  else if (rounds <= 32) launch_shrink<T, 4>(x, ldx, a, scales, index, slots, rank, tokens, K, wide, low, stream);
-  else launch_shrink<T, 8>(x, ldx, a, scales, index, slots, rank, tokens, K, wide, low, stream);
+#define FB_SHRINK(PARTS) \
+  launch_shrink<T, PARTS, PLANES>(x, ldx, a, scales, index, slots, rank, tokens, K, wide, low, planes, stream)
+  if (rounds <= 8) FB_SHRINK(1);
+  else if (rounds <= 16) FB_SHRINK(2);
+  else if (rounds <= 32) FB_SHRINK(4);
+  else FB_SHRINK(8);
+#undef FB_SHRINK
 }
 
 // out[t, n] = sum over the planes of base[., t, n] + sum_j low[t, j] B[a][n, j].
@@ -311,9 +376,22 @@ FB_API int fb_adapter_shrink(const void* x, long long ldx, int dtype, const void
   if (T == 0) return 0;
   const int each = dtype == FB_BF16 ? 8 : 4;
   const int wide = K % each == 0 && ldx % each == 0 && (((uintptr_t)x | (uintptr_t)a) % 16) == 0;
-  FB_DISPATCH_DTYPE(dtype, E, shrink_by_size((const E*)x, ldx, (const E*)a, scales, index, slots, rank, T, K, wide,
-                                             low, stream));
+  FB_DISPATCH_DTYPE(dtype, E, shrink_by_size<E, false>((const E*)x, ldx, (const E*)a, scales, index, slots, rank, T, K,
+                                                      wide, low, ShrinkPlanes{}, stream));
   return fb_check_launch("adapter_shrink");
+}
+
+// The same as planes: u [adapters with tokens * 256, rank], counts [1], slots_of [the same number]. Up to 256 tokens,
+// bfloat16; rows behind the last token are left as they are.
+FB_API int fb_adapter_shrink_planes(const void* x, long long ldx, const void* a, const float* scales,
+                                    const int* index, int slots, int rank, int T, int K, void* u, int* counts,
+                                    int* slots_of, cudaStream_t stream) {
+  FB_REQUIRE(T > 0 && T <= PLANE_ROWS && K > 0 && rank > 0 && slots > 0 && slots <= PLANE_SLOTS && ldx >= K,
+             "adapter_shrink_planes: bad sizes T=%d K=%d rank=%d slots=%d", T, K, rank, slots);
+  const int wide = K % 8 == 0 && ldx % 8 == 0 && (((uintptr_t)x | (uintptr_t)a) % 16) == 0;
+  shrink_by_size<__nv_bfloat16, true>((const __nv_bfloat16*)x, ldx, (const __nv_bfloat16*)a, scales, index, slots, rank, T,
+                                      K, wide, nullptr, ShrinkPlanes{(__nv_bfloat16*)u, counts, slots_of}, stream);
+  return fb_check_launch("adapter_shrink_planes");
 }
 
 FB_API int fb_adapter_expand(const float* base, int planes, long long plane_stride, long long ldb,

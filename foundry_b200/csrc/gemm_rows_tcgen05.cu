@@ -34,6 +34,7 @@
 //   3  the fused q/k/v projection: rotate query and key heads by the token's
 //      position (pairs of ADJACENT features, frequency i for features 2i, 2i+1),
 //      queries to q_out, keys and values into the token's cache page
+//   7  as 0, with the tokens' low-rank adapters (adapter.cu) as more K behind the product's own
 // and, for a product whose input is a norm's output that still lacks its row
 // scale, every token's results are multiplied by 1 / sqrt(mean square + eps).
 //
@@ -112,6 +113,21 @@ template <int NB> struct RowsCfg {
                 "the partial tile and the epilogue's turn table take the stages' place");
 };
 
+// More K behind the product's own (epilogue 7): counts[0] adapters have tokens among the rows, the e-th of them
+// slots[e]; its rank numbers of the tokens, zero for tokens of others, are rows e * ROWS_A_PLANE .. of `u`, and
+// its weights for feature j row slot * N + j of `b`. Each takes `kblocks` K blocks of 64, which the CTAs of a
+// tile take in turn: one sum in tensor memory and one rounding.
+constexpr int ROWS_A_PLANE = 256;
+struct RowsMore {
+  CUtensorMap u, b;
+  const int* counts;
+  const int* slots;
+  int kblocks;
+};
+struct NoRowsMore {};
+template <bool MORE> struct RowsMoreArg { using type = NoRowsMore; };
+template <> struct RowsMoreArg<true> { using type = RowsMore; };
+
 __device__ __forceinline__ void epi_barrier() {  // the four epilogue warps
   asm volatile("bar.sync 1, 128;" ::: "memory");
 }
@@ -132,13 +148,14 @@ __device__ __forceinline__ float ld_cluster(const float* mine, unsigned rank) {
 template <int NB, bool CLUSTER, int EPI>
 __global__ void __launch_bounds__(THREADS)
 gemm_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
-                 const RowsParams p) {
+                 const RowsParams p, const __grid_constant__ typename RowsMoreArg<EPI == 7>::type more) {
   using Cfg = RowsCfg<NB>;
   constexpr int STAGES = Cfg::STAGES;
   // The epilogue is a template parameter: with all four in one kernel the
   // epilogue's straight-line code did not fit the instruction cache and every
   // token's stores waited for instructions (1.1 instead of 0.6 us per 32 tokens).
-  constexpr int epi = EPI;
+  constexpr int epi = EPI == 7 ? 0 : EPI;
+  constexpr bool MORE = EPI == 7;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* tiles = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t* full = (uint64_t*)(tiles + STAGES * Cfg::STAGE_BYTES);
@@ -157,6 +174,11 @@ gemm_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   const int split = CLUSTER ? (int)blockIdx.z : 0;  // = the CTA's rank in its cluster
   const int kb0 = split * p.per;
   const int n = max(min(p.kblocks - kb0, p.per), 0);
+  // this CTA's K blocks of adapters: the split-th of all of them, the one `splits` further, ..
+  auto more_blocks = [&]() {
+    if constexpr (MORE) return max(0, (__ldcg(more.counts) * more.kblocks - split + p.splits - 1) / p.splits);
+    else return 0;
+  };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -198,12 +220,22 @@ gemm_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
       fb_pdl_wait();
       for (int i = 0; i < early; ++i)
         tma_load_2d(tiles + i * Cfg::STAGE_BYTES + A_BYTES, &map_x, &full[i], (kb0 + i) * BK, 0);
-      for (int i = early; i < n; ++i) {
+      const int all = n + more_blocks();
+      for (int i = early; i < all; ++i) {
         const int s = i % STAGES;
         const uint32_t phase = (uint32_t)(i / STAGES) & 1u;
         if (!mbar_wait(&empty[s], phase ^ 1u, abort_flag, 1, i)) break;
         uint8_t* dst = tiles + s * Cfg::STAGE_BYTES;
         mbar_expect_tx(&full[s], Cfg::STAGE_BYTES);
+        if constexpr (MORE) {
+          if (i >= n) {
+            const int of_all = split + (i - n) * p.splits, e = of_all / more.kblocks;
+            const int k = (of_all - e * more.kblocks) * BK;
+            tma_load_2d(dst, &more.b, &full[s], k, __ldcg(more.slots + e) * p.N + tile * BM);
+            tma_load_2d(dst + A_BYTES, &more.u, &full[s], k, e * ROWS_A_PLANE);
+            continue;
+          }
+        }
         tma_load_2d(dst, &map_w, &full[s], (kb0 + i) * BK, tile * BM);
         tma_load_2d(dst + A_BYTES, &map_x, &full[s], (kb0 + i) * BK, 0);
       }
@@ -215,7 +247,9 @@ gemm_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     if (lane == 0) {
       constexpr uint32_t idesc = make_idesc(BM, NB);
       bool ok = true;
-      for (int i = 0; i < n && ok; ++i) {
+      if constexpr (MORE) fb_pdl_wait();  // the adapters among the rows are the work of an earlier kernel
+      const int all = n + more_blocks();
+      for (int i = 0; i < all && ok; ++i) {
         const int s = i % STAGES;
         const uint32_t phase = (uint32_t)(i / STAGES) & 1u;
         ok = mbar_wait(&full[s], phase, abort_flag, 2, i);
@@ -497,7 +531,7 @@ gemm_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 
 template <int NB, int EPI>
 int launch_rows_as(const CUtensorMap& mw, const CUtensorMap& mx, const RowsParams& p, int tiles,
-                   cudaStream_t stream) {
+                   cudaStream_t stream, const typename RowsMoreArg<EPI == 7>::type& more = {}) {
   static bool configured[64] = {};
   if (fb_first_use_on_device(configured)) {
     cudaError_t e = cudaFuncSetAttribute(gemm_rows_kernel<NB, true, EPI>,
@@ -510,10 +544,10 @@ int launch_rows_as(const CUtensorMap& mw, const CUtensorMap& mx, const RowsParam
   }
   if (p.splits > 1)
     fb_launch_cluster(gemm_rows_kernel<NB, true, EPI>, dim3(tiles, 1, p.splits), dim3(THREADS),
-                      RowsCfg<NB>::BYTES, stream, (unsigned)p.splits, mw, mx, p);
+                      RowsCfg<NB>::BYTES, stream, (unsigned)p.splits, mw, mx, p, more);
   else
     fb_launch(gemm_rows_kernel<NB, false, EPI>, dim3(tiles), dim3(THREADS), RowsCfg<NB>::BYTES,
-              stream, mw, mx, p);
+              stream, mw, mx, p, more);
   return fb_check_launch("gemm_rows");
 }
 
@@ -639,6 +673,60 @@ FB_API int fb_gemm_rows(const void* x, long long ldx, int M, const void* w, long
     case 128: return launch_rows<128>(mw, mx, p, tiles, stream);
     default: return launch_rows<256>(mw, mx, p, tiles, stream);
   }
+}
+
+// adapter.cu
+extern "C" int fb_adapter_shrink_planes(const void* x, long long ldx, const void* a, const float* scales,
+                                        const int* index, int slots, int rank, int T, int K, void* u, int* counts,
+                                        int* slots_of, cudaStream_t stream);
+
+// out[t] = scale of t's row * (x[t] w^T + scales[i] (x[t] a[i]^T) b[i]^T), i = index[t] (outside of the bank:
+// without the second part), for up to 64 tokens. a [slots, rank, K], b [slots, N, rank] bfloat16; u [most * 256,
+// rank] bfloat16, counts [1], slots_of [most]: room for the rank numbers, most = the smaller of slots and M; with
+// `made` they are there (fb_adapter_low), else a kernel in front writes them. The rest as in fb_gemm_rows.
+FB_API int fb_gemm_rows_adapted(const void* x, long long ldx, int M, const void* w, long long ldw, int N, int K,
+                                void* out, long long ldo, int out_f32, const float* scale_ss, int scale_count,
+                                int scale_stride, int scale_dim, float scale_eps, const void* a, const void* b,
+                                const float* scales, const int* index, int slots, int rank, void* u, int* counts,
+                                int* slots_of, int made, int splits, cudaStream_t stream) {
+  FB_REQUIRE(M > 0 && M <= 64 && N > 0 && K > 0 && out != nullptr && ldo >= N, "gemm_rows_adapted: bad sizes %d x %d x %d",
+             M, N, K);
+  FB_REQUIRE(K % 8 == 0 && ldx % 8 == 0 && ldw % 8 == 0 &&
+                 (((uintptr_t)x | (uintptr_t)w | (uintptr_t)b | (uintptr_t)u) % 16) == 0,
+             "gemm_rows_adapted: K and the row strides must be multiples of 8 elements and the operands "
+             "16-byte aligned (K=%d ldx=%lld ldw=%lld)", K, ldx, ldw);
+  FB_REQUIRE(slots > 0 && slots <= 1024 && rank > 0 && rank % 8 == 0 && a && b && scales && index && u && counts && slots_of,
+             "gemm_rows_adapted: a bank of %d adapters of rank %d", slots, rank);
+  FB_REQUIRE((long long)slots * N < (1ll << 31) - BM, "gemm_rows_adapted: %d adapters of %d rows", slots, N);
+  if (!made)
+    if (int rc = fb_adapter_shrink_planes(x, ldx, a, scales, index, slots, rank, M, K, u, counts, slots_of, stream))
+      return rc;
+  RowsParams p{};
+  p.M = M; p.N = N; p.K = K;
+  const int tiles = (N + BM - 1) / BM;
+  p.kblocks = (K + BK - 1) / BK;
+  if (splits <= 0) splits = fb_gemm_rows_splits(N, K);
+  FB_REQUIRE(splits <= 8 && splits <= p.kblocks, "gemm_rows_adapted: %d CTAs per tile for %d K blocks "
+             "(at most 8)", splits, p.kblocks);
+  p.per = (p.kblocks + splits - 1) / splits;
+  p.splits = (p.kblocks + p.per - 1) / p.per;
+  p.cols_per = (M + p.splits - 1) / p.splits;
+  p.out = out; p.ldo = ldo; p.out_f32 = out_f32;
+  p.scale = RowsScale{scale_ss, scale_count, scale_stride,
+                      scale_dim > 0 ? 1.0f / (float)scale_dim : 0.f, scale_eps};
+  p.vector_ok = ldo % 4 == 0 && ((uintptr_t)out % 16) == 0;
+  bind_status_mirror(stream);
+  const int NB = M <= 32 ? 32 : 64, most = slots < M ? slots : M;
+  CUtensorMap mw, mx;
+  RowsMore more{};
+  int rc = make_map(&mw, w, N, K, ldw, BM);
+  if (!rc) rc = make_map(&mx, x, M, K, ldx, NB);
+  if (!rc) rc = make_map(&more.u, u, (long long)most * ROWS_A_PLANE, rank, rank, NB);
+  if (!rc) rc = make_map(&more.b, b, (long long)slots * N, rank, rank, BM);
+  if (rc) return rc;
+  more.counts = counts; more.slots = slots_of; more.kblocks = (rank + BK - 1) / BK;
+  return NB == 32 ? launch_rows_as<32, 7>(mw, mx, p, tiles, stream, more)
+                  : launch_rows_as<64, 7>(mw, mx, p, tiles, stream, more);
 }
 
 // As fb_gemm_tc_status, for the kernel of this file.

@@ -125,6 +125,10 @@ _SIGNATURES = {
                                c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p,
                                c_void_p, c_ll, c_int, c_void_p, c_int, c_int, c_int, c_float,
                                c_void_p],
+    "fb_gemm_rows_adapted": [c_void_p, c_ll, c_int, c_void_p, c_ll, c_int, c_int, c_void_p, c_ll, c_int,
+                             c_void_p, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p,
+                             c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                             c_void_p],
     "fb_adapter_low": [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                        c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     "fb_gemm_tc_adapted": [c_void_p, c_ll, c_int, c_void_p, c_ll, c_int, c_int, c_void_p, c_void_p,
@@ -2217,6 +2221,17 @@ def _planes_pay(T: int, N: int) -> bool:
     return PAIRED and PERSISTENT and N >= 128 and T > 64 and T * N >= 3 << 19
 
 
+def _rows_pay(T: int, slots: int, rank: int) -> bool:
+    """Whether adapters ride behind the projection's own K in the product of 17 to 64 rows, a K block of 64
+    for every adapter among the rows and 64 of its ranks; how many those are is known on the device alone,
+    so the bank's size counts. Otherwise the product leaves its 32-bit sums for `adapter_expand` (2,048 ->
+    4,096, 64 rows, behind K and in a pass of its own: rank 16, 4 adapters 12.8 us and 13.3, 64 adapters 21
+    and 13.3; rank 64, 4 adapters 13.6 and 16.0, 64 adapters 22.9 and 17.1; rank 128, 4 adapters 16.3 and
+    26.5; 2,048 -> 28,672, rank 32, 4 adapters 29.7 and 39.9, 64 adapters 73 and 52)."""
+    return (SKINNY_ROWS < T <= min(ROWS_MAX, 64) and slots <= MAX_ADAPTER_SLOTS
+            and min(slots, T) <= 8 + rank // 4)
+
+
 def _adapter_low(x: torch.Tensor, bank: AdapterBank, index: torch.Tensor, most: int, u: int, counts: int,
                  slots: int, low: int) -> None:
     T, K = x.shape
@@ -2257,8 +2272,8 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
                     then_reads: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y[t] = x[t] w^T + scale_a (x[t] a_a^T) b_a^T with a = index[t] (int32, one a token; outside of
     the bank: no adapter). Sums are 32-bit and y is rounded once, to `out_dtype` (the input's type);
-    where the projection runs as the paired tcgen05 product (hundreds of tokens) the rank numbers are
-    rounded to bfloat16 for it (csrc/adapter.cu says which kernels run). `x` may be a `RowScaled`;
+    where the adapters ride behind the projection's own K (hundreds of tokens, or 17 to 64 with few
+    adapters) the rank numbers are rounded to bfloat16 for it (csrc/adapter.cu says which kernels run). `x` may be a `RowScaled`;
     `then_reads` names the weights that the step streams next, a hint."""
     values = x.values if isinstance(x, RowScaled) else x
     if values.dim() != 2 or w.dim() != 2 or values.shape[1] != w.shape[1]:
@@ -2294,6 +2309,21 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
               out.data_ptr(), N, 1 - code, T, N, K, a, b, scales, which, slots, rank, low.data_ptr(),
               *_prefetch_range(then_reads), skinny_plan(N, K, False)[1], *scale, _stream(),
               tag=("t{} n{} k{} r{}", T, N, K, rank))
+        return out
+    if bf16 and _rows_pay(T, slots, rank) and _tc_usable(values, w, w):
+        most = min(slots, T)
+        u = torch.empty((most * ADAPTER_BLOCK, rank), dtype=torch.bfloat16, device=values.device)
+        lists = torch.empty(1 + most, dtype=torch.int32, device=values.device)
+        counts, slots_of = lists.data_ptr(), lists.data_ptr() + 4
+        scale, values = _scale_of(x)
+        made = T * rank > 8192
+        if made:
+            _adapter_low(values, bank, index, most, u.data_ptr(), counts, slots_of, 0)
+        else:
+            _COUNT[0] += 1  # the rank numbers' kernel
+        _call("fb_gemm_rows_adapted", values.data_ptr(), values.stride(0), T, w.data_ptr(), w.stride(0), N,
+              K, out.data_ptr(), N, 1 - code, *scale, a, b, scales, which, slots, rank, u.data_ptr(),
+              counts, slots_of, int(made), ROWS_SPLITS, _stream(), tag=("t{} n{} k{} r{}", T, N, K, rank))
         return out
     x = plain(x)
     if T > ADAPTER_PIECE:

@@ -143,3 +143,10 @@ def test_rank_numbers_on_tensor_maps_by_alignment_and_places():
         return ops._low_fits(x, w, bank)
     assert fits() and fits(pad=8) and fits(slots=1024)
     assert not fits(slots=1025) and not fits(K=60) and not fits(pad=4) and not fits(dtype=torch.float32)
+
+
+@pytest.mark.parametrize("T,slots,rank,pays", [(16, 2, 64, False), (17, 12, 16, True), (17, 13, 16, False), (64, 24, 64, True),
+                                               (64, 25, 64, False), (20, 1000, 48, True), (20, 1025, 48, False),
+                                               (65, 2, 64, False)])
+def test_adapters_behind_k_of_a_few_rows_by_how_many_there_may_be(T, slots, rank, pays):
+    assert ops._rows_pay(T, slots, rank) == pays

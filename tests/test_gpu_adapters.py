@@ -102,6 +102,16 @@ def test_without_an_adapter_it_is_the_product(ops):
         assert torch.allclose(got, want, rtol=2.0 ** -8 * 1.01, atol=1024 * 2.0 ** -24 * 1024 * 0.05)
 
 
+@pytest.mark.parametrize("K,N,R,S", [(512, 384, 64, 24), (520, 132, 48, 20), (4096, 640, 128, 40), (72, 1000, 200, 58)])
+@pytest.mark.parametrize("T", [17, 24, 32, 33, 63, 64, 65])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+def test_many_adapters_behind_the_products_k(ops, T, K, N, R, S, out):
+    """Up to as many as may ride there, all of them among the rows or a few; N past the last tile of 128."""
+    for index in (np.arange(T) * 7 % S, np.where(np.arange(T) % 3 == 0, S - 1, -1), np.arange(T) % (S + 2) - 1):
+        x, w, bank, index = case(ops, T, K, N, R, S, torch.bfloat16, pad=16, index=index.astype(np.int32))
+        check(ops, x, w, bank, index, ops.adapted_product(x, w, bank, index, out_dtype=out), out == torch.bfloat16)
+
+
 @pytest.mark.parametrize("N", [64, 256])  # the rank numbers as rows, and as planes behind K
 @pytest.mark.parametrize("T", [8192, 8193, 8200, 16500])
 def test_more_tokens_than_one_launch_takes(ops, T, N):
