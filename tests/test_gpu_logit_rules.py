@@ -238,6 +238,21 @@ def test_borders_among_many_nearly_equal_logits(ops, V, spread):
     check(ops, dev(logits), logits, rules)
 
 
+@pytest.mark.parametrize("rule", [{}, dict(top_k=[20] * 8), dict(top_p=[0.5] * 8)])
+def test_an_infinite_temperature_gives_equal_shares(ops, rule):
+    n, V = 8, 3000
+    logits = np.random.RandomState(0).randn(n, V).astype(np.float32)
+    logits[:, 5] = -np.inf
+    draw = lambda heat: ops.sample_tokens(dev(logits), ops.SampleRules(  # noqa: E731
+        dev([heat] * n, torch.float32), dev(rule.get("top_k"), torch.int32) if "top_k" in rule else None,
+        dev(rule["top_p"], torch.float32) if "top_p" in rule else None, None,
+        torch.arange(n, device=DEV), torch.arange(n, device=DEV)))
+    tokens, logprobs = draw(np.inf)
+    same_tokens, _ = draw(3e38)
+    assert torch.equal(tokens, same_tokens) and (tokens != 5).all()
+    assert torch.allclose(logprobs, torch.full_like(logprobs, -float(np.log(V - 1))), rtol=1e-6)
+
+
 @pytest.mark.parametrize("m", [1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 257, 600, 3000])
 @pytest.mark.parametrize("V,n", [(7000, 6), (70000, 6), (7000, 200)])
 def test_borders_in_a_bin_of_so_many_tokens(ops, V, n, m):
