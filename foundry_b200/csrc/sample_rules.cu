@@ -309,7 +309,8 @@ sample_rules_kernel(const SampleArgs a) {
   const int lo = (int)rank * a.chunk, hi = min(a.V, lo + a.chunk), mine = max(0, hi - lo);
   const float* from = a.logits + (size_t)r * a.row_stride + lo;
   const FbRowEdits row = fb_row_edits(a.edits, r, a.V);
-  const float T = a.temperature != nullptr ? fminf(a.temperature[r], FLT_MAX) : 0.f;  // (an infinite one: equal shares)
+  const float asked = a.temperature != nullptr ? a.temperature[r] : 0.f;
+  const float T = asked > FLT_MAX ? FLT_MAX : asked;  // (an infinite one: equal shares)
   const bool greedy = !(T > 0.f);
   const int k = a.top_k != nullptr && !greedy ? a.top_k[r] : 0;
   const float p = a.top_p != nullptr && !greedy ? a.top_p[r] : 1.f;

@@ -146,6 +146,22 @@ def test_prompts_and_single_tokens_on_two_streams(ops):
     ops.release_scratch("adapters beside")
 
 
+@pytest.mark.parametrize("S,T", [(1000, 3), (1000, 16), (1000, 40), (1000, 70), (1400, 20), (1000, 600)])
+def test_banks_past_32_bits(ops, S, T):
+    """7 GB of B and more: the last places' rows lie behind 2^32 bytes and 2^31 numbers."""
+    K, N, R = 64, 16640, 136
+    x, w, small, _ = case(ops, T, K, N, R, 2, torch.bfloat16)
+    a = torch.zeros(S, R, K, dtype=torch.bfloat16, device=DEV)
+    b = torch.zeros(S, N, R, dtype=torch.bfloat16, device=DEV)
+    assert b.numel() > 1 << 31
+    a[-2:], b[-2:] = small.a, small.b
+    scales = torch.zeros(S, device=DEV)
+    scales[-2:] = small.scales
+    index = torch.arange(T, dtype=torch.int32, device=DEV) % 2
+    got = ops.adapted_product(x, w, ops.AdapterBank(a, b, scales), index + S - 2)
+    check(ops, x, w, small, index, got, True)
+
+
 def test_no_tokens(ops):
     x, w, bank, index = case(ops, 0, 64, 32, 8, 1, torch.bfloat16, index=[])
     assert ops.adapted_product(x, w, bank, index).shape == (0, 32)

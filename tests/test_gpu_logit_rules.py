@@ -238,6 +238,28 @@ def test_borders_among_many_nearly_equal_logits(ops, V, spread):
     check(ops, dev(logits), logits, rules)
 
 
+def test_rows_and_histories_past_32_bits(ops):
+    """Rows 1.2 billion logits apart, and a history whose last rows lie behind 2^31 counts."""
+    rows = Rows(ops, 3, 128256, seed=6)
+    wide = torch.zeros(3 * 1200000000, device=DEV)
+    logits = wide.view(3, -1)[:, 700:700 + 128256]
+    logits.copy_(rows.device_logits)
+    e = rows.edits
+    many = 17000
+    h = ops.TokenHistory.empty(many, 128256, DEV)
+    assert h.counts.numel() > 1 << 31
+    places = torch.where(e.history_rows >= 0, e.history_rows + many - e.history.rows, -1).to(torch.int32)
+    h.counts[-e.history.rows:] = e.history.counts
+    h.seen[-e.history.rows:] = e.history.seen
+    edits = ops.LogitEdits(h, places, e.repetition, e.frequency, e.presence, e.bias, e.allowed, e.allowed_rows)
+    same(ops.edit_logits(logits, edits), rows.edited())
+    check(ops, logits, rows.edited(), rules_of(3, 1), edits)
+    last = torch.tensor([many - 1] * 3, dtype=torch.int32, device=DEV)
+    before = h.counts[-1, [9, 128255]].clone()
+    ops.record_tokens(h, last, torch.tensor([9, 128255, 9], dtype=torch.int32, device=DEV), "generated")
+    assert torch.equal(h.counts[-1, [9, 128255]] - before, torch.tensor([2, 1], dtype=torch.int32, device=DEV))
+
+
 @pytest.mark.parametrize("rule", [{}, dict(top_k=[20] * 8), dict(top_p=[0.5] * 8)])
 def test_an_infinite_temperature_gives_equal_shares(ops, rule):
     n, V = 8, 3000
