@@ -48,19 +48,25 @@ struct ShrinkPlanes {
 };
 constexpr int PLANE_ROWS = 256, PLANE_SLOTS = 1024;
 
-// low[t, j] = scale * sum_k x[t, k] A[a][j, k], PARTS warps of a block a rank, each with a share of K, so that
-// a warp has few rounds of loads one after another (K = 14,336, 48 tokens, rank 16: one warp a rank 24 us).
-// Block (i, t) has the ranks from i * 8 / PARTS on. `wide`: rows are on 16-byte boundaries. PLANES: the numbers
-// go to the token's row of its adapter's plane, and zeros to its row of the others.
+// low[t, j] = scale * sum_k x[t, k] A[a][j, k]. A warp has four ranks, so that a piece of x in its registers meets
+// four rows of A, and PARTS warps of a block share K; block (i, t) has the ranks from i * BLOCK_RANKS on. Few
+// numbers take many warps each, for a warp's loads are then two rounds, all under way together; many have
+// enough warps without. The whole operator with 8, 4, 2 and 1 parts: 8 tokens of 14,336, rank 64, 27.6, 31, 34 and
+// 46 us; 48 of 4,096, rank 64, 17.6, 16.9, 18.9 and 22.4; 128 of 2,048, rank 64, 24.8, 21.0, 20.5 and 20.6. (A rank
+// a warp: 33, 17.1 and 19.6, and 64 tokens of 14,336 82 us against 47.) `wide`: rows are on 16-byte boundaries.
+// PLANES: the numbers go to the token's row of its adapter's plane, and zeros to its row of the others.
+constexpr int RANKS = 4;  // of a warp
 template <typename T, int PARTS, bool PLANES>
 __global__ void __launch_bounds__(THREADS)
 adapter_shrink_kernel(const T* x, long long ldx, const T* a, const float* scales, const int* index, int slots,
                       int rank, int K, int wide, float* low, const ShrinkPlanes planes) {
-  __shared__ float sums[THREADS / 32];
+  constexpr int WARPS = THREADS / 32;
+  constexpr int BLOCK_RANKS = RANKS * WARPS / PARTS;
+  __shared__ float sums[BLOCK_RANKS][PARTS];
   fb_pdl_wait();
   fb_pdl_launch();
-  const int t = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int j = blockIdx.x * (THREADS / 32 / PARTS) + warp / PARTS;
+  const int t = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j0 = blockIdx.x * BLOCK_RANKS;
+  const int share = warp % PARTS, first = warp / PARTS * RANKS;  // of the block's ranks
   const int slot = index[t];
   const bool own = slot >= 0 && slot < slots;
   __shared__ int s_order;
@@ -98,8 +104,7 @@ adapter_shrink_kernel(const T* x, long long ldx, const T* a, const float* scales
       }
     }
     __syncthreads();
-    constexpr int RANKS = THREADS / 32 / PARTS;
-    const int j0 = blockIdx.x * RANKS, live = min(RANKS, rank - j0);
+    const int live = min(BLOCK_RANKS, rank - j0);
     for (int i = tid; i < s_count * live; i += THREADS) {
       const int e = i / live;
       if (!own || e != s_order)
@@ -109,73 +114,79 @@ adapter_shrink_kernel(const T* x, long long ldx, const T* a, const float* scales
   if (!own) return;  // (the whole block)
   constexpr int EACH = 16 / sizeof(T), ROUND = 32 * EACH;
   const int rounds = (K + ROUND - 1) / ROUND, each = (rounds + PARTS - 1) / PARTS;
-  const int from = (warp % PARTS) * each * ROUND, to = min(K, from + each * ROUND);
+  const int from = share * each * ROUND, to = min(K, from + each * ROUND);
   const T* row = x + (size_t)t * ldx;
-  const T* w = a + ((size_t)slot * rank + min(j, rank - 1)) * K;
-  float sum = 0.f;
+  const T* w[RANKS];
+#pragma unroll
+  for (int q = 0; q < RANKS; ++q) w[q] = a + ((size_t)slot * rank + min(j0 + first + q, rank - 1)) * K;
+  float sum[RANKS] = {};
   int k = from + lane * EACH;
   if (wide) {
-    constexpr int AHEAD = 4;
-    for (; k + (AHEAD - 1) * ROUND < to; k += AHEAD * ROUND) {  // (K is a multiple of EACH)
-      uint4 u[AHEAD], v[AHEAD];
+    constexpr int AHEAD = 2;
+    for (; k < to; k += AHEAD * ROUND) {  // (K is a multiple of EACH)
+      uint4 u[AHEAD], v[AHEAD][RANKS];
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
-        v[i] = ld16(w + k + i * ROUND);
-        u[i] = ld16(row + k + i * ROUND);
+        const bool in = k + i * ROUND < to;
+        u[i] = in ? ld16(row + k + i * ROUND) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int q = 0; q < RANKS; ++q) v[i][q] = in ? ld16(w[q] + k + i * ROUND) : make_uint4(0u, 0u, 0u, 0u);
       }
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
-        if constexpr (sizeof(T) == 2) {
-          sum = dot8(u[i], v[i], sum);
-        } else {
-          const float* p = reinterpret_cast<const float*>(&u[i]);
-          const float* q = reinterpret_cast<const float*>(&v[i]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sum = fmaf(p[e], q[e], sum);
+        for (int q = 0; q < RANKS; ++q) {
+          if constexpr (sizeof(T) == 2) {
+            sum[q] = dot8(u[i], v[i][q], sum[q]);
+          } else {
+            const float* f = reinterpret_cast<const float*>(&u[i]);
+            const float* g = reinterpret_cast<const float*>(&v[i][q]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[q] = fmaf(f[e], g[e], sum[q]);
+          }
         }
       }
     }
-  }
-  for (; k < to; k += ROUND) {
+  } else {
+    for (; k < to; k += ROUND) {
 #pragma unroll
-    for (int e = 0; e < EACH; ++e)
-      if (k + e < to) sum = fmaf(fb_load_coherent(row + k + e), fb_load_coherent(w + k + e), sum);
-  }
-  sum = fb_warp_sum(sum);
-  if constexpr (PARTS > 1) {
-    if (lane == 0) sums[warp] = sum;
-    __syncthreads();
-    if (warp % PARTS != 0) return;
-    sum = 0.f;
+      for (int e = 0; e < EACH; ++e) {
+        if (k + e >= to) break;
+        const float f = fb_load_coherent(row + k + e);
 #pragma unroll
-    for (int i = 0; i < PARTS; ++i) sum += sums[warp + i];
+        for (int q = 0; q < RANKS; ++q) sum[q] = fmaf(f, fb_load_coherent(w[q] + k + e), sum[q]);
+      }
+    }
   }
-  if (lane == 0 && j < rank) {
-    if constexpr (PLANES)
-      planes.u[((size_t)s_order * PLANE_ROWS + t) * rank + j] = __float2bfloat16_rn(scales[slot] * sum);
-    else
-      low[(size_t)t * rank + j] = scales[slot] * sum;
+#pragma unroll
+  for (int q = 0; q < RANKS; ++q) {
+    sum[q] = fb_warp_sum(sum[q]);
+    if (lane == 0) sums[first + q][share] = sum[q];
+  }
+  __syncthreads();
+  if (threadIdx.x < BLOCK_RANKS && j0 + (int)threadIdx.x < rank) {
+    const int j = j0 + threadIdx.x;
+    float whole = 0.f;
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) whole += sums[threadIdx.x][i];
+    whole *= scales[slot];
+    if constexpr (PLANES) planes.u[((size_t)s_order * PLANE_ROWS + t) * rank + j] = __float2bfloat16_rn(whole);
+    else low[(size_t)t * rank + j] = whole;
   }
 }
 
-template <typename T, int PARTS, bool PLANES>
+template <typename T, bool PLANES>
 void launch_shrink(const T* x, long long ldx, const T* a, const float* scales, const int* index, int slots,
                    int rank, int tokens, int K, int wide, float* low, const ShrinkPlanes& planes, cudaStream_t stream) {
-  constexpr int RANKS = THREADS / 32 / PARTS;
-  fb_launch(adapter_shrink_kernel<T, PARTS, PLANES>, dim3((rank + RANKS - 1) / RANKS, tokens), dim3(THREADS), 0,
-            stream, x, ldx, a, scales, index, slots, rank, K, wide, low, planes);
-}
-template <typename T, bool PLANES>
-void shrink_by_size(const T* x, long long ldx, const T* a, const float* scales, const int* index, int slots,
-                    int rank, int tokens, int K, int wide, float* low, const ShrinkPlanes& planes, cudaStream_t stream) {
-  const int rounds = K / (32 * (16 / (int)sizeof(T)));  // of a warp's loads: four go out together
-#define FB_SHRINK(PARTS) \
-  launch_shrink<T, PARTS, PLANES>(x, ldx, a, scales, index, slots, rank, tokens, K, wide, low, planes, stream)
-  if (rounds <= 8) FB_SHRINK(1);
-  else if (rounds <= 16) FB_SHRINK(2);
-  else if (rounds <= 32) FB_SHRINK(4);
-  else FB_SHRINK(8);
-#undef FB_SHRINK
+  auto launch = [&](auto kernel, int ranks) {
+    fb_launch(kernel, dim3((rank + ranks - 1) / ranks, tokens), dim3(THREADS), 0, stream, x, ldx, a, scales, index,
+              slots, rank, K, wide, low, planes);
+  };
+  constexpr int ALL = RANKS * THREADS / 32;
+  const long long numbers = (long long)tokens * rank;
+  if (numbers <= 1024) launch(adapter_shrink_kernel<T, 8, PLANES>, ALL / 8);
+  else if (numbers <= 4096) launch(adapter_shrink_kernel<T, 4, PLANES>, ALL / 4);
+  else launch(adapter_shrink_kernel<T, 2, PLANES>, ALL / 2);
 }
 
 // out[t, n] = sum over the planes of base[., t, n] + sum_j low[t, j] B[a][n, j].
@@ -376,7 +387,7 @@ FB_API int fb_adapter_shrink(const void* x, long long ldx, int dtype, const void
   if (T == 0) return 0;
   const int each = dtype == FB_BF16 ? 8 : 4;
   const int wide = K % each == 0 && ldx % each == 0 && (((uintptr_t)x | (uintptr_t)a) % 16) == 0;
-  FB_DISPATCH_DTYPE(dtype, E, shrink_by_size<E, false>((const E*)x, ldx, (const E*)a, scales, index, slots, rank, T, K,
+  FB_DISPATCH_DTYPE(dtype, E, launch_shrink<E, false>((const E*)x, ldx, (const E*)a, scales, index, slots, rank, T, K,
                                                       wide, low, ShrinkPlanes{}, stream));
   return fb_check_launch("adapter_shrink");
 }
@@ -389,7 +400,7 @@ FB_API int fb_adapter_shrink_planes(const void* x, long long ldx, const void* a,
   FB_REQUIRE(T > 0 && T <= PLANE_ROWS && K > 0 && rank > 0 && slots > 0 && slots <= PLANE_SLOTS && ldx >= K,
              "adapter_shrink_planes: bad sizes T=%d K=%d rank=%d slots=%d", T, K, rank, slots);
   const int wide = K % 8 == 0 && ldx % 8 == 0 && (((uintptr_t)x | (uintptr_t)a) % 16) == 0;
-  shrink_by_size<__nv_bfloat16, true>((const __nv_bfloat16*)x, ldx, (const __nv_bfloat16*)a, scales, index, slots, rank, T,
+  launch_shrink<__nv_bfloat16, true>((const __nv_bfloat16*)x, ldx, (const __nv_bfloat16*)a, scales, index, slots, rank, T,
                                       K, wide, nullptr, ShrinkPlanes{(__nv_bfloat16*)u, counts, slots_of}, stream);
   return fb_check_launch("adapter_shrink_planes");
 }
