@@ -9,10 +9,10 @@
 //   has tokens in the block (zero in the rows of others), and the product takes them as more K behind its
 //   own, [x | planes] [W | B]^T: one sum in tensor memory, one rounding (gemm_tcgen05_pair.cu, MoreK). The
 //   rank numbers are rounded to bfloat16 for that, 2^-9 of the adapter's part on average.
-//   17 to 64 tokens, bfloat16, few adapters: the same with planes by `adapter_shrink` behind the K of the product
+//   Up to 64 tokens, bfloat16, few adapters (below 17 only beside wide projections): the same with planes by `adapter_shrink` behind the K of the product
 //   that shares K in a cluster (gemm_rows_tcgen05.cu, RowsMore): 48 tokens of 4,096 -> 4,096 with 12 adapters of
-//   rank 64 17.3 us, 19.4 with a pass of its own for the sums; 10.1 without adapters.
-//   Up to 16 tokens, bfloat16: `adapter_shrink` leaves them as 32-bit rows, and the weight-streaming product
+//   rank 64 16.9 us, 19.4 with a pass of its own for the sums; 10.1 without adapters.
+//   Else up to 16 tokens, bfloat16: `adapter_shrink` leaves them as 32-bit rows, and the weight-streaming product
 //   adds their product with B in its epilogue (gemm_skinny.cu, MODE_ADAPT). Nothing is rounded in between.
 //   Else: `adapter_shrink` (or, for many numbers, `adapter_low`) leaves them as 32-bit rows, the projection
 //   leaves 32-bit sums (split-K planes), and `adapter_expand` adds up sums and adapters and rounds once.

@@ -2221,15 +2221,18 @@ def _planes_pay(T: int, N: int) -> bool:
     return PAIRED and PERSISTENT and N >= 128 and T > 64 and T * N >= 3 << 19
 
 
-def _rows_pay(T: int, slots: int, rank: int) -> bool:
-    """Whether adapters ride behind the projection's own K in the product of 17 to 64 rows, a K block of 64
+def _rows_pay(T: int, N: int, slots: int, rank: int) -> bool:
+    """Whether adapters ride behind the projection's own K in the product of up to 64 rows, a K block of 64
     for every adapter among the rows and 64 of its ranks; how many those are is known on the device alone,
-    so the bank's size counts. Otherwise the product leaves its 32-bit sums for `adapter_expand` (2,048 ->
-    4,096, 64 rows, behind K and in a pass of its own: rank 16, 4 adapters 12.8 us and 13.3, 64 adapters 21
+    so the bank's size counts. Up to 16 rows the weight-streaming product's epilogue is the other side, which
+    reads a row of B for every result (4,096 -> 28,672, rank 64, 4 adapters: 8 rows 44.7 us and 48.2, 16
+    rows 45 and 78; 4,096 -> 4,096, 16 rows 13.3 and 12.8; rank 16 12.2 and 9.7). Beyond,  the
+    product leaves its 32-bit sums for `adapter_expand` (2,048 -> 4,096, 64 rows, behind K and in a pass of its own: rank 16, 4 adapters 12.8 us and 13.3, 64 adapters 21
     and 13.3; rank 64, 4 adapters 13.6 and 16.0, 64 adapters 22.9 and 17.1; rank 128, 4 adapters 16.3 and
     26.5; 2,048 -> 28,672, rank 32, 4 adapters 29.7 and 39.9, 64 adapters 73 and 52)."""
-    return (SKINNY_ROWS < T <= min(ROWS_MAX, 64) and slots <= MAX_ADAPTER_SLOTS
-            and min(slots, T) <= 8 + rank // 4)
+    if T <= SKINNY_ROWS and T * N * rank <= 1 << (22 if T > 8 else 23):
+        return False
+    return T <= min(ROWS_MAX, 64) and slots <= MAX_ADAPTER_SLOTS and min(slots, T) <= 8 + rank // 4
 
 
 def _adapter_low(x: torch.Tensor, bank: AdapterBank, index: torch.Tensor, most: int, u: int, counts: int,
@@ -2301,16 +2304,8 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
     if T == 0:
         return out
     bf16 = dtype == torch.bfloat16
-    if bf16 and T <= SKINNY_ROWS and _tc_usable(values, w, w):
-        low = torch.empty((T, rank), dtype=torch.float32, device=values.device)
-        scale, values = _scale_of(x)
-        _COUNT[0] += 1  # the rank numbers' kernel
-        _call("fb_gemm_skinny_adapted", values.data_ptr(), values.stride(0), w.data_ptr(), w.stride(0),
-              out.data_ptr(), N, 1 - code, T, N, K, a, b, scales, which, slots, rank, low.data_ptr(),
-              *_prefetch_range(then_reads), skinny_plan(N, K, False)[1], *scale, _stream(),
-              tag=("t{} n{} k{} r{}", T, N, K, rank))
-        return out
-    if bf16 and _rows_pay(T, slots, rank) and _tc_usable(values, w, w):
+    usable = bf16 and _tc_usable(values, w, w)
+    if usable and _rows_pay(T, N, slots, rank):
         most = min(slots, T)
         u = torch.empty((most * ADAPTER_BLOCK, rank), dtype=torch.bfloat16, device=values.device)
         lists = torch.empty(1 + most, dtype=torch.int32, device=values.device)
@@ -2324,6 +2319,15 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
         _call("fb_gemm_rows_adapted", values.data_ptr(), values.stride(0), T, w.data_ptr(), w.stride(0), N,
               K, out.data_ptr(), N, 1 - code, *scale, a, b, scales, which, slots, rank, u.data_ptr(),
               counts, slots_of, int(made), ROWS_SPLITS, _stream(), tag=("t{} n{} k{} r{}", T, N, K, rank))
+        return out
+    if usable and T <= SKINNY_ROWS:
+        low = torch.empty((T, rank), dtype=torch.float32, device=values.device)
+        scale, values = _scale_of(x)
+        _COUNT[0] += 1  # the rank numbers' kernel
+        _call("fb_gemm_skinny_adapted", values.data_ptr(), values.stride(0), w.data_ptr(), w.stride(0),
+              out.data_ptr(), N, 1 - code, T, N, K, a, b, scales, which, slots, rank, low.data_ptr(),
+              *_prefetch_range(then_reads), skinny_plan(N, K, False)[1], *scale, _stream(),
+              tag=("t{} n{} k{} r{}", T, N, K, rank))
         return out
     x = plain(x)
     if T > ADAPTER_PIECE:

@@ -145,8 +145,10 @@ def test_rank_numbers_on_tensor_maps_by_alignment_and_places():
     assert not fits(slots=1025) and not fits(K=60) and not fits(pad=4) and not fits(dtype=torch.float32)
 
 
-@pytest.mark.parametrize("T,slots,rank,pays", [(16, 2, 64, False), (17, 12, 16, True), (17, 13, 16, False), (64, 24, 64, True),
-                                               (64, 25, 64, False), (20, 1000, 48, True), (20, 1025, 48, False),
-                                               (65, 2, 64, False)])
-def test_adapters_behind_k_of_a_few_rows_by_how_many_there_may_be(T, slots, rank, pays):
-    assert ops._rows_pay(T, slots, rank) == pays
+@pytest.mark.parametrize("T,N,slots,rank,pays", [
+    (17, 64, 12, 16, True), (17, 64, 13, 16, False), (64, 64, 24, 64, True), (64, 64, 25, 64, False),
+    (20, 64, 1000, 48, True), (20, 64, 1025, 48, False), (65, 64, 2, 64, False),
+    (16, 4096, 4, 64, False), (16, 4100, 4, 64, True), (9, 28672, 4, 16, False), (10, 28672, 4, 16, True),
+    (8, 28672, 4, 32, False), (8, 28672, 4, 64, True), (16, 28672, 16, 16, False), (1, 28672, 1, 16, False)])
+def test_adapters_behind_k_of_a_few_rows_by_how_many_there_may_be(T, N, slots, rank, pays):
+    assert ops._rows_pay(T, N, slots, rank) == pays

@@ -112,6 +112,27 @@ def test_many_adapters_behind_the_products_k(ops, T, K, N, R, S, out):
         check(ops, x, w, bank, index, ops.adapted_product(x, w, bank, index, out_dtype=out), out == torch.bfloat16)
 
 
+@pytest.mark.parametrize("T,N,R", [(1, 16640, 512), (5, 16400, 128), (8, 16392, 64), (9, 8200, 64), (13, 2000, 256), (16, 16400, 16)])
+@pytest.mark.parametrize("scaled", [False, True])
+def test_a_few_rows_of_wide_projections(ops, T, N, R, scaled):
+    """Where a few rows' adapters leave the weight-streaming product's epilogue; a norm's row scale is then
+    the results' as well."""
+    K = 256
+    x, w, bank, index = case(ops, T, K, N, R, 4, torch.bfloat16)
+    assert ops._rows_pay(T, N, 4, R)
+    if not scaled:
+        check(ops, x, w, bank, index, ops.adapted_product(x, w, bank, index), True)
+        return
+    shares = torch.rand(16, 16, device=DEV) * 40
+    y = ops.adapted_product(ops.RowScaled(x.contiguous(), shares, 1e-5), w, bank, index).float().cpu().numpy().astype(np.float64)
+    host = lambda t: t.float().cpu().numpy()  # noqa: E731
+    scale = 1 / np.sqrt(host(shares).astype(np.float64).sum(0)[:T] / K + 1e-5)
+    want, size, much = (v * scale[:, None] for v in plain.adapted(
+        host(x), host(w), host(bank.a), host(bank.b), host(bank.scales), index.cpu().numpy()))
+    bound = plain.adapted_bound(want, size, much, K + bank.rank + 40, True)
+    assert (np.abs(y - want) <= bound).all(), (np.abs(y - want) / bound).max()
+
+
 @pytest.mark.parametrize("N", [64, 256])  # the rank numbers as rows, and as planes behind K
 @pytest.mark.parametrize("T", [8192, 8193, 8200, 16500])
 def test_more_tokens_than_one_launch_takes(ops, T, N):
