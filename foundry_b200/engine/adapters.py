@@ -68,6 +68,7 @@ class AdapterStore:
         if max_adapters < 1 or max_rank < 1:
             raise AdapterError(f"room for {max_adapters} adapters of rank {max_rank}")
         self.max_rank = (max_rank + 7) // 8 * 8  # the kernels' ranks
+        self.dtype = dtype
         self.sites = sites_of(model.parts())
         if not self.sites:
             raise AdapterError(f"no part of {model.spec.architecture} takes adapters")
@@ -124,8 +125,8 @@ class AdapterStore:
                 wrong.append(f"{p}: A {tuple(a.shape)}, B {tuple(b.shape)} beside [{rows}, {cols}]")
             elif a.shape[0] > self.max_rank:
                 wrong.append(f"{p}: rank {a.shape[0]}, room for {self.max_rank}")
-            elif not (torch.isfinite(a).all() and torch.isfinite(b).all()):
-                wrong.append(f"{p}: not finite")
+            elif not all(torch.isfinite(t.to(self.dtype)).all() for t in (a, b)):
+                wrong.append(f"{p}: not finite (as {self.dtype})")
         if not pairs:
             wrong.append("no tensors")
         if wrong:
