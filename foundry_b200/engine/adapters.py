@@ -53,7 +53,10 @@ def pairs_of(tensors: Mapping[str, torch.Tensor]) -> Dict[str, Tuple[torch.Tenso
         for half in ("lora_A", "lora_B"):
             at = short.find(f".{half}.")
             if at >= 0 and short.endswith("weight"):
-                halves.setdefault(short[:at], {})[half] = tensor
+                of = halves.setdefault(short[:at], {})
+                if half in of:
+                    raise AdapterError(f"{short[:at]}: {half} is given twice")
+                of[half] = tensor
                 break
         else:
             raise AdapterError(f"{name} is neither the A nor the B of a projection")

@@ -74,3 +74,13 @@ def test_numbers_are_finite_in_the_type_that_holds_them(half, value, dtype, fits
         return
     with pytest.raises(AdapterError, match="not finite"):
         store(dtype=dtype)[0].load("x", given)
+
+
+def test_a_projection_that_is_given_twice_is_refused():
+    given = pair("a.o", 6, 4)
+    again = {f"base_model.model.{n}": t for n, t in given.items()}
+    assert set(pairs_of(again)) == {"a.o"}
+    with pytest.raises(AdapterError, match="twice"):
+        pairs_of({**given, **again})
+    with pytest.raises(AdapterError, match="twice"):
+        pairs_of({**given, "a.o.lora_B.other.weight": given["a.o.lora_B.weight"]})
