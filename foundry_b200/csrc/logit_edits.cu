@@ -23,17 +23,17 @@ __device__ __forceinline__ unsigned bits_of(const unsigned* words, int end, int 
 }
 
 // Block (c, r) edits logits [c * TILE, ..) of row r; a warp has 512 side by side, so that it reads whole lines
-// whatever a row's start is aligned to, and a thread 16, all asked for together. Rows with a history or
-// biases take a turn through shared memory: the few tokens that the history holds are put on a list, and
-// the block's threads work it off, one load of a count each, all at once. (Where each thread looked after its
-// own tokens the counts came one after another, and a warp went through the penalties for every 32
-// tokens of which it held one: 64 rows of 128,256 with 4,000 tokens, 300 biases and masks 31 us against 16.6,
-// 68 MB at 4.1 TB/s. What is left to the copy rate's 10.4 are the turn through shared memory and its barriers.)
-__global__ void __launch_bounds__(THREADS)
+// whatever a row's start is aligned to, and a thread 16, all asked for together. They go out as they are, or as
+// -inf, as soon as they are there. The few tokens that the history holds are put on a list meanwhile, and the
+// block's threads then work it off in `out`, one load of a count each, all at once; biases follow. 64 rows of
+// 128,256 with 4,000 tokens, 300 biases and masks: 13.5 us, 68 MB at 5.0 TB/s; what is left to the copy rate's
+// 10.4 are chains of three loads in two rounds of blocks. (Six blocks an SM instead of eight 14.6, 8 logits a thread
+// 15.5, the tile in shared memory until its edits are done 16.6; where each thread looked after its own tokens the counts came one after
+// another, and a warp went through the penalties for every 32 tokens of which it held one: 31.)
+__global__ void __launch_bounds__(THREADS, 8)
 edit_logits_kernel(const float* logits, long long row_stride, int V, float* out, long long out_stride,
                    const FbLogitEdits edits) {
   fb_pdl_wait();
-  __shared__ float tile[TILE];
   __shared__ unsigned short hits[TILE];
   __shared__ int hit_count;
   const int r = blockIdx.y, lo = blockIdx.x * TILE, hi = min(V, lo + TILE), tid = threadIdx.x;
@@ -46,13 +46,10 @@ edit_logits_kernel(const float* logits, long long row_stride, int V, float* out,
   for (int j = 0; j < EACH; ++j) v[j] = first + 32 * j < here ? from[first + 32 * j] : 0.f;
   const FbRowEdits row = fb_row_edits(edits, r, V);
   const int word0 = (lo + first - lane) >> 5, words = ((V + 31) >> 5) - word0;
-  const unsigned held = row.counts != nullptr ? bits_of(row.seen + word0, words, lane) : 0u;
   const unsigned ok = row.allowed != nullptr ? bits_of(row.allowed + word0, words, lane) : ~0u;
-  const bool biased = row.bias_from < row.bias_to;
-  if (row.counts != nullptr || biased) {  // (the whole block)
+  const unsigned held = row.counts != nullptr ? bits_of(row.seen + word0, words, lane) & ok : 0u;
+  if (row.counts != nullptr) {  // (the whole block)
     if (tid == 0) hit_count = 0;
-#pragma unroll
-    for (int j = 0; j < EACH; ++j) tile[first + 32 * j] = v[j];
     __syncthreads();
     // the places of this warp's tokens on the list
     const int mine = __popc(held);
@@ -67,22 +64,21 @@ edit_logits_kernel(const float* logits, long long row_stride, int V, float* out,
     at = __shfl_sync(0xffffffffu, at, 31) + upto - mine;
     for (unsigned left = held; left != 0u; left &= left - 1)
       hits[at++] = (unsigned short)(first + 32 * (__ffs(left) - 1));
-    __syncthreads();
-    for (int i = tid; i < hit_count; i += THREADS) {
-      const int where = hits[i];
-      if (where < here) tile[where] = fb_penalised(row, tile[where], row.counts[lo + where]);
-    }
-    __syncthreads();
-    if (biased) {
-      fb_add_biases(edits, row, tile, lo, hi);
-      __syncthreads();
-    }
-#pragma unroll
-    for (int j = 0; j < EACH; ++j) v[j] = tile[first + 32 * j];
   }
 #pragma unroll
   for (int j = 0; j < EACH; ++j)
     if (first + 32 * j < here) to[first + 32 * j] = (ok >> j & 1u) ? v[j] : -INFINITY;
+  if (row.counts != nullptr) {
+    __syncthreads();  // the list, and what the block's threads wrote
+    for (int i = tid; i < hit_count; i += THREADS) {
+      const int where = hits[i];
+      if (where < here) to[where] = fb_penalised(row, to[where], row.counts[lo + where]);
+    }
+  }
+  if (row.bias_from < row.bias_to) {
+    __syncthreads();
+    fb_add_biases(edits, row, to, lo, hi);
+  }
 }
 
 // Token i goes into history rows[i] (outside of the table: skipped, like a token outside of the

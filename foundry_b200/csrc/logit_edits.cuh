@@ -72,7 +72,7 @@ __device__ __forceinline__ float fb_penalised(const FbRowEdits& e, float v, int 
   return v;
 }
 
-// The biases of a row that fall into [lo, hi), added to values that lie in shared memory from lo
+// The biases of a row that fall into [lo, hi), added to the values of allowed tokens, which lie from lo
 // on. Threads look at the row's whole list side by side (a request has some hundreds at most). Equal
 // ids stand side by side, and the first one's thread adds them all, in order.
 __device__ __forceinline__ void fb_add_biases(const FbLogitEdits& e, const FbRowEdits& row, float* values,
@@ -80,6 +80,7 @@ __device__ __forceinline__ void fb_add_biases(const FbLogitEdits& e, const FbRow
   for (int i = row.bias_from + (int)threadIdx.x; i < row.bias_to; i += (int)blockDim.x) {
     const int id = e.bias_ids[i];
     if (id < lo || id >= hi || (i > row.bias_from && e.bias_ids[i - 1] == id)) continue;
+    if (row.allowed != nullptr && !(row.allowed[id >> 5] >> (id & 31) & 1u)) continue;
     float v = values[id - lo];
     for (int j = i; j < row.bias_to && e.bias_ids[j] == id; ++j) v = __fadd_rn(v, e.bias_values[j]);
     values[id - lo] = v;
