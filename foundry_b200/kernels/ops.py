@@ -2235,6 +2235,15 @@ def _rows_pay(T: int, N: int, slots: int, rank: int) -> bool:
     return T <= min(ROWS_MAX, 64) and slots <= MAX_ADAPTER_SLOTS and min(slots, T) <= 8 + rank // 4
 
 
+def _low_pays(T: int, K: int, slots: int, rank: int) -> bool:
+    """Whether the rank numbers are worth the tensor cores, which multiply every tile of 128 rows with all
+    ranks, 64 a turn, of every adapter in it, where the CUDA cores take each row's own (shrink and low, us:
+    256 rows of 2,048, rank 64, 4 adapters 9.2 and 7.8, 64 of them 9.5 and 17.9; 256 rows of 4,096 15.1 and
+    8.9, 256 adapters 25.6 and 115; 1,024 rows of 2,048, rank 32, 4 adapters 16.3 and 6.7, 64 of them 16.8 and
+    13.7; 64 rows of 4,096, rank 256, 15.3 and 28.6)."""
+    return T * rank * K >= (1 << 26) * ((rank + 63) // 64) * max(1, min(slots, T) // 64)
+
+
 def _adapter_low(x: torch.Tensor, bank: AdapterBank, index: torch.Tensor, most: int, u: int, counts: int,
                  slots: int, low: int) -> None:
     T, K = x.shape
@@ -2311,7 +2320,7 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
         lists = torch.empty(1 + most, dtype=torch.int32, device=values.device)
         counts, slots_of = lists.data_ptr(), lists.data_ptr() + 4
         scale, values = _scale_of(x)
-        made = T * rank > 8192
+        made = _low_pays(T, K, slots, rank)
         if made:
             _adapter_low(values, bank, index, most, u.data_ptr(), counts, slots_of, 0)
         else:
@@ -2340,9 +2349,7 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
         _adapted_planes(x, w, bank, index, out)
         return out
     low = torch.empty((T, rank), dtype=torch.float32, device=x.device)
-    # up to this many rank numbers one warp a number is ahead (64 tokens x 64 ranks of 4,096: 6.9 us
-    # against 12; 256 x 64: 14.3 against 12.3; 512 x 16: 9.1 against 7.3)
-    if on_tensor_cores and T * rank > 8192:
+    if on_tensor_cores and _low_pays(T, K, slots, rank):
         _adapter_low(x, bank, index, min(slots, 128, T), 0, 0, 0, low.data_ptr())
     else:
         _call("fb_adapter_shrink", x.data_ptr(), _rows(x, "x"), code_of(dtype), a, scales, which,

@@ -152,3 +152,10 @@ def test_rank_numbers_on_tensor_maps_by_alignment_and_places():
     (8, 28672, 4, 32, False), (8, 28672, 4, 64, True), (16, 28672, 16, 16, False), (1, 28672, 1, 16, False)])
 def test_adapters_behind_k_of_a_few_rows_by_how_many_there_may_be(T, N, slots, rank, pays):
     assert ops._rows_pay(T, N, slots, rank) == pays
+
+
+@pytest.mark.parametrize("T,K,slots,rank,pays", [(256, 4096, 4, 64, True), (256, 4096, 200, 64, False), (255, 4096, 4, 64, False),
+                                                 (64, 4096, 4, 256, False), (1024, 2048, 64, 32, True), (1024, 2048, 128, 32, False),
+                                                 (4096, 4096, 300, 64, True)])
+def test_rank_numbers_on_the_tensor_cores_by_the_work(T, K, slots, rank, pays):
+    assert ops._low_pays(T, K, slots, rank) == pays

@@ -112,6 +112,17 @@ def test_many_adapters_behind_the_products_k(ops, T, K, N, R, S, out):
         check(ops, x, w, bank, index, ops.adapted_product(x, w, bank, index, out_dtype=out), out == torch.bfloat16)
 
 
+@pytest.mark.parametrize("T,K,N,R,S", [(300, 4096, 512, 64, 3), (300, 4096, 512, 64, 100), (257, 8200, 264, 32, 5), (700, 4096, 136, 128, 9),
+                                       (130, 16384, 200, 200, 70), (1025, 4104, 72, 16, 2), (64, 16392, 264, 64, 20),
+                                       (40, 26216, 136, 64, 3)])
+def test_rank_numbers_on_the_tensor_cores(ops, T, K, N, R, S):
+    """Where they leave rows for a pass behind the projection's sums, or planes for a few rows' product."""
+    assert ops._low_pays(T, K, S, R) and not ops._planes_pay(T, N)
+    for index in (None, (np.arange(T) * 5 // T % S).astype(np.int32)):
+        x, w, bank, index = case(ops, T, K, N, R, S, torch.bfloat16, index=index)
+        check(ops, x, w, bank, index, ops.adapted_product(x, w, bank, index), True)
+
+
 @pytest.mark.parametrize("T,N,R", [(1, 16640, 512), (5, 16400, 128), (8, 16392, 64), (9, 8200, 64), (13, 2000, 256), (16, 16400, 16)])
 @pytest.mark.parametrize("scaled", [False, True])
 def test_a_few_rows_of_wide_projections(ops, T, N, R, scaled):
