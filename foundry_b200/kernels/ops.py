@@ -2213,12 +2213,15 @@ def _low_fits(x: torch.Tensor, w: torch.Tensor, bank: AdapterBank) -> bool:
             and bank.slots <= MAX_ADAPTER_SLOTS and _tc_usable(x, w, w))
 
 
-def _planes_pay(T: int, N: int) -> bool:
+def _planes_pay(T: int, N: int, slots: int, rank: int) -> bool:
     """Whether adapters ride behind the projection's own K in the paired product. Otherwise the
-    projection's best form leaves its 32-bit sums to be read again, T * N of them; the paired one, which is
-    not the best for few tokens, saves that (4,096 -> 4,096, rank 16: 256 tokens 25 us against 31, 512
-    41 against 34; 4,096 -> 28,672, rank 32: 48 tokens 61 against 64, 128 86 against 66)."""
-    return PAIRED and PERSISTENT and N >= 128 and T > 64 and T * N >= 3 << 19
+    projection's best form leaves its 32-bit sums to be read again, T * N of them, for a pass that reads a row
+    of B for each; the paired one, which is not the best for few tokens, saves that and multiplies every block
+    of 256 tokens with every adapter in it, of which a large bank may mean many (unfused and behind K, us:
+    4,096 -> 4,096, 4 adapters, rank 16 256 tokens 25 and 32, 512 40 and 34; rank 64 96 tokens 24 and 32, 192 37
+    and 33; rank 128 96 41 and 40, 256 67 and 41; 64 adapters, rank 64, 256 tokens 52 and 90)."""
+    return PAIRED and PERSISTENT and N >= 128 and T > 64 and \
+        T * N * (rank + 16) >= (3 << 24) * max(1, min(slots, ADAPTER_BLOCK) // 16)
 
 
 def _rows_pay(T: int, N: int, slots: int, rank: int) -> bool:
@@ -2345,7 +2348,7 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
                                                        index[t:t + ADAPTER_PIECE], out_dtype)
         return out
     on_tensor_cores = _low_fits(x, w, bank)
-    if on_tensor_cores and _planes_pay(T, N):
+    if on_tensor_cores and _planes_pay(T, N, slots, rank):
         _adapted_planes(x, w, bank, index, out)
         return out
     low = torch.empty((T, rank), dtype=torch.float32, device=x.device)

@@ -126,11 +126,13 @@ def test_form_of_the_experts_products_by_rows_an_expert(rows, K, gated, form):
     assert ops.grouped_form(16 * rows, 16, K, gated) == form
 
 
-@pytest.mark.parametrize("T,N,pays", [(16, 1 << 20, False), (64, 1 << 20, False), (65, 28672, True), (48, 28672, False),
-                                      (256, 4096, False), (384, 4096, True), (512, 4096, True), (512, 2048, False),
-                                      (8192, 128, False), (12288, 128, True), (1 << 20, 127, False)])
-def test_adapters_behind_k_by_the_sums_that_it_saves(T, N, pays):
-    assert ops._planes_pay(T, N) == pays
+@pytest.mark.parametrize("T,N,slots,rank,pays", [
+    (16, 1 << 20, 4, 16, False), (64, 1 << 20, 4, 16, False), (65, 28672, 4, 16, True), (256, 4096, 4, 16, False),
+    (384, 4096, 4, 16, True), (512, 2048, 4, 16, False), (8192, 128, 4, 16, False), (12288, 128, 4, 16, True),
+    (1 << 20, 127, 4, 16, False), (153, 4096, 4, 64, False), (154, 4096, 4, 64, True), (154, 4096, 31, 64, True),
+    (154, 4096, 32, 64, False), (2048, 6144, 256, 48, True), (2048, 2048, 256, 48, False)])
+def test_adapters_behind_k_by_the_sums_that_it_saves(T, N, slots, rank, pays):
+    assert ops._planes_pay(T, N, slots, rank) == pays
 
 
 def test_rank_numbers_on_tensor_maps_by_alignment_and_places():

@@ -117,10 +117,36 @@ def test_many_adapters_behind_the_products_k(ops, T, K, N, R, S, out):
                                        (40, 26216, 136, 64, 3)])
 def test_rank_numbers_on_the_tensor_cores(ops, T, K, N, R, S):
     """Where they leave rows for a pass behind the projection's sums, or planes for a few rows' product."""
-    assert ops._low_pays(T, K, S, R) and not ops._planes_pay(T, N)
+    assert ops._low_pays(T, K, S, R) and not ops._planes_pay(T, N, S, R)
     for index in (None, (np.arange(T) * 5 // T % S).astype(np.int32)):
         x, w, bank, index = case(ops, T, K, N, R, S, torch.bfloat16, index=index)
         check(ops, x, w, bank, index, ops.adapted_product(x, w, bank, index), True)
+
+
+@pytest.fixture
+def behind_k(ops, monkeypatch):
+    """The paired product with the adapters behind its K, whatever the sizes' rule says."""
+    monkeypatch.setattr(ops, "_planes_pay", lambda T, N, slots, rank: T > 64 and N >= 128)
+    return ops
+
+
+@pytest.mark.parametrize("T", [65, 128, 130, 255, 256, 257, 300, 777])
+@pytest.mark.parametrize("K,N,R,S", [(64, 128, 8, 1), (512, 200, 24, 3), (520, 1024, 64, 9), (1032, 136, 200, 4), (256, 648, 16, 64)])
+def test_behind_the_paired_products_k(behind_k, T, K, N, R, S):
+    for index in (None, (np.arange(T) * 3 // T % S).astype(np.int32), np.arange(T, dtype=np.int32) % S):
+        x, w, bank, index = case(behind_k, T, K, N, R, S, torch.bfloat16, pad=8, index=index)
+        check(behind_k, x, w, bank, index, behind_k.adapted_product(x, w, bank, index), True)
+    check(behind_k, x, w, bank, index, behind_k.adapted_product(x, w, bank, index, out_dtype=torch.float32), False)
+
+
+def test_behind_the_paired_products_k_a_row_depends_on_its_own_adapter_alone(behind_k):
+    test_a_row_depends_on_its_own_adapter_alone(behind_k, 300)
+    test_a_row_depends_on_its_own_adapter_alone(behind_k, 70)
+
+
+def test_behind_the_paired_products_k_on_another_stream_and_replayed(behind_k):
+    test_on_another_stream_and_replayed(behind_k)
+    test_prompts_and_single_tokens_on_two_streams(behind_k)
 
 
 @pytest.mark.parametrize("T,N,R", [(1, 16640, 512), (5, 16400, 128), (8, 16392, 64), (9, 8200, 64), (13, 2000, 256), (16, 16400, 16)])
