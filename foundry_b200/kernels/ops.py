@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import threading
 import weakref
+from array import array
 from typing import Optional, Sequence
 
 import os as _os
@@ -1463,10 +1464,10 @@ def quotients(n: torch.Tensor, d: torch.Tensor) -> torch.Tensor:
 
 
 def _tc_usable(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor) -> bool:
-    K = x.shape[1]
-    return (K % 8 == 0 and x.stride(0) % 8 == 0 and w.stride(0) % 8 == 0
-            and x.data_ptr() % 16 == 0 and w.data_ptr() % 16 == 0 and x.stride(1) == 1
-            and w.stride(1) == 1 and out.stride(1) == 1)
+    x_strides, w_strides = x.stride(), w.stride()  # (a tuple takes half as long as one of its numbers)
+    return (x.shape[1] % 8 == 0 and x_strides[0] % 8 == 0 and w_strides[0] % 8 == 0
+            and x.data_ptr() % 16 == 0 and w.data_ptr() % 16 == 0 and x_strides[1] == 1
+            and w_strides[1] == 1 and out.stride()[1] == 1)
 
 
 def _one_tile_plan(M: int, N: int, K: int):
@@ -2096,15 +2097,17 @@ class LogitEdits:
                 out[12] = 0
         if h is not None and h.rows == 0:
             out[0] = 0
-        return (c_ll * 15)(*out)
+        return array("q", out)  # (a ctypes array of as many takes a microsecond more)
 
 
 def _logit_rows(logits: torch.Tensor, what: str):
     if logits.dim() != 2 or logits.dtype != torch.float32:
         raise KernelError(f"{what}: logits are float32 rows, got {logits.dtype} {tuple(logits.shape)}")
     _on_current_device(logits, "logits")
-    stride = _rows(logits, "logits")
     n, V = logits.shape
+    stride, one = logits.stride()
+    if one != 1:
+        raise KernelError(f"logits must be 2-d with contiguous rows, got strides {logits.stride()}")
     if V == 0:
         raise KernelError(f"{what}: logits of no token")
     return n, V, max(stride, V) if n <= 1 else stride
@@ -2115,12 +2118,12 @@ def edit_logits(logits: torch.Tensor, edits: LogitEdits,
     """The edited logits of every row, float32 (a new tensor, or `out`, which may be `logits`)."""
     n, V, stride = _logit_rows(logits, "edit_logits")
     if out is None:
-        out = torch.empty((n, V), dtype=torch.float32, device=logits.device)
+        out = logits.new_empty(n, V)
     elif out.shape != logits.shape or out.dtype != torch.float32 or out.device != logits.device:
         raise KernelError(f"edit_logits: out is {out.dtype} {tuple(out.shape)} on {out.device}")
     packed = edits.packed(n, V, logits.get_device())
     _call("fb_edit_logits", logits.data_ptr(), stride, n, V, out.data_ptr(),
-          max(_rows(out, "out"), V) if n <= 1 else _rows(out, "out"), ctypes.addressof(packed),
+          max(_rows(out, "out"), V) if n <= 1 else _rows(out, "out"), packed.buffer_info()[0],
           _stream(), tag=("n{} v{}", n, V))
     return out
 
@@ -2156,9 +2159,9 @@ def sample_tokens(logits: torch.Tensor, rules: SampleRules, edits: Optional[Logi
     if V > MAX_SAMPLE_VOCAB:
         raise KernelError(f"sample_tokens: a vocabulary of {V} ({MAX_SAMPLE_VOCAB} at most)")
     if out is None:
-        out = torch.empty(n, dtype=torch.int32, device=device)
+        out = logits.new_empty(n, dtype=torch.int32)
     if logprobs is None:
-        logprobs = torch.empty(n, dtype=torch.float32, device=device)
+        logprobs = logits.new_empty(n)
     if record is not None and (edits is None or edits.history is None):
         raise KernelError("sample_tokens: tokens to record, and no history")
     at = logits.get_device()
@@ -2169,7 +2172,7 @@ def sample_tokens(logits: torch.Tensor, rules: SampleRules, edits: Optional[Logi
         ("min_p", r.min_p, f32), ("streams", r.streams, i64), ("steps", r.steps, i64),
         ("record", record, i32), ("out", out, i32), ("logprobs", logprobs, f32), ("also", also, i32)))
     _call("fb_sample_rules", logits.data_ptr(), stride, n, V, *rows[:6],
-          0 if packed is None else ctypes.addressof(packed), *rows[6:], _stream(),
+          0 if packed is None else packed.buffer_info()[0], *rows[6:], _stream(),
           tag=("n{} v{}", n, V))
     return out, logprobs
 
@@ -2312,35 +2315,37 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
         raise KernelError("adapted_product: the adapters must start on 16-byte boundaries")
     out_dtype = out_dtype or dtype
     code = code_of(out_dtype)
-    out = torch.empty((T, N), dtype=out_dtype, device=values.device)
+    out = values.new_empty(T, N, dtype=out_dtype)
     if T == 0:
         return out
     bf16 = dtype == torch.bfloat16
-    usable = bf16 and _tc_usable(values, w, w)
-    if usable and _rows_pay(T, N, slots, rank):
-        most = min(slots, T)
-        u = torch.empty((most * ADAPTER_BLOCK, rank), dtype=torch.bfloat16, device=values.device)
-        lists = torch.empty(1 + most, dtype=torch.int32, device=values.device)
-        counts, slots_of = lists.data_ptr(), lists.data_ptr() + 4
-        scale, values = _scale_of(x)
-        made = _low_pays(T, K, slots, rank)
-        if made:
-            _adapter_low(values, bank, index, most, u.data_ptr(), counts, slots_of, 0)
-        else:
+    if bf16 and T <= 64 and _tc_usable(values, w, w):
+        w_stride = w.stride()[0]
+        if _rows_pay(T, N, slots, rank):
+            most = min(slots, T)
+            u = values.new_empty(most * ADAPTER_BLOCK, rank)
+            lists = values.new_empty(1 + most, dtype=torch.int32)
+            counts = lists.data_ptr()
+            scale, values = _scale_of(x)
+            made = _low_pays(T, K, slots, rank)
+            if made:
+                _adapter_low(values, bank, index, most, u.data_ptr(), counts, counts + 4, 0)
+            else:
+                _COUNT[0] += 1  # the rank numbers' kernel
+            _call("fb_gemm_rows_adapted", values.data_ptr(), values.stride()[0], T, w.data_ptr(), w_stride,
+                  N, K, out.data_ptr(), N, 1 - code, *scale, a, b, scales, which, slots, rank,
+                  u.data_ptr(), counts, counts + 4, int(made), ROWS_SPLITS, _stream(),
+                  tag=("t{} n{} k{} r{}", T, N, K, rank))
+            return out
+        if T <= SKINNY_ROWS:
+            low = values.new_empty(T, rank, dtype=torch.float32)
+            scale, values = _scale_of(x)
             _COUNT[0] += 1  # the rank numbers' kernel
-        _call("fb_gemm_rows_adapted", values.data_ptr(), values.stride(0), T, w.data_ptr(), w.stride(0), N,
-              K, out.data_ptr(), N, 1 - code, *scale, a, b, scales, which, slots, rank, u.data_ptr(),
-              counts, slots_of, int(made), ROWS_SPLITS, _stream(), tag=("t{} n{} k{} r{}", T, N, K, rank))
-        return out
-    if usable and T <= SKINNY_ROWS:
-        low = torch.empty((T, rank), dtype=torch.float32, device=values.device)
-        scale, values = _scale_of(x)
-        _COUNT[0] += 1  # the rank numbers' kernel
-        _call("fb_gemm_skinny_adapted", values.data_ptr(), values.stride(0), w.data_ptr(), w.stride(0),
-              out.data_ptr(), N, 1 - code, T, N, K, a, b, scales, which, slots, rank, low.data_ptr(),
-              *_prefetch_range(then_reads), skinny_plan(N, K, False)[1], *scale, _stream(),
-              tag=("t{} n{} k{} r{}", T, N, K, rank))
-        return out
+            _call("fb_gemm_skinny_adapted", values.data_ptr(), values.stride()[0], w.data_ptr(), w_stride,
+                  out.data_ptr(), N, 1 - code, T, N, K, a, b, scales, which, slots, rank, low.data_ptr(),
+                  *_prefetch_range(then_reads), skinny_plan(N, K, False)[1], *scale, _stream(),
+                  tag=("t{} n{} k{} r{}", T, N, K, rank))
+            return out
     x = plain(x)
     if T > ADAPTER_PIECE:
         for t in range(0, T, ADAPTER_PIECE):
