@@ -2294,22 +2294,23 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
     adapters) the rank numbers are rounded to bfloat16 for it (csrc/adapter.cu says which kernels run). `x` may be a `RowScaled`;
     `then_reads` names the weights that the step streams next, a hint."""
     values = x.values if isinstance(x, RowScaled) else x
-    if values.dim() != 2 or w.dim() != 2 or values.shape[1] != w.shape[1]:
-        raise KernelError(f"adapted_product: x {tuple(values.shape)}, w {tuple(w.shape)}")
-    (T, K), N, dtype = values.shape, w.shape[0], values.dtype
-    slots, rank = bank.slots, bank.rank
+    shape, w_shape, dtype = values.shape, w.shape, values.dtype
+    if len(shape) != 2 or len(w_shape) != 2 or shape[1] != w_shape[1]:
+        raise KernelError(f"adapted_product: x {tuple(shape)}, w {tuple(w_shape)}")
+    (T, K), N = shape, w_shape[0]
+    slots, rank, a_wide = bank.a.shape
     if w.dtype != dtype:
         raise KernelError(f"adapted_product: x is {dtype}, w is {w.dtype}")
-    if bank.a.shape[2] != K or bank.b.shape[1] != N:
+    if a_wide != K or bank.b.shape != (slots, N, rank):
         raise KernelError(f"adapted_product: adapters {tuple(bank.a.shape)}, {tuple(bank.b.shape)} beside "
-                          f"a projection {tuple(w.shape)}")
+                          f"a projection {tuple(w_shape)}")
     _on_current_device(values, "x")
     at = values.get_device()
     if w.get_device() != at:
         raise KernelError(f"w is on {w.device}, the call's rows are on {values.device}")
     a = _given(bank.a, "a", dtype, None, at)
     b = _given(bank.b, "b", dtype, None, at)
-    scales = _given(bank.scales, "scales", torch.float32, None, at)
+    scales = _given(bank.scales, "scales", torch.float32, (slots,), at)
     which = _given(index, "index", torch.int32, (T,), at)
     if (a | b) % 16:
         raise KernelError("adapted_product: the adapters must start on 16-byte boundaries")
