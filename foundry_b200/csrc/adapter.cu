@@ -5,13 +5,15 @@
 // What it has to read beside the projection is small (a rank of 16 beside 4,096 -> 4,096: 1/128 of W for
 // every adapter in the step), so what counts is that the projection's kernels run as they do without it.
 //   Where the projection itself runs as the paired tcgen05 product (hundreds of tokens, bfloat16):
-//   `adapter_low` (adapter_tcgen05.cu) makes the rank numbers of each block of 256 tokens as planes, one for every adapter that
-//   has tokens in the block (zero in the rows of others), and the product takes them as more K behind its
-//   own, [x | planes] [W | B]^T: one sum in tensor memory, one rounding (gemm_tcgen05_pair.cu, MoreK). The
-//   rank numbers are rounded to bfloat16 for that, 2^-9 of the adapter's part on average.
-//   Up to 64 tokens, bfloat16, few adapters (below 17 only beside wide projections): the same with planes by `adapter_shrink` behind the K of the product
-//   that shares K in a cluster (gemm_rows_tcgen05.cu, RowsMore): 48 tokens of 4,096 -> 4,096 with 12 adapters of
-//   rank 64 16.9 us, 19.4 with a pass of its own for the sums; 10.1 without adapters.
+//   `adapter_low` (adapter_tcgen05.cu) makes the rank numbers of each block of 256 tokens as planes, one for
+//   every adapter that has tokens in the block (zero in the rows of others), and the product takes them as
+//   more K behind its own, [x | planes] [W | B]^T: one sum in tensor memory, one rounding
+//   (gemm_tcgen05_pair.cu, MoreK). The rank numbers are rounded to bfloat16 for that, 2^-9 of the adapter's
+//   part on average.
+//   Up to 64 tokens, bfloat16, few adapters (below 17 only beside wide projections): the same with planes by
+//   `adapter_shrink` behind the K of the product that shares K in a cluster (gemm_rows_tcgen05.cu, RowsMore):
+//   48 tokens of 4,096 -> 4,096 with 12 adapters of rank 64 16.8 us, 19.4 with a pass of its own for the sums;
+//   10.1 without adapters.
 //   Else up to 16 tokens, bfloat16: `adapter_shrink` leaves them as 32-bit rows, and the weight-streaming product
 //   adds their product with B in its epilogue (gemm_skinny.cu, MODE_ADAPT). Nothing is rounded in between.
 //   Else: `adapter_shrink` (or, for many numbers, `adapter_low`) leaves them as 32-bit rows, the projection

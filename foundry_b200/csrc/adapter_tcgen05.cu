@@ -9,8 +9,8 @@
 //
 // What bounds it: the start and the end of a CTA (barriers, tensor memory, the meeting of the shares) around
 // a stream of (128 + ranks) * 128 bytes a K block. 2,048 tokens of 4,096 at rank 48, one or two adapters a
-// block: 9.9 us in graph replays, where x and A alone are 18 MB, 2.7 us at the copy rate. (With mma.sync instead, from registers or
-// through cp.async stages, the same took 15 to 40 us: the instructions' own rate.)
+// block: 9.9 us in graph replays, where x and A alone are 18 MB, 2.7 us at the copy rate. (With mma.sync
+// instead, from registers or through cp.async stages, the same took 15 to 40 us: the instructions' own rate.)
 #define FB_STATUS_KERNEL 6
 #include "gemm_tcgen05.cuh"
 

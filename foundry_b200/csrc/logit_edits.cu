@@ -28,8 +28,9 @@ __device__ __forceinline__ unsigned bits_of(const unsigned* words, int end, int 
 // block's threads then work it off in `out`, one load of a count each, all at once; biases follow. 64 rows of
 // 128,256 with 4,000 tokens, 300 biases and masks: 13.5 us, 68 MB at 5.0 TB/s; what is left to the copy rate's
 // 10.4 are chains of three loads in two rounds of blocks. (Six blocks an SM instead of eight 14.6, 8 logits a thread
-// 15.5, the tile in shared memory until its edits are done 16.6; where each thread looked after its own tokens the counts came one after
-// another, and a warp went through the penalties for every 32 tokens of which it held one: 31.)
+// 15.5, the tile in shared memory until its edits are done 16.6; where each thread looked after its own tokens
+// the counts came one after another, and a warp went through the penalties for every 32 tokens of which it
+// held one: 31.)
 __global__ void __launch_bounds__(THREADS, 8)
 edit_logits_kernel(const float* logits, long long row_stride, int V, float* out, long long out_stride,
                    const FbLogitEdits edits) {

@@ -667,7 +667,8 @@ sample_rules_kernel(const SampleArgs a) {
         {  // as the bins: a thread a block and a slice
           const int at = (int)rank * (SLICES / blocks) + tid / blocks, o = tid & (blocks - 1);
           unsigned count = load_at(&bins.slice_count[at], o);
-          unsigned long long weight = load_at(&bins.slice_low[at], o) + ((unsigned long long)load_at(&bins.slice_high[at], o) << 11);
+          unsigned long long weight = (unsigned long long)load_at(&bins.slice_high[at], o) << 11;
+          weight += load_at(&bins.slice_low[at], o);
           for (int l = blocks / 2; l > 0; l /= 2) {
             count += __shfl_xor_sync(0xffffffffu, count, l);
             weight += __shfl_xor_sync(0xffffffffu, weight, l);

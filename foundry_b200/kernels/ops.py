@@ -2232,10 +2232,11 @@ def _rows_pay(T: int, N: int, slots: int, rank: int) -> bool:
     for every adapter among the rows and 64 of its ranks; how many those are is known on the device alone,
     so the bank's size counts. Up to 16 rows the weight-streaming product's epilogue is the other side, which
     reads a row of B for every result (4,096 -> 28,672, rank 64, 4 adapters: 8 rows 44.7 us and 48.2, 16
-    rows 45 and 78; 4,096 -> 4,096, 16 rows 13.3 and 12.8; rank 16 12.2 and 9.7). Beyond,  the
-    product leaves its 32-bit sums for `adapter_expand` (2,048 -> 4,096, 64 rows, behind K and in a pass of its own: rank 16, 4 adapters 12.8 us and 13.3, 64 adapters 21
-    and 13.3; rank 64, 4 adapters 13.6 and 16.0, 64 adapters 22.9 and 17.1; rank 128, 4 adapters 16.3 and
-    26.5; 2,048 -> 28,672, rank 32, 4 adapters 29.7 and 39.9, 64 adapters 73 and 52)."""
+    rows 45 and 78; 4,096 -> 4,096, 16 rows 13.3 and 12.8; rank 16 12.2 and 9.7). Beyond, the product leaves
+    its 32-bit sums for `adapter_expand` (2,048 -> 4,096, 64 rows, behind K and in a pass of its own: rank 16,
+    4 adapters 12.8 us and 13.3, 64 adapters 21 and 13.3; rank 64, 4 adapters 13.6 and 16.0, 64 adapters 22.9
+    and 17.1; rank 128, 4 adapters 16.3 and 26.5; 2,048 -> 28,672, rank 32, 4 adapters 29.7 and 39.9, 64
+    adapters 73 and 52)."""
     if T <= SKINNY_ROWS and T * N * rank <= 1 << (22 if T > 8 else 23):
         return False
     return T <= min(ROWS_MAX, 64) and slots <= MAX_ADAPTER_SLOTS and min(slots, T) <= 8 + rank // 4
@@ -2290,9 +2291,10 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
                     then_reads: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y[t] = x[t] w^T + scale_a (x[t] a_a^T) b_a^T with a = index[t] (int32, one a token; outside of
     the bank: no adapter). Sums are 32-bit and y is rounded once, to `out_dtype` (the input's type);
-    where the adapters ride behind the projection's own K (hundreds of tokens, or 17 to 64 with few
-    adapters) the rank numbers are rounded to bfloat16 for it (csrc/adapter.cu says which kernels run). `x` may be a `RowScaled`;
-    `then_reads` names the weights that the step streams next, a hint."""
+    where the adapters ride behind the projection's own K (hundreds of tokens, 17 to 64 with few adapters,
+    fewer beside wide projections) the rank numbers are rounded to bfloat16 for it (csrc/adapter.cu says
+    which kernels run). `x` may be a `RowScaled`; `then_reads` names the weights that the step streams next,
+    a hint."""
     values = x.values if isinstance(x, RowScaled) else x
     shape, w_shape, dtype = values.shape, w.shape, values.dtype
     if len(shape) != 2 or len(w_shape) != 2 or shape[1] != w_shape[1]:
