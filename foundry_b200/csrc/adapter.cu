@@ -15,7 +15,8 @@
 //   48 tokens of 4,096 -> 4,096 with 12 adapters of rank 64 16.8 us, 19.4 with a pass of its own for the sums;
 //   10.1 without adapters.
 //   Else up to 16 tokens, bfloat16: `adapter_shrink` leaves them as 32-bit rows, and the weight-streaming product
-//   adds their product with B in its epilogue (gemm_skinny.cu, MODE_ADAPT). Nothing is rounded in between.
+//   adds their product with B to its sums in front of its epilogue (gemm_skinny.cu, ADAPT). Nothing is rounded in
+//   between.
 //   Else: `adapter_shrink` (or, for many numbers, `adapter_low`) leaves them as 32-bit rows, the projection
 //   leaves 32-bit sums (split-K planes), and `adapter_expand` adds up sums and adapters and rounds once.
 #include "common.cuh"

@@ -141,10 +141,10 @@ constexpr int MODE_ROPE = 1;   // rotate and write queries, keys, values
 constexpr int MODE_SINK = 2;   // add into the residual rows in front of a norm
 constexpr int MODE_MANY = 3;   // store; the grid holds several products
 constexpr int MODE_CLAMP = 4;  // (gate, up) pairs with clamped halves and biases
-constexpr int MODE_ADAPT = 5;  // store, each token's low-rank adapter added (adapter.cu)
+// ADAPT, with any of PLAIN, ROPE and SINK: each token's low-rank adapter (adapter.cu) is added to its sums in
+// front of the epilogue: sum_j low[t, j] b[index[t]][n, j] to feature n of token t (an index outside of the bank:
+// nothing).
 constexpr int STAGED_LOW = 1024;  // rank numbers that its blocks fetch ahead
-// What MODE_ADAPT adds to feature n of token t: sum_j low[t, j] b[index[t]][n, j] (an index outside of
-// the bank: nothing), in front of the row scale.
 struct AdapterAdd {
   const float* low;         // [T, rank]
   const __nv_bfloat16* b;   // [slots, N, rank]
@@ -154,7 +154,9 @@ struct AdapterAdd {
 template <int MODE> struct EndArg { using type = NoSink; };
 template <> struct EndArg<MODE_SINK> { using type = ResidualSink; };
 template <> struct EndArg<MODE_CLAMP> { using type = FbGluClamp; };
-template <> struct EndArg<MODE_ADAPT> { using type = AdapterAdd; };
+struct NoAdapter {};
+template <bool ADAPT> struct AdapterArg { using type = NoAdapter; };
+template <> struct AdapterArg<true> { using type = AdapterAdd; };
 
 // NT: token tiles of 8 (1 or 2). WARPS: warps per CTA, each with a K range.
 // UNROLL: chunks whose loads are in flight together.
@@ -165,7 +167,7 @@ template <> struct EndArg<MODE_ADAPT> { using type = AdapterAdd; };
 // tokens the cap holds only because x is fetched one chunk ahead instead of all
 // chunks at once.
 constexpr int min_blocks(int warps) { return 16 / warps; }
-template <int NT, int WARPS, int UNROLL, int MODE>
+template <int NT, int WARPS, int UNROLL, int MODE, bool ADAPT>
 __global__ void __launch_bounds__(WARPS * 32, min_blocks(WARPS))
 gemm_skinny_kernel(const __nv_bfloat16* x, long long ldx,
                    const __nv_bfloat16* __restrict__ w, long long ldw, void* __restrict__ out,
@@ -175,12 +177,12 @@ gemm_skinny_kernel(const __nv_bfloat16* x, long long ldx,
                    const typename RopeArg<MODE == MODE_ROPE>::type rw,
                    const RowScale scale,
                    const typename EndArg<MODE>::type sink,
-                   const typename MoreArg<MODE == MODE_MANY>::type more) {
+                   const typename MoreArg<MODE == MODE_MANY>::type more,
+                   const typename AdapterArg<ADAPT>::type adapt) {
   constexpr bool ROPE = MODE == MODE_ROPE, SINK = MODE == MODE_SINK;
   __shared__ float red[WARPS][16][8 * NT + 1];
   __shared__ float scale_part[4][16];
   extern __shared__ __align__(16) float shares[];  // [scale.count][16] when there is a row scale
-  constexpr bool ADAPT = MODE == MODE_ADAPT;
   constexpr bool AHEAD = ADAPT && NT == 1;  // (the registers of 16 tokens are full)
   constexpr int STAGED = AHEAD ? (WARPS == 4 ? 4 : 2) : 0;  // pieces of b a thread
   __shared__ __align__(16) uint4 b_staged[STAGED + 1][AHEAD ? WARPS * 32 : 1];
@@ -283,19 +285,23 @@ gemm_skinny_kernel(const __nv_bfloat16* x, long long ldx,
   // thread's old residual values and norm weights into registers.
   constexpr int SINK_ITEMS = SINK ? (16 * 8 * NT + WARPS * 32 - 1) / (WARPS * 32) : 1;
   float old_resid[SINK_ITEMS], gamma[SINK_ITEMS];
-  // MODE_ADAPT: neighbouring lanes share a (token, feature)'s row of b, 16 bytes each and round; as many as
+  // ADAPT: neighbouring lanes share a (token, feature)'s row of b, 16 bytes each and round; as many as
   // there are threads for the 16 * T sums, and pieces in a row. A thread has two sums at most.
   constexpr int SUMS = ADAPT ? (16 * 8 * NT + WARPS * 32 - 1) / (WARPS * 32) : 1;
   int sum_lanes = 1, slot_of[SUMS];
   if constexpr (ADAPT)
-    while (sum_lanes < 32 && 8 * sum_lanes < sink.rank && 2 * sum_lanes * 16 * T <= WARPS * 32) sum_lanes *= 2;
+    while (sum_lanes < 32 && 8 * sum_lanes < adapt.rank && 2 * sum_lanes * 16 * T <= WARPS * 32) sum_lanes *= 2;
+  auto b_row = [&](int row) {  // the weight row of this CTA's row, and b's
+    if constexpr (ROPE) return head * rw.D + (row < 8 ? e_lo + row * e_step : e_hi + (row - 8) * e_step);
+    else return n0 + row;
+  };
+  auto live_sum = [&](int at) { return (at >> 4) < T && (ROPE || n0 + (at & 15) < N); };
   auto read_slots = [&]() {
     if constexpr (ADAPT) {
 #pragma unroll
       for (int it = 0; it < SUMS; ++it) {
         const int at = threadIdx.x / sum_lanes + it * (WARPS * 32 / sum_lanes);
-        slot_of[it] = (at >> 4) < T && n0 + (at & 15) < N
-                          ? *reinterpret_cast<const volatile int*>(sink.index + (at >> 4)) : -1;
+        slot_of[it] = live_sum(at) ? *reinterpret_cast<const volatile int*>(adapt.index + (at >> 4)) : -1;
       }
     }
   };
@@ -352,24 +358,24 @@ gemm_skinny_kernel(const __nv_bfloat16* x, long long ldx,
   // The first pieces of b and the rank numbers are asked for beside the weight stream, as the row scale is:
   // fetched by the epilogue, one after the other, they cost 8 tokens of 4,096 -> 28,672 with 4 adapters 3 us of 45.
   bool low_ahead = false;
-  if constexpr (AHEAD) low_ahead = T * sink.rank <= STAGED_LOW;
+  if constexpr (AHEAD) low_ahead = T * adapt.rank <= STAGED_LOW;
   auto ask_for_adapter = [&]() {
     if constexpr (AHEAD) {
       int n = 0;
 #pragma unroll
       for (int it = 0; it < SUMS; ++it) {
         const int at = threadIdx.x / sum_lanes + it * (WARPS * 32 / sum_lanes);
-        const __nv_bfloat16* brow = sink.b + ((size_t)max(slot_of[it], 0) * N + n0 + (at & 15)) * sink.rank;
-        for (int i = lane & (sum_lanes - 1); i < (sink.rank >> 3) && n < STAGED; i += sum_lanes, ++n) {
-          if (slot_of[it] < 0 || slot_of[it] >= sink.slots) continue;
+        const __nv_bfloat16* brow = adapt.b + ((size_t)max(slot_of[it], 0) * N + b_row(at & 15)) * adapt.rank;
+        for (int i = lane & (sum_lanes - 1); i < (adapt.rank >> 3) && n < STAGED; i += sum_lanes, ++n) {
+          if (slot_of[it] < 0 || slot_of[it] >= adapt.slots) continue;
           const uint32_t dst = (uint32_t)__cvta_generic_to_shared(&b_staged[n][threadIdx.x]);
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(brow + i * 8) : "memory");
         }
       }
       if (low_ahead) {
-        for (int i = threadIdx.x * 4; i < T * sink.rank; i += WARPS * 128) {
+        for (int i = threadIdx.x * 4; i < T * adapt.rank; i += WARPS * 128) {
           const uint32_t dst = (uint32_t)__cvta_generic_to_shared(low_staged + i);
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(sink.low + i) : "memory");
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(adapt.low + i) : "memory");
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -469,6 +475,39 @@ gemm_skinny_kernel(const __nv_bfloat16* x, long long ldx,
   };
   float* out_f = reinterpret_cast<float*>(out) + (size_t)blockIdx.y * plane_stride;
   __nv_bfloat16* out_h = reinterpret_cast<__nv_bfloat16*>(out);
+  if constexpr (ADAPT) {
+    const int lanes = sum_lanes, pieces = adapt.rank >> 3, part = lane & (lanes - 1);
+    if constexpr (!AHEAD) read_slots();
+    int n = 0;  // of the staged pieces
+#pragma unroll
+    for (int it = 0; it < SUMS; ++it) {
+      const int at = threadIdx.x / lanes + it * (WARPS * 32 / lanes);
+      const int row = at & 15, tok = at >> 4, slot = slot_of[it];
+      float v = 0.f;
+      const __nv_bfloat16* brow = adapt.b + ((size_t)max(slot, 0) * N + b_row(row)) * adapt.rank;
+      for (int i = part; i < pieces; i += lanes, ++n) {
+        if (slot < 0 || slot >= adapt.slots) continue;
+        const float* low = (low_ahead ? low_staged : adapt.low) + tok * adapt.rank + i * 8;
+        const uint4 q = n < STAGED ? b_staged[n][threadIdx.x] : ld_cached(brow + i * 8);
+        const uint4 lo = low_ahead ? *reinterpret_cast<const uint4*>(low) : ld_cached(low);
+        const uint4 hi = low_ahead ? *reinterpret_cast<const uint4*>(low + 4) : ld_cached(low + 4);
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
+        const float* f0 = reinterpret_cast<const float*>(&lo);
+        const float* f1 = reinterpret_cast<const float*>(&hi);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 b0 = __bfloat1622float2(h[e]), b1 = __bfloat1622float2(h[e + 2]);
+          v = fmaf(f0[2 * e], b0.x, v);
+          v = fmaf(f0[2 * e + 1], b0.y, v);
+          v = fmaf(f1[2 * e], b1.x, v);
+          v = fmaf(f1[2 * e + 1], b1.y, v);
+        }
+      }
+      for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (part == 0 && slot >= 0) red[0][row][tok] += v;
+    }
+    __syncthreads();
+  }
   if constexpr (ROPE) {
     // rows p and p + 8 are elements e_lo + p * e_step and e_hi + p * e_step of the head
     for (int idx = threadIdx.x; idx < 8 * T; idx += WARPS * 32) {
@@ -544,46 +583,6 @@ gemm_skinny_kernel(const __nv_bfloat16* x, long long ldx,
       const float rs = row_scale(tok);
       out_h[(size_t)tok * ldo + (row >> 1)] =
           __float2bfloat16_rn(fb_glu_clamped(sink, gate * rs + b0, up * rs + b1));
-    }
-  } else if constexpr (MODE == MODE_ADAPT) {
-    const int lanes = sum_lanes, pieces = sink.rank >> 3, part = lane & (lanes - 1);
-    if constexpr (!AHEAD) read_slots();
-    int n = 0;  // of the staged pieces
-#pragma unroll
-    for (int it = 0; it < SUMS; ++it) {
-      const int at = threadIdx.x / lanes + it * (WARPS * 32 / lanes);
-      const int row = at & 15, tok = at >> 4, slot = slot_of[it];
-      const bool live = tok < T && n0 + row < N;
-      float v = 0.f;
-      const __nv_bfloat16* brow = sink.b + ((size_t)max(slot, 0) * N + n0 + row) * sink.rank;
-      for (int i = part; i < pieces; i += lanes, ++n) {
-        if (slot < 0 || slot >= sink.slots) continue;
-        const float* low = (low_ahead ? low_staged : sink.low) + tok * sink.rank + i * 8;
-        const uint4 q = n < STAGED ? b_staged[n][threadIdx.x] : ld_cached(brow + i * 8);
-        const uint4 lo = low_ahead ? *reinterpret_cast<const uint4*>(low) : ld_cached(low);
-        const uint4 hi = low_ahead ? *reinterpret_cast<const uint4*>(low + 4) : ld_cached(low + 4);
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
-        const float* f0 = reinterpret_cast<const float*>(&lo);
-        const float* f1 = reinterpret_cast<const float*>(&hi);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float2 b0 = __bfloat1622float2(h[e]), b1 = __bfloat1622float2(h[e + 2]);
-          v = fmaf(f0[2 * e], b0.x, v);
-          v = fmaf(f0[2 * e + 1], b0.y, v);
-          v = fmaf(f1[2 * e], b1.x, v);
-          v = fmaf(f1[2 * e + 1], b1.y, v);
-        }
-      }
-      for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (live && part == 0) {
-        float whole = 0.f;
-#pragma unroll
-        for (int wi = 0; wi < WARPS; ++wi) whole += red[wi][row][tok];
-        v = (whole + v) * row_scale(tok);
-        const size_t o = (size_t)tok * ldo + n0 + row;
-        if (out_f32) out_f[o] = v;
-        else out_h[o] = __float2bfloat16_rn(v);
-      }
     }
   } else {
     if (epilogue == 0 || epilogue == 5) {
@@ -673,18 +672,25 @@ int launch_skinny(const void* x, long long ldx, const void* w, long long ldw, vo
   const int unroll = per >= 4 ? 4 : per >= 3 ? 3 : 2;
   // CTAs from this one on are the last half round of the grid (16 / warps CTAs fit an SM)
   const int early_from = blocks * ksplit - (16 / warps) * (sm_count() / 2);
-#define FB_SKINNY_R(NT, W, U, MODE, ROPE_ARG, SINK_ARG, MORE_ARG)                                       \
+  FB_REQUIRE(adapter.low == nullptr || (epilogue != 6 && epilogue != 5 && ksplit == 1 && more.count == 0),
+             "gemm_skinny: no adapters beside epilogue %d, %d K shares or further products", epilogue, ksplit);
+#define FB_SKINNY_A(NT, W, U, MODE, ADAPT, ROPE_ARG, SINK_ARG, MORE_ARG, ADAPT_ARG)                    \
   do {                                                                                         \
-  fb_launch(gemm_skinny_kernel<NT, W, U, MODE>, dim3(blocks, ksplit), dim3(W * 32),            \
+  fb_launch(gemm_skinny_kernel<NT, W, U, MODE, ADAPT>, dim3(blocks, ksplit), dim3(W * 32),            \
             shares_bytes, stream, (const __nv_bfloat16*)x, ldx, (const __nv_bfloat16*)w, ldw,   \
             out, ldo, out_f32, T, N, K, epilogue, next, next_bytes, plane_stride,               \
-            late_trigger, early_from, ROPE_ARG, scale, SINK_ARG, MORE_ARG); } while (0)
+            late_trigger, early_from, ROPE_ARG, scale, SINK_ARG, MORE_ARG, ADAPT_ARG); } while (0)
+#define FB_SKINNY_R(NT, W, U, MODE, ROPE_ARG, SINK_ARG, MORE_ARG) \
+  FB_SKINNY_A(NT, W, U, MODE, false, ROPE_ARG, SINK_ARG, MORE_ARG, NoAdapter{})
 #define FB_SKINNY(NT, W, U)                                                      \
   do {                                                                           \
-    if (epilogue == 2) FB_SKINNY_R(NT, W, U, MODE_ROPE, rw, NoSink{}, NoMore{});            \
+    if (adapter.low != nullptr) {                                                              \
+      if (epilogue == 2) FB_SKINNY_A(NT, W, U, MODE_ROPE, true, rw, NoSink{}, NoMore{}, adapter); \
+      else if (epilogue == 3) FB_SKINNY_A(NT, W, U, MODE_SINK, true, NoRope{}, sink, NoMore{}, adapter); \
+      else FB_SKINNY_A(NT, W, U, MODE_PLAIN, true, NoRope{}, NoSink{}, NoMore{}, adapter);       \
+    } else if (epilogue == 2) FB_SKINNY_R(NT, W, U, MODE_ROPE, rw, NoSink{}, NoMore{});        \
     else if (epilogue == 3) FB_SKINNY_R(NT, W, U, MODE_SINK, NoRope{}, sink, NoMore{});     \
     else if (epilogue == 6) FB_SKINNY_R(NT, W, U, MODE_CLAMP, NoRope{}, clamp, NoMore{});   \
-    else if (adapter.low != nullptr) FB_SKINNY_R(NT, W, U, MODE_ADAPT, NoRope{}, adapter, NoMore{}); \
     else if (more.count > 0) FB_SKINNY_R(NT, W, U, MODE_MANY, NoRope{}, NoSink{}, more);      \
     else FB_SKINNY_R(NT, W, U, MODE_PLAIN, NoRope{}, NoSink{}, NoMore{});                   \
   } while (0)
@@ -705,10 +711,33 @@ int launch_skinny(const void* x, long long ldx, const void* w, long long ldw, vo
 #undef FB_SKINNY_U
 #undef FB_SKINNY
 #undef FB_SKINNY_R
+#undef FB_SKINNY_A
   return fb_check_launch("gemm_skinny");
 }
 
 }  // namespace
+
+// adapter.cu
+extern "C" int fb_adapter_shrink(const void* x, long long ldx, int dtype, const void* a, const float* scales,
+                                 const int* index, int slots, int rank, int T, int K, float* low,
+                                 cudaStream_t stream);
+
+// What `adapter` (on the host, or null: none) says of the tokens' adapters: a [slots, rank, K] and b [slots, N, rank]
+// bfloat16, scales [slots], index [T] (outside of the bank: none), slots, rank, and low [T, rank] float32, which
+// a kernel in front of the product fills: token t's results then are those of x[t] w^T + scales[i] (x[t] a[i]^T) b[i]^T.
+static int adapter_of(const long long* adapter, const void* x, long long ldx, int T, int K, cudaStream_t stream,
+                      AdapterAdd* add) {
+  *add = AdapterAdd{};
+  if (adapter == nullptr) return 0;
+  const int slots = (int)adapter[4], rank = (int)adapter[5];
+  float* low = (float*)adapter[6];
+  FB_REQUIRE(slots > 0 && rank > 0 && rank % 8 == 0 && adapter[0] && adapter[1] && adapter[2] && adapter[3] && low &&
+                 ((adapter[1] | adapter[6]) % 16) == 0,
+             "gemm_skinny: a bank of %d adapters of rank %d, or operands not on 16-byte boundaries", slots, rank);
+  *add = AdapterAdd{low, (const __nv_bfloat16*)adapter[1], (const int*)adapter[3], slots, rank};
+  return fb_adapter_shrink(x, ldx, FB_BF16, (const void*)adapter[0], (const float*)adapter[2], add->index, slots, rank,
+                           T, K, low, stream);
+}
 
 // x: [T, K] bf16 (row stride ldx), w: [N, K] bf16 (row stride ldw), T <= 16.
 // epilogue 0: out[T, N] (bf16 or float32, row stride ldo).
@@ -727,7 +756,7 @@ FB_API int fb_gemm_skinny(const void* x, long long ldx, const void* w, long long
                           long long plane_stride, int warps, const float* scale_ss,
                           int scale_count, int scale_stride, int scale_dim, float scale_eps,
                           float glu_limit, float glu_alpha, float glu_shift, const float* glu_bias,
-                          cudaStream_t stream) {
+                          const long long* adapter, cudaStream_t stream) {
   // epilogue 4: as 1 with the tanh form of GELU on the gate
   // epilogue 5: as 0 with out = max(out, 0)^2
   // epilogue 6: as 1 with clamped halves and biases (glu_*; glu_bias null: none)
@@ -736,9 +765,11 @@ FB_API int fb_gemm_skinny(const void* x, long long ldx, const void* w, long long
   FB_REQUIRE(epilogue != 6 || glu_limit > 0.f, "gemm_skinny: the clamped epilogue needs a positive limit");
   const RowScale scale{scale_ss, scale_count, scale_stride,
                        scale_dim > 0 ? 1.0f / (float)scale_dim : 0.f, scale_eps};
+  AdapterAdd add;
+  if (int rc = adapter_of(adapter, x, ldx, T, K, stream, &add)) return rc;
   return launch_skinny(x, ldx, w, ldw, out, ldo, out_f32, T, N, K, epilogue, next, next_bytes,
                        ksplit, plane_stride, warps, 1, RopeWrite{}, scale, ResidualSink{}, stream,
-                       MoreProducts{}, FbGluClamp{glu_limit, glu_alpha, glu_shift, glu_bias});
+                       MoreProducts{}, FbGluClamp{glu_limit, glu_alpha, glu_shift, glu_bias}, add);
 }
 
 // Two products of the same T tokens in one launch, float32 out: out1 = x1 w1^T ([T, N1]) and
@@ -790,10 +821,13 @@ FB_API int fb_gemm_skinny_residual(const void* x, long long ldx, const void* w, 
                                    int T, int N, int K, float* resid, long long ldr,
                                    const float* gamma, void* xg, long long ldxg, float* ss_out,
                                    int ss_stride, float scale, const void* next,
-                                   long long next_bytes, int warps, cudaStream_t stream) {
+                                   long long next_bytes, int warps, const long long* adapter,
+                                   cudaStream_t stream) {
   ResidualSink sink{resid, ldr, gamma, (__nv_bfloat16*)xg, ldxg, ss_out, ss_stride, scale};
+  AdapterAdd add;
+  if (int rc = adapter_of(adapter, x, ldx, T, K, stream, &add)) return rc;
   return launch_skinny(x, ldx, w, ldw, resid, ldr, 1, T, N, K, 3, next, next_bytes, 1, 0, warps,
-                       1, RopeWrite{}, RowScale{}, sink, stream);
+                       1, RopeWrite{}, RowScale{}, sink, stream, MoreProducts{}, FbGluClamp{}, add);
 }
 
 // Most shares of a row scale that the products behind a norm take
@@ -819,7 +853,7 @@ FB_API int fb_gemm_skinny_rope(const void* x, long long ldx, const void* w, long
                                int interleaved, const void* next, long long next_bytes, int warps,
                                int late_trigger, const float* scale_ss, int scale_count,
                                int scale_stride, int scale_dim, float scale_eps,
-                               cudaStream_t stream) {
+                               const long long* adapter, cudaStream_t stream) {
   FB_REQUIRE(A > 0 && Kh > 0 && D > 0 && D % 16 == 0,
              "gemm_skinny_rope: head size %d is not a multiple of 16", D);
   FB_REQUIRE(rotary_dim >= 0 && rotary_dim <= D && rotary_dim % 16 == 0,
@@ -837,33 +871,9 @@ FB_API int fb_gemm_skinny_rope(const void* x, long long ldx, const void* w, long
   rw.interleaved = interleaved ? 1 : 0;
   const RowScale scale{scale_ss, scale_count, scale_stride,
                        scale_dim > 0 ? 1.0f / (float)scale_dim : 0.f, scale_eps};
+  AdapterAdd add;
+  if (int rc = adapter_of(adapter, x, ldx, T, K, stream, &add)) return rc;
   return launch_skinny(x, ldx, w, ldw, q_out, q_stride, 0, T, (A + 2 * Kh) * D, K, 2, next,
-                       next_bytes, 1, 0, warps, late_trigger, rw, scale, ResidualSink{}, stream);
-}
-
-// adapter.cu
-extern "C" int fb_adapter_shrink(const void* x, long long ldx, int dtype, const void* a, const float* scales,
-                                 const int* index, int slots, int rank, int T, int K, float* low,
-                                 cudaStream_t stream);
-
-// out[t] = scale of t's row * (x[t] w^T + scales[i] (x[t] a[i]^T) b[i]^T), i = index[t] (outside of the bank:
-// without the second part), for up to 16 tokens: two kernels, the rank numbers (low [T, rank] float32,
-// written here) and the product with them in its epilogue. a [slots, rank, K], b [slots, N, rank] bfloat16.
-// scale_*: as in fb_gemm_skinny.
-FB_API int fb_gemm_skinny_adapted(const void* x, long long ldx, const void* w, long long ldw, void* out,
-                                  long long ldo, int out_f32, int T, int N, int K, const void* a, const void* b,
-                                  const float* scales, const int* index, int slots, int rank, float* low,
-                                  const void* next, long long next_bytes, int warps, const float* scale_ss,
-                                  int scale_count, int scale_stride, int scale_dim, float scale_eps,
-                                  cudaStream_t stream) {
-  FB_REQUIRE(slots > 0 && rank > 0 && rank % 8 == 0 && a && b && scales && index && low &&
-                 (((uintptr_t)b | (uintptr_t)low) % 16) == 0,
-             "gemm_skinny_adapted: a bank of %d adapters of rank %d, or operands not on 16-byte boundaries", slots,
-             rank);
-  if (int rc = fb_adapter_shrink(x, ldx, FB_BF16, a, scales, index, slots, rank, T, K, low, stream)) return rc;
-  const RowScale scale{scale_ss, scale_count, scale_stride,
-                       scale_dim > 0 ? 1.0f / (float)scale_dim : 0.f, scale_eps};
-  return launch_skinny(x, ldx, w, ldw, out, ldo, out_f32, T, N, K, 0, next, next_bytes, 1, 0, warps, 1,
-                       RopeWrite{}, scale, ResidualSink{}, stream, MoreProducts{}, FbGluClamp{},
-                       AdapterAdd{low, (const __nv_bfloat16*)b, index, slots, rank});
+                       next_bytes, 1, 0, warps, late_trigger, rw, scale, ResidualSink{}, stream, MoreProducts{},
+                       FbGluClamp{}, add);
 }

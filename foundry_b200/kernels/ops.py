@@ -75,16 +75,16 @@ _SIGNATURES = {
                             c_void_p],
     "fb_gemm_skinny": [c_void_p, c_ll, c_void_p, c_ll, c_void_p, c_ll, c_int, c_int, c_int, c_int,
                        c_int, c_void_p, c_ll, c_int, c_ll, c_int, c_void_p, c_int, c_int, c_int,
-                       c_float, c_float, c_float, c_float, c_void_p, c_void_p],
+                       c_float, c_float, c_float, c_float, c_void_p, c_void_p, c_void_p],
     "fb_gemm_skinny_residual": [c_void_p, c_ll, c_void_p, c_ll, c_int, c_int, c_int, c_void_p,
                                 c_ll, c_void_p, c_void_p, c_ll, c_void_p, c_int, c_float, c_void_p,
-                                c_ll, c_int, c_void_p],
+                                c_ll, c_int, c_void_p, c_void_p],
     "fb_apply_row_scale": [c_void_p, c_ll, c_void_p, c_int, c_int, c_int, c_float, c_void_p,
                            c_ll, c_int, c_int, c_void_p],
     "fb_gemm_skinny_rope": [c_void_p, c_ll, c_void_p, c_ll, c_int, c_int, c_void_p, c_void_p,
                             c_void_p, c_int, c_void_p, c_int, c_void_p, c_ll, c_void_p, c_void_p,
                             c_ll, c_ll, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_ll,
-                            c_int, c_int, c_void_p, c_int, c_int, c_int, c_float, c_void_p],
+                            c_int, c_int, c_void_p, c_int, c_int, c_int, c_float, c_void_p, c_void_p],
     "fb_attention_prefill": [c_void_p, c_ll, c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_int,
                              c_void_p, c_void_p, c_ll, c_ll, c_int, c_int, c_int, c_int, c_int,
                              c_float, c_void_p],
@@ -122,10 +122,6 @@ _SIGNATURES = {
                         c_void_p],
     "fb_adapter_shrink": [c_void_p, c_ll, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                           c_int, c_void_p, c_void_p],
-    "fb_gemm_skinny_adapted": [c_void_p, c_ll, c_void_p, c_ll, c_void_p, c_ll, c_int, c_int, c_int,
-                               c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p,
-                               c_void_p, c_ll, c_int, c_void_p, c_int, c_int, c_int, c_float,
-                               c_void_p],
     "fb_gemm_rows_adapted": [c_void_p, c_ll, c_int, c_void_p, c_ll, c_int, c_int, c_void_p, c_ll, c_int,
                              c_void_p, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p,
                              c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
@@ -954,7 +950,7 @@ def _prefetch_range(then_reads: Optional[torch.Tensor]):
 
 def gemm_skinny(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, epilogue: int = 0,
                 then_reads: Optional[torch.Tensor] = None, ksplit: int = 1, warps: int = 0,
-                clamp: Optional[GluClamp] = None) -> torch.Tensor:
+                clamp: Optional[GluClamp] = None, adapters=None) -> torch.Tensor:
     """Up to 16 token rows: the weight-streaming kernel (csrc/gemm_skinny.cu).
     epilogue 1: `w` rows are (gate, up) pairs and out is [M, N/2] = SiLU(gate)*up
     (4: the tanh form of GELU instead; 6: the rule `clamp`); epilogue 5: out = max(x w^T, 0)^2.
@@ -962,7 +958,8 @@ def gemm_skinny(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, epilogue: i
     blocks ask for their start to be brought into L2 as they finish.
     `ksplit` > 1: K is shared by that many CTAs per row group and `out` is
     float32 planes [ksplit, M, N]. `warps`: 4, 8 or 16 per CTA (0: the
-    launcher's choice)."""
+    launcher's choice). `adapters`: (an `AdapterBank`, each row's place in it), added to the sums in
+    front of the epilogue (0, 1 or 4)."""
     scale, x = _scale_of(x)
     M, K = x.shape
     N = w.shape[0]
@@ -980,8 +977,29 @@ def gemm_skinny(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, epilogue: i
           _rows(out, "out") if ksplit == 1 else N, 1 if out.dtype == torch.float32 else 0,
           M, N, K, epilogue,
           *_prefetch_range(then_reads), ksplit, M * N if ksplit > 1 else 0, warps, *scale,
-          *(_NO_CLAMP if clamp is None else clamp.args()), _stream(), tag=("m{} k{} n{}", M, K, N))
+          *(_NO_CLAMP if clamp is None else clamp.args()), *_adapter_args(x, w, adapters), _stream(),
+          tag=("m{} k{} n{}", M, K, N))
     return out
+
+
+def _adapter_args(x: torch.Tensor, w: torch.Tensor, adapters):
+    """The weight-streaming kernel's argument for `adapters` (None: without)."""
+    if adapters is None:
+        return (0,)
+    bank, index = adapters
+    T, _, _, slots, rank, a, b, scales, which = _bank_args(x, w, bank, index)
+    low = x.new_empty(T, rank, dtype=torch.float32)
+    _COUNT[0] += 1  # the rank numbers' kernel
+    packed = array("q", (a, b, scales, which, slots, rank, low.data_ptr()))
+    return (_AdapterArgument(packed, low),)
+
+
+class _AdapterArgument(ctypes.c_void_p):
+    """The address of the packed numbers, with what has to live until the call."""
+
+    def __init__(self, packed, low):
+        super().__init__(packed.buffer_info()[0])
+        self.held = (packed, low)
 
 
 def skinny_pair_fits(x1: torch.Tensor, w1: torch.Tensor, x2: torch.Tensor, w2: torch.Tensor) -> bool:
@@ -1045,7 +1063,8 @@ def gemm_skinny_many(pairs, then_reads: Optional[torch.Tensor] = None):
 
 
 def gemm_skinny_residual(x: torch.Tensor, w: torch.Tensor, sink: ResidualSink,
-                         then_reads: Optional[torch.Tensor] = None, warps: int = 0) -> NormPending:
+                         then_reads: Optional[torch.Tensor] = None, warps: int = 0,
+                         adapters=None) -> NormPending:
     """Up to 16 token rows in front of a norm: sink.resid += x w^T in the
     product's epilogue, which also leaves resid * gamma in bfloat16 and each
     CTA's share of the rows' sums of squares for the product behind the norm."""
@@ -1063,7 +1082,7 @@ def gemm_skinny_residual(x: torch.Tensor, w: torch.Tensor, sink: ResidualSink,
           _dev(w, "w", contiguous=False), _rows(w, "w"), M, N, K,
           _dev(resid, "resid", torch.float32, contiguous=False), _rows(resid, "resid"),
           _dev(sink.gamma, "gamma", torch.float32), values.data_ptr(), N, shares.data_ptr(), 16,
-          float(sink.scale), *_prefetch_range(then_reads), warps, _stream(),
+          float(sink.scale), *_prefetch_range(then_reads), warps, *_adapter_args(x, w, adapters), _stream(),
           tag=("m{} k{} n{}", M, K, N))
     return NormPending(sink, values, shares)
 
@@ -1095,7 +1114,7 @@ def gemm_skinny_rope(x: torch.Tensor, w: torch.Tensor, positions: torch.Tensor,
                      v_cache: Optional[torch.Tensor], num_heads: int, num_kv_heads: int,
                      head_dim: int, ring_pages: int = 0, write_cache: bool = True,
                      then_reads: Optional[torch.Tensor] = None,
-                     pairing: str = "half") -> torch.Tensor:
+                     pairing: str = "half", adapters=None) -> torch.Tensor:
     """The fused q/k/v projection of up to 16 tokens, rotated and stored by the
     product's epilogue: returns the rotated queries [T, heads * head_dim]; the
     rotated keys and the values go into the cache pages (`rope_kv_write` has
@@ -1129,8 +1148,8 @@ def gemm_skinny_rope(x: torch.Tensor, w: torch.Tensor, positions: torch.Tensor,
           q_out.data_ptr(), q_out.stride(0), kp, vp, page_stride, head_stride, ring_pages,
           num_heads, num_kv_heads, head_dim, 1 if write_cache else 0, _pairing_code(pairing),
           *_prefetch_range(then_reads), skinny_plan(w.shape[0], K, False)[1],
-          1 if page_table.shape[1] <= ROPE_TRIGGER_PAGES else 0, *scale, _stream(),
-          tag=("m{} k{} n{}", T, K, w.shape[0]))
+          1 if page_table.shape[1] <= ROPE_TRIGGER_PAGES else 0, *scale, *_adapter_args(x, w, adapters),
+          _stream(), tag=("m{} k{} n{}", T, K, w.shape[0]))
     return q_out
 
 
@@ -2286,6 +2305,31 @@ def _adapted_planes(x: torch.Tensor, w: torch.Tensor, bank: AdapterBank, index: 
           tag=("t{} n{} k{} r{} tile{}", T, N, K, bank.rank, bn))
 
 
+def _bank_args(x: torch.Tensor, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor):
+    """(T, K, N, slots, rank, the addresses of a, b, scales and index) of a checked call."""
+    shape, w_shape, dtype = x.shape, w.shape, x.dtype
+    if len(shape) != 2 or len(w_shape) != 2 or shape[1] != w_shape[1]:
+        raise KernelError(f"adapted_product: x {tuple(shape)}, w {tuple(w_shape)}")
+    (T, K), N = shape, w_shape[0]
+    slots, rank, a_wide = bank.a.shape
+    if w.dtype != dtype:
+        raise KernelError(f"adapted_product: x is {dtype}, w is {w.dtype}")
+    if a_wide != K or bank.b.shape != (slots, N, rank):
+        raise KernelError(f"adapted_product: adapters {tuple(bank.a.shape)}, {tuple(bank.b.shape)} beside "
+                          f"a projection {tuple(w_shape)}")
+    _on_current_device(x, "x")
+    at = x.get_device()
+    if w.get_device() != at:
+        raise KernelError(f"w is on {w.device}, the call's rows are on {x.device}")
+    a = _given(bank.a, "a", dtype, None, at)
+    b = _given(bank.b, "b", dtype, None, at)
+    scales = _given(bank.scales, "scales", torch.float32, (slots,), at)
+    which = _given(index, "index", torch.int32, (T,), at)
+    if (a | b) % 16:
+        raise KernelError("adapted_product: the adapters must start on 16-byte boundaries")
+    return T, K, N, slots, rank, a, b, scales, which
+
+
 def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
                     out_dtype: Optional[torch.dtype] = None,
                     then_reads: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -2296,26 +2340,8 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
     which kernels run). `x` may be a `RowScaled`; `then_reads` names the weights that the step streams next,
     a hint."""
     values = x.values if isinstance(x, RowScaled) else x
-    shape, w_shape, dtype = values.shape, w.shape, values.dtype
-    if len(shape) != 2 or len(w_shape) != 2 or shape[1] != w_shape[1]:
-        raise KernelError(f"adapted_product: x {tuple(shape)}, w {tuple(w_shape)}")
-    (T, K), N = shape, w_shape[0]
-    slots, rank, a_wide = bank.a.shape
-    if w.dtype != dtype:
-        raise KernelError(f"adapted_product: x is {dtype}, w is {w.dtype}")
-    if a_wide != K or bank.b.shape != (slots, N, rank):
-        raise KernelError(f"adapted_product: adapters {tuple(bank.a.shape)}, {tuple(bank.b.shape)} beside "
-                          f"a projection {tuple(w_shape)}")
-    _on_current_device(values, "x")
-    at = values.get_device()
-    if w.get_device() != at:
-        raise KernelError(f"w is on {w.device}, the call's rows are on {values.device}")
-    a = _given(bank.a, "a", dtype, None, at)
-    b = _given(bank.b, "b", dtype, None, at)
-    scales = _given(bank.scales, "scales", torch.float32, (slots,), at)
-    which = _given(index, "index", torch.int32, (T,), at)
-    if (a | b) % 16:
-        raise KernelError("adapted_product: the adapters must start on 16-byte boundaries")
+    dtype = values.dtype
+    T, K, N, slots, rank, a, b, scales, which = _bank_args(values, w, bank, index)
     out_dtype = out_dtype or dtype
     code = code_of(out_dtype)
     out = values.new_empty(T, N, dtype=out_dtype)
@@ -2342,11 +2368,12 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
             return out
         if T <= SKINNY_ROWS:
             low = values.new_empty(T, rank, dtype=torch.float32)
+            packed = array("q", (a, b, scales, which, slots, rank, low.data_ptr()))
             scale, values = _scale_of(x)
             _COUNT[0] += 1  # the rank numbers' kernel
-            _call("fb_gemm_skinny_adapted", values.data_ptr(), values.stride()[0], w.data_ptr(), w_stride,
-                  out.data_ptr(), N, 1 - code, T, N, K, a, b, scales, which, slots, rank, low.data_ptr(),
-                  *_prefetch_range(then_reads), skinny_plan(N, K, False)[1], *scale, _stream(),
+            _call("fb_gemm_skinny", values.data_ptr(), values.stride()[0], w.data_ptr(), w_stride,
+                  out.data_ptr(), N, 1 - code, T, N, K, 0, *_prefetch_range(then_reads), 1, 0,
+                  skinny_plan(N, K, False)[1], *scale, *_NO_CLAMP, packed.buffer_info()[0], _stream(),
                   tag=("t{} n{} k{} r{}", T, N, K, rank))
             return out
     x = plain(x)
@@ -2376,6 +2403,40 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
           which, slots, rank, T, N, out.data_ptr(), code, N, _stream(),
           tag=("t{} n{} r{}", T, N, rank))
     return out
+
+
+def adapted_epilogue_fits(x, w: torch.Tensor, bank: AdapterBank) -> bool:
+    """Whether the weight-streaming product takes this projection with its adapters, and with them its other
+    epilogues (`gemm_skinny`, `gemm_skinny_rope`, `gemm_skinny_residual`)."""
+    values = x.values if isinstance(x, RowScaled) else x
+    T = values.shape[0]
+    return (0 < T <= SKINNY_ROWS and values.dtype == w.dtype == torch.bfloat16 and _tc_usable(values, w, w)
+            and not _rows_pay(T, w.shape[0], bank.slots, bank.rank))
+
+
+def adapted_silu_mul(x, w_pairs: torch.Tensor, bank: AdapterBank, index: torch.Tensor, out: torch.Tensor,
+                     then_reads: Optional[torch.Tensor] = None, act: str = "silu") -> torch.Tensor:
+    """out = act(gate) * up of the adapted product with (gate, up) pairs of weight rows ("silu" or
+    "gelu_tanh"), in the product's epilogue for a few rows."""
+    if adapted_epilogue_fits(x, w_pairs, bank):
+        return gemm_skinny(x, w_pairs, out, epilogue=GLU_EPILOGUE[act], then_reads=then_reads,
+                           warps=skinny_plan(w_pairs.shape[0], w_pairs.shape[1], False)[1],
+                           adapters=(bank, index))
+    both = adapted_product(x, w_pairs, bank, index, out_dtype=torch.float32, then_reads=then_reads)
+    return silu_mul(both, out, interleaved=True, act=act)
+
+
+def adapted_residual(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
+                     then_reads: Optional[torch.Tensor] = None, residual: Optional[ResidualSink] = None):
+    """The adapted product as 32-bit `Planes`; or, for a few rows in front of a norm, added to the residual
+    rows in the product's epilogue (a `NormPending`, as `gemm_bf16` has it)."""
+    if (residual is not None and NORM_FUSION and not isinstance(x, RowScaled)
+            and tuple(residual.resid.shape) == (x.shape[0], w.shape[0])
+            and (w.shape[0] + 15) // 16 <= MAX_SCALE_SHARES and adapted_epilogue_fits(x, w, bank)):
+        return gemm_skinny_residual(x, w, residual, then_reads=then_reads,
+                                    warps=skinny_plan(w.shape[0], w.shape[1], False)[1],
+                                    adapters=(bank, index))
+    return Planes(adapted_product(x, w, bank, index, out_dtype=torch.float32, then_reads=then_reads)[None])
 
 
 # --------------------------------------------------- layer norm, sinusoidal embedding

@@ -165,6 +165,13 @@ class GQAAttention(Part):
             q = rotated_projection(ctx, x, self.qkv.weight, self.inv_freq, self.rotary_dim,
                                    self.pairing, self.angles_key, cache, self.num_heads,
                                    self.num_kv_heads, self.head_dim)
+        elif ops.qkv_rope_fusable(x, self.qkv.weight, self.rotary_dim, self.head_dim, cache.k) \
+                and ops.adapted_epilogue_fits(x, self.qkv.weight, self.qkv_site.bank):
+            q = ops.gemm_skinny_rope(x, self.qkv.weight, ctx.positions, ctx.seq_of_token, table,
+                                     self.inv_freq, self.rotary_dim, cache.k, cache.v, self.num_heads,
+                                     self.num_kv_heads, self.head_dim, ring_pages=cache.group.ring_pages,
+                                     write_cache=cache.writes, pairing=self.pairing,
+                                     adapters=(self.qkv_site.bank, adapters))
         else:  # 32-bit sums of projection and adapters, then rotation and cache write
             qkv = ops.adapted_product(x, self.qkv.weight, self.qkv_site.bank, adapters,
                                       out_dtype=torch.float32, then_reads=self.o.weight)
@@ -172,15 +179,15 @@ class GQAAttention(Part):
                                   self.inv_freq, self.rotary_dim, cache.k, cache.v, self.num_heads,
                                   self.num_kv_heads, self.head_dim,
                                   ring_pages=cache.group.ring_pages, write_cache=cache.writes,
-                                  dtype=x.dtype, pairing=self.pairing)
+                                  dtype=ops.plain(x).dtype, pairing=self.pairing)
         attn = torch.empty((x.shape[0], self.q_size), dtype=x.dtype, device=x.device)
         ops.attention(ctx, q, attn, table, cache.k, cache.v, self.num_heads, self.num_kv_heads,
                       self.head_dim, self.scale, window=cache.group.window,
                       ring_pages=cache.group.ring_pages, then_reads=self.o.weight)
-        if adapters is not None:  # 32-bit sums for whoever adds them to the stream
-            return ops.Planes(ops.adapted_product(
-                attn, self.o.weight, self.o_site.bank, adapters, out_dtype=torch.float32,
-                then_reads=getattr(ctx, "reads_after_part", None))[None])
+        if adapters is not None:
+            return ops.adapted_residual(attn, self.o.weight, self.o_site.bank, adapters,
+                                        then_reads=getattr(ctx, "reads_after_part", None),
+                                        residual=getattr(ctx, "residual_sink", None))
         return self.o.forward(attn, allow_planes=True,
                               then_reads=getattr(ctx, "reads_after_part", None),
                               residual=getattr(ctx, "residual_sink", None))

@@ -36,7 +36,7 @@ Optional, any part
     adapter_sites() -> [AdapterSite]: the projections of a loaded part that take low-rank
     adapters (parts/adapters.py). `ctx.adapters` is then either None or int32 [tokens], each
     token's place in the sites' banks; a part with sites adds its adapters' share
-    (ops.adapted_product) in a step where it is not None. Other parts need not look at it.
+    (ops.adapted_product and its kin) in a step where it is not None. Other parts need not look at it.
     first_weight() -> the weight tensor its forward streams first, or None.
     `ctx.reads_after_part` holds the first weight of whatever runs after the
     part being called (the block sets it for its mixer and feed-forward, the

@@ -69,13 +69,12 @@ class SwiGLU(Part):
 
     def _adapted(self, ctx, x, adapters: torch.Tensor):
         """`forward` of a step of which some tokens have an adapter."""
-        both = ops.adapted_product(x, self.gate_up, self.gate_up_site.bank, adapters,
-                                   out_dtype=torch.float32, then_reads=self.down.weight)
         hidden = torch.empty((x.shape[0], self.intermediate_size), dtype=x.dtype, device=x.device)
-        ops.silu_mul(both, hidden, interleaved=True, act=self.activation)
-        return ops.Planes(ops.adapted_product(
-            hidden, self.down.weight, self.down_site.bank, adapters, out_dtype=torch.float32,
-            then_reads=getattr(ctx, "reads_after_part", None))[None])
+        ops.adapted_silu_mul(x, self.gate_up, self.gate_up_site.bank, adapters, hidden,
+                             then_reads=self.down.weight, act=self.activation)
+        return ops.adapted_residual(hidden, self.down.weight, self.down_site.bank, adapters,
+                                    then_reads=getattr(ctx, "reads_after_part", None),
+                                    residual=getattr(ctx, "residual_sink", None))
 
     def hidden(self, x) -> torch.Tensor:
         """act(gate(x)) * up(x) in the activation type: what the down projection reads."""

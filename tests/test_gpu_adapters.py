@@ -220,6 +220,87 @@ def test_banks_past_32_bits(ops, S, T):
     check(ops, x, w, small, index, got, True)
 
 
+# The weight-streaming product's other epilogues, with adapters in their sums
+def sums_of(x, w, bank, index, scale=1.0):
+    """The sums in 64 bits, and what 32-bit ones may be off by."""
+    host = lambda t: t.float().cpu().numpy()  # noqa: E731
+    want, _, much = plain.adapted(host(x), host(w), host(bank.a), host(bank.b), host(bank.scales), index.cpu().numpy())
+    return want, (x.shape[1] + bank.rank + 8) * 2.0 ** -24 * much
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("T", [1, 3, 8, 9, 16, 17, 40])
+@pytest.mark.parametrize("K,I,R,S", [(256, 128, 16, 4), (520, 100, 48, 3), (2048, 1024, 128, 9)])
+def test_gated_pairs(ops, T, K, I, R, S, act):
+    x, w, bank, index = case(ops, T, K, 2 * I, R, S, torch.bfloat16)
+    out = torch.empty(T, I, dtype=torch.bfloat16, device=DEV)
+    assert ops.adapted_epilogue_fits(x, w, bank) == (T <= 16)
+    ops.adapted_silu_mul(x, w, bank, index, out, act=act)
+    sums, off = sums_of(x, w, bank, index)
+    if T > 16:  # the rank numbers may be bfloat16 there
+        _, size, _ = plain.adapted(*(t.float().cpu().numpy() for t in (x, w, bank.a, bank.b, bank.scales)),
+                                   index.cpu().numpy())
+        off = off + 2.0 ** -8 * size
+    gate, up, d_gate, d_up = sums[:, ::2], sums[:, 1::2], off[:, ::2], off[:, 1::2]
+    if act == "silu":
+        value = gate / (1 + np.exp(-gate))
+    else:
+        value = 0.5 * gate * (1 + np.tanh(np.sqrt(2 / np.pi) * (gate + 0.044715 * gate ** 3)))
+    # both activations have slopes below 1.13; 2^-20 of the value for their own exponentials
+    want = value * up
+    bound = 1.13 * d_gate * (np.abs(up) + d_up) + np.abs(value) * d_up + (2.0 ** -8 * 1.01 + 2.0 ** -20) * np.abs(want) + 1e-30
+    assert (np.abs(out.float().cpu().numpy() - want) <= bound).all()
+
+
+@pytest.mark.parametrize("T", [1, 5, 8, 9, 16])
+@pytest.mark.parametrize("K,N,R,S,scale", [(256, 128, 16, 4, 1.0), (520, 200, 48, 3, 0.5), (4096, 2048, 64, 9, 1.0)])
+def test_sums_into_the_residual_rows(ops, T, K, N, R, S, scale):
+    x, w, bank, index = case(ops, T, K, N, R, S, torch.bfloat16)
+    g = torch.Generator().manual_seed(T)
+    before, gamma = torch.randn(T, N, generator=g).to(DEV), torch.rand(N, generator=g).to(DEV)
+    resid = before.clone()
+    got = ops.adapted_residual(x, w, bank, index, residual=ops.ResidualSink(resid, gamma, 1e-5, scale))
+    assert isinstance(got, ops.NormPending)
+    sums, off = sums_of(x, w, bank, index)
+    want = before.double().cpu().numpy() + scale * sums
+    bound = scale * off + 2.0 ** -23 * (np.abs(want) + scale * np.abs(sums))
+    assert (np.abs(resid.double().cpu().numpy() - want) <= bound).all()
+    assert torch.equal(got.values, (resid * gamma).bfloat16())
+    squares = resid.double().square().sum(1)
+    assert torch.allclose(got.shares.double().sum(0)[:T], squares, rtol=1e-5)
+    # without a sink, and for more rows than the kernel takes: 32-bit sums
+    planes = ops.adapted_residual(x, w, bank, index)
+    off = np.abs(planes.sum(torch.float32).double().cpu().numpy() - sums) - off
+    assert isinstance(planes, ops.Planes) and (off <= 2.0 ** -24 * np.abs(sums)).all()
+
+
+@pytest.mark.parametrize("pairing", ["half", "interleaved"])
+@pytest.mark.parametrize("T", [1, 6, 8, 13, 16])
+@pytest.mark.parametrize("A,Kh,D,rot", [(4, 2, 16, 16), (6, 3, 32, 32), (3, 1, 48, 32), (8, 2, 128, 128), (2, 2, 64, 0)])
+@pytest.mark.parametrize("scaled", [False, True])
+def test_rotated_projections(ops, A, Kh, D, rot, T, pairing, scaled):
+    """Against the 32-bit sums' own rotation: both round once, what they round differs by their sums' order."""
+    K, N = 264, (A + 2 * Kh) * D
+    x, w, bank, index = case(ops, T, K, N, 24, 5, torch.bfloat16)
+    inv_freq = (10000.0 ** (-torch.arange(0, rot, 2, dtype=torch.float32) / max(rot, 1))).to(DEV)
+    as_int = lambda a: torch.tensor(a, dtype=torch.int32, device=DEV)  # noqa: E731
+    positions, seqs = as_int([(37 * t) % 700 for t in range(T)]), as_int([-1 if t == 5 else 0 for t in range(T)])
+    table = torch.arange(11, dtype=torch.int32, device=DEV).view(1, 11)
+    ops_args = (positions, seqs, table, inv_freq, rot)
+    caches = [torch.zeros(11, Kh, 64, D, dtype=torch.bfloat16, device=DEV) for _ in range(4)]
+    given = ops.RowScaled(x.contiguous(), torch.rand(16, 16, device=DEV) * 40 + 1, 1e-5) if scaled else x
+    q = ops.gemm_skinny_rope(given, w, *ops_args, caches[0], caches[1], A, Kh, D, pairing=pairing, adapters=(bank, index))
+    sums = ops.adapted_product(given, w, bank, index, out_dtype=torch.float32)
+    q2 = ops.rope_kv_write(ops.Planes(sums[None].clone()), *ops_args, caches[2], caches[3], A, Kh, D,
+                           dtype=torch.bfloat16, pairing=pairing)
+    live = [t for t in range(T) if t != 5]
+    most = float(sums.abs().max())
+    for one, two in ((q[live], q2[live]), (caches[0], caches[2]), (caches[1], caches[3])):
+        one, two = one.float(), two.float()
+        # a rounding each, and 32-bit sums of K + 24 products of which none passes the largest sum by much
+        assert ((one - two).abs() <= 2.0 ** -7 * torch.maximum(one.abs(), two.abs()) + 2.0 ** -15 * most).all()
+
+
 def test_no_tokens(ops):
     x, w, bank, index = case(ops, 0, 64, 32, 8, 1, torch.bfloat16, index=[])
     assert ops.adapted_product(x, w, bank, index).shape == (0, 32)
