@@ -34,7 +34,7 @@
 //   3  the fused q/k/v projection: rotate query and key heads by the token's
 //      position (pairs of ADJACENT features, frequency i for features 2i, 2i+1),
 //      queries to q_out, keys and values into the token's cache page
-//   7  as 0, with the tokens' low-rank adapters (adapter.cu) as more K behind the product's own
+// With MORE the tokens' low-rank adapters (adapter.cu) are more K behind the product's own, whatever the epilogue;
 // and, for a product whose input is a norm's output that still lacks its row
 // scale, every token's results are multiplied by 1 / sqrt(mean square + eps).
 //
@@ -113,7 +113,7 @@ template <int NB> struct RowsCfg {
                 "the partial tile and the epilogue's turn table take the stages' place");
 };
 
-// More K behind the product's own (epilogue 7): counts[0] adapters have tokens among the rows, the e-th of them
+// More K behind the product's own: counts[0] adapters have tokens among the rows, the e-th of them
 // slots[e]; its rank numbers of the tokens, zero for tokens of others, are rows e * ROWS_A_PLANE .. of `u`, and
 // its weights for feature j row slot * N + j of `b`. Each takes `kblocks` K blocks of 64, which the CTAs of a
 // tile take in turn: one sum in tensor memory and one rounding.
@@ -145,17 +145,16 @@ __device__ __forceinline__ float ld_cluster(const float* mine, unsigned rank) {
   return v;
 }
 
-template <int NB, bool CLUSTER, int EPI>
+template <int NB, bool CLUSTER, int EPI, bool MORE>
 __global__ void __launch_bounds__(THREADS)
 gemm_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
-                 const RowsParams p, const __grid_constant__ typename RowsMoreArg<EPI == 7>::type more) {
+                 const RowsParams p, const __grid_constant__ typename RowsMoreArg<MORE>::type more) {
   using Cfg = RowsCfg<NB>;
   constexpr int STAGES = Cfg::STAGES;
   // The epilogue is a template parameter: with all four in one kernel the
   // epilogue's straight-line code did not fit the instruction cache and every
   // token's stores waited for instructions (1.1 instead of 0.6 us per 32 tokens).
-  constexpr int epi = EPI == 7 ? 0 : EPI;
-  constexpr bool MORE = EPI == 7;
+  constexpr int epi = EPI;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* tiles = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t* full = (uint64_t*)(tiles + STAGES * Cfg::STAGE_BYTES);
@@ -529,37 +528,47 @@ gemm_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   }
 }
 
-template <int NB, int EPI>
+template <int NB, int EPI, bool MORE>
 int launch_rows_as(const CUtensorMap& mw, const CUtensorMap& mx, const RowsParams& p, int tiles,
-                   cudaStream_t stream, const typename RowsMoreArg<EPI == 7>::type& more = {}) {
+                   cudaStream_t stream, const typename RowsMoreArg<MORE>::type& more) {
   static bool configured[64] = {};
   if (fb_first_use_on_device(configured)) {
-    cudaError_t e = cudaFuncSetAttribute(gemm_rows_kernel<NB, true, EPI>,
+    cudaError_t e = cudaFuncSetAttribute(gemm_rows_kernel<NB, true, EPI, MORE>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          RowsCfg<NB>::BYTES);
     if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(gemm_rows_kernel<NB, false, EPI>,
+      e = cudaFuncSetAttribute(gemm_rows_kernel<NB, false, EPI, MORE>,
                                cudaFuncAttributeMaxDynamicSharedMemorySize, RowsCfg<NB>::BYTES);
     if (e != cudaSuccess) return fb_fail(2, "gemm_rows: shared memory opt-in: %s", cudaGetErrorString(e));
   }
   if (p.splits > 1)
-    fb_launch_cluster(gemm_rows_kernel<NB, true, EPI>, dim3(tiles, 1, p.splits), dim3(THREADS),
+    fb_launch_cluster(gemm_rows_kernel<NB, true, EPI, MORE>, dim3(tiles, 1, p.splits), dim3(THREADS),
                       RowsCfg<NB>::BYTES, stream, (unsigned)p.splits, mw, mx, p, more);
   else
-    fb_launch(gemm_rows_kernel<NB, false, EPI>, dim3(tiles), dim3(THREADS), RowsCfg<NB>::BYTES,
+    fb_launch(gemm_rows_kernel<NB, false, EPI, MORE>, dim3(tiles), dim3(THREADS), RowsCfg<NB>::BYTES,
               stream, mw, mx, p, more);
   return fb_check_launch("gemm_rows");
 }
 
 template <int NB>
 int launch_rows(const CUtensorMap& mw, const CUtensorMap& mx, const RowsParams& p, int tiles,
-                cudaStream_t stream) {
+                cudaStream_t stream, const RowsMore* more) {
+  if constexpr (NB <= 64) {
+    if (more != nullptr) {
+      switch (p.epilogue) {
+        case 0: return launch_rows_as<NB, 0, true>(mw, mx, p, tiles, stream, *more);
+        case 1: return launch_rows_as<NB, 1, true>(mw, mx, p, tiles, stream, *more);
+        case 2: return launch_rows_as<NB, 2, true>(mw, mx, p, tiles, stream, *more);
+        default: return launch_rows_as<NB, 3, true>(mw, mx, p, tiles, stream, *more);
+      }
+    }
+  }
   switch (p.epilogue) {
-    case 0: return launch_rows_as<NB, 0>(mw, mx, p, tiles, stream);
-    case 1: return launch_rows_as<NB, 1>(mw, mx, p, tiles, stream);
-    case 2: return launch_rows_as<NB, 2>(mw, mx, p, tiles, stream);
-    case 4: return launch_rows_as<NB, 4>(mw, mx, p, tiles, stream);
-    default: return launch_rows_as<NB, 3>(mw, mx, p, tiles, stream);
+    case 0: return launch_rows_as<NB, 0, false>(mw, mx, p, tiles, stream, {});
+    case 1: return launch_rows_as<NB, 1, false>(mw, mx, p, tiles, stream, {});
+    case 2: return launch_rows_as<NB, 2, false>(mw, mx, p, tiles, stream, {});
+    case 4: return launch_rows_as<NB, 4, false>(mw, mx, p, tiles, stream, {});
+    default: return launch_rows_as<NB, 3, false>(mw, mx, p, tiles, stream, {});
   }
 }
 
@@ -578,6 +587,41 @@ FB_API int fb_gemm_rows_splits(int N, int K) {
   return (kblocks + per - 1) / per;  // no CTA without a K block
 }
 
+// adapter.cu
+extern "C" int fb_adapter_shrink_planes(const void* x, long long ldx, const void* a, const float* scales,
+                                        const int* index, int slots, int rank, int T, int K, void* u, int* counts,
+                                        int* slots_of, cudaStream_t stream);
+
+// What `adapter` (on the host) says of the adapters of up to 64 tokens: a [slots, rank, K] and b [slots, N, rank]
+// bfloat16, scales [slots], index [M] (outside of the bank: none), slots, rank; u [most * 256, rank] bfloat16,
+// counts [1], slots_of [most]: room for the rank numbers, most = the smaller of slots and M; and whether they are
+// there (fb_adapter_low), else a kernel in front writes them.
+static int rows_more_of(const long long* adapter, const void* x, long long ldx, int M, int N, int K, int NB,
+                        cudaStream_t stream, RowsMore* more) {
+  const void* a = (const void*)adapter[0];
+  const void* b = (const void*)adapter[1];
+  const float* scales = (const float*)adapter[2];
+  const int* index = (const int*)adapter[3];
+  const int slots = (int)adapter[4], rank = (int)adapter[5];
+  void* u = (void*)adapter[6];
+  int* counts = (int*)adapter[7];
+  int* slots_of = (int*)adapter[8];
+  FB_REQUIRE(M <= 64 && slots > 0 && slots <= 1024 && rank > 0 && rank % 8 == 0 && a && b && scales && index && u &&
+                 counts && slots_of && (((uintptr_t)b | (uintptr_t)u) % 16) == 0,
+             "gemm_rows: a bank of %d adapters of rank %d for %d tokens", slots, rank, M);
+  FB_REQUIRE((long long)slots * N < (1ll << 31) - BM, "gemm_rows: %d adapters of %d rows", slots, N);
+  if (adapter[9] == 0)
+    if (int rc = fb_adapter_shrink_planes(x, ldx, a, scales, index, slots, rank, M, K, u, counts, slots_of, stream))
+      return rc;
+  const int most = slots < M ? slots : M;
+  int rc = make_map(&more->u, u, (long long)most * ROWS_A_PLANE, rank, rank, NB);
+  if (!rc) rc = make_map(&more->b, b, (long long)slots * N, rank, rank, BM);
+  more->counts = counts;
+  more->slots = slots_of;
+  more->kblocks = (rank + BK - 1) / BK;
+  return rc;
+}
+
 // out = x W^T with the epilogue named; see the head of the file.
 //   x: [M, K] bf16, row stride ldx, 17 <= M <= 256 (fewer work, at the cost of a
 //      mostly empty tile); w: [N, K] bf16, row stride ldw
@@ -589,6 +633,7 @@ FB_API int fb_gemm_rows_splits(int N, int K) {
 //      features, so the caller's weight rows must be laid out that way
 //   scale_*: the input's row scale (scale_ss null: none)
 //   splits: CTAs per weight tile, 1 to 8 (0: fb_gemm_rows_splits' choice)
+//   adapter: null, or the tokens' adapters (rows_more_of), beside epilogues 0 to 3
 FB_API int fb_gemm_rows(const void* x, long long ldx, int M, const void* w, long long ldw, int N,
                         int K, void* out, long long ldo, int out_f32, int epilogue,
                         const float* scale_ss, int scale_count, int scale_stride, int scale_dim,
@@ -599,7 +644,7 @@ FB_API int fb_gemm_rows(const void* x, long long ldx, int M, const void* w, long
                         long long q_stride, void* k_cache, void* v_cache, long long page_stride,
                         long long head_stride, int ring_pages, int A, int Kh, int D, int splits,
                         float glu_limit, float glu_alpha, float glu_shift, const float* glu_bias,
-                        cudaStream_t stream) {
+                        const long long* adapter, cudaStream_t stream) {
   FB_REQUIRE(M > 0 && M <= 256 && N > 0 && K > 0, "gemm_rows: bad sizes %d x %d x %d", M, N, K);
   FB_REQUIRE(K % 8 == 0 && ldx % 8 == 0 && ldw % 8 == 0 && ((uintptr_t)x % 16) == 0 &&
                  ((uintptr_t)w % 16) == 0,
@@ -610,6 +655,7 @@ FB_API int fb_gemm_rows(const void* x, long long ldx, int M, const void* w, long
   if (epilogue == 4) epilogue = 1;
   FB_REQUIRE((epilogue >= 0 && epilogue <= 3) || epilogue == 6, "gemm_rows: unknown epilogue %d",
              epilogue);
+  FB_REQUIRE(adapter == nullptr || epilogue != 6, "gemm_rows: no adapters beside the clamped epilogue");
   RowsParams p{};
   p.glu_act = glu_act;
   if (epilogue == 6) {  // as 1 with clamped halves and biases (glu_*; glu_bias null: none)
@@ -667,66 +713,26 @@ FB_API int fb_gemm_rows(const void* x, long long ldx, int M, const void* w, long
   if (rc) return rc;
   rc = make_map(&mx, x, M, K, ldx, NB);
   if (rc) return rc;
+  RowsMore added{};
+  if (adapter != nullptr)
+    if (int failed = rows_more_of(adapter, x, ldx, M, N, K, NB, stream, &added)) return failed;
+  const RowsMore* more = adapter != nullptr ? &added : nullptr;
   switch (NB) {
-    case 32: return launch_rows<32>(mw, mx, p, tiles, stream);
-    case 64: return launch_rows<64>(mw, mx, p, tiles, stream);
-    case 128: return launch_rows<128>(mw, mx, p, tiles, stream);
-    default: return launch_rows<256>(mw, mx, p, tiles, stream);
+    case 32: return launch_rows<32>(mw, mx, p, tiles, stream, more);
+    case 64: return launch_rows<64>(mw, mx, p, tiles, stream, more);
+    case 128: return launch_rows<128>(mw, mx, p, tiles, stream, nullptr);
+    default: return launch_rows<256>(mw, mx, p, tiles, stream, nullptr);
   }
 }
 
-// adapter.cu
-extern "C" int fb_adapter_shrink_planes(const void* x, long long ldx, const void* a, const float* scales,
-                                        const int* index, int slots, int rank, int T, int K, void* u, int* counts,
-                                        int* slots_of, cudaStream_t stream);
-
-// out[t] = scale of t's row * (x[t] w^T + scales[i] (x[t] a[i]^T) b[i]^T), i = index[t] (outside of the bank:
-// without the second part), for up to 64 tokens. a [slots, rank, K], b [slots, N, rank] bfloat16; u [most * 256,
-// rank] bfloat16, counts [1], slots_of [most]: room for the rank numbers, most = the smaller of slots and M; with
-// `made` they are there (fb_adapter_low), else a kernel in front writes them. The rest as in fb_gemm_rows.
+// fb_gemm_rows with epilogue 0 and adapters, in fewer arguments.
 FB_API int fb_gemm_rows_adapted(const void* x, long long ldx, int M, const void* w, long long ldw, int N, int K,
                                 void* out, long long ldo, int out_f32, const float* scale_ss, int scale_count,
-                                int scale_stride, int scale_dim, float scale_eps, const void* a, const void* b,
-                                const float* scales, const int* index, int slots, int rank, void* u, int* counts,
-                                int* slots_of, int made, int splits, cudaStream_t stream) {
-  FB_REQUIRE(M > 0 && M <= 64 && N > 0 && K > 0 && out != nullptr && ldo >= N, "gemm_rows_adapted: bad sizes %d x %d x %d",
-             M, N, K);
-  FB_REQUIRE(K % 8 == 0 && ldx % 8 == 0 && ldw % 8 == 0 &&
-                 (((uintptr_t)x | (uintptr_t)w | (uintptr_t)b | (uintptr_t)u) % 16) == 0,
-             "gemm_rows_adapted: K and the row strides must be multiples of 8 elements and the operands "
-             "16-byte aligned (K=%d ldx=%lld ldw=%lld)", K, ldx, ldw);
-  FB_REQUIRE(slots > 0 && slots <= 1024 && rank > 0 && rank % 8 == 0 && a && b && scales && index && u && counts && slots_of,
-             "gemm_rows_adapted: a bank of %d adapters of rank %d", slots, rank);
-  FB_REQUIRE((long long)slots * N < (1ll << 31) - BM, "gemm_rows_adapted: %d adapters of %d rows", slots, N);
-  if (!made)
-    if (int rc = fb_adapter_shrink_planes(x, ldx, a, scales, index, slots, rank, M, K, u, counts, slots_of, stream))
-      return rc;
-  RowsParams p{};
-  p.M = M; p.N = N; p.K = K;
-  const int tiles = (N + BM - 1) / BM;
-  p.kblocks = (K + BK - 1) / BK;
-  if (splits <= 0) splits = fb_gemm_rows_splits(N, K);
-  FB_REQUIRE(splits <= 8 && splits <= p.kblocks, "gemm_rows_adapted: %d CTAs per tile for %d K blocks "
-             "(at most 8)", splits, p.kblocks);
-  p.per = (p.kblocks + splits - 1) / splits;
-  p.splits = (p.kblocks + p.per - 1) / p.per;
-  p.cols_per = (M + p.splits - 1) / p.splits;
-  p.out = out; p.ldo = ldo; p.out_f32 = out_f32;
-  p.scale = RowsScale{scale_ss, scale_count, scale_stride,
-                      scale_dim > 0 ? 1.0f / (float)scale_dim : 0.f, scale_eps};
-  p.vector_ok = ldo % 4 == 0 && ((uintptr_t)out % 16) == 0;
-  bind_status_mirror(stream);
-  const int NB = M <= 32 ? 32 : 64, most = slots < M ? slots : M;
-  CUtensorMap mw, mx;
-  RowsMore more{};
-  int rc = make_map(&mw, w, N, K, ldw, BM);
-  if (!rc) rc = make_map(&mx, x, M, K, ldx, NB);
-  if (!rc) rc = make_map(&more.u, u, (long long)most * ROWS_A_PLANE, rank, rank, NB);
-  if (!rc) rc = make_map(&more.b, b, (long long)slots * N, rank, rank, BM);
-  if (rc) return rc;
-  more.counts = counts; more.slots = slots_of; more.kblocks = (rank + BK - 1) / BK;
-  return NB == 32 ? launch_rows_as<32, 7>(mw, mx, p, tiles, stream, more)
-                  : launch_rows_as<64, 7>(mw, mx, p, tiles, stream, more);
+                                int scale_stride, int scale_dim, float scale_eps, int splits,
+                                const long long* adapter, cudaStream_t stream) {
+  return fb_gemm_rows(x, ldx, M, w, ldw, N, K, out, ldo, out_f32, 0, scale_ss, scale_count, scale_stride, scale_dim,
+                      scale_eps, nullptr, 0, nullptr, nullptr, 0, nullptr, 0, nullptr, nullptr, nullptr, 0, nullptr, 0,
+                      nullptr, 0, nullptr, nullptr, 0, 0, 0, 0, 0, 0, splits, 0.f, 0.f, 0.f, nullptr, adapter, stream);
 }
 
 // As fb_gemm_tc_status, for the kernel of this file.

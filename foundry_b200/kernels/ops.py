@@ -101,7 +101,7 @@ _SIGNATURES = {
                      c_int, c_void_p, c_int, c_int, c_int, c_float, c_void_p, c_ll, c_void_p,
                      c_void_p, c_ll, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int,
                      c_void_p, c_int, c_void_p, c_ll, c_void_p, c_void_p, c_ll, c_ll, c_int, c_int,
-                     c_int, c_int, c_int, c_float, c_float, c_float, c_void_p, c_void_p],
+                     c_int, c_int, c_int, c_float, c_float, c_float, c_void_p, c_void_p, c_void_p],
     "fb_gemm_rows_status": [c_void_p],
     "fb_event_create": [c_void_p],
     "fb_event_synchronize": [c_void_p],
@@ -123,9 +123,7 @@ _SIGNATURES = {
     "fb_adapter_shrink": [c_void_p, c_ll, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                           c_int, c_void_p, c_void_p],
     "fb_gemm_rows_adapted": [c_void_p, c_ll, c_int, c_void_p, c_ll, c_int, c_int, c_void_p, c_ll, c_int,
-                             c_void_p, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p,
-                             c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
-                             c_void_p],
+                             c_void_p, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p],
     "fb_adapter_low": [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                        c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     "fb_gemm_tc_adapted": [c_void_p, c_ll, c_int, c_void_p, c_ll, c_int, c_int, c_void_p, c_void_p,
@@ -1170,8 +1168,9 @@ def rows_usable(x, w) -> bool:
 
 
 def _gemm_rows(x, w, epilogue: int, out=None, sink: Optional[ResidualSink] = None,
-               sink_out=None, rope=None, clamp: Optional[GluClamp] = None) -> None:
-    """The launcher's face; `x` may be a `RowScaled`."""
+               sink_out=None, rope=None, clamp: Optional[GluClamp] = None, adapters=None) -> None:
+    """The launcher's face; `x` may be a `RowScaled`. `adapters`: (an `AdapterBank`, each row's place in
+    it), for up to 64 rows."""
     scale = _NO_SCALE
     if isinstance(x, RowScaled):
         scale, x = x.scale_args(), x.values
@@ -1193,13 +1192,35 @@ def _gemm_rows(x, w, epilogue: int, out=None, sink: Optional[ResidualSink] = Non
     _call("fb_gemm_rows", _dev(x, "x", torch.bfloat16, contiguous=False), _rows(x, "x"), M,
           _dev(w, "w", torch.bfloat16, contiguous=False), _rows(w, "w"), N, K, *out_args, epilogue,
           *scale, *sink_args, *rope_args, ROWS_SPLITS,
-          *(_NO_CLAMP if clamp is None else clamp.args()), _stream(),
+          *(_NO_CLAMP if clamp is None else clamp.args()), *_rows_adapter_args(x, w, adapters), _stream(),
           tag=("m{} k{} n{} e{}", M, K, N, epilogue))
+
+
+def _rows_adapter(values, T, K, bank, index, slots, rank, addresses):
+    """The few-rows product's numbers for a bank, and the tensors that they point to; the rank numbers are made
+    here if the tensor cores are to make them."""
+    most = min(slots, T)
+    u = values.new_empty(most * ADAPTER_BLOCK, rank)
+    lists = values.new_empty(1 + most, dtype=torch.int32)
+    counts = lists.data_ptr()
+    made = _low_pays(T, K, slots, rank)
+    if made:
+        _adapter_low(values, bank, index, most, u.data_ptr(), counts, counts + 4, 0)
+    else:
+        _COUNT[0] += 1  # the rank numbers' kernel
+    return array("q", (*addresses, slots, rank, u.data_ptr(), counts, counts + 4, made)), (u, lists)
+
+
+def _rows_adapter_args(x: torch.Tensor, w: torch.Tensor, adapters):
+    if adapters is None:
+        return (0,)
+    T, K, _, slots, rank, *addresses = _bank_args(x, w, *adapters)
+    return (_AdapterArgument(*_rows_adapter(x, T, K, *adapters, slots, rank, addresses)),)
 
 
 def gemm_rows(x, w: torch.Tensor, out: Optional[torch.Tensor] = None,
               out_dtype: Optional[torch.dtype] = None, silu_mul: bool = False,
-              act: str = "silu", clamp: Optional[GluClamp] = None) -> torch.Tensor:
+              act: str = "silu", clamp: Optional[GluClamp] = None, adapters=None) -> torch.Tensor:
     """out[M, N] = x[M, K] @ w[N, K]^T for 17 to 256 token rows (any count up to
     256 works); with `silu_mul` the weight rows are (gate, up) pairs and out is
     [M, N / 2] = act(gate) * up. `x` may be a `RowScaled`."""
@@ -1209,11 +1230,11 @@ def gemm_rows(x, w: torch.Tensor, out: Optional[torch.Tensor] = None,
                           device=w.device)
     if tuple(out.shape) != (M, N // 2 if silu_mul else N) or out.stride(1) != 1:
         raise KernelError(f"gemm_rows: out is {tuple(out.shape)} for x {tuple(x.shape)}, w {tuple(w.shape)}")
-    _gemm_rows(x, w, GLU_EPILOGUE[act] if silu_mul else 0, out=out, clamp=clamp)
+    _gemm_rows(x, w, GLU_EPILOGUE[act] if silu_mul else 0, out=out, clamp=clamp, adapters=adapters)
     return out
 
 
-def gemm_rows_residual(x: torch.Tensor, w: torch.Tensor, sink: ResidualSink) -> NormPending:
+def gemm_rows_residual(x: torch.Tensor, w: torch.Tensor, sink: ResidualSink, adapters=None) -> NormPending:
     """The same product in front of a norm: sink.resid += x w^T in the epilogue,
     which also leaves resid * gamma in bfloat16 and each weight tile's share of
     the rows' sums of squares (see `gemm_skinny_residual`)."""
@@ -1223,7 +1244,7 @@ def gemm_rows_residual(x: torch.Tensor, w: torch.Tensor, sink: ResidualSink) -> 
                           f"{tuple(sink.gamma.shape)} for a product of {(M, N)}")
     values = torch.empty((M, N), dtype=torch.bfloat16, device=w.device)
     shares = torch.empty(((N + 127) // 128, (M + 31) // 32 * 32), dtype=torch.float32, device=w.device)
-    _gemm_rows(x, w, 2, sink=sink, sink_out=(values, shares))
+    _gemm_rows(x, w, 2, sink=sink, sink_out=(values, shares), adapters=adapters)
     return NormPending(sink, values, shares)
 
 
@@ -1231,7 +1252,7 @@ def gemm_rows_rope(x, w: torch.Tensor, positions: torch.Tensor, seq_of_token: to
                    page_table: torch.Tensor, inv_freq: torch.Tensor, rotary_dim: int,
                    k_cache: Optional[torch.Tensor], v_cache: Optional[torch.Tensor],
                    num_heads: int, num_kv_heads: int, head_dim: int, ring_pages: int = 0,
-                   write_cache: bool = True) -> torch.Tensor:
+                   write_cache: bool = True, adapters=None) -> torch.Tensor:
     """The fused q/k/v projection of 17 to 256 tokens, rotated and stored by the
     product's epilogue (see `gemm_skinny_rope`). The rotation pairs ADJACENT
     features (frequency i turns features 2i and 2i + 1 of a head): the caller's
@@ -1256,7 +1277,7 @@ def gemm_rows_rope(x, w: torch.Tensor, positions: torch.Tensor, seq_of_token: to
             _dev(inv_freq, "inv_freq", torch.float32) if rotary_dim else 0, rotary_dim,
             q_out.data_ptr(), q_out.stride(0), kp, vp, page_stride, head_stride, ring_pages,
             num_heads, num_kv_heads, head_dim)
-    _gemm_rows(x, w, 3, rope=rope)
+    _gemm_rows(x, w, 3, rope=rope, adapters=adapters)
     return q_out
 
 
@@ -2351,20 +2372,11 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
     if bf16 and T <= 64 and _tc_usable(values, w, w):
         w_stride = w.stride()[0]
         if _rows_pay(T, N, slots, rank):
-            most = min(slots, T)
-            u = values.new_empty(most * ADAPTER_BLOCK, rank)
-            lists = values.new_empty(1 + most, dtype=torch.int32)
-            counts = lists.data_ptr()
             scale, values = _scale_of(x)
-            made = _low_pays(T, K, slots, rank)
-            if made:
-                _adapter_low(values, bank, index, most, u.data_ptr(), counts, counts + 4, 0)
-            else:
-                _COUNT[0] += 1  # the rank numbers' kernel
+            packed, held = _rows_adapter(values, T, K, bank, index, slots, rank, (a, b, scales, which))
             _call("fb_gemm_rows_adapted", values.data_ptr(), values.stride()[0], T, w.data_ptr(), w_stride,
-                  N, K, out.data_ptr(), N, 1 - code, *scale, a, b, scales, which, slots, rank,
-                  u.data_ptr(), counts, counts + 4, int(made), ROWS_SPLITS, _stream(),
-                  tag=("t{} n{} k{} r{}", T, N, K, rank))
+                  N, K, out.data_ptr(), N, 1 - code, *scale, ROWS_SPLITS, packed.buffer_info()[0],
+                  _stream(), tag=("t{} n{} k{} r{}", T, N, K, rank))
             return out
         if T <= SKINNY_ROWS:
             low = values.new_empty(T, rank, dtype=torch.float32)
@@ -2414,6 +2426,13 @@ def adapted_epilogue_fits(x, w: torch.Tensor, bank: AdapterBank) -> bool:
             and not _rows_pay(T, w.shape[0], bank.slots, bank.rank))
 
 
+def adapted_rows_fit(x, w: torch.Tensor, bank: AdapterBank) -> bool:
+    """The same of the few-rows tcgen05 product (`gemm_rows`, `gemm_rows_rope`, `gemm_rows_residual`)."""
+    values = x.values if isinstance(x, RowScaled) else x
+    return (values.dtype == w.dtype == torch.bfloat16 and values.shape[0] > 0 and _tc_usable(values, w, w)
+            and _rows_pay(values.shape[0], w.shape[0], bank.slots, bank.rank))
+
+
 def adapted_silu_mul(x, w_pairs: torch.Tensor, bank: AdapterBank, index: torch.Tensor, out: torch.Tensor,
                      then_reads: Optional[torch.Tensor] = None, act: str = "silu") -> torch.Tensor:
     """out = act(gate) * up of the adapted product with (gate, up) pairs of weight rows ("silu" or
@@ -2422,6 +2441,8 @@ def adapted_silu_mul(x, w_pairs: torch.Tensor, bank: AdapterBank, index: torch.T
         return gemm_skinny(x, w_pairs, out, epilogue=GLU_EPILOGUE[act], then_reads=then_reads,
                            warps=skinny_plan(w_pairs.shape[0], w_pairs.shape[1], False)[1],
                            adapters=(bank, index))
+    if adapted_rows_fit(x, w_pairs, bank):
+        return gemm_rows(x, w_pairs, out, silu_mul=True, act=act, adapters=(bank, index))
     both = adapted_product(x, w_pairs, bank, index, out_dtype=torch.float32, then_reads=then_reads)
     return silu_mul(both, out, interleaved=True, act=act)
 
@@ -2431,11 +2452,13 @@ def adapted_residual(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
     """The adapted product as 32-bit `Planes`; or, for a few rows in front of a norm, added to the residual
     rows in the product's epilogue (a `NormPending`, as `gemm_bf16` has it)."""
     if (residual is not None and NORM_FUSION and not isinstance(x, RowScaled)
-            and tuple(residual.resid.shape) == (x.shape[0], w.shape[0])
-            and (w.shape[0] + 15) // 16 <= MAX_SCALE_SHARES and adapted_epilogue_fits(x, w, bank)):
-        return gemm_skinny_residual(x, w, residual, then_reads=then_reads,
-                                    warps=skinny_plan(w.shape[0], w.shape[1], False)[1],
-                                    adapters=(bank, index))
+            and tuple(residual.resid.shape) == (x.shape[0], w.shape[0])):
+        if (w.shape[0] + 15) // 16 <= MAX_SCALE_SHARES and adapted_epilogue_fits(x, w, bank):
+            return gemm_skinny_residual(x, w, residual, then_reads=then_reads,
+                                        warps=skinny_plan(w.shape[0], w.shape[1], False)[1],
+                                        adapters=(bank, index))
+        if x.shape[0] > SKINNY_ROWS and residual.scale == 1.0 and adapted_rows_fit(x, w, bank):
+            return gemm_rows_residual(x, w, residual, adapters=(bank, index))
     return Planes(adapted_product(x, w, bank, index, out_dtype=torch.float32, then_reads=then_reads)[None])
 
 

@@ -172,6 +172,13 @@ class GQAAttention(Part):
                                      self.num_kv_heads, self.head_dim, ring_pages=cache.group.ring_pages,
                                      write_cache=cache.writes, pairing=self.pairing,
                                      adapters=(self.qkv_site.bank, adapters))
+        elif ops.qkv_rows_rope_fusable(x, self.qkv.weight, self.rotary_dim, self.head_dim, cache.k,
+                                       self.pairing) and cache.writes \
+                and ops.adapted_rows_fit(x, self.qkv.weight, self.qkv_site.bank):
+            q = ops.gemm_rows_rope(x, self.qkv.weight, ctx.positions, ctx.seq_of_token, table, self.inv_freq,
+                                   self.rotary_dim, cache.k, cache.v, self.num_heads, self.num_kv_heads,
+                                   self.head_dim, ring_pages=cache.group.ring_pages,
+                                   write_cache=cache.writes, adapters=(self.qkv_site.bank, adapters))
         else:  # 32-bit sums of projection and adapters, then rotation and cache write
             qkv = ops.adapted_product(x, self.qkv.weight, self.qkv_site.bank, adapters,
                                       out_dtype=torch.float32, then_reads=self.o.weight)

@@ -229,12 +229,12 @@ def sums_of(x, w, bank, index, scale=1.0):
 
 
 @pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
-@pytest.mark.parametrize("T", [1, 3, 8, 9, 16, 17, 40])
+@pytest.mark.parametrize("T", [1, 3, 8, 9, 16, 17, 32, 40, 64, 70])
 @pytest.mark.parametrize("K,I,R,S", [(256, 128, 16, 4), (520, 100, 48, 3), (2048, 1024, 128, 9)])
 def test_gated_pairs(ops, T, K, I, R, S, act):
     x, w, bank, index = case(ops, T, K, 2 * I, R, S, torch.bfloat16)
     out = torch.empty(T, I, dtype=torch.bfloat16, device=DEV)
-    assert ops.adapted_epilogue_fits(x, w, bank) == (T <= 16)
+    assert ops.adapted_epilogue_fits(x, w, bank) == (T <= 16) and ops.adapted_rows_fit(x, w, bank) == (17 <= T <= 64)
     ops.adapted_silu_mul(x, w, bank, index, out, act=act)
     sums, off = sums_of(x, w, bank, index)
     if T > 16:  # the rank numbers may be bfloat16 there
@@ -252,7 +252,7 @@ def test_gated_pairs(ops, T, K, I, R, S, act):
     assert (np.abs(out.float().cpu().numpy() - want) <= bound).all()
 
 
-@pytest.mark.parametrize("T", [1, 5, 8, 9, 16])
+@pytest.mark.parametrize("T", [1, 5, 8, 9, 16, 17, 40, 64])
 @pytest.mark.parametrize("K,N,R,S,scale", [(256, 128, 16, 4, 1.0), (520, 200, 48, 3, 0.5), (4096, 2048, 64, 9, 1.0)])
 def test_sums_into_the_residual_rows(ops, T, K, N, R, S, scale):
     x, w, bank, index = case(ops, T, K, N, R, S, torch.bfloat16)
@@ -260,8 +260,15 @@ def test_sums_into_the_residual_rows(ops, T, K, N, R, S, scale):
     before, gamma = torch.randn(T, N, generator=g).to(DEV), torch.rand(N, generator=g).to(DEV)
     resid = before.clone()
     got = ops.adapted_residual(x, w, bank, index, residual=ops.ResidualSink(resid, gamma, 1e-5, scale))
-    assert isinstance(got, ops.NormPending)
     sums, off = sums_of(x, w, bank, index)
+    if T > 16:
+        _, size, _ = plain.adapted(*(t.float().cpu().numpy() for t in (x, w, bank.a, bank.b, bank.scales)),
+                                   index.cpu().numpy())
+        off = off + 2.0 ** -8 * size
+    if T > 16 and scale != 1.0:  # that product adds its sums as they are
+        assert isinstance(got, ops.Planes) and torch.equal(resid, before)
+        return
+    assert isinstance(got, ops.NormPending)
     want = before.double().cpu().numpy() + scale * sums
     bound = scale * off + 2.0 ** -23 * (np.abs(want) + scale * np.abs(sums))
     assert (np.abs(resid.double().cpu().numpy() - want) <= bound).all()
@@ -275,7 +282,7 @@ def test_sums_into_the_residual_rows(ops, T, K, N, R, S, scale):
 
 
 @pytest.mark.parametrize("pairing", ["half", "interleaved"])
-@pytest.mark.parametrize("T", [1, 6, 8, 13, 16])
+@pytest.mark.parametrize("T", [1, 6, 8, 13, 16, 17, 40, 64])
 @pytest.mark.parametrize("A,Kh,D,rot", [(4, 2, 16, 16), (6, 3, 32, 32), (3, 1, 48, 32), (8, 2, 128, 128), (2, 2, 64, 0)])
 @pytest.mark.parametrize("scaled", [False, True])
 def test_rotated_projections(ops, A, Kh, D, rot, T, pairing, scaled):
@@ -288,8 +295,18 @@ def test_rotated_projections(ops, A, Kh, D, rot, T, pairing, scaled):
     table = torch.arange(11, dtype=torch.int32, device=DEV).view(1, 11)
     ops_args = (positions, seqs, table, inv_freq, rot)
     caches = [torch.zeros(11, Kh, 64, D, dtype=torch.bfloat16, device=DEV) for _ in range(4)]
-    given = ops.RowScaled(x.contiguous(), torch.rand(16, 16, device=DEV) * 40 + 1, 1e-5) if scaled else x
-    q = ops.gemm_skinny_rope(given, w, *ops_args, caches[0], caches[1], A, Kh, D, pairing=pairing, adapters=(bank, index))
+    given = ops.RowScaled(x.contiguous(), torch.rand(16, (T + 15) // 16 * 16, device=DEV) * 40 + 1, 1e-5) if scaled else x
+    if T <= 16:
+        q = ops.gemm_skinny_rope(given, w, *ops_args, caches[0], caches[1], A, Kh, D, pairing=pairing,
+                                 adapters=(bank, index))
+    else:
+        if pairing == "half":
+            pytest.skip("that product rotates neighbours")
+        assert ops.qkv_rows_rope_fusable(given, w, rot, D, caches[0], pairing) and ops.adapted_rows_fit(given, w, bank)
+        q = ops.gemm_rows_rope(given, w, *ops_args, caches[0], caches[1], A, Kh, D, adapters=(bank, index))
+        # (without the cache's rows its weights would be fewer than the bank's)
+        with pytest.raises(ops.KernelError):
+            ops.gemm_rows_rope(given, w, *ops_args, None, None, A, Kh, D, write_cache=False, adapters=(bank, index))
     sums = ops.adapted_product(given, w, bank, index, out_dtype=torch.float32)
     q2 = ops.rope_kv_write(ops.Planes(sums[None].clone()), *ops_args, caches[2], caches[3], A, Kh, D,
                            dtype=torch.bfloat16, pairing=pairing)
