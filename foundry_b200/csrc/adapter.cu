@@ -403,8 +403,9 @@ FB_API int fb_adapter_shrink_planes(const void* x, long long ldx, const void* a,
   FB_REQUIRE(T > 0 && T <= PLANE_ROWS && K > 0 && rank > 0 && slots > 0 && slots <= PLANE_SLOTS && ldx >= K,
              "adapter_shrink_planes: bad sizes T=%d K=%d rank=%d slots=%d", T, K, rank, slots);
   const int wide = K % 8 == 0 && ldx % 8 == 0 && (((uintptr_t)x | (uintptr_t)a) % 16) == 0;
-  launch_shrink<__nv_bfloat16, true>((const __nv_bfloat16*)x, ldx, (const __nv_bfloat16*)a, scales, index, slots, rank, T,
-                                      K, wide, nullptr, ShrinkPlanes{(__nv_bfloat16*)u, counts, slots_of}, stream);
+  launch_shrink<__nv_bfloat16, true>((const __nv_bfloat16*)x, ldx, (const __nv_bfloat16*)a, scales, index, slots,
+                                     rank, T, K, wide, nullptr, ShrinkPlanes{(__nv_bfloat16*)u, counts, slots_of},
+                                     stream);
   return fb_check_launch("adapter_shrink_planes");
 }
 

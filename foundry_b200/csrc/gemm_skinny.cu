@@ -724,7 +724,8 @@ extern "C" int fb_adapter_shrink(const void* x, long long ldx, int dtype, const 
 
 // What `adapter` (on the host, or null: none) says of the tokens' adapters: a [slots, rank, K] and b [slots, N, rank]
 // bfloat16, scales [slots], index [T] (outside of the bank: none), slots, rank, and low [T, rank] float32, which
-// a kernel in front of the product fills: token t's results then are those of x[t] w^T + scales[i] (x[t] a[i]^T) b[i]^T.
+// a kernel in front of the product fills: token t's results then are those of
+// x[t] w^T + scales[i] (x[t] a[i]^T) b[i]^T.
 static int adapter_of(const long long* adapter, const void* x, long long ldx, int T, int K, cudaStream_t stream,
                       AdapterAdd* add) {
   *add = AdapterAdd{};
