@@ -8,17 +8,19 @@
 //   `adapter_low` (adapter_tcgen05.cu) makes the rank numbers of each block of 256 tokens as planes, one for
 //   every adapter that has tokens in the block (zero in the rows of others), and the product takes them as
 //   more K behind its own, [x | planes] [W | B]^T: one sum in tensor memory, one rounding
-//   (gemm_tcgen05_pair.cu, MoreK). The rank numbers are rounded to bfloat16 for that, 2^-9 of the adapter's
-//   part on average.
+//   (gemm_tcgen05_pair.cu, MoreK). A rank number goes there as the sum of two bfloat16 numbers
+//   (adapter_planes.cuh), 16 bits of it, and its rounding is 2^-16 of the adapter's part at most, a 256th of a
+//   bfloat16 result's own. (Rounded to one bfloat16 number: 16.8 us where 18.6 stands below, 2,048 tokens the same.)
 //   Up to 64 tokens, bfloat16, few adapters (below 17 only beside wide projections): the same with planes by
 //   `adapter_shrink` behind the K of the product that shares K in a cluster (gemm_rows_tcgen05.cu, RowsMore):
-//   48 tokens of 4,096 -> 4,096 with 12 adapters of rank 64 16.8 us, 19.4 with a pass of its own for the sums;
+//   48 tokens of 4,096 -> 4,096 with 12 adapters of rank 64 18.6 us, 19.6 with a pass of its own for the sums;
 //   10.1 without adapters.
 //   Else up to 16 tokens, bfloat16: `adapter_shrink` leaves them as 32-bit rows, and the weight-streaming product
 //   adds their product with B to its sums in front of its epilogue (gemm_skinny.cu, ADAPT). Nothing is rounded in
 //   between.
 //   Else: `adapter_shrink` (or, for many numbers, `adapter_low`) leaves them as 32-bit rows, the projection
 //   leaves 32-bit sums (split-K planes), and `adapter_expand` adds up sums and adapters and rounds once.
+#include "adapter_planes.cuh"
 #include "common.cuh"
 
 namespace {
@@ -43,7 +45,7 @@ __device__ __forceinline__ float dot8(const uint4& a, const uint4& b, float sum)
 }
 
 // The rank numbers as planes for a product that takes them as more K (fb_gemm_rows_adapted): adapter by
-// adapter [256 rows, rank] bfloat16, zero in the rows of other adapters' tokens.
+// adapter [256 rows, fb_plane_width(rank)] bfloat16, zero in the rows of other adapters' tokens.
 struct ShrinkPlanes {
   __nv_bfloat16* u;
   int* counts;    // [1]: adapters with tokens
@@ -107,11 +109,12 @@ adapter_shrink_kernel(const T* x, long long ldx, const T* a, const float* scales
       }
     }
     __syncthreads();
-    const int live = min(BLOCK_RANKS, rank - j0);
+    // (the last block's part reaches to the end of the last 32 ranks)
+    const int live = (j0 + BLOCK_RANKS >= rank ? fb_plane_ranks(rank) : j0 + BLOCK_RANKS) - j0;
     for (int i = tid; i < s_count * live; i += THREADS) {
-      const int e = i / live;
-      if (!own || e != s_order)
-        planes.u[((size_t)e * PLANE_ROWS + t) * rank + j0 + i % live] = __float2bfloat16_rn(0.f);
+      const int e = i / live, j = j0 + i % live;
+      if (!own || e != s_order || j >= rank)
+        fb_store_halves(planes.u + ((size_t)e * PLANE_ROWS + t) * fb_plane_width(rank), j, 0.f);
     }
   }
   if (!own) return;  // (the whole block)
@@ -173,7 +176,7 @@ adapter_shrink_kernel(const T* x, long long ldx, const T* a, const float* scales
 #pragma unroll
     for (int i = 0; i < PARTS; ++i) whole += sums[threadIdx.x][i];
     whole *= scales[slot];
-    if constexpr (PLANES) planes.u[((size_t)s_order * PLANE_ROWS + t) * rank + j] = __float2bfloat16_rn(whole);
+    if constexpr (PLANES) fb_store_halves(planes.u + ((size_t)s_order * PLANE_ROWS + t) * fb_plane_width(rank), j, whole);
     else low[(size_t)t * rank + j] = whole;
   }
 }
@@ -395,7 +398,7 @@ FB_API int fb_adapter_shrink(const void* x, long long ldx, int dtype, const void
   return fb_check_launch("adapter_shrink");
 }
 
-// The same as planes: u [adapters with tokens * 256, rank], counts [1], slots_of [the same number]. Up to 256 tokens,
+// The same as planes: u [adapters with tokens * 256, fb_plane_width(rank)], counts [1], slots_of [the same number]. Up to 256 tokens,
 // bfloat16; rows behind the last token are left as they are.
 FB_API int fb_adapter_shrink_planes(const void* x, long long ldx, const void* a, const float* scales,
                                     const int* index, int slots, int rank, int T, int K, void* u, int* counts,

@@ -12,6 +12,7 @@
 // block: 9.9 us in graph replays, where x and A alone are 18 MB, 2.7 us at the copy rate. (With mma.sync
 // instead, from registers or through cp.async stages, the same took 15 to 40 us: the instructions' own rate.)
 #define FB_STATUS_KERNEL 6
+#include "adapter_planes.cuh"
 #include "gemm_tcgen05.cuh"
 
 namespace {
@@ -43,7 +44,7 @@ __device__ __forceinline__ float ld_peer(const float* mine, unsigned rank) {
 }
 
 // CTA (i, y, z): 128 tokens, the adapters y, y + gridDim.y, .. of their block, share z of K. PLANES: a block
-// is 256 tokens, and every adapter of it gets a plane of bfloat16 rows, zero in those of others; else a
+// is 256 tokens, and every adapter of it gets a plane of rows (adapter_planes.cuh), zero in those of others; else a
 // block is the tile, and a token's own rank numbers go to its row of `low`.
 template <int RB, bool PLANES>
 __global__ void __launch_bounds__(THREADS, 2)
@@ -133,11 +134,12 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
   int it = 0, turn = 0;
   for (int e = blockIdx.y; e < count; e += gridDim.y) {
     const int slot = s_listed[e];
-    __nv_bfloat16* rows = PLANES ? u + ((size_t)(block * most + e) * BLOCK_ROWS + t0 % BLOCK_ROWS) * rank : nullptr;
+    const int width = fb_plane_width(rank);
+    __nv_bfloat16* rows = PLANES ? u + ((size_t)(block * most + e) * BLOCK_ROWS + t0 % BLOCK_ROWS) * width : nullptr;
     if (!__syncthreads_or(tid < BM && s_index[tid & (BM - 1)] == slot)) {  // none of these tokens: zeros
       if (PLANES && share == 0) {
         const int live = min(BM, T - t0);
-        for (int i = tid; i < live * rank / 8; i += THREADS)
+        for (int i = tid; i < live * width / 8; i += THREADS)
           reinterpret_cast<uint4*>(rows)[i] = make_uint4(0u, 0u, 0u, 0u);
       }
       continue;
@@ -194,11 +196,14 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
       tc_fence_after();
       // the cluster's CTAs share the tokens; a token's ranks side by side
       const int wide = min(RB, rank - r0), mine = BM / shares;
-      for (int i = tid; i < mine * wide; i += THREADS) {
-        const int t = share * mine + i / wide, j = i % wide;
+      const int reach = PLANES ? fb_plane_ranks(wide) : wide;  // (a plane's ranks behind the last one are zeros)
+      for (int i = tid; i < mine * reach; i += THREADS) {
+        const int t = share * mine + i / reach, j = i % reach;
         if (t0 + t >= T) break;
+        const bool own = s_index[t] == slot;
         float v = 0.f;
-        if (shares > 1) {
+        if (PLANES && (j >= wide || !own)) {
+        } else if (shares > 1) {
           float p[8];
 #pragma unroll
           for (int z = 0; z < 8; ++z) p[z] = z < shares ? ld_peer(&part[t][j], z) : 0.f;
@@ -207,8 +212,7 @@ adapter_low_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         } else {
           v = part[t][j];
         }
-        const bool own = s_index[t] == slot;
-        if constexpr (PLANES) rows[(size_t)t * rank + r0 + j] = __float2bfloat16_rn(own ? scale * v : 0.f);
+        if constexpr (PLANES) fb_store_halves(rows + (size_t)t * width, r0 + j, own && j < wide ? scale * v : 0.f);
         else if (own) low[(size_t)(t0 + t) * rank + r0 + j] = scale * v;
       }
       // nobody's sums are overwritten, or gone, while a peer still reads them
@@ -247,7 +251,7 @@ int launch_low(const CUtensorMap& mx, const CUtensorMap& ma, const float* scales
 }
 }  // namespace
 
-// u != null: planes for fb_gemm_tc_adapted, u [ceil(T / 256) * most * 256, rank] bfloat16, counts [blocks],
+// u != null: planes for fb_gemm_tc_adapted, u [ceil(T / 256) * most * 256, fb_plane_width(rank)] bfloat16, counts [blocks],
 // slots_of [blocks, most]; rows behind the last token are left as they are (what the product makes of them
 // goes nowhere). Else: low [T, rank] float32, rows of tokens without an adapter left as they are. `most`: at
 // least the adapters that one block (256 tokens, or 128) can have. side: CTAs that share the adapters of a

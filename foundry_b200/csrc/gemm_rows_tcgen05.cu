@@ -47,6 +47,7 @@
 // Every mbarrier wait is bounded as in the other tcgen05 kernels; a CTA whose
 // wait ran out still passes both cluster barriers, so its peers never hang.
 #define FB_STATUS_KERNEL 4
+#include "adapter_planes.cuh"
 #include "gemm_tcgen05.cuh"
 
 namespace {
@@ -115,8 +116,8 @@ template <int NB> struct RowsCfg {
 
 // More K behind the product's own: counts[0] adapters have tokens among the rows, the e-th of them
 // slots[e]; its rank numbers of the tokens, zero for tokens of others, are rows e * ROWS_A_PLANE .. of `u`, and
-// its weights for feature j row slot * N + j of `b`. Each takes `kblocks` K blocks of 64, which the CTAs of a
-// tile take in turn: one sum in tensor memory and one rounding.
+// its weights for feature j row slot * N + j of `b`. Each takes `kblocks` K blocks of 32 ranks, in two halves
+// (adapter_planes.cuh), which the CTAs of a tile take in turn: one sum in tensor memory and one rounding.
 constexpr int ROWS_A_PLANE = 256;
 struct RowsMore {
   CUtensorMap u, b;
@@ -229,9 +230,9 @@ gemm_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         if constexpr (MORE) {
           if (i >= n) {
             const int of_all = split + (i - n) * p.splits, e = of_all / more.kblocks;
-            const int k = (of_all - e * more.kblocks) * BK;
-            tma_load_2d(dst, &more.b, &full[s], k, __ldcg(more.slots + e) * p.N + tile * BM);
-            tma_load_2d(dst + A_BYTES, &more.u, &full[s], k, e * ROWS_A_PLANE);
+            const int k = of_all - e * more.kblocks;
+            tma_load_2d(dst, &more.b, &full[s], k * FB_PLANE_RANKS, __ldcg(more.slots + e) * p.N + tile * BM);
+            tma_load_2d(dst + A_BYTES, &more.u, &full[s], k * BK, e * ROWS_A_PLANE);
             continue;
           }
         }
@@ -257,9 +258,12 @@ gemm_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         const uint32_t a_addr = smem_u32(tiles + s * Cfg::STAGE_BYTES);
         const uint32_t b_addr = a_addr + A_BYTES;
 #pragma unroll
-        for (int k = 0; k < BK / UMMA_K; ++k)
-          umma(tmem_base, make_desc(a_addr + k * UMMA_K * 2), make_desc(b_addr + k * UMMA_K * 2),
+        for (int k = 0; k < BK / UMMA_K; ++k) {
+          // (a block of adapters: both halves of the rank numbers meet the same 32 columns of their B)
+          const int ka = MORE && i >= n ? k % (FB_PLANE_RANKS / UMMA_K) : k;
+          umma(tmem_base, make_desc(a_addr + ka * UMMA_K * 2), make_desc(b_addr + k * UMMA_K * 2),
                idesc, (i | k) != 0 ? 1u : 0u);
+        }
         tc_commit(&empty[s]);
       }
       if (ok) tc_commit(acc_full);
@@ -593,7 +597,7 @@ extern "C" int fb_adapter_shrink_planes(const void* x, long long ldx, const void
                                         int* slots_of, cudaStream_t stream);
 
 // What `adapter` (on the host) says of the adapters of up to 64 tokens: a [slots, rank, K] and b [slots, N, rank]
-// bfloat16, scales [slots], index [M] (outside of the bank: none), slots, rank; u [most * 256, rank] bfloat16,
+// bfloat16, scales [slots], index [M] (outside of the bank: none), slots, rank; u [most * 256, fb_plane_width(rank)],
 // counts [1], slots_of [most]: room for the rank numbers, most = the smaller of slots and M; and whether they are
 // there (fb_adapter_low), else a kernel in front writes them.
 static int rows_more_of(const long long* adapter, const void* x, long long ldx, int M, int N, int K, int NB,
@@ -614,11 +618,11 @@ static int rows_more_of(const long long* adapter, const void* x, long long ldx, 
     if (int rc = fb_adapter_shrink_planes(x, ldx, a, scales, index, slots, rank, M, K, u, counts, slots_of, stream))
       return rc;
   const int most = slots < M ? slots : M;
-  int rc = make_map(&more->u, u, (long long)most * ROWS_A_PLANE, rank, rank, NB);
+  int rc = make_map(&more->u, u, (long long)most * ROWS_A_PLANE, fb_plane_width(rank), fb_plane_width(rank), NB);
   if (!rc) rc = make_map(&more->b, b, (long long)slots * N, rank, rank, BM);
   more->counts = counts;
   more->slots = slots_of;
-  more->kblocks = (rank + BK - 1) / BK;
+  more->kblocks = fb_plane_width(rank) / BK;
   return rc;
 }
 

@@ -1,6 +1,7 @@
 // The tcgen05 product with two SMs on one tile (cta_group::2); the one-CTA forms
 // and the entry point `fb_gemm_tc` are in gemm_tcgen05.cu.
 #define FB_STATUS_KERNEL 2
+#include "adapter_planes.cuh"
 #include "gemm_tcgen05.cuh"
 #include "tcgen05_pair.cuh"
 
@@ -67,8 +68,9 @@ __device__ __forceinline__ PairUnit pair_unit(const GemmParams& p, int u, int ti
 // More K behind a tile's own, for adapters beside the projection (adapter.cu): block `ta` of 256 rows has
 // counts[ta] adapters with tokens in it, the e-th of them slots[ta * most + e]; its rank numbers of the
 // block's rows, zero in rows of others, are rows (ta * most + e) * 256 .. of `u`, and its weights for
-// feature j row slot * rows_b + j of `b`. Each takes `kblocks` K blocks of 64, so a product with them is
-// one sum in tensor memory and one rounding. (A tile's last share of K carries them.)
+// feature j row slot * rows_b + j of `b`. Each takes `kblocks` K blocks of 32 ranks, in two halves
+// (adapter_planes.cuh), so a product with them is one sum in tensor memory and one rounding. (A tile's last share of
+// K carries them.)
 struct MoreK {
   CUtensorMap u, b;
   const int* counts;
@@ -185,10 +187,11 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a,
           const uint32_t bar = full_leader + (uint32_t)(s * 8);
           if constexpr (MORE) {
             if (kb >= nkb) {
-              const int e = (kb - nkb) / more.kblocks, k = (kb - nkb - e * more.kblocks) * BK;
+              const int e = (kb - nkb) / more.kblocks, k = kb - nkb - e * more.kblocks;
               const int slot = __ldcg(more.slots + w.ta * more.most + e);
-              tma_load_2d_pair(a_dst, &more.u, bar, k, (w.ta * more.most + e) * 2 * BM + (int)rank * BM);
-              tma_load_2d_pair(b_dst, &more.b, bar, k, slot * p.rows_b + w.tb * BN + (int)rank * (BN / 2));
+              tma_load_2d_pair(a_dst, &more.u, bar, k * BK, (w.ta * more.most + e) * 2 * BM + (int)rank * BM);
+              tma_load_2d_pair(b_dst, &more.b, bar, k * FB_PLANE_RANKS,
+                               slot * p.rows_b + w.tb * BN + (int)rank * (BN / 2));
               continue;
             }
           }
@@ -223,10 +226,13 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a,
           const uint32_t a_addr = smem_u32(tiles + s * SmemPair<BN>::STAGE_BYTES);
           const uint32_t b_addr = a_addr + SmemPair<BN>::A_BYTES;
 #pragma unroll
-          for (int k = 0; k < BK / UMMA_K; ++k)
+          for (int k = 0; k < BK / UMMA_K; ++k) {
+            // (a block of adapters: both halves of the rank numbers meet the same 32 columns of their B)
+            const int k_of_b = MORE && kb >= nkb ? k % (FB_PLANE_RANKS / UMMA_K) : k;
             umma_pair(d_tmem, make_desc(a_addr + k * UMMA_K * 2),
-                      make_desc(b_addr + k * UMMA_K * 2), idesc,
+                      make_desc(b_addr + k_of_b * UMMA_K * 2), idesc,
                       (kb != w.kb0 || k != 0) ? 1u : 0u);
+          }
           tc_commit_pair(&empty[s]);
         }
         if (!ok) break;
@@ -785,8 +791,8 @@ int fb_gemm_tc_pair(const void* a, long long lda, int rows_a, const void* b, lon
   }
 }
 
-// out[T, N] = x w^T + the adapters' share: u and b2 as MoreK has them, u [blocks * most * 256, rank], b2
-// [adapters * N, rank], counts [blocks], slots [blocks, most], written by fb_adapter_planes. bfloat16 or
+// out[T, N] = x w^T + the adapters' share: u and b2 as MoreK has them, u [blocks * most * 256, fb_plane_width(rank)], b2
+// [adapters * N, rank], counts [blocks], slots [blocks, most], written by fb_adapter_low. bfloat16 or
 // float32 rows of `out`.
 FB_API int fb_gemm_tc_adapted(const void* x, long long ldx, int T, const void* w, long long ldw, int N, int K,
                               const void* u, const void* b2, const int* counts, const int* slots, int most,
@@ -816,10 +822,10 @@ FB_API int fb_gemm_tc_adapted(const void* x, long long ldx, int T, const void* w
   MoreK more{};
   int rc = make_map(&ma, x, T, K, ldx, BM);
   if (!rc) rc = make_map(&mb, w, N, K, ldw, bn / 2);
-  if (!rc) rc = make_map(&more.u, u, (long long)blocks * most * 2 * BM, rank, rank, BM);
+  if (!rc) rc = make_map(&more.u, u, (long long)blocks * most * 2 * BM, fb_plane_width(rank), fb_plane_width(rank), BM);
   if (!rc) rc = make_map(&more.b, b2, (long long)adapters * N, rank, rank, bn / 2);
   if (rc) return rc;
-  more.counts = counts; more.slots = slots; more.most = most; more.kblocks = (rank + BK - 1) / BK;
+  more.counts = counts; more.slots = slots; more.most = most; more.kblocks = fb_plane_width(rank) / BK;
   const int tiles_b = (N + bn - 1) / bn;
   switch (bn) {
 #define FB_ADAPTED_CASE(W)                                                                                   \

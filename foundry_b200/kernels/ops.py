@@ -1200,7 +1200,7 @@ def _rows_adapter(values, T, K, bank, index, slots, rank, addresses):
     """The few-rows product's numbers for a bank, and the tensors that they point to; the rank numbers are made
     here if the tensor cores are to make them."""
     most = min(slots, T)
-    u = values.new_empty(most * ADAPTER_BLOCK, rank)
+    u = values.new_empty(most * ADAPTER_BLOCK, _plane_width(rank))
     lists = values.new_empty(1 + most, dtype=torch.int32)
     counts = lists.data_ptr()
     made = _low_pays(T, K, slots, rank)
@@ -2246,8 +2246,14 @@ class AdapterBank:
 
 
 ADAPTER_BLOCK = 256      # tokens whose adapters share the planes of a tile (csrc/adapter.cu)
+PLANE_RANKS = 32         # ranks of a K block of a plane (csrc/adapter_planes.cuh)
 ADAPTER_PIECE = 8192     # tokens of one launch: the planes' workspace is made for this many
 MAX_ADAPTER_SLOTS = 1024
+
+
+def _plane_width(rank: int) -> int:
+    """bfloat16 numbers of a plane's row: the two halves of each rank number, of whole K blocks."""
+    return (rank + PLANE_RANKS - 1) // PLANE_RANKS * 2 * PLANE_RANKS
 
 
 def _low_fits(x: torch.Tensor, w: torch.Tensor, bank: AdapterBank) -> bool:
@@ -2261,25 +2267,27 @@ def _planes_pay(T: int, N: int, slots: int, rank: int) -> bool:
     projection's best form leaves its 32-bit sums to be read again, T * N of them, for a pass that reads a row
     of B for each; the paired one, which is not the best for few tokens, saves that and multiplies every block
     of 256 tokens with every adapter in it, of which a large bank may mean many (unfused and behind K, us:
-    4,096 -> 4,096, 4 adapters, rank 16 256 tokens 25 and 32, 512 40 and 34; rank 64 96 tokens 24 and 32, 192 37
-    and 33; rank 128 96 41 and 40, 256 67 and 41; 64 adapters, rank 64, 256 tokens 52 and 90)."""
+    4,096 -> 4,096, 4 adapters, rank 16 256 tokens 25.8 and 31.7, 512 41.8 and 34.6; rank 64 128 tokens 26.7 and
+    34.6, 192 37.6 and 34.8; rank 128 96 41.1 and 44.4, 128 47.8 and 45.0, 256 66.7 and 45.7; 64 adapters, rank 64,
+    256 tokens 87 and 135)."""
     return PAIRED and PERSISTENT and N >= 128 and T > 64 and \
         T * N * (rank + 16) >= (3 << 24) * max(1, min(slots, ADAPTER_BLOCK) // 16)
 
 
 def _rows_pay(T: int, N: int, slots: int, rank: int) -> bool:
     """Whether adapters ride behind the projection's own K in the product of up to 64 rows, a K block of 64
-    for every adapter among the rows and 64 of its ranks; how many those are is known on the device alone,
+    for every adapter among the rows and 32 of its ranks; how many those are is known on the device alone,
     so the bank's size counts. Up to 16 rows the weight-streaming product's epilogue is the other side, which
-    reads a row of B for every result (4,096 -> 28,672, rank 64, 4 adapters: 8 rows 44.7 us and 48.2, 16
-    rows 45 and 78; 4,096 -> 4,096, 16 rows 13.3 and 12.8; rank 16 12.2 and 9.7). Beyond, the product leaves
-    its 32-bit sums for `adapter_expand` (2,048 -> 4,096, 64 rows, behind K and in a pass of its own: rank 16,
-    4 adapters 12.8 us and 13.3, 64 adapters 21 and 13.3; rank 64, 4 adapters 13.6 and 16.0, 64 adapters 22.9
-    and 17.1; rank 128, 4 adapters 16.3 and 26.5; 2,048 -> 28,672, rank 32, 4 adapters 29.7 and 39.9, 64
-    adapters 73 and 52)."""
+    reads a row of B for every result (4,096 -> 28,672, rank 64, 4 adapters: 8 rows 46.5 us and 49.0, 16
+    rows 48 and 78; 4,096 -> 4,096, 16 rows 13.6 and 13.1; rank 16 12.2 and 9.9). Beyond, the product leaves
+    its 32-bit sums for `adapter_expand` (64 rows, 2,048 -> 4,096 and -> 28,672, behind K and in a pass of its own,
+    every adapter among the rows: rank 16, 8 adapters 13.1 us and 13.0, 30.5 and 37.1, 12 of them 13.8 and 13.0, 32.9
+    and 37.5, 64 of them 21.7 and 13.1; rank 64, 4 adapters 14.5 and 17.7, 24 of them 20.1 and 18.0, 54.7 and 63;
+    rank 128, 20 adapters 26.5 and 27.5, 75 and 136, 40 of them 38 and 29, 119 and 137; rank 256, 64 adapters 96 and
+    59, 321 and 276)."""
     if T <= SKINNY_ROWS and T * N * rank <= 1 << (22 if T > 8 else 23):
         return False
-    return T <= min(ROWS_MAX, 64) and slots <= MAX_ADAPTER_SLOTS and min(slots, T) <= 8 + rank // 4
+    return T <= min(ROWS_MAX, 64) and slots <= MAX_ADAPTER_SLOTS and min(slots, T) <= min(24, 8 + rank // 4)
 
 
 def _low_pays(T: int, K: int, slots: int, rank: int) -> bool:
@@ -2311,7 +2319,7 @@ def _adapted_planes(x: torch.Tensor, w: torch.Tensor, bank: AdapterBank, index: 
     (T, K), N = x.shape, w.shape[0]
     blocks = (T + ADAPTER_BLOCK - 1) // ADAPTER_BLOCK
     most = min(bank.slots, ADAPTER_BLOCK, T)
-    u = torch.empty((blocks * most * ADAPTER_BLOCK, bank.rank), dtype=torch.bfloat16, device=x.device)
+    u = torch.empty((blocks * most * ADAPTER_BLOCK, _plane_width(bank.rank)), dtype=torch.bfloat16, device=x.device)
     lists = torch.empty(blocks * (1 + most), dtype=torch.int32, device=x.device)
     counts, slots = lists.data_ptr(), lists.data_ptr() + 4 * blocks
     _adapter_low(x, bank, index, most, u.data_ptr(), counts, slots, 0)
@@ -2357,7 +2365,7 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
     """y[t] = x[t] w^T + scale_a (x[t] a_a^T) b_a^T with a = index[t] (int32, one a token; outside of
     the bank: no adapter). Sums are 32-bit and y is rounded once, to `out_dtype` (the input's type);
     where the adapters ride behind the projection's own K (hundreds of tokens, 17 to 64 with few adapters,
-    fewer beside wide projections) the rank numbers are rounded to bfloat16 for it (csrc/adapter.cu says
+    fewer beside wide projections) 16 bits of a rank number go with them (csrc/adapter.cu says
     which kernels run). `x` may be a `RowScaled`; `then_reads` names the weights that the step streams next,
     a hint."""
     values = x.values if isinstance(x, RowScaled) else x
