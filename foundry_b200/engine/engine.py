@@ -283,6 +283,10 @@ class Engine:
         step of several tokens every sequence then wants one row). The penalties'
         histories count what a row brings as the prompt's while its count is 0,
         and as generated afterwards."""
+        if not isinstance(params, SamplingParams):
+            params = params_of_rows(params, len(steps))
+            if params and not is_ruled(params):
+                params = params[0]  # the same plain one for every row
         ruled = is_ruled(params)
         # (a row that has generated nothing yet brings a prompt, of a single token maybe)
         if self._is_decode(steps) and not (ruled and any(c == 0 for c in counts)):
