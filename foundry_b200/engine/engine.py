@@ -347,7 +347,7 @@ class Engine:
         session = self._session
         if session is None or session.slots != slots or session.sampling != params \
                 or session.keys != keys or session.adapters != self.adapters_of(slots) \
-                or (session.rules is not None and any(s in self._unread for s in slots)):
+                or any(row in self._unread for row in session.history_rows):
             self._settle()
             session = self._session = DecodeSession(self, slots, params, keys, counts)
         return session
