@@ -24,7 +24,9 @@ __device__ __forceinline__ float uniform24(unsigned long long stream, unsigned l
                                            unsigned long long i) {
   unsigned long long z = mix64(stream + GOLDEN * (step + 1));
   z = mix64(z + GOLDEN * (i + 1));
-  return ((float)(z >> 40) + 0.5f) * (1.0f / 16777216.0f);  // in (0, 1), exact in 32-bit
+  // in (0, 1): 24 bits and a half are 25, and the largest rounds to one, whose noise would be infinite, so that any
+  // token would win with it (V / 2^24 of all draws)
+  return fminf(((float)(z >> 40) + 0.5f) * (1.0f / 16777216.0f), 1.0f - 0x1p-24f);
 }
 
 // A warp finds the best of a row's chunk results; every lane gets it (no number at all: token 0).

@@ -42,7 +42,8 @@ def uniform24(seed: int, key: int, step: int, count: int) -> np.ndarray:
         z = _mix64(z + np.uint64(_GOLDEN) * np.uint64(step + 1))
         i = np.arange(1, count + 1, dtype=np.uint64)
         z = _mix64(z + np.uint64(_GOLDEN) * i)
-    return ((z >> np.uint64(40)).astype(np.float32) + np.float32(0.5)) * np.float32(1.0 / 16777216.0)
+    u = ((z >> np.uint64(40)).astype(np.float32) + np.float32(0.5)) * np.float32(1.0 / 16777216.0)
+    return np.minimum(u, np.float32(1.0 - 2.0 ** -24))  # (the largest rounds to one, whose noise is infinite)
 
 
 def gumbel_scores(logits: np.ndarray, temperature: float, seed: int, key: int,
