@@ -31,6 +31,7 @@ constexpr int MAX_CLUSTER = 16;
 // A block's logits in shared memory, 129 KB. With more of them in one bin the fractions of their
 // weights could pass 32 bits (see Bins).
 constexpr int MAX_CHUNK = 33024;
+constexpr float SMALLEST_TEMPERATURE = 0x1p-120f;
 constexpr unsigned ID_BITS = 20, ID_MASK = (1u << ID_BITS) - 1;
 
 struct SampleArgs {
@@ -310,7 +311,9 @@ sample_rules_kernel(const SampleArgs a) {
   const float* from = a.logits + (size_t)r * a.row_stride + lo;
   const FbRowEdits row = fb_row_edits(a.edits, r, a.V);
   const float asked = a.temperature != nullptr ? a.temperature[r] : 0.f;
-  const float T = asked > FLT_MAX ? FLT_MAX : asked;  // (an infinite one: equal shares)
+  // (an infinite one: equal shares. The smallest: 32 / T and log2(e) / T stay finite, so that the best token's lead of
+  // zero is no NaN; a smaller one would draw otherwise only between logits less than 2^-113 apart.)
+  const float T = asked > 0.f ? fminf(fmaxf(asked, SMALLEST_TEMPERATURE), FLT_MAX) : 0.f;
   const bool greedy = !(T > 0.f);
   const int k = a.top_k != nullptr && !greedy ? a.top_k[r] : 0;
   const float p = a.top_p != nullptr && !greedy ? a.top_p[r] : 1.f;

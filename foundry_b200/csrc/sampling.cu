@@ -9,6 +9,8 @@
 // on the batch it runs in, and the host can restate them.
 #include "common.cuh"
 
+#include <cfloat>
+
 namespace {
 __host__ __device__ __forceinline__ unsigned long long mix64(unsigned long long z) {
   // the SplitMix64 finaliser (src/bench/rng.rs:21-27 uses the same constants)
@@ -68,9 +70,12 @@ select_tokens_kernel(const float* logits, long long row_stride, int V, int chunk
   __shared__ int best_i[32];
   const int r = blockIdx.x, c = blockIdx.y, chunks = gridDim.y;
   const float* row = logits + (size_t)r * row_stride;
-  const float temp = temperature ? temperature[r] : 0.f;
+  const float asked = temperature ? temperature[r] : 0.f;
+  const float temp = asked > FLT_MAX ? FLT_MAX : asked;  // (one that is no number stays none: greedy)
   const bool greedy = !(temp > 0.f);
-  const float inv_t = greedy ? 1.f : 1.0f / temp;
+  // scores are v / T + g; below 2^-96, where v / T may pass the largest number, v + T g, which are in the same order
+  const bool cold = !greedy && temp < 0x1p-96f;
+  const float inv_t = greedy || cold ? 1.f : 1.0f / temp, of_noise = cold ? temp : 1.f;
   const unsigned long long stream = (!greedy && streams) ? (unsigned long long)streams[r] : 0ULL;
   const unsigned long long step = (!greedy && steps) ? (unsigned long long)steps[r] : 0ULL;
   const int lo = c * chunk, hi = min(V, lo + chunk);
@@ -92,7 +97,7 @@ select_tokens_kernel(const float* logits, long long row_stride, int V, int chunk
       float v = got[a];
       if (!greedy) {
         const float u = uniform24(stream, step, (unsigned long long)i);
-        v = v * inv_t - logf(-logf(u));
+        v = v * inv_t - logf(-logf(u)) * of_noise;
       }
       // indices ascend within a thread, so `>` keeps the first of equal values;
       // a NaN compares false and never wins

@@ -270,7 +270,7 @@ class DecodeSession:
                      for s, p in zip(self.slots, self.params)])
             self.h2d_bytes_per_step += runner.rules.set_steps(self.streams, self.counts)
             return
-        temperature = float(self.params[0].temperature)
+        temperature = self.params[0].held_temperature
         if runner.temperature_value != temperature:
             runner.temperature.fill_(temperature)
             runner.temperature_value = temperature

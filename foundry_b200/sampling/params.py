@@ -26,6 +26,8 @@ import math
 from dataclasses import dataclass
 from typing import Callable, Iterable, Mapping, Optional, Sequence, Tuple, Union
 
+SMALLEST_TEMPERATURE, LARGEST_TEMPERATURE = 2.0 ** -120, float.fromhex("0x1.fffffep127")  # csrc/sample_rules.cu
+
 Allowed = Callable[[Sequence[int]], Optional[Iterable[int]]]
 
 
@@ -68,6 +70,12 @@ class SamplingParams:
     @property
     def greedy(self) -> bool:
         return self.temperature == 0.0
+
+    @property
+    def held_temperature(self) -> float:
+        """The temperature as the kernels calculate with it (32 bits would make zero, the greedy choice, of the
+        smallest ones)."""
+        return min(max(self.temperature, SMALLEST_TEMPERATURE), LARGEST_TEMPERATURE) if self.temperature else 0.0
 
     @property
     def needs_history(self) -> bool:

@@ -93,7 +93,7 @@ class RowRules:
         i[:n] = [min(p.top_k, self.vocab) for p in params]
         i[b:3 * b] = -1
         i[b:b + n] = history_rows
-        f[:n] = [p.temperature for p in params]
+        f[:n] = [p.held_temperature for p in params]
         f[b:2 * b] = 1.0
         f[b:b + n] = [p.top_p for p in params]
         f[2 * b:2 * b + n] = [p.min_p for p in params]

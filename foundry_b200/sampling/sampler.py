@@ -50,8 +50,12 @@ def gumbel_scores(logits: np.ndarray, temperature: float, seed: int, key: int,
                   step: int) -> np.ndarray:
     """logit_i / T - log(-log(u_i)) in float32: the quantity whose argmax is the sample."""
     u = uniform24(seed, key, step, logits.shape[-1])
-    inv_t = np.float32(1.0) / np.float32(temperature)
-    return logits.astype(np.float32) * inv_t - np.log(-np.log(u)).astype(np.float32)
+    temp = np.float32(SamplingParams(temperature).held_temperature)
+    noise = -np.log(-np.log(u)).astype(np.float32)
+    if temp < 2.0 ** -96:  # in the same order, and no logit over it is infinite
+        return logits.astype(np.float32) + temp * noise
+    inv_t = np.float32(1.0) / temp
+    return logits.astype(np.float32) * inv_t + noise
 
 
 class Sampler:
@@ -84,6 +88,6 @@ class Sampler:
             return ops.select_tokens(logits, out, None)
         streams = [stream_key(params.seed, int(k)) for k in keys]
         meta = torch.tensor([streams, list(steps)], dtype=torch.int64).to(logits.device)
-        temp = torch.full((n,), float(params.temperature), dtype=torch.float32,
+        temp = torch.full((n,), params.held_temperature, dtype=torch.float32,
                           device=logits.device)
         return ops.select_tokens(logits, out, temp, meta[0], meta[1])
