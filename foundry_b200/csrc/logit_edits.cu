@@ -121,9 +121,9 @@ FB_API int fb_edit_logits(const float* logits, long long row_stride, int n, int 
                           long long out_stride, const long long* edits, cudaStream_t stream) {
   FB_REQUIRE(n >= 0 && V > 0 && row_stride >= V && out_stride >= V, "edit_logits: bad sizes n=%d V=%d", n, V);
   FB_REQUIRE(n <= 65535, "edit_logits: %d rows (65535 at most)", n);
+  if (n == 0) return 0;  // (its rows' arrays are empty too, and have no address)
   const FbLogitEdits e = fb_unpack_edits(edits);
   if (int rc = fb_check_edits("edit_logits", e, V)) return rc;
-  if (n == 0) return 0;
   fb_launch(edit_logits_kernel, dim3((V + TILE - 1) / TILE, n), dim3(THREADS), 0, stream, logits,
             row_stride, V, out, out_stride, e);
   return fb_check_launch("edit_logits");

@@ -959,11 +959,11 @@ FB_API int fb_sample_rules(const float* logits, long long row_stride, int n, int
   FB_REQUIRE(n >= 0 && V > 0 && row_stride >= V, "sample_rules: bad sizes n=%d V=%d", n, V);
   FB_REQUIRE(V <= MAX_CLUSTER * MAX_CHUNK, "sample_rules: %d tokens (a vocabulary of %d at most)", V,
              MAX_CLUSTER * MAX_CHUNK);
+  if (n == 0) return 0;  // (its rows' arrays are empty too, and have no address)
   SampleArgs a{};
   a.edits = fb_unpack_edits(edits);
   if (int rc = fb_check_edits("sample_rules", a.edits, V)) return rc;
   FB_REQUIRE(record == nullptr || a.edits.counts != nullptr, "sample_rules: tokens to record, and no history");
-  if (n == 0) return 0;
   int blocks = 0, an_sm = 1;
   if (int rc = blocks_a_row(n, V, &blocks, &an_sm)) return rc;
   FB_REQUIRE(V <= blocks * MAX_CHUNK, "sample_rules: a vocabulary of %d (%d at most here)", V, blocks * MAX_CHUNK);
