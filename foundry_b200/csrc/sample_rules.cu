@@ -402,7 +402,8 @@ sample_rules_kernel(const SampleArgs a) {
   }
   // where it comes first: looked for by the threads that have their warp's best value alone
   int top_at = -1;
-  if (top > -INFINITY && ordered(top) == __reduce_max_sync(__activemask(), ordered(top))) {
+  const unsigned top_of_warp = __reduce_max_sync(0xffffffffu, ordered(top));
+  if (top > -INFINITY && ordered(top) == top_of_warp) {
     for (int i = 4 * tid; top_at < 0; i += 4 * THREADS) {
       const float4 f = *reinterpret_cast<float4*>(values + i);
       if (f.x == top) top_at = i;
