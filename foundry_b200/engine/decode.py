@@ -34,7 +34,7 @@ import torch
 from ..cache.pages import PAGE
 from ..kernels import ops
 from ..sampling.params import SamplingParams, is_ruled, params_of_rows
-from ..sampling.rules import RowRules, bias_room, check_vocabulary
+from ..sampling.rules import RowRules, bias_room, check_vocabulary, masks_of
 from .context import StepContext, lengths_are_unequal
 from .generate import NoTokenLeft
 from .staging import StagingRing
@@ -251,7 +251,7 @@ class DecodeSession:
             runner.ctx.kv_lens_host = [length + 1 for length in lengths] + [0] * pad
         return runner
 
-    def _upload(self, runner: DecodeRunner, tokens: Optional[Sequence[int]]) -> None:
+    def _upload(self, runner: DecodeRunner, tokens: Optional[Sequence[int]], masks=None) -> None:
         n = len(self.slots)
         start = runner.meta_start
         if tokens is not None:
@@ -264,10 +264,8 @@ class DecodeSession:
             if runner.rules_of != filled:
                 self.h2d_bytes_per_step += runner.rules.fill(*filled)
                 runner.rules_of = filled
-            if self.rules[1]:
-                self.h2d_bytes_per_step += runner.rules.set_masks(
-                    [None if p.allowed_tokens is None else p.allowed_tokens(self.engine.tokens_said(s))
-                     for s, p in zip(self.slots, self.params)])
+            if masks is not None:
+                self.h2d_bytes_per_step += runner.rules.set_masks(masks)
             self.h2d_bytes_per_step += runner.rules.set_steps(self.streams, self.counts)
             return
         temperature = self.params[0].held_temperature
@@ -296,8 +294,13 @@ class DecodeSession:
         self._pending_tokens = None
 
     def _launch(self, tokens: Optional[Sequence[int]]) -> DecodeRunner:
+        masks = None
+        if self.rules is not None and self.rules[1]:  # (a grammar may raise: nothing has changed then)
+            said = [() if p.allowed_tokens is None else self.engine.tokens_said(s) + [t]
+                    for p, s, t in zip(self.params, self.slots, tokens)]
+            masks = masks_of(self.params, said, self.engine.spec.vocab_size)
         runner = self._prepare()
-        self._upload(runner, tokens)
+        self._upload(runner, tokens, masks)
         runner.run()
         self.counts = [c + 1 for c in self.counts]
         return runner
@@ -373,11 +376,12 @@ class DecodeSession:
         (sampling only). `more`: the caller expects to come back with the same
         rows and the tokens returned here, so the step after this one is
         started before this one's tokens are handed out."""
-        if self.rules is not None and self.rules[1]:
+        tokens = [int(t) for t in tokens]
+        runner = self._started(tokens, counts)
+        if self.rules is not None and self.rules[1]:  # (a step that was refused may come again)
             for slot, p, token in zip(self.slots, self.params, tokens):
                 if p.allowed_tokens is not None:
-                    self.engine.tokens_said(slot).append(int(token))
-        runner = self._started([int(t) for t in tokens], counts)
+                    self.engine.tokens_said(slot).append(token)
         n = len(self.slots)
         runner.tokens_host[:n].copy_(runner.next_tokens[:n], non_blocking=True)
         if runner.rules is not None:

@@ -19,6 +19,7 @@ from ..cache.store import SequenceCache
 from ..config import load_model_config
 from ..config.spec import ModelSpec
 from ..sampling import Sampler, SamplingParams, is_ruled, params_of_rows
+from ..sampling.rules import check_vocabulary, masks_of
 from ..weights.safetensors_io import WeightFiles
 from . import generate as loop
 from ..cache.pages import CacheFull
@@ -304,6 +305,11 @@ class Engine:
         """A step of several tokens whose rows draw under rules of their own."""
         if any(len(s.want) != 1 for s in steps):
             raise ValueError("rows that draw under rules of their own want one place each")
+        # what may refuse the step comes in front of it
+        check_vocabulary(params, self.spec.vocab_size)
+        behind = [() if p.allowed_tokens is None else self.tokens_said(s.slot) + [int(t) for t in s.tokens if c > 0]
+                  for p, s, c in zip(params, steps, counts)]
+        masks = masks_of(params, behind, self.spec.vocab_size)
         logits = self.step(steps)
         said = [p.needs_history for p in params]
         rows = [self.history_row(s.slot) if h else -1 for s, h in zip(steps, said)]
@@ -316,8 +322,6 @@ class Engine:
         for s, p, c in zip(steps, params, counts):
             if p.allowed_tokens is not None and c > 0:
                 self.tokens_said(s.slot).extend(int(t) for t in s.tokens)
-        masks = [None if p.allowed_tokens is None else p.allowed_tokens(self.tokens_said(s.slot))
-                 for s, p in zip(steps, params)]
         tokens, logprobs = self.sampler.draw(logits, params, keys, counts,
                                              self.token_history() if any(said) else None, rows, masks)
         self._last_logprobs = logprobs.tolist()

@@ -42,6 +42,15 @@ def mask_bits(allowed: Iterable[int], vocab: int) -> np.ndarray:
     return np.packbits(flags, bitorder="little").view(np.int32)
 
 
+def masks_of(params: Sequence[SamplingParams], said: Sequence[Sequence[int]], vocab: int):
+    """The bits of what each row's grammar allows behind these tokens of its own, or None: all."""
+    masks = []
+    for p, tokens in zip(params, said):
+        allowed = None if p.allowed_tokens is None else p.allowed_tokens(tokens)
+        masks.append(None if allowed is None else mask_bits(allowed, vocab))
+    return masks
+
+
 class _Copied:
     """A `StagingRing`'s interface for values that are sent once."""
 
@@ -117,14 +126,14 @@ class RowRules:
         m[b:b + n] = counts
         return self.meta.upload()
 
-    def set_masks(self, masks: Sequence[Optional[Iterable[int]]]) -> int:
-        """Which tokens each row allows (None: all)."""
+    def set_masks(self, masks: Sequence[Optional[np.ndarray]]) -> int:
+        """Which tokens each row allows, as `masks_of` gives them."""
         b, words = self.rows, (self.vocab + 31) // 32
         bits, where = self.bits.values.reshape(b, words), self.ints.values
         where[2 * b:3 * b] = -1
-        for r, allowed in enumerate(masks):
-            if allowed is not None:
-                bits[r] = mask_bits(allowed, self.vocab)
+        for r, mask in enumerate(masks):
+            if mask is not None:
+                bits[r] = mask
                 where[2 * b + r] = r
         return self.bits.upload() + self.ints.upload()
 

@@ -65,7 +65,7 @@ class Sampler:
     def draw(self, logits: torch.Tensor, params, keys: Sequence[int], steps: Sequence[int],
              history: Optional[ops.TokenHistory], history_rows: Sequence[int], masks):
         """(tokens, log-probabilities) of rows that draw under rules of their own: `history_rows` are
-        the rows' places in `history`, `masks` the tokens that each row allows (None: all)."""
+        the rows' places in `history`, `masks` what each row allows (`rules.masks_of`)."""
         n, vocab = logits.shape
         rows = params_of_rows(params, n)
         check_vocabulary(rows, vocab)
