@@ -183,8 +183,10 @@ class DecodeSession:
             check_vocabulary(self.params, engine.spec.vocab_size)
             self.rules = (bias_room(self.params), any(p.allowed_tokens is not None for p in self.params),
                           any(p.needs_history for p in self.params))
-            self.history_rows = [engine.history_row(s) if p.needs_history else -1
-                                 for s, p in zip(self.slots, self.params)]
+            self.history_rows = [s if p.needs_history else -1 for s, p in zip(self.slots, self.params)]
+        self.said_rows = [r for r in self.history_rows if r >= 0]
+        if self.said_rows:
+            engine.complete_history(self.said_rows)
         self.adapters = engine.adapters_of(self.slots)
         self.counts = list(counts) if counts is not None else [0] * len(slots)
         self.runner: Optional[DecodeRunner] = None
@@ -300,6 +302,8 @@ class DecodeSession:
                     for p, s, t in zip(self.params, self.slots, tokens)]
             masks = masks_of(self.params, said, self.engine.spec.vocab_size)
         runner = self._prepare()
+        if self.said_rows:  # (other steps of these sequences may have come between)
+            self.engine.complete_history(self.said_rows)
         self._upload(runner, tokens, masks)
         runner.run()
         self.counts = [c + 1 for c in self.counts]
@@ -359,11 +363,21 @@ class DecodeSession:
             self.counts = list(counts)
         return self._launch(tokens)
 
+    def _note(self, tokens: Sequence[int], prompt: bool = False) -> None:
+        """These were a step's input tokens: a row with a history has its own in it by the step itself."""
+        for slot, token, row in zip(self.slots, tokens, self.history_rows):
+            told = self.engine.told(slot)
+            if row >= 0:
+                told.recorded["generated"] += 1
+            (told.prompt if prompt and row < 0 else told.said).append(token)
+
     def step_logits(self, tokens: Sequence[int]) -> torch.Tensor:
-        """One step fed from the host; returns its float32 logits [rows, vocab], the
-        caller's own. Their copy is queued behind the step, and one wait covers both (the
+        """One step fed from the host, whose tokens count as the prompt's where a row has no history; returns its
+        float32 logits [rows, vocab], the caller's own. Their copy is queued behind the step, and one wait covers both (the
         tokens fetched, waited for, then the logits waited for and copied: 40 us more a step)."""
-        runner = self._started([int(t) for t in tokens])
+        tokens = [int(t) for t in tokens]
+        runner = self._started(tokens)
+        self._note(tokens, prompt=True)
         logits = runner.logits[:len(self.slots)].clone()
         ops.wait_for_stream()
         ops.raise_on_device_failure()
@@ -378,10 +392,7 @@ class DecodeSession:
         started before this one's tokens are handed out."""
         tokens = [int(t) for t in tokens]
         runner = self._started(tokens, counts)
-        if self.rules is not None and self.rules[1]:  # (a step that was refused may come again)
-            for slot, p, token in zip(self.slots, self.params, tokens):
-                if p.allowed_tokens is not None:
-                    self.engine.tokens_said(slot).append(token)
+        self._note(tokens)  # (behind the launch: a step that was refused may come again)
         n = len(self.slots)
         runner.tokens_host[:n].copy_(runner.next_tokens[:n], non_blocking=True)
         if runner.rules is not None:

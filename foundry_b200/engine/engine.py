@@ -52,6 +52,20 @@ def require_cuda(device) -> torch.device:
     return device
 
 
+class Told:
+    """The tokens of an open sequence, as far as they passed the host, and how many of them its row of the
+    history holds."""
+    __slots__ = ("prompt", "said", "recorded")
+
+    def __init__(self):
+        self.prompt: List[int] = []
+        self.said: List[int] = []
+        self.recorded = {"prompt": 0, "generated": 0}
+
+    def kinds(self):
+        return (("prompt", self.prompt), ("generated", self.said))
+
+
 class Engine:
     def __init__(self, spec: ModelSpec, config, dtype=torch.bfloat16, device="cuda:0",
                  max_tokens: int = 8192, max_slots: int = 256):
@@ -70,7 +84,7 @@ class Engine:
         self._prompts = None  # graphs of short prompt steps, made at the first one
         self._history: Optional[ops.TokenHistory] = None  # made for the first row with a penalty
         self._unread = set()  # slots whose row of the history is another sequence's
-        self._said: Dict[int, List[int]] = {}  # tokens generated, for rows with a grammar
+        self._told: Dict[int, Told] = {}  # slot -> its sequence's tokens
         self._last_logprobs: List[float] = []
         self.adapters: Optional[AdapterStore] = None
         self._adapter_of: Dict[int, int] = {}  # slot -> place of its adapter
@@ -132,7 +146,7 @@ class Engine:
         place = None if adapter is None else self._adapters().place_of(adapter)
         slot = self.cache.open_sequence()
         self._unread.add(slot)
-        self._said.pop(slot, None)
+        self._told[slot] = Told()
         self._adapter_of.pop(slot, None)
         if place is not None:
             self._adapter_of[slot] = place
@@ -141,6 +155,7 @@ class Engine:
 
     def close_sequence(self, slot: int) -> None:
         self.cache.close_sequence(slot)
+        self._told.pop(slot, None)
         place = self._adapter_of.pop(slot, None)
         if place is not None:
             self.adapters.release(place)
@@ -182,16 +197,39 @@ class Engine:
         return self._history
 
     def history_row(self, slot: int) -> int:
-        """The slot's row of the history, cleared if another sequence's tokens are in it."""
-        history = self.token_history()
-        if slot in self._unread:
-            history.clear([slot])
-            self._unread.discard(slot)
+        """The slot's row of the history, with all of its sequence's tokens in it that passed the host."""
+        self.complete_history([slot])
         return slot
 
+    def complete_history(self, slots: Sequence[int]) -> None:
+        """Record what the slots' sequences were given and have generated since their rows were last complete, by
+        steps that looked at no history (pieces of a prompt, draws without a penalty); a row with another
+        sequence's tokens is cleared first."""
+        told = [self._told.get(s) for s in slots]
+        if not any(s in self._unread or t is not None and any(t.recorded[what] < len(tokens) for what, tokens in t.kinds())
+                   for s, t in zip(slots, told)):
+            return
+        history = self.token_history()
+        other = [s for s in slots if s in self._unread]
+        if other:
+            history.clear(other)
+            self._unread.difference_update(other)
+        pairs = {"prompt": [], "generated": []}
+        for s, t in zip(slots, told):
+            for what, tokens in t.kinds() if t is not None else ():
+                pairs[what] += [(s, token) for token in tokens[t.recorded[what]:]]
+                t.recorded[what] = len(tokens)
+        for what, some in pairs.items():
+            if some:
+                where = torch.tensor(some, dtype=torch.int32).t().contiguous().to(self.device)
+                ops.record_tokens(history, where[0], where[1], what)
+
     def tokens_said(self, slot: int) -> List[int]:
-        """The tokens that the slot's sequence has generated, as far as a grammar was asked."""
-        return self._said.setdefault(slot, [])
+        """The tokens that the slot's sequence has generated, as far as they passed the host."""
+        return self.told(slot).said
+
+    def told(self, slot: int) -> Told:
+        return self._told.setdefault(slot, Told())
 
     def last_logprobs(self) -> List[float]:
         """The log-probabilities of the tokens that the last `step_select` returned."""
@@ -218,10 +256,18 @@ class Engine:
     # ---------------------------------------------------------------- step
     def step(self, steps: Sequence[SequenceStep]) -> torch.Tensor:
         """Run the given tokens from the cache; float32 logits [wanted, vocab]
-        in the order of `steps` and of each `want`."""
+        in the order of `steps` and of each `want`. The penalties' histories count the
+        tokens as the prompt's (`step_select` knows better)."""
         if self._is_decode(steps):
             return self._session_of(steps, SamplingParams(), None, None).step_logits(
                 [int(s.tokens[0]) for s in steps])
+        logits = self._run(steps)
+        for s in steps:
+            self.told(s.slot).prompt.extend(int(t) for t in s.tokens)
+        return logits
+
+    def _run(self, steps: Sequence[SequenceStep]) -> torch.Tensor:
+        """`step` of more than single tokens, or of rows that want nothing."""
         self._settle()
         limit = self.cache.step_token_limit()
         if limit is not None and any(len(s.tokens) > limit for s in steps):
@@ -265,7 +311,7 @@ class Engine:
                           if start <= w < start + len(chunk)]
                 portion.append(SequenceStep(s.slot, chunk, [w for _, w in wanted]))
                 keys.extend((i, k) for k, _ in wanted)
-            logits = self.step(portion)
+            logits = self._run(portion)
             for row, key in zip(logits, keys):
                 rows[key] = row
         ordered = [rows[(i, k)] for i, s in enumerate(plan_check) for k in range(len(s.want))]
@@ -283,7 +329,8 @@ class Engine:
         `params`: one `SamplingParams` for all wanted rows, or one each (in a
         step of several tokens every sequence then wants one row). The penalties'
         histories count what a row brings as the prompt's while its count is 0,
-        and as generated afterwards."""
+        and as generated afterwards, whether the row has a penalty by then or
+        only later; pieces of a prompt may go through `step` before."""
         if not isinstance(params, SamplingParams):
             params = params_of_rows(params, len(steps))
             if params and not is_ruled(params):
@@ -293,13 +340,25 @@ class Engine:
         if self._is_decode(steps) and not (ruled and any(c == 0 for c in counts)):
             session = self._session_of(steps, params, keys, counts)
             tokens = session.step_host([int(s.tokens[0]) for s in steps], more, counts)
+            if not ruled:
+                for s, c in zip(steps, counts):
+                    if c == 0:  # a prompt of one token, which the session took for one of the row's own
+                        told = self.told(s.slot)
+                        told.prompt.append(told.said.pop())
             self._last_logprobs = session.last_logprobs
             return tokens
         if ruled:
             return self._draw_behind(steps, params_of_rows(params, len(steps)), keys, counts)
-        logits = self.step(steps)
+        logits = self._run_noted(steps, counts)
         tokens = self.sampler.select(logits, params, keys, counts)
         return tokens.tolist()
+
+    def _run_noted(self, steps, counts) -> torch.Tensor:
+        logits = self._run(steps)
+        for s, c in zip(steps, counts):
+            told = self.told(s.slot)
+            (told.prompt if c == 0 else told.said).extend(int(t) for t in s.tokens)
+        return logits
 
     def _draw_behind(self, steps, params, keys, counts) -> List[int]:
         """A step of several tokens whose rows draw under rules of their own."""
@@ -310,20 +369,13 @@ class Engine:
         behind = [() if p.allowed_tokens is None else self.tokens_said(s.slot) + [int(t) for t in s.tokens if c > 0]
                   for p, s, c in zip(params, steps, counts)]
         masks = masks_of(params, behind, self.spec.vocab_size)
-        logits = self.step(steps)
-        said = [p.needs_history for p in params]
-        rows = [self.history_row(s.slot) if h else -1 for s, h in zip(steps, said)]
-        for what, wanted in (("prompt", lambda c: c == 0), ("generated", lambda c: c > 0)):
-            pairs = [(row, int(t)) for s, row, c in zip(steps, rows, counts) if row >= 0 and wanted(c)
-                     for t in s.tokens]
-            if pairs:
-                where = torch.tensor(pairs, dtype=torch.int32).t().contiguous().to(self.device)
-                ops.record_tokens(self.token_history(), where[0], where[1], what)
-        for s, p, c in zip(steps, params, counts):
-            if p.allowed_tokens is not None and c > 0:
-                self.tokens_said(s.slot).extend(int(t) for t in s.tokens)
+        logits = self._run_noted(steps, counts)
+        rows = [s.slot if p.needs_history else -1 for s, p in zip(steps, params)]
+        said = [r for r in rows if r >= 0]
+        if said:
+            self.complete_history(said)
         tokens, logprobs = self.sampler.draw(logits, params, keys, counts,
-                                             self.token_history() if any(said) else None, rows, masks)
+                                             self.token_history() if said else None, rows, masks)
         self._last_logprobs = logprobs.tolist()
         tokens = tokens.tolist()
         if min(tokens) < 0:

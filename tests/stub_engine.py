@@ -4,6 +4,7 @@ import types
 import torch
 
 from foundry_b200.engine import engine as module
+from foundry_b200.engine.decode import DecodeSession
 from foundry_b200.engine.engine import Engine
 from foundry_b200.kernels import ops
 from foundry_b200.sampling import is_ruled, params_of_rows
@@ -45,6 +46,11 @@ class Cache:
 class Session:
     """As `DecodeSession`, with steps that are counted and started on a guess whenever they may be."""
     made, cancelled, used = 0, 0, 0
+    _note = DecodeSession._note
+
+    def step_logits(self, tokens):
+        self._note(tokens, prompt=True)
+        return torch.zeros(len(tokens), 100)
 
     def __init__(self, engine, slots, sampling, keys=None, counts=None):
         type(self).made += 1
@@ -52,10 +58,11 @@ class Session:
         self.sampling = sampling if not isinstance(sampling, (list, tuple)) else list(sampling)
         self.params = params_of_rows(sampling, len(self.slots))
         self.rules = (0, False, False) if is_ruled(self.sampling) else None
-        self.history_rows = [engine.history_row(s) if self.rules and p.needs_history else -1
+        self.history_rows = [s if self.rules and p.needs_history else -1
                              for s, p in zip(self.slots, self.params)]
         self.adapters = engine.adapters_of(self.slots)
         self.last_logprobs, self.ahead = [], False
+        engine.complete_history([r for r in self.history_rows if r >= 0])
 
     def cancel_ahead(self):
         type(self).cancelled += self.ahead
@@ -64,6 +71,11 @@ class Session:
     def step_host(self, tokens, more=False, counts=None):
         type(self).used += self.ahead
         self.ahead = more
+        said = [(r, t) for r, t in zip(self.history_rows, tokens) if r >= 0]
+        self.engine.complete_history([r for r, _ in said])
+        for r, t in said:
+            self.engine._history.rows[r].append(("generated", t))
+        self._note(tokens)
         self.last_logprobs = [-1.0] * len(tokens)
         return [t + 1 for t in tokens]
 
@@ -84,7 +96,7 @@ def make(monkeypatch):
     engine = Engine.__new__(Engine)
     engine.spec = types.SimpleNamespace(vocab_size=100, eos_token_ids=(), max_positions=1000)
     engine.device, engine.cache = torch.device("cpu"), Cache()
-    for name, value in dict(_session=None, _history=History(), _unread=set(), _said={}, _last_logprobs=[],
+    for name, value in dict(_session=None, _history=History(), _unread=set(), _told={}, _last_logprobs=[],
                             adapters=None, _adapter_of={}, _runners={}, scratch=("test", 0), use_graphs=False,
                             _prompts=types.SimpleNamespace(wants=lambda steps: True, step=lambda steps: torch.zeros(
                                 sum(len(s.want) for s in steps), 100))).items():

@@ -72,7 +72,7 @@ def session(monkeypatch):
 
     engine.cache.table.length = {slot: 5}
     for name, value in dict(engine=engine, slots=[slot], params=[SamplingParams(allowed_tokens=grammar)], streams=[0], counts=[1],
-                            rules=(0, True, False), history_rows=[-1], _ahead=None, full=False, runner=runner, _prepare=prepare,
+                            rules=(0, True, False), history_rows=[-1], said_rows=[], _ahead=None, full=False, runner=runner, _prepare=prepare,
                             _read=types.SimpleNamespace(record=lambda: None, synchronize=lambda: None)).items():
         setattr(made, name, value)
     monkeypatch.setattr(ops, "raise_on_device_failure", lambda: None)

@@ -62,6 +62,62 @@ def test_a_slot_opened_again_has_a_session_of_its_own(stub, other):
         engine.step_select(steps, sampling, [0, 1], [0, 0])
         for count in (1, 2):
             engine.step_select([prompt(s, 7) for s in slots], sampling, [0, 1], [count] * 2, count == 1)
-        assert history.rows[slots[0]] == [("prompt", t) for t in tokens]
+        assert history.rows[slots[0]] == [("prompt", t) for t in tokens] + [("generated", 7)] * 2
         for s in slots:
             engine.close_sequence(s)
+
+
+def held(history, slot):
+    """(the prompt's tokens in the slot's row, the generated ones)"""
+    return tuple(sorted(t for w, t in history.rows[slot] if w == what) for what in ("prompt", "generated"))
+
+
+@pytest.mark.parametrize("pieces", [[[1, 2], [3, 4, 5]], [[1], [2], [3, 4, 5]], [[1, 2, 3, 4], [5]]])
+@pytest.mark.parametrize("wants", [False, True])
+def test_pieces_of_a_prompt_are_in_the_history(stub, pieces, wants):
+    """Whichever step took them: pieces that want nothing, or logits, and single tokens of it."""
+    engine, _, history = stub
+    for _ in range(2):  # (the slot's next sequence as well)
+        slot, other = engine.open_sequence(), engine.open_sequence()
+        for piece in pieces[:-1]:
+            engine.step([SequenceStep(slot, piece, [len(piece) - 1] if wants else [])])
+        engine.step([SequenceStep(other, [50, 51], [])])
+        engine.step_select([prompt(slot, *pieces[-1])], PENALTY, [0], [0])
+        assert held(history, slot) == ([1, 2, 3, 4, 5], [])
+        engine.step_select([prompt(slot, 7)], PENALTY, [0], [1])
+        assert held(history, slot) == ([1, 2, 3, 4, 5], [7])
+        assert other not in history.rows or not history.rows[other]
+        engine.close_sequence(slot)
+        engine.close_sequence(other)
+
+
+@pytest.mark.parametrize("first", [[1, 2, 3], [1]])
+@pytest.mark.parametrize("before", [SamplingParams(), SamplingParams(0.8, 1, top_k=9)])
+def test_tokens_drawn_without_a_penalty_are_in_the_history(stub, first, before):
+    """What a sequence was given and drew before its first penalty, and between two, counts when one comes."""
+    engine, _, history = stub
+    slot = engine.open_sequence()
+    engine.step_select([prompt(slot, *first)], before, [0], [0])
+    for count in (1, 2):
+        engine.step_select([prompt(slot, 20 + count)], before, [0], [count])
+    assert slot not in history.rows
+    engine.step_select([prompt(slot, 23)], PENALTY, [0], [3])
+    assert held(history, slot) == (first, [21, 22, 23])
+    engine.step_select([prompt(slot, 24)], before, [0], [4])
+    assert held(history, slot) == (first, [21, 22, 23])
+    engine.step_select([prompt(slot, 25, 26)], PENALTY, [0], [5])  # (two tokens of its own at once)
+    assert held(history, slot) == (first, [21, 22, 23, 24, 25, 26])
+    engine.step([SequenceStep(slot, [30, 31], [])])
+    engine.step_select([prompt(slot, 27)], [PENALTY], [0], [7])
+    assert held(history, slot) == (first + [30, 31], [21, 22, 23, 24, 25, 26, 27])
+    assert engine.tokens_said(slot) == [21, 22, 23, 24, 25, 26, 27]
+
+
+def test_a_grammar_knows_the_tokens_drawn_before_it(stub):
+    engine, _, _ = stub
+    slot, asked = engine.open_sequence(), []
+    grammar = SamplingParams(allowed_tokens=lambda said: asked.append(list(said)))
+    engine.step_select([prompt(slot, 1, 2)], SamplingParams(), [0], [0])
+    engine.step_select([prompt(slot, 7)], SamplingParams(), [0], [1])
+    engine.step_select([prompt(slot, 8, 9)], grammar, [0], [2])
+    assert asked == [[7, 8, 9]]
