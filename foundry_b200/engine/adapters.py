@@ -12,6 +12,7 @@ from typing import Dict, List, Mapping, Optional, Tuple
 
 import torch
 
+from ..kernels import ops
 from ..parts.adapters import sites_of
 from ..weights.safetensors_io import WeightFiles, parse_header
 
@@ -75,6 +76,10 @@ class AdapterStore:
         self.sites = sites_of(model.parts())
         if not self.sites:
             raise AdapterError(f"no part of {model.spec.architecture} takes adapters")
+        # (the projections of one matrix stand side by side in its bank's ranks)
+        most = ops.MAX_ADAPTER_RANK // max(len(site.names) for site in self.sites) // 8 * 8
+        if self.max_rank > most:
+            raise AdapterError(f"adapters of rank {max_rank}: up to {most} beside this model's projections")
         for site in self.sites:
             site.make(max_adapters, self.max_rank, dtype, device)
         self.places: Dict[str, int] = {}

@@ -163,7 +163,8 @@ class Engine:
     # ------------------------------------------------------------ adapters
     def enable_adapters(self, max_adapters: int = 8, max_rank: int = 16) -> None:
         """Make room for low-rank adapters beside the projections that take them (q, k, v, o, gate, up
-        and down of the Llama decoder): `max_adapters` at a time, of rank `max_rank` at most."""
+        and down of the Llama decoder): `max_adapters` at a time, of rank `max_rank` at most (which may be 168:
+        q, k and v share the 512 ranks of their matrix's bank)."""
         if self.adapters is not None:
             raise ValueError("adapters are enabled already")
         self.adapters = AdapterStore(self.model, max_adapters, max_rank, self.dtype, self.device)

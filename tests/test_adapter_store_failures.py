@@ -1,0 +1,36 @@
+"""What an engine's adapters do where a step of theirs fails, on the host."""
+import types
+
+import pytest
+import torch
+
+from foundry_b200.engine.adapters import AdapterError, AdapterStore
+from foundry_b200.kernels import ops
+from foundry_b200.parts.adapters import AdapterSite
+
+
+def model_of(sites):
+    part = types.SimpleNamespace(adapter_sites=lambda: sites)
+    return types.SimpleNamespace(parts=lambda: [part], spec=types.SimpleNamespace(architecture="Toy"))
+
+
+def sites():
+    return [AdapterSite([("a.o", 6)], 8), AdapterSite([("a.q", 4), ("a.k", 2), ("a.v", 1)], 8), AdapterSite([("a.g", 3), ("a.u", 3)], 8)]
+
+
+def pairs(rank=2):
+    return {f"{name}.lora_{half}.weight": torch.ones(shape) for name, rows in (("a.o", 6), ("a.q", 4))
+            for half, shape in (("A", (rank, 8)), ("B", (rows, rank)))}
+
+
+@pytest.mark.parametrize("rank", [161, 168, 169, 512])
+def test_the_largest_rank_is_that_of_the_fused_matrices(rank):
+    """Three projections of one matrix share its bank's ranks (ops.MAX_ADAPTER_RANK)."""
+    some = sites()
+    if rank <= ops.MAX_ADAPTER_RANK // 3 // 8 * 8:
+        assert AdapterStore(model_of(some), 2, rank, torch.float32, "cpu").max_rank == 168
+        return
+    with pytest.raises(AdapterError, match=f"rank {rank}: up to 168 beside this model"):
+        AdapterStore(model_of(some), 2, rank, torch.float32, "cpu")
+    assert all(s.bank is None for s in some)  # nothing was made
+    assert AdapterStore(model_of(some[:1]), 2, rank, torch.float32, "cpu").max_rank >= rank
