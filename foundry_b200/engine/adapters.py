@@ -80,8 +80,13 @@ class AdapterStore:
         most = ops.MAX_ADAPTER_RANK // max(len(site.names) for site in self.sites) // 8 * 8
         if self.max_rank > most:
             raise AdapterError(f"adapters of rank {max_rank}: up to {most} beside this model's projections")
-        for site in self.sites:
-            site.make(max_adapters, self.max_rank, dtype, device)
+        try:
+            for site in self.sites:
+                site.make(max_adapters, self.max_rank, dtype, device)
+        except BaseException:
+            for site in self.sites:  # (what was made before would hold its memory)
+                site.bank = None
+            raise
         self.places: Dict[str, int] = {}
         self._free: List[int] = list(range(max_adapters))
         self._held: Dict[int, int] = {}
@@ -115,9 +120,10 @@ class AdapterStore:
             raise AdapterError(f"an adapter's scale is {scale}")
         pairs = pairs_of(tensors)
         self._check(name, pairs)
-        place = self._free.pop(0)
+        place = self._free[0]  # taken when all of it is written: every site's numbers there are then this adapter's
         for site in self.sites:
             site.write(place, pairs, scale)
+        self._free.pop(0)
         self.places[name] = place
 
     def _check(self, name: str, pairs) -> None:

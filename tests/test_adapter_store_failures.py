@@ -34,3 +34,30 @@ def test_the_largest_rank_is_that_of_the_fused_matrices(rank):
         AdapterStore(model_of(some), 2, rank, torch.float32, "cpu")
     assert all(s.bank is None for s in some)  # nothing was made
     assert AdapterStore(model_of(some[:1]), 2, rank, torch.float32, "cpu").max_rank >= rank
+
+
+def test_a_place_is_taken_by_what_is_written():
+    """An adapter whose writing failed (no memory, say) leaves its place to the next one, and nothing of itself there."""
+    some = sites()
+    store = AdapterStore(model_of(some), 1, 8, torch.float32, "cpu")
+    write = some[1].write
+
+    def fails(*args):
+        write(*args)
+        raise MemoryError("no room")
+    some[1].write = fails
+    for _ in range(3):
+        with pytest.raises(MemoryError):
+            store.load("x", pairs())
+    assert store.places == {}
+    some[1].write = write
+    store.load("y", {k: v for k, v in pairs().items() if k.startswith("a.q")}, 2.0)
+    assert store.place_of("y") == 0 and not some[0].bank.b.any() and not some[0].bank.a.any()
+
+
+def test_room_that_cannot_be_made_leaves_none():
+    some = sites()
+    some[2].make = lambda *args: (_ for _ in ()).throw(MemoryError("no room"))
+    with pytest.raises(MemoryError):
+        AdapterStore(model_of(some), 1, 8, torch.float32, "cpu")
+    assert all(s.bank is None for s in some)
