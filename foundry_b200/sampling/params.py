@@ -26,7 +26,8 @@ import math
 from dataclasses import dataclass
 from typing import Callable, Iterable, Mapping, Optional, Sequence, Tuple, Union
 
-SMALLEST_TEMPERATURE, LARGEST_TEMPERATURE = 2.0 ** -120, float.fromhex("0x1.fffffep127")  # csrc/sample_rules.cu
+LARGEST = float.fromhex("0x1.fffffep127")  # of 32 bits
+SMALLEST_TEMPERATURE, SMALLEST_PENALTY = 2.0 ** -120, 2.0 ** -126  # csrc/sample_rules.cu; not rounded to zero
 
 Allowed = Callable[[Sequence[int]], Optional[Iterable[int]]]
 
@@ -48,23 +49,24 @@ class SamplingParams:
     def __post_init__(self):
         if not (self.temperature >= 0.0):
             raise ValueError(f"temperature must not be negative, got {self.temperature}")
-        if int(self.top_k) != self.top_k or not 0 <= self.top_k < 1 << 31:
+        if not 0 <= self.top_k < 1 << 31 or int(self.top_k) != self.top_k:
             raise ValueError(f"top_k must be a whole number of tokens or 0, got {self.top_k}")
         if not 0.0 < self.top_p <= 1.0:
             raise ValueError(f"top_p must lie in (0, 1], got {self.top_p}")
         if not 0.0 <= self.min_p <= 1.0:
             raise ValueError(f"min_p must lie in [0, 1], got {self.min_p}")
-        if not (self.repetition_penalty > 0.0 and math.isfinite(self.repetition_penalty)):
-            raise ValueError(f"repetition_penalty must be positive, got {self.repetition_penalty}")
+        # (the kernels' numbers are of 32 bits: what is finite in 64 may be infinite there, or zero)
+        if not SMALLEST_PENALTY <= self.repetition_penalty <= LARGEST:
+            raise ValueError(f"repetition_penalty must be positive and finite in 32 bits, got {self.repetition_penalty}")
         for name in ("frequency_penalty", "presence_penalty"):
-            if not math.isfinite(getattr(self, name)):
-                raise ValueError(f"{name} must be finite, got {getattr(self, name)}")
+            if not abs(getattr(self, name)) <= LARGEST:
+                raise ValueError(f"{name} must be finite in 32 bits, got {getattr(self, name)}")
         pairs = self.logit_bias.items() if isinstance(self.logit_bias, Mapping) else self.logit_bias
         pairs = tuple(sorted((int(t), float(b)) for t, b in pairs))
         if len({t for t, _ in pairs}) != len(pairs) or any(t < 0 for t, _ in pairs):
             raise ValueError("logit_bias names a token twice, or a negative one")
-        if any(math.isnan(b) or b == math.inf for _, b in pairs):
-            raise ValueError("logit_bias values are finite or -inf")
+        if not all(abs(b) <= LARGEST or b == -math.inf for _, b in pairs):
+            raise ValueError("logit_bias values are finite in 32 bits, or -inf")
         object.__setattr__(self, "logit_bias", pairs)
 
     @property
@@ -75,7 +77,7 @@ class SamplingParams:
     def held_temperature(self) -> float:
         """The temperature as the kernels calculate with it (32 bits would make zero, the greedy choice, of the
         smallest ones)."""
-        return min(max(self.temperature, SMALLEST_TEMPERATURE), LARGEST_TEMPERATURE) if self.temperature else 0.0
+        return min(max(self.temperature, SMALLEST_TEMPERATURE), LARGEST) if self.temperature else 0.0
 
     @property
     def needs_history(self) -> bool:
