@@ -204,7 +204,8 @@ def load_adapter(engine, folder: str) -> str:
     """Make room for the folder's adapter and load it; returns its name."""
     from .engine.adapters import pairs_of, read_folder
     tensors, scale = read_folder(folder)
-    engine.enable_adapters(1, max(a.shape[0] for a, _ in pairs_of(tensors).values()))
+    ranks = [a.shape[0] for a, _ in pairs_of(tensors).values() if a.dim() == 2]
+    engine.enable_adapters(1, max(ranks, default=1))  # (what does not fit is `load_adapter`'s to say)
     engine.load_adapter(folder, tensors, scale)
     return folder
 
