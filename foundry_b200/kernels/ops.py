@@ -2249,6 +2249,7 @@ ADAPTER_BLOCK = 256      # tokens whose adapters share the planes of a tile (csr
 PLANE_RANKS = 32         # ranks of a K block of a plane (csrc/adapter_planes.cuh)
 ADAPTER_PIECE = 8192     # tokens of one launch: the planes' workspace is made for this many
 MAX_ADAPTER_SLOTS = 1024
+PLANES_ROOM = 1 << 28    # bytes of planes at a time
 
 
 def _plane_width(rank: int) -> int:
@@ -2272,6 +2273,13 @@ def _planes_pay(T: int, N: int, slots: int, rank: int) -> bool:
     256 tokens 87 and 135)."""
     return PAIRED and PERSISTENT and N >= 128 and T > 64 and \
         T * N * (rank + 16) >= (3 << 24) * max(1, min(slots, ADAPTER_BLOCK) // 16)
+
+
+def _planes_piece(T: int, slots: int, rank: int) -> int:
+    """How many of T tokens go through the planes at a time: a block of 256 has room for a plane of every adapter
+    that it may have, 134 MB at 256 places of rank 512, whatever it does have (only the device knows that)."""
+    block = min(slots, ADAPTER_BLOCK, T) * ADAPTER_BLOCK * _plane_width(rank) * 2
+    return min(T, max(1, PLANES_ROOM // block) * ADAPTER_BLOCK)
 
 
 def _rows_pay(T: int, N: int, slots: int, rank: int) -> bool:
@@ -2404,7 +2412,9 @@ def adapted_product(x, w: torch.Tensor, bank: AdapterBank, index: torch.Tensor,
         return out
     on_tensor_cores = _low_fits(x, w, bank)
     if on_tensor_cores and _planes_pay(T, N, slots, rank):
-        _adapted_planes(x, w, bank, index, out)
+        piece = _planes_piece(T, slots, rank)
+        for t in range(0, T, piece):
+            _adapted_planes(x[t:t + piece], w, bank, index[t:t + piece], out[t:t + piece])
         return out
     low = torch.empty((T, rank), dtype=torch.float32, device=x.device)
     if on_tensor_cores and _low_pays(T, K, slots, rank):
