@@ -233,7 +233,8 @@ class Engine:
         return self._told.setdefault(slot, Told())
 
     def last_logprobs(self) -> List[float]:
-        """The log-probabilities of the tokens that the last `step_select` returned."""
+        """The log-probabilities of the tokens that the last `step_select` returned, if a row of it had rules
+        (else none)."""
         return self._last_logprobs
 
     def _settle(self) -> None:
@@ -332,6 +333,7 @@ class Engine:
         histories count what a row brings as the prompt's while its count is 0,
         and as generated afterwards, whether the row has a penalty by then or
         only later; pieces of a prompt may go through `step` before."""
+        self._last_logprobs = []
         if not isinstance(params, SamplingParams):
             params = params_of_rows(params, len(steps))
             if params and not is_ruled(params):

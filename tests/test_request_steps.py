@@ -121,3 +121,19 @@ def test_a_grammar_knows_the_tokens_drawn_before_it(stub):
     engine.step_select([prompt(slot, 7)], SamplingParams(), [0], [1])
     engine.step_select([prompt(slot, 8, 9)], grammar, [0], [2])
     assert asked == [[7, 8, 9]]
+
+
+def test_log_probabilities_are_the_last_steps(stub):
+    """A step whose rows ask for none, or that fails, leaves none of an earlier one's."""
+    engine, _, _ = stub
+    slot = engine.open_sequence()
+    engine.step_select([prompt(slot, 1, 2)], SamplingParams(logprobs=True), [0], [0])
+    assert engine.last_logprobs() == [-0.5]
+    other = engine.open_sequence()
+    engine.step_select([prompt(other, 1, 2)], SamplingParams(), [0], [0])
+    assert engine.last_logprobs() == []
+    engine.step_select([prompt(slot, 7)], SamplingParams(logprobs=True), [0], [1])
+    assert engine.last_logprobs() == [-1.0]
+    with pytest.raises(ValueError):
+        engine.step_select([prompt(slot, 7)], SamplingParams(logit_bias={100: 1.0}), [0], [0])
+    assert engine.last_logprobs() == []
