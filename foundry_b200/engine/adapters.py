@@ -116,7 +116,7 @@ class AdapterStore:
         else:
             tensors, scale = source, 1.0 if scale is None else scale
         scale = float(scale)
-        if not abs(scale) < float("inf"):
+        if not abs(scale) <= torch.finfo(torch.float32).max:  # (what the banks hold it in)
             raise AdapterError(f"an adapter's scale is {scale}")
         pairs = pairs_of(tensors)
         self._check(name, pairs)

@@ -61,3 +61,13 @@ def test_room_that_cannot_be_made_leaves_none():
     with pytest.raises(MemoryError):
         AdapterStore(model_of(some), 1, 8, torch.float32, "cpu")
     assert all(s.bank is None for s in some)
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39, float("inf"), float("nan")])
+def test_a_scale_is_finite_in_the_type_that_holds_it(scale):
+    some = sites()
+    store = AdapterStore(model_of(some), 1, 8, torch.float32, "cpu")
+    with pytest.raises(AdapterError, match="scale"):
+        store.load("x", pairs(), scale)
+    store.load("x", pairs(), 3e38)
+    assert torch.isfinite(some[0].bank.scales).all()
