@@ -213,14 +213,15 @@ class DecodeSession:
         bucket = bucket_of(n)
         unequal = lengths_are_unequal(lengths)
         runner = self.runner
+        self.adapters = engine.adapters_of(slots)  # (a slot may have been opened again with another)
+        adapted = self.adapters is not None
         if runner is None or runner.bucket != bucket or runner.width < need \
-                or runner.unequal != unequal:
+                or runner.unequal != unequal or runner.adapted != adapted:
             width = 8 if runner is None or runner.bucket != bucket else runner.width
             while width < need:
                 width *= 2
             previous = runner
-            runner = self.runner = engine.decode_runner(bucket, width, unequal, self.rules,
-                                                        self.adapters is not None)
+            runner = self.runner = engine.decode_runner(bucket, width, unequal, self.rules, adapted)
             if previous is not None and previous is not runner and previous.bucket == bucket:
                 # tokens that stay on the device (`step`) move on with the session
                 runner.ctx.token_ids.copy_(previous.next_tokens)
@@ -234,7 +235,7 @@ class DecodeSession:
             h[6][n:] = 0
             runner.row_sig[n:] = [None] * (bucket - n)
             runner.filled_for = list(slots)
-        if runner.adapted:  # (a slot may have been opened again with another)
+        if adapted:
             h[-1][:n] = self.adapters
             h[-1][n:] = -1
         h[1][:n] = lengths

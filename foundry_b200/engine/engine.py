@@ -186,6 +186,8 @@ class Engine:
 
     def adapters_of(self, slots: Sequence[int]) -> Optional[List[int]]:
         """The places of these sequences' adapters (-1: none), or None if no one has one."""
+        if not self._adapter_of:
+            return None
         places = [self._adapter_of.get(s, -1) for s in slots]
         return places if any(p >= 0 for p in places) else None
 
