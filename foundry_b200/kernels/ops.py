@@ -2461,6 +2461,13 @@ def adapted_silu_mul(x, w_pairs: torch.Tensor, bank: AdapterBank, index: torch.T
                            adapters=(bank, index))
     if adapted_rows_fit(x, w_pairs, bank):
         return gemm_rows(x, w_pairs, out, silu_mul=True, act=act, adapters=(bank, index))
+    T = index.shape[0]
+    if T > ADAPTER_PIECE:  # (the 32-bit sums of a long prompt's pairs are its largest tensor)
+        x = plain(x)
+        for t in range(0, T, ADAPTER_PIECE):
+            end = t + ADAPTER_PIECE
+            adapted_silu_mul(x[t:end], w_pairs, bank, index[t:end], out[t:end], then_reads, act)
+        return out
     both = adapted_product(x, w_pairs, bank, index, out_dtype=torch.float32, then_reads=then_reads)
     return silu_mul(both, out, interleaved=True, act=act)
 

@@ -55,3 +55,26 @@ def test_a_long_prompt_beside_a_large_bank_takes_little_memory():
     before = torch.cuda.memory_allocated()
     ops.adapted_product(x, w, bank, index)
     assert torch.cuda.max_memory_allocated() - before < (1 << 28) + (1 << 26)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_long_prompts_gated_pairs_take_a_pieces_room(dtype, act):
+    """32-bit gate and up rows stand in memory for 8,192 tokens at a time."""
+    T, K, I, R = 20000, 64, 512, 8
+    g = torch.Generator(device=DEV).manual_seed(0)
+    make = lambda *shape: torch.randn(*shape, generator=g, device=DEV).to(dtype)  # noqa: E731
+    x, w = make(T, K), make(2 * I, K) * 0.1
+    bank = ops.AdapterBank(make(3, R, K) / 8, make(3, 2 * I, R) * 0.1, torch.ones(3, device=DEV))
+    index = torch.arange(T, device=DEV, dtype=torch.int32) * 5 // T % 4
+    out = torch.empty(T, I, dtype=dtype, device=DEV)
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    ops.adapted_silu_mul(x, w, bank, index, out, act=act)
+    assert torch.cuda.max_memory_allocated() - before < 2.5 * 8192 * 2 * I * 4
+    for t in (0, 8191, 8192, 16383, 16384, T - 1):
+        some = torch.empty(1, I, dtype=dtype, device=DEV)
+        ops.adapted_silu_mul(x[t:t + 1], w, bank, index[t:t + 1], some, act=act)
+        assert torch.allclose(out[t].float(), some[0].float(), rtol=2.0 ** -6, atol=1e-4)
