@@ -92,13 +92,15 @@ constexpr int UMMA_K = 16;         // K of one tcgen05.mma for 16-bit inputs
 constexpr int THREADS = 192;       // 6 warps
 using GemmParams = FbGemmParams;
 
+__device__ __forceinline__ bool on_16_bytes(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
 // Epilogue 1 with clamped halves, feature pairs in this thread's registers (`base`: where the
 // first result goes).
 template <int CHUNK>
 __device__ __forceinline__ void store_clamped(const GemmParams& p, const float (&v)[CHUNK],
                                               long long base, long long j0, __nv_bfloat16* out_h) {
   const float* bias = p.clamp.bias;
-  if (j0 + CHUNK <= p.rows_b && (base % 8) == 0) {
+  if (j0 + CHUNK <= p.rows_b && on_16_bytes(out_h + base)) {
     float b[CHUNK];  // all of the chunk's biases asked for before the first is needed
     if (bias != nullptr) {
 #pragma unroll
@@ -156,7 +158,7 @@ __device__ __forceinline__ void store_chunk(const GemmParams& p, const float (&v
         const long long base = i_global * p.stride_a + (j0 >> 1);
         if (p.glu_act == 2) {
           store_clamped<CHUNK>(p, v, base, j0, out_h);
-        } else if (j0 + CHUNK <= p.rows_b && (base % 8) == 0) {
+        } else if (j0 + CHUNK <= p.rows_b && on_16_bytes(out_h + base)) {
 #pragma unroll
           for (int e = 0; e < CHUNK; e += 16) {  // 8 results = 16 bytes per store
             float r8[8];
@@ -208,7 +210,9 @@ __device__ __forceinline__ void store_chunk(const GemmParams& p, const float (&v
     }
   } else if (i_global < p.rows_a) {
     const long long base = i_global * p.stride_a + j0 * p.stride_b;
-    if (p.stride_b == 1 && j0 + CHUNK <= p.rows_b && (base % 8) == 0) {
+    // (by the address: a plane of K shares may start at any multiple of four bytes, an output where its caller says)
+    const bool whole = p.out_f32 ? on_16_bytes(out_f + base) : on_16_bytes(out_h + base);
+    if (p.stride_b == 1 && j0 + CHUNK <= p.rows_b && whole) {
       // this thread's elements are contiguous: vector stores
       if (p.out_f32) {
 #pragma unroll
