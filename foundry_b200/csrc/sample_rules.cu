@@ -870,7 +870,8 @@ sample_rules_kernel(const SampleArgs a) {
   if (tid == 0 && token >= lo && token < hi) {
     a.out[r] = token;
     if (a.also != nullptr) a.also[r] = token;
-    a.logprobs[r] = (float)(-(double)distance(values[token - lo]) - log_all);
+    // (in 64 bits, rounded once: what the sum's weights are off by is all that is left, below a rounding's size)
+    a.logprobs[r] = (float)(((double)values[token - lo] - (double)M) / (greedy ? 1.0 : (double)T) - log_all);
   }
   // (the last meeting's barrier is behind every word to another block)
 }
