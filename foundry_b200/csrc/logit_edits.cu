@@ -26,8 +26,8 @@ __device__ __forceinline__ unsigned bits_of(const unsigned* words, int end, int 
 // whatever a row's start is aligned to, and a thread 16, all asked for together. They go out as they are, or as
 // -inf, as soon as they are there. The few tokens that the history holds are put on a list meanwhile, and the
 // block's threads then work it off in `out`, one load of a count each, all at once; biases follow. 64 rows of
-// 128,256 with 4,000 tokens, 300 biases and masks: 13.5 us, 68 MB at 5.0 TB/s; what is left to the copy rate's
-// 10.4 are chains of three loads in two rounds of blocks. (Six blocks an SM instead of eight 14.6, 8 logits a thread
+// 128,256 with 4,000 tokens, 300 biases and masks: 18.0 us from memory, 68 MB at 3.8 TB/s (13.5 from L2); what is
+// left to the copy rate's 10.4 are chains of three loads in two rounds of blocks. (From L2: six blocks an SM instead of eight 14.6, 8 logits a thread
 // 15.5, the tile in shared memory until its edits are done 16.6; where each thread looked after its own tokens
 // the counts came one after another, and a warp went through the penalties for every 32 tokens of which it
 // held one: 31.)

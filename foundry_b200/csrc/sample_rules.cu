@@ -18,7 +18,8 @@
 // under mixed rules) and the meetings of the cluster one after another, 1 to 1.5 us each: the maximum, the bins,
 // a border, the winner. Device times in graph replays at 128,256 tokens, by rule (greedy, plain, top-k, top-p):
 // one row 6.1, 7.4, 14.1, 14.4 us; 8 rows 7.7, 10.8, 19, 27; 33 rows 10.1, 15.4, 23.5, 41; 64 rows, two rounds
-// of clusters, 19, 32, 51, 77.
+// of clusters, 19, 32, 51, 77. Where fewer than top_k tokens are within 32 temperatures of the best one, the border
+// lies in the last bin and is found bit by bit: k = 50 at T = 0.1 240 us for one row, 690 for 64.
 #include "logit_edits.cuh"
 
 #include <cfloat>
