@@ -220,7 +220,7 @@ class Engine:
         pairs = {"prompt": [], "generated": []}
         for s, t in zip(slots, told):
             for what, tokens in t.kinds() if t is not None else ():
-                pairs[what] += [(s, token) for token in tokens[t.recorded[what]:]]
+                pairs[what] += [(s, int(token)) for token in tokens[t.recorded[what]:]]
                 t.recorded[what] = len(tokens)
         for what, some in pairs.items():
             if some:
@@ -267,7 +267,7 @@ class Engine:
                 [int(s.tokens[0]) for s in steps])
         logits = self._run(steps)
         for s in steps:
-            self.told(s.slot).prompt.extend(int(t) for t in s.tokens)
+            self.told(s.slot).prompt.extend(s.tokens)
         return logits
 
     def _run(self, steps: Sequence[SequenceStep]) -> torch.Tensor:
@@ -362,7 +362,10 @@ class Engine:
         logits = self._run(steps)
         for s, c in zip(steps, counts):
             told = self.told(s.slot)
-            (told.prompt if c == 0 else told.said).extend(int(t) for t in s.tokens)
+            if c == 0:
+                told.prompt.extend(s.tokens)
+            else:
+                told.said.extend(int(t) for t in s.tokens)
         return logits
 
     def _draw_behind(self, steps, params, keys, counts) -> List[int]:

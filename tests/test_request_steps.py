@@ -1,5 +1,7 @@
 """What the engine makes of requests' own sampling, without a device (tests/stub_engine.py)."""
+import numpy as np
 import pytest
+import torch
 
 import stub_engine
 from foundry_b200.engine.context import SequenceStep
@@ -137,3 +139,16 @@ def test_log_probabilities_are_the_last_steps(stub):
     with pytest.raises(ValueError):
         engine.step_select([prompt(slot, 7)], SamplingParams(logit_bias={100: 1.0}), [0], [0])
     assert engine.last_logprobs() == []
+
+
+@pytest.mark.parametrize("kind", [list, np.array, torch.tensor])
+def test_a_callers_tokens_are_its_own_again_behind_the_step(stub, kind):
+    engine, _, history = stub
+    slot = engine.open_sequence()
+    tokens, more = kind([1, 2, 3]), kind([4, 5])
+    engine.step([SequenceStep(slot, tokens, [])])
+    engine.step_select([SequenceStep(slot, more, [1])], SamplingParams(), [0], [0])
+    if kind is list:
+        tokens[0] = more[0] = 99
+    engine.step_select([prompt(slot, 7)], PENALTY, [0], [1])
+    assert held(history, slot) == ([1, 2, 3, 4, 5], [7])
