@@ -2153,17 +2153,31 @@ def _logit_rows(logits: torch.Tensor, what: str):
     return n, V, max(stride, V) if n <= 1 else stride
 
 
+def _partly_the_same(one: int, stride: int, other: int, other_stride: int, n: int, width: int) -> bool:
+    """Whether two sets of n rows of `width` (where they start, and their strides, in elements) share some and are
+    not the same rows. Rows of different strides in one range count as such."""
+    if n == 0 or (one == other and (stride == other_stride or n == 1)):
+        return False
+    if one + (n - 1) * stride + width <= other or other + (n - 1) * other_stride + width <= one:
+        return False
+    return stride != other_stride or n == 1 or not width <= (other - one) % stride <= stride - width
+
+
 def edit_logits(logits: torch.Tensor, edits: LogitEdits,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """The edited logits of every row, float32 (a new tensor, or `out`, which may be `logits`)."""
+    """The edited logits of every row, float32 (a new tensor, or `out`, which may be `logits`, or rows beside
+    them in the same buffer, but no rows that are partly theirs)."""
     n, V, stride = _logit_rows(logits, "edit_logits")
     if out is None:
-        out = logits.new_empty(n, V)
+        out, out_stride = logits.new_empty(n, V), V
     elif out.shape != logits.shape or out.dtype != torch.float32 or out.device != logits.device:
         raise KernelError(f"edit_logits: out is {out.dtype} {tuple(out.shape)} on {out.device}")
+    else:
+        out_stride = max(_rows(out, "out"), V) if n <= 1 else _rows(out, "out")
+        if _partly_the_same(logits.data_ptr() // 4, stride, out.data_ptr() // 4, out_stride, n, V):
+            raise KernelError("edit_logits: out overlaps the logits, and is not the logits")
     packed = edits.packed(n, V, logits.get_device())
-    _call("fb_edit_logits", logits.data_ptr(), stride, n, V, out.data_ptr(),
-          max(_rows(out, "out"), V) if n <= 1 else _rows(out, "out"), packed.buffer_info()[0],
+    _call("fb_edit_logits", logits.data_ptr(), stride, n, V, out.data_ptr(), out_stride, packed.buffer_info()[0],
           _stream(), tag=("n{} v{}", n, V))
     return out
 
