@@ -56,8 +56,8 @@ constexpr int PLANE_ROWS = 256, PLANE_SLOTS = 1024;
 // low[t, j] = scale * sum_k x[t, k] A[a][j, k]. A warp has four ranks, so that a piece of x in its registers meets
 // four rows of A, and PARTS warps of a block share K; block (i, t) has the ranks from i * BLOCK_RANKS on. Few
 // numbers take many warps each, for a warp's loads are then two rounds, all under way together; many have
-// enough warps without. The whole operator (planes of one number a rank) with 8, 4, 2 and 1 parts: 8 tokens of 14,336, rank 64, 27.6, 31, 34 and
-// 46 us; 48 of 4,096, rank 64, 17.6, 16.9, 18.9 and 22.4; 128 of 2,048, rank 64, 24.8, 21.0, 20.5 and 20.6. (A rank
+// enough warps without. The whole operator (planes of one number a rank) with 8, 4, 2 and 1 parts: 8 tokens of
+// 14,336, rank 64, 27.6, 31, 34 and 46 us; 48 of 4,096, rank 64, 17.6, 16.9, 18.9 and 22.4; 128 of 2,048, rank 64, 24.8, 21.0, 20.5 and 20.6. (A rank
 // a warp: 33, 17.1 and 19.6, and 64 tokens of 14,336 82 us against 47.) `wide`: rows are on 16-byte boundaries.
 // PLANES: the numbers go to the token's row of its adapter's plane, and zeros to its row of the others.
 constexpr int RANKS = 4;  // of a warp
@@ -398,8 +398,8 @@ FB_API int fb_adapter_shrink(const void* x, long long ldx, int dtype, const void
   return fb_check_launch("adapter_shrink");
 }
 
-// The same as planes: u [adapters with tokens * 256, fb_plane_width(rank)], counts [1], slots_of [the same number]. Up to 256 tokens,
-// bfloat16; rows behind the last token are left as they are.
+// The same as planes: u [adapters with tokens * 256, fb_plane_width(rank)], counts [1], slots_of [the same number].
+// Up to 256 tokens, bfloat16; rows behind the last token are left as they are.
 FB_API int fb_adapter_shrink_planes(const void* x, long long ldx, const void* a, const float* scales,
                                     const int* index, int slots, int rank, int T, int K, void* u, int* counts,
                                     int* slots_of, cudaStream_t stream) {

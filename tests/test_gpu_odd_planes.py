@@ -65,3 +65,20 @@ def test_outputs_that_start_anywhere(ops, M, N, K, shift, dtype):
     assert torch.equal(out, (x.double() @ w.double().T).to(dtype))
     flat[shift:shift + M * (N + 8)].view(M, N + 8)[:, :N] = 7.0
     assert (flat == 7.0).all()
+
+
+@pytest.mark.parametrize("act", ["silu", "clamped"])
+@pytest.mark.parametrize("shift", [0, 1, 4, 8])
+@pytest.mark.parametrize("M,I,K", [(40, 132, 256), (100, 200, 256), (300, 132, 256), (700, 256, 512), (2100, 136, 128)])
+def test_gated_outputs_that_start_anywhere(ops, M, I, K, shift, act):
+    """The same bits as in rows of their own, and nothing beside them."""
+    x, w = operands(M, 2 * I, K)
+    x, w = x * 0.1, w * 0.1
+    clamp = ops.GluClamp(7.0, 1.7, 1.0, None) if act == "clamped" else None
+    want = ops.gemm_bf16_silu_mul(x, w, torch.empty(M, I, dtype=torch.bfloat16, device=DEV), act=act, clamp=clamp)
+    flat = torch.full((M * (I + 12) + 16,), 7.0, dtype=torch.bfloat16, device=DEV)
+    out = flat[shift:shift + M * (I + 12)].view(M, I + 12)[:, :I]
+    ops.gemm_bf16_silu_mul(x, w, out, act=act, clamp=clamp)
+    assert torch.equal(out, want)
+    out.fill_(7.0)
+    assert (flat == 7.0).all()
